@@ -485,6 +485,157 @@ int wpcg_model_generate(wpcg_model* m, const uint32_t* prompt, uint32_t n_prompt
  * reads the residual. */
 int wpcg_model_debug_read(wpcg_model* m, int which, float* out, uint64_t n);
 
+/* ---- batched serving: pages of keys and values, attention over them -------
+ * No reference counterpart (the reference decodes one sequence with a
+ * contiguous cache, wpc-runtime/src/model.rs:419-547): the operators between
+ * the projections (wpcg_linear_gemm over the rows of several sequences) of a
+ * step that serves many sequences at once, each with as many new rows as it
+ * has (one token, drafts to verify, a prompt).
+ *
+ * Keys and values of one layer live in pages of page_size tokens; a sequence
+ * is a list of page ids (a row of `table`), so sequences grow without copies
+ * and may share pages. Element (page, head, token, i) of the keys is at
+ * k_dev + page*page_stride + head*head_stride + token*token_stride + i, the
+ * values alike; strides count elements, and all three 0 mean the packed order
+ * [page][head][token][head_dim]. dtype: WPCG_DTYPE_F32, WPCG_DTYPE_BF16 or
+ * WPCG_DTYPE_E4M3 (8 bits: 1 sign, 4 exponent, 3 mantissa, largest value 448;
+ * the value a byte stands for is its own times its head's scale). Limits:
+ * head_dim 64 or 128 (else E_UNSUPPORTED); page_size a power of two in
+ * 16..256; pointers and strides multiples of 16 bytes; scales positive.
+ *
+ * A batch's rows are numbered through: sequence s owns rows q_start[s] ..
+ * q_start[s+1]-1 (q_start null: sequence s is row s alone), the newest tokens
+ * of its kv_len[s] ones, so its row i is at position kv_len[s] - n + i of n.
+ * n_rows, max_q and max_kv bound the rows, a sequence's rows and its length;
+ * the arrays themselves are read on the device, so a captured graph follows
+ * them. Rows of no sequence are left as they were. Nothing outside the
+ * arrays is read or written whatever the device arrays hold: a sequence whose
+ * row range is not within 0..n_rows, in order and at most max_q long is left
+ * out; one whose kv_len is not in 0..max_kv, or that needs a page whose id is
+ * not in 0..n_pages-1, gets NaN in its output rows and nothing is stored for
+ * the tokens concerned. A sequence longer in rows than in tokens (kv_len < n)
+ * has rows before position 0; they append nothing and see nothing. */
+#define WPCG_DTYPE_E4M3 3
+typedef struct wpcg_kv_pages_s {
+    void* k_dev;
+    void* v_dev;
+    int32_t dtype;
+    uint32_t n_pages, page_size, n_kv_heads, head_dim;
+    uint64_t page_stride, head_stride, token_stride;
+    const float* k_scale_dev; /* n_kv_heads floats; E4M3 only, null = 1 */
+    const float* v_scale_dev;
+} wpcg_kv_pages;
+typedef struct wpcg_kv_batch_s {
+    uint32_t n_seq, n_rows, max_q, max_kv;
+    uint32_t table_stride;      /* page ids per sequence in table */
+    const int32_t* q_start_dev; /* n_seq + 1, or null */
+    const int32_t* kv_len_dev;  /* n_seq, the new rows counted in */
+    const int32_t* table_dev;   /* [n_seq][table_stride] */
+} wpcg_kv_batch;
+
+/* Stores the rows' keys and values in their sequences' pages, after the
+ * query/key head norm and the rotation (wpc-runtime/src/model.rs:419-547 does
+ * these for one token), and writes the queries that attention reads. Per
+ * head of q and k, with D = head_dim:
+ *   y = x / sqrt(mean(x^2) + eps) * w        (w null: y = x)
+ *   (y_i, y_{i+D/2}) -> (y_i cos a - y_{i+D/2} sin a, y_{i+D/2} cos a + y_i sin a),
+ *   a = position * freq[i], freq being D/2 doubles    (freq null: y as it is)
+ * computed in fp32 with the angle in fp64, and rounded once: to the cache's
+ * type (E4M3: divided by the head's scale and clamped to +-448) and to
+ * q_out_dtype. q, k, v are rows of dtype F32 or BF16, row r at r * stride
+ * elements (0 = packed: heads * head_dim), heads side by side. q and q_out
+ * may both be null (keys and values alone), and q_out may be q itself where
+ * type and stride are the same. Two rows for one place in the pages: the
+ * place holds one of them, which one is not defined. */
+typedef struct wpcg_kv_rows_s {
+    const void* q_dev;
+    const void* k_dev;
+    const void* v_dev;
+    int32_t dtype, q_out_dtype;
+    uint32_t n_heads;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride;
+    void* q_out_dev;
+    const float* q_norm_dev; /* head_dim floats or null */
+    const float* k_norm_dev;
+    const double* freq_dev;  /* head_dim / 2 doubles or null */
+    float eps;
+} wpcg_kv_rows;
+int wpcg_kv_append(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch,
+                   const wpcg_kv_rows* rows, wpcg_stream stream);
+
+/* out = softmax(scale * q K^T) V for every row and query head, query head h
+ * reading key-value head h / (n_heads / n_kv_heads), over the tokens t that
+ * the row at position p sees: t <= p, and, with window > 0, t > p - window or
+ * t < sinks (the first tokens stay visible). A row that sees nothing gives
+ * zeros; what the cache holds at tokens a row does not see (NaN, infinities)
+ * does not reach it, and pages whose tokens no row sees are not looked at, so
+ * a window's old pages may be given away and their ids be anything.
+ * q and out are rows of dtype F32 or BF16 (0 strides = packed). An F32 q keeps
+ * fp32 accuracy whatever the cache holds; a BF16 q goes with a BF16 or E4M3
+ * cache (an F32 cache is E_UNSUPPORTED) and rounds the softmax's terms to
+ * bf16 before they meet V. Sums and softmax statistics are fp32. One pass over
+ * the pages with a running maximum; long sequences are split over workgroups
+ * and joined by a second launch. How a batch is split depends on the batch's
+ * bounds (n_seq, max_q, max_kv), not on what the arrays hold; the same call
+ * gives the same bits.
+ * ws_dev: device memory of at least wpcg_paged_attention_workspace bytes
+ * (16-byte aligned; may be null if that is 0), whose contents are nothing
+ * before or after the call. Calls that may overlap need one each, also as
+ * parts of graphs. The query needs no GPU. */
+typedef struct wpcg_attention_s {
+    const void* q_dev;
+    void* out_dev;
+    int32_t dtype;
+    uint32_t n_heads;
+    uint64_t q_stride, out_stride;
+    float scale;             /* > 0 */
+    uint32_t window, sinks;  /* 0: no window */
+} wpcg_attention;
+int wpcg_paged_attention_workspace(const wpcg_kv_pages* kv, const wpcg_kv_batch* batch,
+                                   const wpcg_attention* att, uint64_t* bytes);
+int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch,
+                         const wpcg_attention* att, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream);
+
+/* Verification of drafted tokens by sampling, beside wpcg_model_verify's
+ * greedy one: the accepted tokens are distributed as the target's own samples.
+ * Sequence s owns rows q_start[s] .. q_start[s+1]-1 (q_start null: max_rows
+ * rows each), as wpcg_model_verify takes them: the last accepted token, then
+ * its drafts, so that k = rows - 1 drafts are checked. Row r holds the
+ * target's logits after tokens[r]; p_r = softmax(logits / temperature[s]),
+ * q_r = draft_probs row r, what the drafter drew tokens[r+1] from (draft_probs
+ * null: the drafts were chosen outright, q_r is 1 there and 0 elsewhere).
+ *   draft r is accepted while u[r] * q_r(tokens[r+1]) < p_r(tokens[r+1]);
+ *   the first rejected row's next token comes from max(0, p_r - q_r), the
+ *   last row's (all accepted) from p_r: the lowest id whose running sum of
+ *   weights passes u_next[s] times their total (where p_r - q_r leaves no
+ *   weight at all: from p_r).
+ * A temperature not above 0 (null: all 1) is greedy: a draft is accepted while it is the
+ * first largest logit, which also is the next token. accepted[s] receives the
+ * number of accepted drafts, out the rows' tokens: the accepted drafts, the
+ * next token, then -1. Probabilities, running sums and comparisons are fp64;
+ * u and u_next are in [0, 1). A row without any weight (NaN, or no logit
+ * above -inf) accepts nothing and gives next token -1; a draft id outside the
+ * vocabulary is rejected; a sequence whose row range is empty, longer than max_rows or not within n_rows gets
+ * accepted = -1 and none of its out is written. vocab <= 2^30, max_rows <=
+ * WPCG_DRAFT_MAX. Workspace and streams as for wpcg_paged_attention. */
+#define WPCG_DRAFT_MAX 64
+typedef struct wpcg_draft_s {
+    uint32_t n_seq, n_rows, max_rows, vocab;
+    const int32_t* q_start_dev;      /* n_seq + 1, or null */
+    const float* logits_dev;         /* [n_rows][vocab], rows logits_stride floats apart (0 = vocab) */
+    uint64_t logits_stride;
+    const float* draft_probs_dev;    /* alike, or null; a sequence's last row is not read */
+    uint64_t draft_stride;
+    const uint32_t* tokens_dev;      /* n_rows */
+    const float* u_dev;              /* n_rows; a sequence's last is not read */
+    const float* u_next_dev;         /* n_seq */
+    const float* temperature_dev;    /* n_seq, or null */
+    int32_t* accepted_dev;           /* n_seq */
+    int32_t* out_dev;                /* n_rows */
+} wpcg_draft;
+int wpcg_draft_verify_workspace(const wpcg_draft* d, uint64_t* bytes);
+int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream);
+
 /* ---- HIP graphs over the context stream (no reference counterpart) ----
  * wpcg_graph_begin starts capturing the context's stream; device calls with
  * stream NULL are then recorded instead of run, until wpcg_graph_end

@@ -1,0 +1,304 @@
+"""GPU tests of wpcg_paged_attention against a plain 64-bit implementation:
+one to many rows a sequence, every pair of types, head layouts, lengths from
+none to split ones, windows and sinks, page orders and strides; what a row does
+not see (NaN, infinities, ids of no page) does not reach it; bad pages and
+lengths; graphs, streams. Bounds are derived in serve_ref.attention_bound."""
+import numpy as np
+import pytest
+
+import serve_ref as R
+import wpcg
+from serve_ref import BF16, E4M3, F32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = wpcg.Context(0)
+    yield c
+    c.close()
+
+
+def expected(pg, q, rows, heads, q_dtype, scale, window, sinks):
+    """(outputs, bounds) [row][head][d] from the stored values."""
+    outs, bounds = [], []
+    at = 0
+    for s, n in enumerate(rows):
+        m = pg.kv_len[s]
+        x = R.decode(q[at:at + n], q_dtype)
+        o, mag, reach = R.attention(x, pg.real["k"][s], pg.real["v"][s], np.arange(m - n, m), scale, window, sinks)
+        outs.append(o)
+        bounds.append(R.attention_bound(o, mag, reach, pg.d, m, q_dtype))
+        at += n
+    return np.concatenate(outs), np.concatenate(bounds)
+
+
+def check(got, want, bound):
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    off = np.abs(got - want) - bound
+    i = np.unravel_index(np.nanargmax(off), off.shape)
+    assert not (off > 0).any(), f"{(off > 0).sum()} of {off.size} off, worst {i}: {got[i]} for {want[i]} +- {bound[i]}"
+
+
+def run(ctx, pg, batch, q, heads, q_dtype, scale, window=0, sinks=0, fill=0x5A, stream=None):
+    """Output rows as values; rows that nothing is written to keep the fill."""
+    rows = q.shape[0]
+    out = ctx.upload(np.full(rows * heads * pg.d * R.SIZE[q_dtype], fill, np.uint8))
+    qd = ctx.upload(q)
+    op = wpcg.PagedAttention(ctx, pg.kv, batch, heads, q_dtype, scale=scale, window=window, sinks=sinks)
+    if op.workspace is not None:  # the workspace may hold anything
+        op.workspace.write(np.full(op.workspace_bytes, 0xFF, np.uint8))
+    op.run(qd, out, stream)
+    ctx.sync()
+    bits = out.read(R.BITS[q_dtype], rows * heads * pg.d).reshape(rows, heads, pg.d)
+    return R.decode(bits, q_dtype), op
+
+
+TYPES = [(BF16, BF16), (BF16, E4M3), (F32, F32), (F32, BF16), (F32, E4M3)]
+LENGTHS = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129, 200, 0, 257]
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("d,heads,hkv", [(128, 8, 2), (64, 14, 2), (64, 3, 3), (128, 20, 1), (128, 32, 1)])
+def test_one_row_every_length(ctx, q_dtype, dtype, d, heads, hkv):
+    """Groups of 4, 7, 1, 20 and 32 query heads (the last in the kernel for
+    many rows); a length of none gives zeros."""
+    print(f"[gpu] one row: {q_dtype}/{dtype} {heads}/{hkv}x{d}", flush=True)
+    rng = np.random.default_rng(d + heads + 100 * q_dtype + dtype)
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 16, LENGTHS, scales=dtype == E4M3).upload()
+    q = R.encode(rng.standard_normal((len(LENGTHS), heads, d)) * 1.5, q_dtype)
+    scale = d ** -0.5
+    got, _ = run(ctx, pg, pg.batch(None), q, heads, q_dtype, scale)
+    check(got, *expected(pg, q, [1] * len(LENGTHS), heads, q_dtype, scale, 0, 0))
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (16, 3), (33, 16), (50, 40), (1000, 4), (7, 300)])
+def test_few_rows_windows(ctx, q_dtype, dtype, window, sinks):
+    """Three rows a sequence (drafts): causal among themselves, windows that
+    end inside tiles, sinks that meet the window and that exceed the length."""
+    print(f"[gpu] few rows: {q_dtype}/{dtype} window {window} sinks {sinks}", flush=True)
+    rng = np.random.default_rng(window * 7 + sinks + q_dtype + 10 * dtype)
+    lens = [3, 5, 20, 50, 64, 97, 150, 258]
+    pg = R.Paged(ctx, rng, dtype, 2, 128, 32, lens, order="token", scales=dtype == E4M3).upload()
+    q = R.encode(rng.standard_normal((3 * len(lens), 8, 128)) * 1.5, q_dtype)
+    got, _ = run(ctx, pg, pg.batch([3] * len(lens)), q, 8, q_dtype, 0.1, window, sinks)
+    check(got, *expected(pg, q, [3] * len(lens), 8, q_dtype, 0.1, window, sinks))
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("d,heads,hkv,window,sinks", [(128, 8, 2, 0, 0), (64, 7, 1, 0, 0), (128, 4, 4, 40, 5),
+                                                      (64, 4, 2, 64, 0), (128, 16, 1, 100, 70)])
+def test_many_rows(ctx, q_dtype, dtype, d, heads, hkv, window, sinks):
+    """Ragged prompts, with and without cached tokens before them, and a
+    sequence with more rows than tokens (its first rows see nothing)."""
+    print(f"[gpu] many rows: {q_dtype}/{dtype} {heads}/{hkv}x{d} window {window} sinks {sinks}", flush=True)
+    rng = np.random.default_rng(d + heads + window + q_dtype + 10 * dtype)
+    rows, lens = [70, 1, 133, 40, 9], [70, 200, 190, 167, 5]
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 64, lens, scales=dtype == E4M3).upload()
+    q = R.encode(rng.standard_normal((sum(rows), heads, d)) * 1.5, q_dtype)
+    scale = d ** -0.5
+    got, _ = run(ctx, pg, pg.batch(rows), q, heads, q_dtype, scale, window, sinks)
+    check(got, *expected(pg, q, rows, heads, q_dtype, scale, window, sinks))
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("rows,lens,heads,hkv,window", [([1, 1], [5000, 37], 4, 2, 0), ([2, 2], [3001, 1], 8, 2, 700),
+                                                        ([40, 3], [2500, 3], 8, 2, 0), ([65], [4000], 4, 1, 900)])
+def test_split_and_joined(ctx, q_dtype, dtype, rows, lens, heads, hkv, window):
+    """Sequences split over workgroups, beside ones too short for a second
+    part; the same call gives the same bits."""
+    print(f"[gpu] split: {q_dtype}/{dtype} rows {rows} lens {lens}", flush=True)
+    rng = np.random.default_rng(sum(lens) + q_dtype + 10 * dtype)
+    pg = R.Paged(ctx, rng, dtype, hkv, 128, 16, lens, scales=dtype == E4M3).upload()
+    q = R.encode(rng.standard_normal((sum(rows), heads, 128)) * 1.5, q_dtype)
+    b = pg.batch(rows)
+    got, op = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, 4)
+    assert op.workspace_bytes > 0
+    check(got, *expected(pg, q, rows, heads, q_dtype, 0.09, window, 4))
+    again, _ = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, 4)
+    assert np.array_equal(got.view(np.uint64), again.view(np.uint64))
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("rows", [2, 30])
+def test_infinite_values_reach_only_rows_that_see_them(ctx, q_dtype, dtype, rows):
+    """The last token's values hold NaN (and infinities where the type has
+    them): rows before it are as if they were not there, its own row has them."""
+    print(f"[gpu] not finite: {q_dtype}/{dtype} rows {rows}", flush=True)
+    rng = np.random.default_rng(rows + dtype)
+    n = 75
+    pg = R.Paged(ctx, rng, dtype, 1, 64, 16, [n])
+    odd = [np.nan] if dtype == E4M3 else [np.inf, -np.inf, np.nan]
+    last = pg.real["v"][0][n - 1, 0].copy()
+    for i, x in enumerate(odd):
+        last[5 + 17 * i] = x
+    words = R.encode(last, dtype)
+    pg.put("v", 0, words[None, None], [n - 1])
+    pg.upload()
+    q = R.encode(rng.standard_normal((rows, 4, 64)), q_dtype)
+    got, _ = run(ctx, pg, pg.batch([rows]), q, 4, q_dtype, 0.125)
+    want, bound = expected(pg, q, [rows], 4, q_dtype, 0.125, 0, 0)
+    check(got[:-1], want[:-1], bound[:-1])
+    clean = np.isfinite(last)
+    check(got[-1][:, clean], want[-1][:, clean], bound[-1][:, clean])
+    for i, x in enumerate(odd):
+        assert np.array_equal(got[-1][:, 5 + 17 * i], np.full(4, x), equal_nan=True)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_bad_pages_lengths_and_row_ranges(ctx, rows):
+    """NaN for sequences with an id of no page or an impossible length, others
+    as they should be; rows of no sequence stay as they were. Ids of pages that
+    no row sees are not looked at."""
+    print(f"[gpu] bad pages, rows {rows}", flush=True)
+    rng = np.random.default_rng(rows)
+    lens = [300] * 6
+    pg = R.Paged(ctx, rng, BF16, 2, 128, 16, lens).upload()
+    pg.table[1, 18] = pg.n_pages       # one past the last
+    pg.table[2, 3] = -1                # in the window's gap below, seen without it
+    pg.kv_len[3] = 301                 # above max_kv
+    pg.kv_len[4] = -5
+    nr = [rows] * 6
+    batch = pg.batch(nr, n_rows=6 * rows + 5, max_kv=300)
+    pg.kv_len = lens
+    q = R.encode(rng.standard_normal((6 * rows + 5, 4, 128)), BF16)
+    for window in (0, 100):
+        got, _ = run(ctx, pg, batch, q, 4, BF16, 0.1, window, 16)
+        want, bound = expected(pg, q, nr, 4, BF16, 0.1, window, 16)
+        ok = [0, 5] + ([2] if window else [])
+        for s in range(6):
+            part = slice(s * rows, (s + 1) * rows)
+            if s in ok:
+                check(got[part], want[part], bound[part])
+            elif s != 2:
+                assert np.isnan(got[part]).all(), s
+        if not window:
+            assert np.isnan(got[2 * rows:3 * rows]).all()
+        fill = R.decode(np.full(1, 0x5A5A, np.uint16), BF16)[0]
+        assert (got[6 * rows:] == fill).all()
+    # row ranges out of order or beyond the rows: left out
+    start = np.cumsum([0] + nr).astype(np.int32)
+    start[4] = 6 * rows + 6
+    pg.d_start.write(start)
+    got, _ = run(ctx, pg, batch, q, 4, BF16, 0.1, 100, 16)
+    assert (got[3 * rows:4 * rows] == fill).all() and (got[4 * rows:5 * rows] == fill).all()
+    check(got[:rows], want[:rows], bound[:rows])
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_strided_rows_leave_the_gaps(ctx, rows):
+    """q and out as slices of wider rows."""
+    rng = np.random.default_rng(9)
+    lens = [90, 130]
+    pg = R.Paged(ctx, rng, BF16, 2, 64, 128, lens, order="token").upload()
+    heads, width = 6, 6 * 64 + 72
+    n = 2 * rows
+    q = R.encode(rng.standard_normal((n, width)), F32)
+    qd, out = ctx.upload(q), ctx.upload(np.full((n, width), 0x5A5A5A5A, np.uint32))
+    op = wpcg.PagedAttention(ctx, pg.kv, pg.batch([rows] * 2), heads, F32, scale=0.2, q_stride=width, out_stride=width)
+    op.run(qd, out)
+    ctx.sync()
+    bits = out.read(np.uint32, n * width).reshape(n, width)
+    assert (bits[:, heads * 64:] == 0x5A5A5A5A).all()
+    x = np.ascontiguousarray(q[:, :heads * 64]).reshape(n, heads, 64)
+    check(R.decode(np.ascontiguousarray(bits[:, :heads * 64]), F32).reshape(n, heads, 64),
+          *expected(pg, x, [rows] * 2, heads, F32, 0.2, 0, 0))
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_pages_beyond_32_bit_offsets(ctx, rows):
+    """A cache of 5 GiB keys and as many values, the sequence's pages at its
+    far end."""
+    print(f"[gpu] far pages, rows {rows}", flush=True)
+    rng = np.random.default_rng(4)
+    hkv, d, page = 2, 128, 16
+    elems = hkv * page * d
+    total = (5 << 30) // (2 * elems)
+    pg = R.Paged(ctx, rng, BF16, hkv, d, page, [100], spare=0)
+    near = {n: pg.bits[n] for n in "kv"}
+    big = [ctx.alloc(total * elems * 2) for _ in range(2)]
+    first = total - pg.n_pages
+    for b, n in zip(big, "kv"):
+        wpcg.check(wpcg.lib.wpcg_memcpy_h2d(ctx.h, b.ptr.value + first * elems * 2, near[n].ctypes.data,
+                                            near[n].nbytes))
+    pg.kv = wpcg.PagedKv(ctx, total, page, hkv, d, BF16, k=big[0], v=big[1])
+    keep = pg.table.copy()
+    pg.table[0, :7] += first
+    batch = pg.batch([rows])
+    pg.table = keep
+    q = R.encode(rng.standard_normal((rows, 8, d)), BF16)
+    got, _ = run(ctx, pg, batch, q, 8, BF16, 0.09)
+    check(got, *expected(pg, q, [rows], 8, BF16, 0.09, 0, 0))
+    for b in big:
+        b.free()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_captured_graph_follows_the_lengths(ctx, rows):
+    """One graph, replayed while the lengths change on the device, with other
+    calls (and another operator object with its own workspace) between."""
+    print(f"[gpu] graph, rows {rows}", flush=True)
+    rng = np.random.default_rng(rows + 1)
+    full = [900, 1500]
+    pg = R.Paged(ctx, rng, BF16, 2, 128, 16, full).upload()
+    batch = pg.batch([rows] * 2)
+    q = R.encode(rng.standard_normal((2 * rows, 8, 128)), F32)
+    qd = ctx.upload(q)
+    outs = [ctx.alloc(q.nbytes) for _ in range(2)]
+    ops = [wpcg.PagedAttention(ctx, pg.kv, batch, 8, F32, scale=0.09) for _ in range(2)]
+    assert ops[0].workspace_bytes > 0
+    g = ctx.capture(lambda: ops[0].run(qd, outs[0]))
+    g2 = ctx.capture(lambda: ops[1].run(qd, outs[1]))
+    for lens in ([900, 1500], [rows, 777], [450, rows + 1], [900, 1500]):
+        pg.d_len.write(np.array(lens, np.int32))
+        outs[0].write(np.full(q.size, 0xFFFFFFFF, np.uint32))
+        g.launch()
+        g2.launch()
+        g.launch()
+        ctx.sync()
+        pg.kv_len = lens
+        kept = pg.real
+        pg.real = {n: [x[:m] for x, m in zip(kept[n], lens)] for n in "kv"}
+        want, bound = expected(pg, q, [rows] * 2, 8, F32, 0.09, 0, 0)
+        pg.real = kept
+        bits = [o.read(np.uint32, q.size).reshape(q.shape) for o in outs]
+        assert np.array_equal(bits[0], bits[1])
+        check(R.decode(bits[0], F32), want, bound)
+    del g, g2
+
+
+def test_other_streams(ctx):
+    """Calls of two objects on streams of other contexts, at once."""
+    rng = np.random.default_rng(12)
+    pg = R.Paged(ctx, rng, E4M3, 2, 64, 32, [2000, 1000], scales=True).upload()
+    batch = pg.batch(None)
+    q = R.encode(rng.standard_normal((2, 6, 64)), F32)
+    qd = ctx.upload(q)
+    want, bound = expected(pg, q, [1, 1], 6, F32, 0.125, 0, 0)
+    others = [wpcg.Context(0) for _ in range(2)]
+    ops = [wpcg.PagedAttention(ctx, pg.kv, batch, 6, F32, scale=0.125) for _ in others]
+    outs = [ctx.alloc(q.nbytes) for _ in others]
+    for _ in range(20):
+        for o, op, out in zip(others, ops, outs):
+            op.run(qd, out, o.stream)
+    for o, out in zip(others, outs):
+        o.sync()
+        check(R.decode(out.read(np.uint32, q.size).reshape(q.shape), F32), want, bound)
+        o.close()
+
+
+def test_nothing_to_do(ctx):
+    rng = np.random.default_rng(1)
+    pg = R.Paged(ctx, rng, BF16, 1, 64, 16, [10]).upload()
+    batch = pg.batch(None)
+    q = ctx.upload(R.encode(rng.standard_normal((1, 1, 64)), BF16))
+    for n_seq, n_rows in ((0, 0), (0, 1)):
+        b = wpcg.KvBatch(n_seq, n_rows, batch.kv_len, batch.table, 2, 10)
+        op = wpcg.PagedAttention(ctx, pg.kv, b, 1, BF16)
+        op.run(q, q)
+    # a batch that has room for tokens and holds none
+    pg.d_len.write(np.zeros(1, np.int32))
+    got, _ = run(ctx, pg, batch, R.encode(rng.standard_normal((1, 1, 64)), BF16), 1, BF16, 0.125)
+    assert (got == 0).all()

@@ -1,0 +1,574 @@
+// Attention of few rows over paged keys and values: one new token of each
+// sequence, or the drafts being verified.
+//
+// Every key and value is read once for the query heads of its group, and with
+// one to a few rows that is all there is to do: the memory is the bound (two
+// flops a byte and query head). So the kernel is built to keep loads in
+// flight. Nothing is staged: a wave loads 32 tokens' keys and values straight
+// into the matrix cores' operand layout, 16 bytes a lane, and the next tile's
+// keys are on their way while this tile's softmax runs. A wave owns every
+// fourth tile of the workgroup's chunk, with a running maximum and sum of its
+// own; the four are put together through LDS at the end.
+//
+// Layout. Columns are (row, query head) pairs, 16 a workgroup: lane l holds
+// column l % 16 throughout, lane group g = l / 16. With keys as the A operand
+// (16 tokens) and queries as B, the scores S^T leave lane (column, g) the
+// tokens 4g .. 4g+3 of a 16-token half. That is what the second product needs
+// as its B operand already: a contraction may take its terms in any order, so
+// V^T's A operand just takes tokens 4g .. 4g+3 of both halves in lane group
+// g too, and the terms never leave their lane. The running maximum, the sum
+// and the rescaling factor are one number a lane. V^T needs one dimension's
+// eight tokens side by side: a lane loads D/16 dimensions of eight tokens
+// and transposes them in registers, one byte permute per two values.
+//
+// Precision. With BF16 queries the products are bf16 x bf16 (keys, values and
+// queries exact), the softmax's terms rounded to bf16 for the second: half a
+// step of relative error on each term, as the output's own rounding has.
+// With F32 queries, q and the terms are carried as three bf16 each, exactly,
+// over a BF16 or E4M3 cache, and an F32 cache takes the fp32 matrix cores.
+#include "paged.h"
+
+namespace wpcg {
+namespace {
+
+constexpr int WAVES = 4;
+constexpr int THREADS = 64 * WAVES;
+constexpr int TILE = ATTN_FEW_TILE, COLS = ATTN_FEW_COLS;
+
+// Keys of 16 tokens as A fragments. BF16 and E4M3: D/32 fragments of 32
+// dimensions; lane (token, g) holds dimensions key_dim(f, g) + 0..7. F32:
+// D/16 of four products of 4 dimensions, product e of fragment f taking
+// dimension 16 f + 4 g + e from lane group g.
+template <int CT>
+__device__ __forceinline__ int key_dim(int f, int g)
+{
+    return CT == CT_F32 ? 16 * f + 4 * g : CT == CT_BF16 ? 32 * f + 8 * g : 64 * (f / 2) + 16 * g + 8 * (f % 2);
+}
+
+template <int D, int CT>
+struct Keys {
+    static constexpr int LOADS = D * ct_size<CT>() / 64;  // of 16 bytes
+    pu32x4 w[LOADS];
+    __device__ __forceinline__ void load(const uint8_t* row, int g)  // row: the lane's token
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) w[i] = *(const pu32x4*)(row + i * 64 + g * 16);
+    }
+    __device__ __forceinline__ pbf16x8 frag(int f) const  // not F32
+    {
+        if (CT == CT_BF16) return __builtin_bit_cast(pbf16x8, w[f]);
+        const uint32_t a = w[f / 2][f % 2 * 2], b = w[f / 2][f % 2 * 2 + 1];
+        const pu32x4 r = {e4m3_bf16<false>(a), e4m3_bf16<true>(a), e4m3_bf16<false>(b), e4m3_bf16<true>(b)};
+        return __builtin_bit_cast(pbf16x8, r);
+    }
+};
+
+// Values of a tile: lane (n, g) holds dimensions n*DV .. n*DV + DV-1 of its
+// eight tokens 4g .. 4g+3 and 16 + 4g .. 16 + 4g+3.
+template <int D, int CT>
+struct Values {
+    static constexpr int DV = D / 16;
+    static constexpr int WORDS = DV * ct_size<CT>() / 4;  // of one token
+    uint32_t w[8][WORDS];
+    __device__ __forceinline__ void load(int x, const uint8_t* row, int n)
+    {
+        const uint8_t* p = row + n * DV * ct_size<CT>();
+        if constexpr (WORDS >= 4) {
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; i++) {
+                const pu32x4 v = *(const pu32x4*)(p + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[x][4 * i + j] = v[j];
+            }
+        } else if constexpr (WORDS == 2) {
+            const pu32x2 v = *(const pu32x2*)p;
+            w[x][0] = v[0];
+            w[x][1] = v[1];
+        } else {
+            w[x][0] = *(const uint32_t*)p;
+        }
+    }
+    __device__ __forceinline__ void clear(int x)
+    {
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) w[x][i] = 0;
+    }
+    // bf16 pair of dimensions 2 i, 2 i + 1 of token x (not F32)
+    __device__ __forceinline__ uint32_t pair(int x, int i) const
+    {
+        if (CT == CT_BF16) return w[x][i];
+        return i % 2 ? e4m3_bf16<true>(w[x][i / 2]) : e4m3_bf16<false>(w[x][i / 2]);
+    }
+    __device__ __forceinline__ bool odd() const  // a value that is not finite
+    {
+        bool r = false;
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+            if constexpr (CT == CT_F32) {
+#pragma unroll
+                for (int i = 0; i < WORDS; i++) r |= (w[x][i] & 0x7f800000u) == 0x7f800000u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < DV / 2; i++) r |= bf16_odd(pair(x, i));
+            }
+        }
+        return r;
+    }
+};
+
+// acc[j] += A_j B over the tile's 32 tokens, A_j being dimension n*DV + j of
+// the values, for NT bf16 terms of B. ODD: what is not finite in A is kept out
+// of the products and added to the columns of `see` (1.0 where the column sees
+// the token) alone; three more products count the +inf, -inf and NaN a column
+// sees.
+template <int D, int CT, int NT, bool ODD>
+__device__ __forceinline__ void add_values(const Values<D, CT>& v, const pbf16x8 (&b)[NT], pf32x4 (&acc)[D / 16],
+                                           pbf16x8 see)
+{
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        uint32_t t[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) t[x] = v.pair(x, i);
+        const auto side = [&](const uint32_t (&w)[8], bool high) {
+            pu32x4 r;
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                r[x] = __builtin_amdgcn_perm(w[2 * x + 1], w[2 * x], high ? 0x07060302u : 0x05040100u);
+            return __builtin_bit_cast(pbf16x8, r);
+        };
+        if constexpr (ODD) {
+#pragma unroll 1
+            for (int kind = 0; kind < 3; kind++) {
+                uint32_t is[8];
+#pragma unroll
+                for (int x = 0; x < 8; x++) is[x] = bf16_is(t[x], kind);
+                const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const pf32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(side(is, e), see, (pf32x4){}, 0, 0, 0);
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if (n[y] > 0.0f) acc[2 * i + e][y] += add;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 8; x++) t[x] = bf16_finite(t[x]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const pbf16x8 a = side(t, e);
+#pragma unroll
+            for (int n = NT - 1; n >= 0; n--)  // small terms first
+                acc[2 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[n], acc[2 * i + e], 0, 0, 0);
+        }
+    }
+}
+
+template <int D, int CT, bool QF32>
+__global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
+{
+    constexpr bool F32MM = CT == CT_F32;  // the fp32 matrix cores
+    constexpr int NT = QF32 ? 3 : 1;      // bf16 terms of q and of the softmax's terms
+    constexpr int DV = D / 16;
+    constexpr int ES = ct_size<CT>();
+    __shared__ float s_o[WAVES][COLS][D + 4];
+    __shared__ float s_ml[WAVES][COLS][2];
+
+    // block -> (column block, chunk, sequence and head); the heads of a
+    // sequence are neighbours
+    const int pairs = p.b.n_seq * p.n_kv;
+    const int pair = (int)(blockIdx.x % (unsigned)pairs), rest = (int)(blockIdx.x / (unsigned)pairs);
+    const int cb = rest % p.col_blocks, split = rest / p.col_blocks;
+    const int seq = pair / p.n_kv, kvh = pair % p.n_kv;
+    const SeqRows sq = seq_rows(p.b, seq);
+    const int cols = sq.n * p.group;  // of this sequence and head
+    if (cb * COLS >= cols) return;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int c = lane & 15, g = lane >> 4;
+    const int col = cb * COLS + c;
+    const bool live = col < cols;
+    const int row = live ? col / p.group : 0;
+    const int head = kvh * p.group + (live ? col % p.group : 0);
+    const int len = sq.bad ? 0 : sq.len;
+    const int pos0 = len - sq.n;  // position of the sequence's row 0
+    const int first = cb * COLS / p.group, last = min(cols, (cb + 1) * COLS) - 1;
+    const SeenTiles<TILE> seen = seen_tiles<TILE>(pos0 + first, pos0 + last / p.group, p.window, p.sinks);
+    const int v0 = split * p.chunk, v1 = min(v0 + p.chunk, seen.total());
+    if (v0 >= v1 && split > 0) return;
+    const int pos = pos0 + row;
+    // tokens that every column of the block sees: no mask there
+    const int all_hi = pos0 + first + 1;
+    const int all_lo = p.window > 0 ? pos0 + last / p.group - p.window + 1 : 0;
+
+    // q as B fragments, in the keys' order of dimensions
+    const uint64_t q_at = (uint64_t)(sq.a + row) * p.q_row + (uint64_t)head * D;
+    constexpr int QF = F32MM ? 1 : D / 32, QW = F32MM ? D / 16 : 1;
+    pbf16x8 qb[QF][NT];
+    pf32x4 qf[QW];
+    if constexpr (F32MM) {
+#pragma unroll
+        for (int f = 0; f < QW; f++)
+            qf[f] = live ? *(const pf32x4*)((const float*)p.q + q_at + key_dim<CT>(f, g)) : (pf32x4){};
+    } else {
+#pragma unroll
+        for (int f = 0; f < QF; f++) {
+            const int d = key_dim<CT>(f, g);
+            if constexpr (QF32) {
+                pf32x4 a = {}, b = {};
+                if (live) {
+                    a = *(const pf32x4*)((const float*)p.q + q_at + d);
+                    b = *(const pf32x4*)((const float*)p.q + q_at + d + 4);
+                }
+                uint32_t t[4][3];
+                split3(a[0], a[1], t[0]);
+                split3(a[2], a[3], t[1]);
+                split3(b[0], b[1], t[2]);
+                split3(b[2], b[3], t[3]);
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+                    qb[f][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
+            } else {
+                const pu32x4 w = live ? *(const pu32x4*)((const uint16_t*)p.q + q_at + d) : (pu32x4){};
+                qb[f][0] = __builtin_bit_cast(pbf16x8, w);
+            }
+        }
+    }
+    const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
+
+    const uint8_t* const kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
+    const uint8_t* const vp = (const uint8_t*)p.v + (uint64_t)kvh * p.head_stride * ES;
+    const int32_t* const table = p.b.table + (uint64_t)seq * p.b.table_stride;
+    const uint64_t page_bytes = p.page_stride * ES, token_bytes = p.token_stride * ES;
+
+    // a half tile's place in the pages (elements from the head's start); false
+    // where it needs a page that is none. Halves that no row sees read page 0
+    // unlooked at: they are masked.
+    bool fault = false;
+    const auto place = [&](int t0) -> uint64_t {
+        if (!seen.any(t0, t0 + 16)) return 0;
+        const uint32_t id = (uint32_t)table[t0 >> p.b.page_shift];
+        if (id >= p.b.n_pages) {
+            fault = true;
+            return 0;
+        }
+        return (uint64_t)id * page_bytes + (uint64_t)(t0 & (p.b.page_size - 1)) * token_bytes;
+    };
+
+    Keys<D, CT> K[2];
+    Values<D, CT> V;
+    pf32x4 acc[DV] = {};
+    float m = -INFINITY, l = 0.0f;
+
+    int vt = v0 + wave;
+    uint64_t at[2] = {0, 0};
+    if (vt < v1) {
+        const int t0 = seen.tile(vt) * TILE;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            at[h] = place(t0 + 16 * h);
+            K[h].load(kp + at[h] + (uint64_t)c * token_bytes, g);
+        }
+    }
+    for (; vt < v1; vt += WAVES) {
+        const int t0 = seen.tile(vt) * TILE;
+#pragma unroll
+        for (int x = 0; x < 8; x++)
+            V.load(x, vp + at[x / 4] + (uint64_t)(4 * g + x % 4) * token_bytes, c);
+        uint64_t next[2] = {0, 0};
+        if (vt + WAVES < v1) {
+            const int t1 = seen.tile(vt + WAVES) * TILE;
+            next[0] = place(t1);
+            next[1] = place(t1 + 16);
+        }
+        // scores
+        pf32x4 s[2] = {};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if constexpr (F32MM) {
+#pragma unroll
+                for (int f = 0; f < QW; f++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(K[h].w[f][e]), qf[f][e], s[h], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int n = NT - 1; n >= 0; n--)
+#pragma unroll
+                    for (int f = 0; f < QF; f++)
+                        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K[h].frag(f), qb[f][n], s[h], 0, 0, 0);
+            }
+        }
+        if (vt + WAVES < v1) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) K[h].load(kp + next[h] + (uint64_t)c * token_bytes, g);
+        }
+        at[0] = next[0];
+        at[1] = next[1];
+        // mask
+        const bool whole = t0 + TILE <= all_hi && t0 >= all_lo;
+        if (!whole) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const int t = t0 + 16 * (x / 4) + 4 * g + x % 4;
+                if (!row_sees(pos, t, p.window, p.sinks)) s[x / 4][x % 4] = -INFINITY;
+            }
+        }
+        // running maximum and terms
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = max_x16_32(top) * sc;
+        const float now = fmaxf(m, top);
+        const float base = now == -INFINITY ? 0.0f : now;
+        if (__any(now > m)) {
+            const float f = exp2_fast(m - base);
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < DV; j++) acc[j] *= f;
+            m = now;
+        }
+        float e[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+            e[x] = exp2_fast(fmaf(s[x / 4][x % 4], sc, -base));
+            l += e[x];
+        }
+        // what a masked token's value holds stays out: tokens that no column
+        // sees are cleared, and values that are not finite and that only some
+        // columns see are added to those alone
+        bool odd = false;
+        if (!whole) {
+#pragma unroll
+            for (int x = 0; x < 8; x++)
+                if (!seen.some(t0 + 16 * (x / 4) + 4 * g + x % 4)) V.clear(x);
+            odd = __any(V.odd());
+        }
+        if constexpr (F32MM) {
+            if (odd) {
+#pragma unroll 1
+                for (int kind = 0; kind < 3; kind++) {
+                    const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+                    for (int j = 0; j < DV; j++) {
+                        pf32x4 n = {};
+#pragma unroll
+                        for (int x = 0; x < 8; x++) {
+                            const int t = t0 + 16 * (x / 4) + 4 * g + x % 4;
+                            const uint32_t w = V.w[x][j];
+                            const bool hit = kind == 0 ? w == 0x7f800000u : kind == 1 ? w == 0xff800000u
+                                                                                    : (w & 0x7fffffffu) > 0x7f800000u;
+                            n = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                hit ? 1.0f : 0.0f, row_sees(pos, t, p.window, p.sinks) ? 1.0f : 0.0f, n, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (n[i] > 0.0f) acc[j][i] += add;
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+#pragma unroll
+                    for (int j = 0; j < DV; j++)
+                        if ((V.w[x][j] & 0x7f800000u) == 0x7f800000u) V.w[x][j] = 0;
+            }
+#pragma unroll
+            for (int x = 0; x < 8; x++)
+#pragma unroll
+                for (int j = 0; j < DV; j++)
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(V.w[x][j]), e[x], acc[j], 0, 0, 0);
+        } else {
+            pbf16x8 b[NT];
+            if constexpr (QF32) {
+                uint32_t t[4][3];
+#pragma unroll
+                for (int x = 0; x < 4; x++) split3(e[2 * x], e[2 * x + 1], t[x]);
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+                    b[n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
+            } else {
+                pu32x4 t;
+#pragma unroll
+                for (int x = 0; x < 4; x++) t[x] = pk_bf16_rne(e[2 * x], e[2 * x + 1]);
+                b[0] = __builtin_bit_cast(pbf16x8, t);
+            }
+            if (odd) {
+                pu32x4 see;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int t = t0 + 16 * (x / 2) + 4 * g + 2 * x % 4;
+                    see[x] = (row_sees(pos, t, p.window, p.sinks) ? 0x3f80u : 0u) |
+                             (row_sees(pos, t + 1, p.window, p.sinks) ? 0x3f800000u : 0u);
+                }
+                add_values<D, CT, NT, true>(V, b, acc, __builtin_bit_cast(pbf16x8, see));
+            } else {
+                add_values<D, CT, NT, false>(V, b, acc, pbf16x8{});
+            }
+        }
+    }
+    l = sum_x16_32(l);
+    if (__any(fault)) l = __builtin_nanf("");
+
+    // the four waves' parts together; a lane's D/4 outputs are dimensions
+    // (4g + i) * DV + j of column c
+    if (g == 0) {
+        s_ml[wave][c][0] = m;
+        s_ml[wave][c][1] = l;
+    }
+    __syncthreads();
+    float top = s_ml[0][c][0];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) top = fmaxf(top, s_ml[w][c][0]);
+    const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+#pragma unroll
+    for (int j = 0; j < DV; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s_o[wave][c][(4 * g + i) * DV + j] = f == 0.0f ? 0.0f : acc[j][i] * f;
+    __syncthreads();
+
+    // thread -> column tid / 16, DV dimensions
+    const int oc = (int)threadIdx.x / 16, od = (int)threadIdx.x % 16 * DV;
+    const int ocol = cb * COLS + oc;
+    if (ocol >= cols) return;
+    float om = s_ml[0][oc][0], ol = 0.0f;
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) om = fmaxf(om, s_ml[w][oc][0]);
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        const float wm = s_ml[w][oc][0], wl = s_ml[w][oc][1];
+        ol += wm == -INFINITY ? (wl != wl ? wl : 0.0f) : wl * exp2_fast(wm - om);
+    }
+    float o[DV];
+#pragma unroll
+    for (int j = 0; j < DV; j++) {
+        o[j] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) o[j] += s_o[w][oc][od + j];
+    }
+    const int orow = ocol / p.group, ohead = kvh * p.group + ocol % p.group;
+    if (p.splits > 1) {
+        const uint64_t slot = ((uint64_t)split * p.b.n_rows + sq.a + orow) * p.n_heads + ohead;
+#pragma unroll
+        for (int j = 0; j < DV; j += 4)
+            *(pf32x4*)(p.part_o + slot * D + od + j) = (pf32x4){o[j], o[j + 1], o[j + 2], o[j + 3]};
+        if (od == 0) {
+            p.part_ml[slot * 2] = om;
+            p.part_ml[slot * 2 + 1] = ol;
+        }
+        return;
+    }
+    attn_store<DV, QF32>(p, sq, orow, ohead, od, D, o, ol, p.v_scale ? p.v_scale[kvh] : 1.0f);
+}
+
+template <int D, int CT, bool QF32>
+void go(const PagedAttnArgs& p, unsigned blocks, hipStream_t s)
+{
+    k_attn_few<D, CT, QF32><<<dim3(blocks), dim3(THREADS), 0, s>>>(p);
+}
+
+template <int D>
+void go_types(const PagedAttnArgs& p, int q_dtype, int cache_dtype, unsigned blocks, hipStream_t s)
+{
+    if (q_dtype == WPCG_DTYPE_BF16) {
+        if (cache_dtype == WPCG_DTYPE_BF16) go<D, CT_BF16, false>(p, blocks, s);
+        else go<D, CT_E4M3, false>(p, blocks, s);
+    } else {
+        if (cache_dtype == WPCG_DTYPE_F32) go<D, CT_F32, true>(p, blocks, s);
+        else if (cache_dtype == WPCG_DTYPE_BF16) go<D, CT_BF16, true>(p, blocks, s);
+        else go<D, CT_E4M3, true>(p, blocks, s);
+    }
+}
+
+// ---- the chunks' states joined -------------------------------------------------
+// A workgroup per (row, query head): out = sum_i 2^(m_i - M) o_i / sum_i
+// 2^(m_i - M) l_i over the chunks that the row's workgroup had, in an order
+// that depends on their number alone. Four chunks are read at a time.
+template <int D, bool QF32, bool MANY>
+__global__ __launch_bounds__(256) void k_attn_join(PagedAttnArgs p)
+{
+    constexpr int COLS_ = MANY ? ATTN_MANY_COLS : ATTN_FEW_COLS;
+    constexpr int TILE_ = MANY ? ATTN_MANY_TILE : ATTN_FEW_TILE;
+    constexpr int TH = D / 4, PAR = 256 / TH;  // threads of a chunk, chunks at a time
+    __shared__ float s_o[PAR][D];
+    __shared__ float s_l[PAR], s_red[4];
+    const int head = (int)(blockIdx.x % (unsigned)p.n_heads), rest = (int)(blockIdx.x / (unsigned)p.n_heads);
+    const int seq = rest % p.b.n_seq, row = rest / p.b.n_seq;
+    const SeqRows sq = seq_rows(p.b, seq);
+    if (row >= sq.n) return;
+    const int kvh = head / p.group;
+    const int cols = sq.n * p.group, cb = (row * p.group + head % p.group) / COLS_;
+    const int len = sq.bad ? 0 : sq.len, pos0 = len - sq.n;
+    const int first = cb * COLS_ / p.group, last = (min(cols, (cb + 1) * COLS_) - 1) / p.group;
+    const int tiles = seen_tiles<TILE_>(pos0 + first, pos0 + last, p.window, p.sinks).total();
+    const int n = max(1, (tiles + p.chunk - 1) / p.chunk);
+    const int tid = (int)threadIdx.x;
+    const uint64_t slot0 = (uint64_t)(sq.a + row) * p.n_heads + head;
+    const uint64_t step = (uint64_t)p.b.n_rows * p.n_heads;
+
+    float m = -INFINITY;
+    for (int i = tid; i < n; i += 256) m = fmaxf(m, p.part_ml[(slot0 + i * step) * 2]);
+    m = max_x16_32(m);
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if ((tid & 63) == 0) s_red[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float base = m == -INFINITY ? 0.0f : m;
+
+    const int part = tid / TH, d = tid % TH * 4;
+    float l = 0.0f;
+    pf32x4 o = {};
+    for (int i = part; i < n; i += PAR) {
+        const uint64_t slot = slot0 + i * step;
+        const float f = exp2_fast(p.part_ml[slot * 2] - base);
+        const float li = p.part_ml[slot * 2 + 1];
+        const pf32x4 oi = *(const pf32x4*)(p.part_o + slot * D + d);
+        l += f == 0.0f && li == li ? 0.0f : li * f;
+        if (f != 0.0f) o += oi * f;
+    }
+    *(pf32x4*)&s_o[part][d] = o;
+    if (d == 0) s_l[part] = l;
+    __syncthreads();
+    // sums over the parts, in their order
+    if (part != 0) return;
+    float lt = 0.0f, out[4] = {};
+#pragma unroll
+    for (int i = 0; i < PAR; i++) {
+        lt += s_l[i];
+#pragma unroll
+        for (int j = 0; j < 4; j++) out[j] += s_o[i][d + j];
+    }
+    attn_store<4, QF32>(p, sq, row, head, d, D, out, lt, p.v_scale ? p.v_scale[kvh] : 1.0f);
+}
+
+}  // namespace
+
+hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s)
+{
+    const uint64_t blocks = (uint64_t)p.b.n_seq * p.n_kv * p.col_blocks * p.splits;
+    if (blocks == 0) return hipSuccess;
+    if (head_dim == 128) go_types<128>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
+    else go_types<64>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_attn_join(const PagedAttnArgs& p, int head_dim, int q_dtype, bool many, hipStream_t s)
+{
+    const uint64_t blocks = (uint64_t)p.b.n_seq * p.b.max_q * p.n_heads;
+    if (blocks == 0) return hipSuccess;
+    const dim3 grid((unsigned)blocks), block(256);
+    const bool f32 = q_dtype == WPCG_DTYPE_F32;
+#define WPCG_JOIN(D, F, M) \
+    if (head_dim == D && f32 == F && many == M) k_attn_join<D, F, M><<<grid, block, 0, s>>>(p)
+    WPCG_JOIN(64, false, false);
+    WPCG_JOIN(64, true, false);
+    WPCG_JOIN(128, false, false);
+    WPCG_JOIN(128, true, false);
+    WPCG_JOIN(64, false, true);
+    WPCG_JOIN(64, true, true);
+    WPCG_JOIN(128, false, true);
+    WPCG_JOIN(128, true, true);
+#undef WPCG_JOIN
+    return hipGetLastError();
+}
+
+}  // namespace wpcg

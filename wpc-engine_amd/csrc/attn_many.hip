@@ -1,0 +1,461 @@
+// Attention of many rows over paged keys and values: prompts, and chunks of
+// prompts behind cached tokens; causal, with a window and sinks.
+//
+// The work is two matrix products a tile and the exponentials between them:
+// the matrix cores are the bound for long prompts, and the exponentials (a
+// quarter-rate instruction each) come close behind. A workgroup takes 128
+// columns ((row, query head) pairs of one key-value head, so that keys and
+// values are shared by the heads of a group) and walks the 64-token tiles
+// they see; each of its four waves owns 32 columns and keeps their running
+// maximum, sum and output in registers. Tiles no column of a wave sees are
+// skipped, tiles that all see whole take no mask.
+//
+// Layout. 32 x 32 x 16 products with keys as A and queries as B leave the
+// scores S^T with column l % 32 in lane l and tokens 8a + 4(l/32) + b, which
+// is the second product's B operand as it stands if V^T's A operand takes its
+// tokens in the same order. So the softmax's terms stay in their lane, the
+// maximum needs one lane exchange, and the rescaling factor is one number a
+// lane. Keys go to LDS in 16-byte pieces [8 dimensions][token], the token
+// index XORed with the piece's so that neither the writes (along a row) nor
+// the reads (along tokens) meet in a bank; values are transposed in registers
+// by byte permutes on their way to LDS and lie in the order the operand is
+// read, 1 KiB a wave without conflicts. The next tile's loads are in flight
+// during the products.
+//
+// Precision is that of attn_few.hip; an F32 cache is carried as three bf16
+// terms too, and a product of two fp32 values takes the six of its nine terms
+// that reach 2^-24.
+#include "paged.h"
+
+namespace wpcg {
+namespace {
+
+constexpr int WAVES = 4;
+constexpr int THREADS = 64 * WAVES;
+constexpr int TILE = ATTN_MANY_TILE, COLS = ATTN_MANY_COLS;
+
+template <int D, int CT, bool QF32>
+struct Shape {
+    static constexpr int NQ = QF32 ? 3 : 1;         // bf16 terms of q and of the softmax's terms
+    static constexpr int NK = CT == CT_F32 ? 3 : 1;  // of keys and values
+    static constexpr int NBUF = NK == 1 ? 2 : 1;     // tiles in LDS
+    static constexpr int CW = CT == CT_F32 ? 4 : 8;  // dimensions of a value load
+    static constexpr int NCH = D / CW;
+    static constexpr int PLANE = TILE * D;           // bf16 elements of one term of a tile
+    static constexpr int KT = 16 * (D / 8) / 64;     // key pieces of a lane and tile
+    static constexpr int VT = (4 * NCH + 63) / 64;   // value pieces (4 tokens) of a lane and tile
+};
+
+// A tile on its way: what one lane carries of the 16 tokens that its wave
+// brings in.
+template <int D, int CT>
+struct Carried {
+    using S = Shape<D, CT, true>;
+    static constexpr int KW = 8 * ct_size<CT>() / 4, VW = S::CW * ct_size<CT>() / 4;  // words
+    uint32_t k[S::KT][KW];
+    uint32_t v[S::VT][4][VW];
+};
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p)
+{
+    if constexpr (W >= 4) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const pu32x4 x = *(const pu32x4*)(p + 4 * i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[i + j] = x[j];
+        }
+    } else {
+        static_assert(W == 2, "8 bytes");
+        const pu32x2 x = *(const pu32x2*)p;
+        w[0] = x[0];
+        w[1] = x[1];
+    }
+}
+
+// Place of the 16-byte piece (dimensions 8c .. 8c+7, token t) of a tile's keys.
+__device__ __forceinline__ int key_at(int c, int t) { return (c * TILE + (t ^ (c & 15))) * 8; }
+// Place of slot (h, p) of 16-token group j of its values: the eight tokens
+// 16j + 4h + 0..3 and 16j + 8 + 4h + 0..3 of dimension CW * (p % NCH) + p / NCH.
+template <int D>
+__device__ __forceinline__ int value_at(int j, int h, int p)
+{
+    return ((j * (D / 32) + p / 32) * 64 + h * 32 + p % 32) * 8;
+}
+
+// acc += a b over their bf16 terms, small products first; of two three-term
+// numbers the products below 2^-24 of the first are left out.
+template <int NA, int NB>
+__device__ __forceinline__ pf32x16 mul_terms(const pbf16x8 (&a)[NA], const pbf16x8 (&b)[NB], pf32x16 acc)
+{
+    if constexpr (NA == 3) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], acc, 0, 0, 0);
+    }
+    if constexpr (NB == 3) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], acc, 0, 0, 0);
+    if constexpr (NA == 3) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], acc, 0, 0, 0);
+    if constexpr (NB == 3) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], acc, 0, 0, 0);
+}
+
+template <int D, int CT, bool QF32>
+__global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p)
+{
+    using S = Shape<D, CT, QF32>;
+    constexpr int ES = ct_size<CT>();
+    constexpr int CW = S::CW, NCH = S::NCH;
+    __shared__ __attribute__((aligned(16))) uint16_t s_k[S::NBUF][S::NK][S::PLANE];
+    __shared__ __attribute__((aligned(16))) uint16_t s_v[S::NBUF][S::NK][S::PLANE];
+    __shared__ int s_odd[S::NBUF][WAVES], s_fault[WAVES];
+
+    // block -> (column block, chunk, sequence and head): the blocks of a head
+    // are `pairs` apart, so that with a multiple of 8 pairs they run on one
+    // die and share its L2; the last column blocks, which see most, come first
+    const int pairs = p.b.n_seq * p.n_kv;
+    const int pair = (int)(blockIdx.x % (unsigned)pairs), rest = (int)(blockIdx.x / (unsigned)pairs);
+    const int split = rest % p.splits, cb = p.col_blocks - 1 - rest / p.splits;
+    const int seq = pair / p.n_kv, kvh = pair % p.n_kv;
+    const SeqRows sq = seq_rows(p.b, seq);
+    const int cols = sq.n * p.group;
+    if (cb * COLS >= cols) return;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int c = lane & 31, h = lane >> 5;
+    const int len = sq.bad ? 0 : sq.len;
+    const int pos0 = len - sq.n;
+    const int first = cb * COLS / p.group, last = (min(cols, (cb + 1) * COLS) - 1) / p.group;
+    const SeenTiles<TILE> seen = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks);
+    const int v0 = split * p.chunk, v1 = min(v0 + p.chunk, seen.total());
+    if (v0 >= v1 && split > 0) return;
+    const int all_hi = pos0 + first + 1;
+    const int all_lo = p.window > 0 ? pos0 + last - p.window + 1 : 0;
+
+    // the wave's columns
+    const int w0 = cb * COLS + 32 * wave;
+    const bool active = w0 < cols;
+    const int col = w0 + c;
+    const bool live = col < cols;
+    const int row = live ? col / p.group : 0, head = kvh * p.group + (live ? col % p.group : 0);
+    const int pos = pos0 + row;
+    const int wfirst = active ? w0 / p.group : 0, wlast = active ? (min(cols, w0 + 32) - 1) / p.group : 0;
+    const SeenTiles<TILE> wseen = seen_tiles<TILE>(pos0 + wfirst, pos0 + wlast, p.window, p.sinks);
+    const int w_hi = pos0 + wfirst + 1;
+    const int w_lo = p.window > 0 ? pos0 + wlast - p.window + 1 : 0;
+
+    // q as B fragments: lane (column, h) holds dimensions 16 f + 8 h + 0..7
+    pbf16x8 qb[D / 16][S::NQ];
+    {
+        const uint64_t at = (uint64_t)(sq.a + row) * p.q_row + (uint64_t)head * D + 8 * h;
+#pragma unroll
+        for (int f = 0; f < D / 16; f++) {
+            if constexpr (QF32) {
+                pf32x4 a = {}, b = {};
+                if (live) {
+                    a = *(const pf32x4*)((const float*)p.q + at + 16 * f);
+                    b = *(const pf32x4*)((const float*)p.q + at + 16 * f + 4);
+                }
+                uint32_t t[4][3];
+                split3(a[0], a[1], t[0]);
+                split3(a[2], a[3], t[1]);
+                split3(b[0], b[1], t[2]);
+                split3(b[2], b[3], t[3]);
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+                    qb[f][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
+            } else {
+                qb[f][0] = __builtin_bit_cast(
+                    pbf16x8, live ? *(const pu32x4*)((const uint16_t*)p.q + at + 16 * f) : (pu32x4){});
+            }
+        }
+    }
+    const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
+
+    const uint8_t* const kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
+    const uint8_t* const vp = (const uint8_t*)p.v + (uint64_t)kvh * p.head_stride * ES;
+    const int32_t* const table = p.b.table + (uint64_t)seq * p.b.table_stride;
+    const uint64_t page_bytes = p.page_stride * ES, token_bytes = p.token_stride * ES;
+    bool fault = false;
+
+    // wave w brings in tokens 16 w .. 16 w + 15 of a tile
+    Carried<D, CT> in;
+    const auto fetch = [&](int vt) {
+        const int t0 = __builtin_amdgcn_readfirstlane(seen.tile(vt) * TILE + 16 * wave);
+        uint64_t at = 0;
+        if (seen.any(t0, t0 + 16)) {
+            const uint32_t id = (uint32_t)table[t0 >> p.b.page_shift];
+            if (id >= p.b.n_pages) fault = true;
+            else at = (uint64_t)id * page_bytes + (uint64_t)(t0 & (p.b.page_size - 1)) * token_bytes;
+        }
+#pragma unroll
+        for (int i = 0; i < S::KT; i++) {
+            const int x = lane + 64 * i;
+            load_words(in.k[i], kp + at + (uint64_t)(x / (D / 8)) * token_bytes + x % (D / 8) * 8 * ES);
+        }
+#pragma unroll
+        for (int i = 0; i < S::VT; i++) {
+            const int x = lane + 64 * i;
+            if (4 * NCH % 64 == 0 || x < 4 * NCH) {
+                const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    load_words(in.v[i][y], vp + at + (uint64_t)(8 * xh + 4 * vh + y) * token_bytes + n * CW * ES);
+            }
+        }
+    };
+    const auto put = [&](int vt, int buf) {
+        const int t0 = seen.tile(vt) * TILE;
+        const bool whole = t0 + TILE <= all_hi && t0 >= all_lo;
+#pragma unroll
+        for (int i = 0; i < S::KT; i++) {
+            const int x = lane + 64 * i;
+            const int at = key_at(x % (D / 8), 16 * wave + x / (D / 8));
+            if constexpr (CT == CT_F32) {
+                uint32_t t[4][3];
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    split3(__uint_as_float(in.k[i][2 * y]), __uint_as_float(in.k[i][2 * y + 1]), t[y]);
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+                    *(pu32x4*)&s_k[buf][n][at] = (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]};
+            } else if constexpr (CT == CT_BF16) {
+                *(pu32x4*)&s_k[buf][0][at] = (pu32x4){in.k[i][0], in.k[i][1], in.k[i][2], in.k[i][3]};
+            } else {
+                *(pu32x4*)&s_k[buf][0][at] = (pu32x4){e4m3_bf16<false>(in.k[i][0]), e4m3_bf16<true>(in.k[i][0]),
+                                                      e4m3_bf16<false>(in.k[i][1]), e4m3_bf16<true>(in.k[i][1])};
+            }
+        }
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < S::VT; i++) {
+            const int x = lane + 64 * i;
+            if (4 * NCH % 64 == 0 || x < 4 * NCH) {
+                const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
+                bool some[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) some[k] = whole || seen.some(t0 + 16 * wave + 8 * xh + 4 * vh + k);
+#pragma unroll
+                for (int y = 0; y < CW / 2; y++) {
+                    // bf16 pairs of dimensions 2 y, 2 y + 1 of the four tokens
+                    uint32_t t[4][S::NK];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if constexpr (CT == CT_F32)
+                            split3(__uint_as_float(in.v[i][k][2 * y]), __uint_as_float(in.v[i][k][2 * y + 1]), t[k]);
+                        else if constexpr (CT == CT_BF16)
+                            t[k][0] = in.v[i][k][y];
+                        else
+                            t[k][0] = y % 2 ? e4m3_bf16<true>(in.v[i][k][y / 2]) : e4m3_bf16<false>(in.v[i][k][y / 2]);
+                    }
+                    if (!whole) {  // tokens that no column sees hold anything
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+#pragma unroll
+                            for (int e = 0; e < S::NK; e++) {
+                                t[k][e] = some[k] ? t[k][e] : 0u;
+                                odd |= bf16_odd(t[k][e]);
+                            }
+                    }
+#pragma unroll
+                    for (int e = 0; e < S::NK; e++) {
+                        const pu32x2 lo = {__builtin_amdgcn_perm(t[1][e], t[0][e], 0x05040100u),
+                                           __builtin_amdgcn_perm(t[3][e], t[2][e], 0x05040100u)};
+                        const pu32x2 hi = {__builtin_amdgcn_perm(t[1][e], t[0][e], 0x07060302u),
+                                           __builtin_amdgcn_perm(t[3][e], t[2][e], 0x07060302u)};
+                        *(pu32x2*)&s_v[buf][e][value_at<D>(wave, vh, 2 * y * NCH + n) + 4 * xh] = lo;
+                        *(pu32x2*)&s_v[buf][e][value_at<D>(wave, vh, (2 * y + 1) * NCH + n) + 4 * xh] = hi;
+                    }
+                }
+            }
+        }
+        odd = __any(odd);
+        if (lane == 0) s_odd[buf][wave] = odd;
+    };
+
+    pf32x16 acc[D / 32] = {};
+    float m = -INFINITY, l = 0.0f;
+    if (v0 < v1) fetch(v0);
+    for (int vt = v0; vt < v1; vt++) {
+        const int buf = (vt - v0) % S::NBUF;
+        if (S::NBUF == 1 && vt > v0) __syncthreads();  // the tile before is read
+        put(vt, buf);
+        __syncthreads();
+        if (vt + 1 < v1) fetch(vt + 1);
+        const int t0 = seen.tile(vt) * TILE;
+        if (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3]) {
+            // values that are not finite: added to the columns that see their
+            // token (products with ones count the +inf, -inf and NaN a column
+            // sees), and zeros for the products below
+            if (active) {
+#pragma unroll
+                for (int d = 0; d < D / 32; d++) {
+#pragma unroll 1
+                    for (int j = 0; j < 4; j++) {
+                        pu32x4 see;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int t = t0 + 16 * j + 8 * (i / 2) + 4 * h + 2 * i % 4;
+                            see[i] = (row_sees(pos, t, p.window, p.sinks) ? 0x3f80u : 0u) |
+                                     (row_sees(pos, t + 1, p.window, p.sinks) ? 0x3f800000u : 0u);
+                        }
+#pragma unroll 1
+                        for (int kind = 0; kind < 3; kind++) {
+                            pf32x16 n = {};
+#pragma unroll
+                            for (int e = 0; e < S::NK; e++) {
+                                const pu32x4 w = *(const pu32x4*)&s_v[buf][e][value_at<D>(j, 0, 32 * d) + lane * 8];
+                                const pu32x4 is = {bf16_is(w[0], kind), bf16_is(w[1], kind), bf16_is(w[2], kind),
+                                                   bf16_is(w[3], kind)};
+                                n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pbf16x8, is),
+                                                                            __builtin_bit_cast(pbf16x8, see), n, 0, 0, 0);
+                            }
+                            const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (n[i] > 0.0f) acc[d][i] += add;
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            for (int i = (int)threadIdx.x; i < S::NK * S::PLANE / 2; i += THREADS) {
+                uint32_t* w = (uint32_t*)&s_v[buf][0][0] + i;
+                *w = bf16_finite(*w);
+            }
+            __syncthreads();
+        }
+        if (!active || !wseen.any(t0, t0 + TILE)) continue;
+
+        // scores of two 32-token halves
+        pf32x16 s[2] = {};
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int f = 0; f < D / 16; f++) {
+                pbf16x8 k[S::NK];
+#pragma unroll
+                for (int e = 0; e < S::NK; e++) k[e] = *(const pbf16x8*)&s_k[buf][e][key_at(2 * f + h, 32 * u + c)];
+                s[u] = mul_terms(k, qb[f], s[u]);
+            }
+        }
+        const bool whole = t0 + TILE <= w_hi && t0 >= w_lo;
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int t = t0 + 32 * u + 8 * (i / 4) + 4 * h + i % 4;
+                    if (!row_sees(pos, t, p.window, p.sinks)) s[u][i] = -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
+        top = max_x32(top) * sc;
+        const float now = fmaxf(m, top);
+        const float base = now == -INFINITY ? 0.0f : now;
+        if (__any(now > m)) {
+            // (what a first tile's infinities left in acc is kept)
+            const float f = m == -INFINITY ? 1.0f : exp2_fast(m - base);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < D / 32; d++) acc[d] *= f;
+            m = now;
+        }
+        pbf16x8 b[4][S::NQ];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                e[i] = exp2_fast(fmaf(s[j / 2][8 * (j % 2) + i], sc, -base));
+                sum += e[i];
+            }
+            if constexpr (QF32) {
+                uint32_t t[4][3];
+#pragma unroll
+                for (int i = 0; i < 4; i++) split3(e[2 * i], e[2 * i + 1], t[i]);
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+                    b[j][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
+            } else {
+                b[j][0] = __builtin_bit_cast(pbf16x8, (pu32x4){pk_bf16_rne(e[0], e[1]), pk_bf16_rne(e[2], e[3]),
+                                                               pk_bf16_rne(e[4], e[5]), pk_bf16_rne(e[6], e[7])});
+            }
+        }
+        l += sum;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+#pragma unroll
+            for (int d = 0; d < D / 32; d++) {
+                pbf16x8 v[S::NK];
+#pragma unroll
+                for (int e = 0; e < S::NK; e++)
+                    v[e] = *(const pbf16x8*)&s_v[buf][e][value_at<D>(j, 0, 32 * d) + lane * 8];
+                acc[d] = mul_terms(v, b[j], acc[d]);
+            }
+        }
+    }
+    if (lane == 0) s_fault[wave] = 0;
+    if (__any(fault) && lane == 0) s_fault[wave] = 1;
+    __syncthreads();
+    if (!live) return;
+    l = sum_x32(l);
+    if (s_fault[0] | s_fault[1] | s_fault[2] | s_fault[3]) l = __builtin_nanf("");
+
+    const float v_scale = p.v_scale ? p.v_scale[kvh] : 1.0f;
+    const uint64_t slot = ((uint64_t)split * p.b.n_rows + sq.a + row) * p.n_heads + head;
+#pragma unroll
+    for (int a0 = 0; a0 < NCH / 8; a0++)
+#pragma unroll
+        for (int b0 = 0; b0 < 4; b0++) {
+            float o[CW];
+#pragma unroll
+            for (int j = 0; j < CW; j++) o[j] = acc[j * NCH / 32][4 * (j * NCH % 32 / 8 + a0) + b0];
+            const int d = CW * (8 * a0 + 4 * h + b0);
+            if (p.splits > 1) {
+#pragma unroll
+                for (int j = 0; j < CW; j += 4)
+                    *(pf32x4*)(p.part_o + slot * D + d + j) = (pf32x4){o[j], o[j + 1], o[j + 2], o[j + 3]};
+            } else {
+                attn_store<CW, QF32>(p, sq, row, head, d, D, o, l, v_scale);
+            }
+        }
+    if (p.splits > 1 && h == 0) {
+        p.part_ml[slot * 2] = m;
+        p.part_ml[slot * 2 + 1] = l;
+    }
+}
+
+template <int D, int CT, bool QF32>
+void go(const PagedAttnArgs& p, unsigned blocks, hipStream_t s)
+{
+    k_attn_many<D, CT, QF32><<<dim3(blocks), dim3(THREADS), 0, s>>>(p);
+}
+
+template <int D>
+void go_types(const PagedAttnArgs& p, int q_dtype, int cache_dtype, unsigned blocks, hipStream_t s)
+{
+    if (q_dtype == WPCG_DTYPE_BF16) {
+        if (cache_dtype == WPCG_DTYPE_BF16) go<D, CT_BF16, false>(p, blocks, s);
+        else go<D, CT_E4M3, false>(p, blocks, s);
+    } else {
+        if (cache_dtype == WPCG_DTYPE_F32) go<D, CT_F32, true>(p, blocks, s);
+        else if (cache_dtype == WPCG_DTYPE_BF16) go<D, CT_BF16, true>(p, blocks, s);
+        else go<D, CT_E4M3, true>(p, blocks, s);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s)
+{
+    const uint64_t blocks = (uint64_t)p.b.n_seq * p.n_kv * p.col_blocks * p.splits;
+    if (blocks == 0) return hipSuccess;
+    if (head_dim == 128) go_types<128>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
+    else go_types<64>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
+    return hipGetLastError();
+}
+
+}  // namespace wpcg

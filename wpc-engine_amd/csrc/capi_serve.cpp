@@ -1,0 +1,360 @@
+// The C boundary of the operators of batched serving (include/wpcg.h): paged
+// keys and values, attention over them, verification of drafts. Everything a
+// kernel indexes with is bounded here or, where it comes from device arrays,
+// in the kernels.
+#include <algorithm>
+#include <cmath>
+
+#include "wpcg_internal.hpp"
+
+namespace wpcg {
+namespace {
+
+constexpr uint64_t INT_BOUND = 1u << 30;  // of rows, tokens, heads: sums of two stay ints
+
+uint64_t type_size(int dtype) { return dtype == WPCG_DTYPE_F32 ? 4 : dtype == WPCG_DTYPE_BF16 ? 2 : 1; }
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_rows_dtype(int dtype)
+{
+    if (dtype != WPCG_DTYPE_F32 && dtype != WPCG_DTYPE_BF16) return fail(WPCG_E_ARG, "rows are F32 or BF16");
+    return WPCG_OK;
+}
+
+// A row stride in elements (0 = packed): at least the row, 16-byte steps.
+int row_stride(uint64_t stride, uint64_t width, int dtype, uint64_t* out)
+{
+    if (stride == 0) stride = width;
+    if (stride < width) return fail(WPCG_E_SHAPE, "row stride shorter than the row");
+    if (stride * type_size(dtype) % 16 != 0) return fail(WPCG_E_SHAPE, "row stride not a multiple of 16 bytes");
+    if (stride >> 40) return fail(WPCG_E_ARG, "row stride too large");
+    *out = stride;
+    return WPCG_OK;
+}
+
+struct Pages {
+    uint64_t page, head, token;  // strides
+};
+
+int check_pages(const wpcg_kv_pages* kv, Pages* s)
+{
+    if (!kv) return fail(WPCG_E_ARG, "null pages");
+    if (kv->dtype != WPCG_DTYPE_F32 && kv->dtype != WPCG_DTYPE_BF16 && kv->dtype != WPCG_DTYPE_E4M3)
+        return fail(WPCG_E_ARG, "pages are F32, BF16 or E4M3");
+    if (kv->head_dim != 64 && kv->head_dim != 128) return fail(WPCG_E_UNSUPPORTED, "head_dim is 64 or 128");
+    if (kv->page_size < 16 || kv->page_size > 256 || (kv->page_size & (kv->page_size - 1)))
+        return fail(WPCG_E_SHAPE, "page_size is a power of two in 16..256");
+    if (kv->n_pages == 0 || kv->n_pages > INT_BOUND) return fail(WPCG_E_ARG, "n_pages out of range");
+    if (kv->n_kv_heads == 0 || kv->n_kv_heads > 65536) return fail(WPCG_E_ARG, "n_kv_heads out of range");
+    if ((kv->k_scale_dev || kv->v_scale_dev) && kv->dtype != WPCG_DTYPE_E4M3)
+        return fail(WPCG_E_ARG, "scales are of an E4M3 cache");
+    *s = {kv->page_stride, kv->head_stride, kv->token_stride};
+    const uint64_t d = kv->head_dim;
+    if (!s->page && !s->head && !s->token) {
+        s->token = d;
+        s->head = d * kv->page_size;
+        s->page = s->head * kv->n_kv_heads;
+    }
+    const uint64_t es = type_size(kv->dtype);
+    for (uint64_t x : {s->page, s->head, s->token}) {
+        if (x < d) return fail(WPCG_E_SHAPE, "a page stride is shorter than a head");
+        if (x * es % 16 != 0) return fail(WPCG_E_SHAPE, "a page stride is not a multiple of 16 bytes");
+        if (x >> 40) return fail(WPCG_E_ARG, "a page stride is too large");
+    }
+    return WPCG_OK;
+}
+
+int check_batch(const wpcg_kv_batch* b, const wpcg_kv_pages* kv, PagedBatch* out)
+{
+    if (!b) return fail(WPCG_E_ARG, "null batch");
+    if (b->n_seq > INT_BOUND || b->n_rows > INT_BOUND || b->max_q > INT_BOUND || b->max_kv > INT_BOUND)
+        return fail(WPCG_E_ARG, "batch bounds out of range");
+    if (b->n_seq > 0) {
+        if (b->max_q == 0) return fail(WPCG_E_ARG, "max_q is 0");
+        if (!b->q_start_dev && (b->max_q != 1 || b->n_rows < b->n_seq))
+            return fail(WPCG_E_ARG, "without q_start every sequence has one row");
+        if ((uint64_t)b->table_stride * kv->page_size < b->max_kv)
+            return fail(WPCG_E_SHAPE, "the table's rows do not hold max_kv tokens");
+    }
+    int shift = 0;
+    while ((1u << shift) < kv->page_size) shift++;
+    *out = {(int)b->n_seq, (int)b->n_rows, (int)std::min(b->max_q, b->n_rows), (int)b->max_kv, kv->n_pages,
+            (int)kv->page_size, shift, b->table_stride, b->q_start_dev, b->kv_len_dev, b->table_dev};
+    return WPCG_OK;
+}
+
+// After the checks that need no pointers: what a call must have.
+int check_pointers(const wpcg_kv_pages* kv, const wpcg_kv_batch* b)
+{
+    if (!kv->k_dev || !kv->v_dev || !b->kv_len_dev || (!b->table_dev && b->max_kv > 0))
+        return fail(WPCG_E_ARG, "null argument");
+    if (!aligned(kv->k_dev) || !aligned(kv->v_dev)) return fail(WPCG_E_ARG, "pages not aligned to 16 bytes");
+    return WPCG_OK;
+}
+
+struct Plan {
+    bool many;
+    int col_blocks, chunk, splits;
+    uint64_t bytes;
+};
+
+// Which kernel, and how many workgroups share a sequence's tokens.
+//
+// Few rows: up to FEW_BLOCKS column blocks of 16, each reading the keys and
+// values again.
+//
+// A batch is split over the tokens until it has about TARGET workgroups, in
+// chunks of at least the given tiles: a shorter chunk pays more for its state
+// than it gains. The bounds stand in for the lengths, which only the device
+// knows; a shorter sequence just has fewer chunks.
+int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attention* a, Plan* out)
+{
+    const int64_t group = a->n_heads / kv->n_kv_heads, cols = (int64_t)b.max_q * group;
+    constexpr int64_t FEW_COLS = 2 * ATTN_FEW_COLS;
+    Plan p;
+    p.many = cols > FEW_COLS;
+    const int64_t cw = p.many ? ATTN_MANY_COLS : ATTN_FEW_COLS, tw = p.many ? ATTN_MANY_TILE : ATTN_FEW_TILE;
+    const int64_t blocks = (cols + cw - 1) / cw;
+    // tiles that a column block can see
+    int64_t tiles = (b.max_kv + tw - 1) / tw;
+    if (a->window > 0) {
+        const int64_t rows = std::min<int64_t>(b.max_q, cw / group + 2);
+        const int64_t seen = (std::min<int64_t>(a->sinks, b.max_kv) + tw - 1) / tw +
+                             ((int64_t)std::min<uint64_t>(a->window, INT_BOUND) + rows + tw - 1) / tw + 1;
+        tiles = std::min(tiles, seen);
+    }
+    const int64_t base = (int64_t)b.n_seq * kv->n_kv_heads * blocks;
+    const int64_t target = p.many ? 512 : 1024, least = p.many ? 8 : 4;
+    int64_t chunk = tiles;
+    if (base > 0 && base < target) {
+        const int64_t want = (target + base - 1) / base;
+        chunk = std::max(least, (tiles + want - 1) / want);
+    }
+    p.chunk = (int)std::max<int64_t>(1, chunk);
+    p.splits = (int)std::max<int64_t>(1, (tiles + p.chunk - 1) / p.chunk);
+    p.col_blocks = (int)std::max<int64_t>(1, blocks);
+    if (base * p.splits >= (int64_t)1 << 31 || (uint64_t)b.n_seq * b.max_q * a->n_heads >= 1u << 31)
+        return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
+    p.bytes = p.splits > 1 ? (uint64_t)p.splits * b.n_rows * a->n_heads * (kv->head_dim + 2) * sizeof(float) : 0;
+    *out = p;
+    return WPCG_OK;
+}
+
+int check_attention(const wpcg_kv_pages* kv, const wpcg_attention* a)
+{
+    if (!a) return fail(WPCG_E_ARG, "null argument");
+    if (int rc = check_rows_dtype(a->dtype)) return rc;
+    if (a->dtype == WPCG_DTYPE_BF16 && kv->dtype == WPCG_DTYPE_F32)
+        return fail(WPCG_E_UNSUPPORTED, "BF16 queries take a BF16 or E4M3 cache");
+    if (a->n_heads == 0 || a->n_heads > 65536 || a->n_heads % kv->n_kv_heads)
+        return fail(WPCG_E_SHAPE, "n_heads is a multiple of n_kv_heads");
+    if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return fail(WPCG_E_ARG, "scale is positive");
+    return WPCG_OK;
+}
+
+// ids of a chunk of a row's logits: short ones while the rows are few, so
+// that a single sequence's five rows still have a few hundred workgroups
+int draft_chunk(const wpcg_draft* d)
+{
+    return (uint64_t)d->n_rows * ((d->vocab + 8191) / 8192) >= 1024 ? 8192 : 2048;
+}
+
+int check_draft(const wpcg_draft* d, int* chunk, int* chunks, uint64_t* bytes)
+{
+    if (!d) return fail(WPCG_E_ARG, "null argument");
+    if (d->vocab == 0 || d->vocab > INT_BOUND) return fail(WPCG_E_ARG, "vocab out of range");
+    if (d->n_seq > INT_BOUND || d->n_rows > INT_BOUND) return fail(WPCG_E_ARG, "batch bounds out of range");
+    if (d->n_seq > 0) {
+        if (d->max_rows == 0 || d->max_rows > WPCG_DRAFT_MAX)
+            return fail(WPCG_E_ARG, "max_rows is in 1.." + std::to_string(WPCG_DRAFT_MAX));
+        if (!d->q_start_dev && (uint64_t)d->n_seq * d->max_rows > d->n_rows)
+            return fail(WPCG_E_ARG, "without q_start every sequence has max_rows rows");
+    }
+    if ((d->logits_stride && d->logits_stride < d->vocab) || (d->draft_stride && d->draft_stride < d->vocab))
+        return fail(WPCG_E_SHAPE, "row stride shorter than the row");
+    if (d->logits_stride >> 40 || d->draft_stride >> 40) return fail(WPCG_E_ARG, "row stride too large");
+    *chunk = draft_chunk(d);
+    *chunks = (int)((d->vocab + *chunk - 1) / *chunk);
+    if ((uint64_t)std::max(d->n_rows, d->n_seq) * *chunks >= 1u << 31)
+        return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
+    *bytes = (uint64_t)d->n_rows * *chunks * sizeof(DraftPart) + (uint64_t)d->n_seq * *chunks * sizeof(double) +
+             (uint64_t)d->n_seq * sizeof(DraftChoice);
+    return WPCG_OK;
+}
+
+}  // namespace
+}  // namespace wpcg
+
+using namespace wpcg;
+
+extern "C" {
+
+int wpcg_kv_append(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch, const wpcg_kv_rows* r,
+                   wpcg_stream stream)
+{
+    Pages st;
+    if (int rc = check_pages(kv, &st)) return rc;
+    KvAppendArgs a{};
+    if (int rc = check_batch(batch, kv, &a.b)) return rc;
+    if (!r) return fail(WPCG_E_ARG, "null argument");
+    if (int rc = check_rows_dtype(r->dtype)) return rc;
+    const bool with_q = r->q_dev || r->q_out_dev;
+    const uint64_t d = kv->head_dim;
+    if (with_q) {
+        if (int rc = check_rows_dtype(r->q_out_dtype)) return rc;
+        if (r->n_heads == 0 || r->n_heads > 65536 || r->n_heads % kv->n_kv_heads)
+            return fail(WPCG_E_SHAPE, "n_heads is a multiple of n_kv_heads");
+        if (int rc = row_stride(r->q_stride, r->n_heads * d, r->dtype, &a.q_row)) return rc;
+        if (int rc = row_stride(r->q_out_stride, r->n_heads * d, r->q_out_dtype, &a.q_out_row)) return rc;
+        if (r->q_dev == r->q_out_dev && (r->dtype != r->q_out_dtype || a.q_row != a.q_out_row))
+            return fail(WPCG_E_ARG, "q_out may be q itself only in q's type and stride");
+    }
+    if (int rc = row_stride(r->k_stride, kv->n_kv_heads * d, r->dtype, &a.k_row)) return rc;
+    if (int rc = row_stride(r->v_stride, kv->n_kv_heads * d, r->dtype, &a.v_row)) return rc;
+    if ((r->q_norm_dev || r->k_norm_dev) && !(r->eps >= 0.0f)) return fail(WPCG_E_ARG, "eps is not negative");
+    a.n_q = with_q ? (int)r->n_heads : 0;
+    a.n_kv = (int)kv->n_kv_heads;
+    a.n_units = a.n_q + 2 * a.n_kv;
+    const uint64_t per = 2048 / d;  // heads of a workgroup
+    if ((uint64_t)batch->n_rows * ((a.n_units + per - 1) / per) >= 1u << 31)
+        return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
+    if (batch->n_seq == 0 || batch->n_rows == 0) return check_ctx(ctx);
+    if (int rc = check_pointers(kv, batch)) return rc;
+    if ((with_q && (!r->q_dev || !r->q_out_dev)) || !r->k_dev || !r->v_dev) return fail(WPCG_E_ARG, "null argument");
+    for (const void* x : {r->q_dev, (const void*)r->q_out_dev, r->k_dev, r->v_dev, (const void*)r->q_norm_dev,
+                          (const void*)r->k_norm_dev})
+        if (!aligned(x)) return fail(WPCG_E_ARG, "rows or weights not aligned to 16 bytes");
+    if (int rc = check_ctx(ctx)) return rc;
+    a.q = r->q_dev;
+    a.k = r->k_dev;
+    a.v = r->v_dev;
+    a.q_out = r->q_out_dev;
+    a.q_out_dtype = r->q_out_dtype;
+    a.k_pages = kv->k_dev;
+    a.v_pages = kv->v_dev;
+    a.cache_dtype = kv->dtype;
+    a.page_stride = st.page;
+    a.head_stride = st.head;
+    a.token_stride = st.token;
+    a.k_scale = kv->k_scale_dev;
+    a.v_scale = kv->v_scale_dev;
+    a.q_norm = r->q_norm_dev;
+    a.k_norm = r->k_norm_dev;
+    a.freq = r->freq_dev;
+    a.eps = r->eps;
+    WPCG_HIP(launch_kv_append(a, (int)d, r->dtype == WPCG_DTYPE_BF16, pick(ctx, stream)));
+    return WPCG_OK;
+}
+
+int wpcg_paged_attention_workspace(const wpcg_kv_pages* kv, const wpcg_kv_batch* batch, const wpcg_attention* att,
+                                   uint64_t* bytes)
+{
+    if (!bytes) return fail(WPCG_E_ARG, "null output");
+    *bytes = 0;
+    Pages st;
+    if (int rc = check_pages(kv, &st)) return rc;
+    PagedBatch b;
+    if (int rc = check_batch(batch, kv, &b)) return rc;
+    if (int rc = check_attention(kv, att)) return rc;
+    Plan plan;
+    if (int rc = plan_attention(kv, b, att, &plan)) return rc;
+    *bytes = plan.bytes;
+    return WPCG_OK;
+}
+
+int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch, const wpcg_attention* att,
+                         void* ws_dev, uint64_t ws_bytes, wpcg_stream stream)
+{
+    Pages st;
+    if (int rc = check_pages(kv, &st)) return rc;
+    PagedAttnArgs a{};
+    if (int rc = check_batch(batch, kv, &a.b)) return rc;
+    if (int rc = check_attention(kv, att)) return rc;
+    const uint64_t width = (uint64_t)att->n_heads * kv->head_dim;
+    if (int rc = row_stride(att->q_stride, width, att->dtype, &a.q_row)) return rc;
+    if (int rc = row_stride(att->out_stride, width, att->dtype, &a.out_row)) return rc;
+    Plan plan;
+    if (int rc = plan_attention(kv, a.b, att, &plan)) return rc;
+    if (batch->n_seq == 0 || batch->n_rows == 0) return check_ctx(ctx);
+    if (int rc = check_pointers(kv, batch)) return rc;
+    if (!att->q_dev || !att->out_dev) return fail(WPCG_E_ARG, "null argument");
+    if (!aligned(att->q_dev) || !aligned(att->out_dev)) return fail(WPCG_E_ARG, "rows not aligned to 16 bytes");
+    if (plan.bytes) {
+        if (!ws_dev || ws_bytes < plan.bytes)
+            return fail(WPCG_E_ARG, "the call needs " + std::to_string(plan.bytes) + " bytes of workspace");
+        if (!aligned(ws_dev)) return fail(WPCG_E_ARG, "workspace not aligned to 16 bytes");
+    }
+    if (int rc = check_ctx(ctx)) return rc;
+    a.q = att->q_dev;
+    a.out = att->out_dev;
+    a.k = kv->k_dev;
+    a.v = kv->v_dev;
+    a.page_stride = st.page;
+    a.head_stride = st.head;
+    a.token_stride = st.token;
+    a.k_scale = kv->k_scale_dev;
+    a.v_scale = kv->v_scale_dev;
+    a.n_heads = (int)att->n_heads;
+    a.n_kv = (int)kv->n_kv_heads;
+    a.group = a.n_heads / a.n_kv;
+    a.scale = (float)((double)att->scale * 1.4426950408889634);
+    a.window = (int)std::min<uint64_t>(att->window, INT_BOUND);
+    a.sinks = (int)std::min<uint64_t>(att->sinks, INT_BOUND);
+    a.col_blocks = plan.col_blocks;
+    a.chunk = plan.chunk;
+    a.splits = plan.splits;
+    a.part_o = (float*)ws_dev;
+    a.part_ml = a.part_o + (uint64_t)plan.splits * a.b.n_rows * a.n_heads * kv->head_dim;
+    const hipStream_t s = pick(ctx, stream);
+    const int d = (int)kv->head_dim;
+    WPCG_HIP(plan.many ? launch_attn_many(a, d, att->dtype, kv->dtype, s) : launch_attn_few(a, d, att->dtype, kv->dtype, s));
+    if (plan.splits > 1) WPCG_HIP(launch_attn_join(a, d, att->dtype, plan.many, s));
+    return WPCG_OK;
+}
+
+int wpcg_draft_verify_workspace(const wpcg_draft* d, uint64_t* bytes)
+{
+    if (!bytes) return fail(WPCG_E_ARG, "null output");
+    *bytes = 0;
+    int chunk, chunks;
+    return check_draft(d, &chunk, &chunks, bytes);
+}
+
+int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream)
+{
+    DraftArgs a{};
+    uint64_t bytes = 0;
+    if (int rc = check_draft(d, &a.chunk, &a.chunks, &bytes)) return rc;
+    if (d->n_seq == 0) return check_ctx(ctx);
+    if (!d->accepted_dev) return fail(WPCG_E_ARG, "null argument");
+    if (d->n_rows > 0) {
+        if (!d->logits_dev || !d->tokens_dev || !d->u_dev || !d->u_next_dev || !d->out_dev)
+            return fail(WPCG_E_ARG, "null argument");
+        if (!ws_dev || ws_bytes < bytes)
+            return fail(WPCG_E_ARG, "the call needs " + std::to_string(bytes) + " bytes of workspace");
+        if (!aligned(ws_dev)) return fail(WPCG_E_ARG, "workspace not aligned to 16 bytes");
+    }
+    if (int rc = check_ctx(ctx)) return rc;
+    a.n_seq = (int)d->n_seq;
+    a.n_rows = (int)d->n_rows;
+    a.max_rows = (int)d->max_rows;
+    a.vocab = (int)d->vocab;
+    a.q_start = d->q_start_dev;
+    a.logits = d->logits_dev;
+    a.logits_row = d->logits_stride ? d->logits_stride : d->vocab;
+    a.probs = d->draft_probs_dev;
+    a.probs_row = d->draft_stride ? d->draft_stride : d->vocab;
+    a.tokens = d->tokens_dev;
+    a.u = d->u_dev;
+    a.u_next = d->u_next_dev;
+    a.temperature = d->temperature_dev;
+    a.accepted = d->accepted_dev;
+    a.out = d->out_dev;
+    a.part = (DraftPart*)ws_dev;
+    a.choice = (DraftChoice*)(a.part + (uint64_t)d->n_rows * a.chunks);
+    a.rest = (double*)(a.choice + d->n_seq);
+    WPCG_HIP(launch_draft_verify(a, pick(ctx, stream)));
+    return WPCG_OK;
+}
+
+}  // extern "C"

@@ -468,6 +468,87 @@ hipError_t launch_argmax_next(const float* logits, int n, DecodeState* st, uint3
 // out[r] = the first index of the largest logit of row r (logits [rows][n]).
 hipError_t launch_argmax_rows(const float* logits, int n, int rows, uint32_t* out, hipStream_t s);
 
+// ---- paged keys and values (kv_append.hip, attn_few.hip, attn_many.hip) -----
+// wpcg_kv_batch and the page geometry as the kernels take them; every bound
+// fits an int (capi_serve.cpp checks).
+struct PagedBatch {
+    int n_seq, n_rows, max_q, max_kv;
+    uint32_t n_pages;
+    int page_size, page_shift;
+    uint64_t table_stride;
+    const int32_t *q_start, *kv_len, *table;
+};
+struct KvAppendArgs {
+    PagedBatch b;
+    const void *q, *k, *v;  // q null: n_q = 0
+    uint64_t q_row, k_row, v_row, q_out_row;
+    void *q_out, *k_pages, *v_pages;
+    int q_out_dtype, cache_dtype;
+    int n_q, n_kv, n_units;  // query and key heads; n_q + 2 n_kv
+    uint64_t page_stride, head_stride, token_stride;
+    const float *k_scale, *v_scale, *q_norm, *k_norm;
+    const double* freq;
+    float eps;
+};
+hipError_t launch_kv_append(const KvAppendArgs& p, int head_dim, bool bf16, hipStream_t s);
+// Attention over pages. A column is a (row, query head) pair: column c of a
+// sequence's key-value head is row c / group, query head c % group of its
+// group. The kernel for few rows takes ATTN_FEW_COLS columns a workgroup,
+// that for many ATTN_MANY_COLS; each reads a chunk of `chunk` tiles
+// (ATTN_FEW_TILE, ATTN_MANY_TILE tokens) of those its columns see, the chunks
+// are `splits` at most. With splits > 1 chunk i leaves a column's
+// unnormalised output (fp32) at part_o[(i * n_rows + row) * n_heads + head]
+// (head_dim values) and its maximum (of the scores times log2 e) and sum of
+// terms at part_ml [same][2], and launch_attn_join puts them together.
+constexpr int ATTN_FEW_COLS = 16, ATTN_FEW_TILE = 32;
+constexpr int ATTN_MANY_COLS = 128, ATTN_MANY_TILE = 64;
+struct PagedAttnArgs {
+    PagedBatch b;
+    const void *q, *k, *v;
+    void* out;
+    uint64_t q_row, out_row;
+    uint64_t page_stride, head_stride, token_stride;
+    const float *k_scale, *v_scale;
+    int n_heads, n_kv, group;
+    float scale;  // times log2 e
+    int window, sinks;
+    int col_blocks;  // of a sequence's key-value head
+    int chunk, splits;
+    float *part_o, *part_ml;
+};
+hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
+hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
+hipError_t launch_attn_join(const PagedAttnArgs& p, int head_dim, int q_dtype, bool many, hipStream_t s);
+
+// ---- verification of drafts (draft.hip) -------------------------------------
+// A chunk's state of a row: sum of exp((x - max) / T), the largest logit and
+// its first place; and what was decided for a sequence: Z and M of the row the
+// next token comes from, its first largest logit, the accepted drafts.
+struct DraftPart {
+    double sum;
+    float max;
+    int at;
+};
+struct DraftChoice {
+    double z;
+    float m;
+    int at, accepted, pad;
+};
+struct DraftArgs {
+    int n_seq, n_rows, max_rows, vocab;
+    int chunk, chunks;  // ids of a chunk, chunks of a row
+    const int32_t* q_start;
+    const float *logits, *probs;  // probs may be null
+    uint64_t logits_row, probs_row;
+    const uint32_t* tokens;
+    const float *u, *u_next, *temperature;
+    int32_t *accepted, *out;
+    DraftPart* part;      // [n_rows][chunks]
+    double* rest;         // [n_seq][chunks]
+    DraftChoice* choice;  // [n_seq]
+};
+hipError_t launch_draft_verify(const DraftArgs& p, hipStream_t s);
+
 // ---- JSON DOM (json.cpp): safetensors headers, their index, config.json ----
 struct JsonValue {
     enum Kind { NUL, BOOL, NUM, STR, ARR, OBJ } kind = NUL;

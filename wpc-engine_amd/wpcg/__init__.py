@@ -32,7 +32,7 @@ SCHEME_V3, SCHEME_V4 = 3, 4
 MODE_EXACT, MODE_FAST = 0, 1
 FAST_KERNEL_MFMA, FAST_KERNEL_VALU = 0, 1
 ROUND_FMA, ROUND_TWO = 0, 1
-DTYPE_F32, DTYPE_BF16, DTYPE_F32_SPLIT = 0, 1, 2
+DTYPE_F32, DTYPE_BF16, DTYPE_F32_SPLIT, DTYPE_E4M3 = 0, 1, 2, 3
 
 _ERR_NAMES = {0: "OK", 1: "E_IO", 2: "E_FORMAT", 3: "E_SHAPE", 4: "E_NOTFOUND", 5: "E_DEVICE",
               6: "E_ARG", 7: "E_NOMEM", 8: "E_UNSUPPORTED"}
@@ -143,6 +143,11 @@ _SIGS = {
     "wpcg_moe_load_experts": (C.c_int, [_p, _p, C.c_uint32]),
     "wpcg_moe_set_mode": (C.c_int, [_p, C.c_int]),
     "wpcg_moe_forward": (C.c_int, [_p, _p, _p, _p, _p, _p]),
+    "wpcg_kv_append": (C.c_int, [_p, _p, _p, _p, _p]),
+    "wpcg_paged_attention_workspace": (C.c_int, [_p, _p, _p, _u64p]),
+    "wpcg_paged_attention": (C.c_int, [_p, _p, _p, _p, _p, _u64, _p]),
+    "wpcg_draft_verify_workspace": (C.c_int, [_p, _u64p]),
+    "wpcg_draft_verify": (C.c_int, [_p, _p, _p, _u64, _p]),
     "wpcg_graph_begin": (C.c_int, [_p]),
     "wpcg_graph_end": (C.c_int, [_p, _pp]),
     "wpcg_graph_launch": (C.c_int, [_p, _p]),
@@ -744,6 +749,148 @@ class MoeLayer:
             self.close()
         except Exception:
             pass
+
+
+# ------------------------------------------------------------------ batched serving
+def _ptr(b):
+    """The device pointer of a buffer (anything with .ptr), or None."""
+    return b.ptr if b is not None else None
+
+
+_PAGE_ELEMENT = {DTYPE_F32: 4, DTYPE_BF16: 2, DTYPE_E4M3: 1}
+
+
+class _KvPages(C.Structure):
+    """wpcg_kv_pages (include/wpcg.h)."""
+    _fields_ = [("k", _p), ("v", _p), ("dtype", C.c_int32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("page_stride", _u64), ("head_stride", _u64),
+                ("token_stride", _u64), ("k_scale", _p), ("v_scale", _p)]
+
+
+class _KvBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("n_rows", C.c_uint32), ("max_q", C.c_uint32), ("max_kv", C.c_uint32),
+                ("table_stride", C.c_uint32), ("q_start", _p), ("kv_len", _p), ("table", _p)]
+
+
+class _KvRows(C.Structure):
+    _fields_ = [("q", _p), ("k", _p), ("v", _p), ("dtype", C.c_int32), ("q_out_dtype", C.c_int32),
+                ("n_heads", C.c_uint32), ("q_stride", _u64), ("k_stride", _u64), ("v_stride", _u64),
+                ("q_out_stride", _u64), ("q_out", _p), ("q_norm", _p), ("k_norm", _p), ("freq", _p),
+                ("eps", C.c_float)]
+
+
+class _Attention(C.Structure):
+    _fields_ = [("q", _p), ("out", _p), ("dtype", C.c_int32), ("n_heads", C.c_uint32), ("q_stride", _u64),
+                ("out_stride", _u64), ("scale", C.c_float), ("window", C.c_uint32), ("sinks", C.c_uint32)]
+
+
+class _Draft(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("n_rows", C.c_uint32), ("max_rows", C.c_uint32), ("vocab", C.c_uint32),
+                ("q_start", _p), ("logits", _p), ("logits_stride", _u64), ("draft_probs", _p), ("draft_stride", _u64),
+                ("tokens", _p), ("u", _p), ("u_next", _p), ("temperature", _p), ("accepted", _p), ("out", _p)]
+
+
+def rope_frequencies(theta: float, head_dim: int) -> np.ndarray:
+    """theta^(-2i/head_dim), i < head_dim/2 (apply_rope, wpc-runtime/src/rope.rs:10-40)
+    as the doubles that KvAppend takes."""
+    return float(theta) ** (-np.arange(0, head_dim, 2, dtype=np.float64) / head_dim)
+
+
+class PagedKv:
+    """One layer's keys and values in pages (wpcg_kv_pages): page buffers of
+    its own, or the caller's k and v. strides: (page, head, token) in
+    elements; None = packed [page][head][token][head_dim]."""
+
+    def __init__(self, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 dtype: int = DTYPE_BF16, k=None, v=None, k_scale=None, v_scale=None, strides=None):
+        self.ctx = ctx
+        if k is None or v is None:
+            if strides is not None:
+                raise ValueError("strides go with the caller's own k and v")
+            if dtype not in _PAGE_ELEMENT:
+                raise WpcgError(E_ARG, "pages are F32, BF16 or E4M3")
+            n = n_pages * page_size * n_kv_heads * head_dim * _PAGE_ELEMENT[dtype]
+            k, v = (ctx.alloc(n) if b is None else b for b in (k, v))
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.desc = _KvPages(k.ptr, v.ptr, dtype, n_pages, page_size, n_kv_heads, head_dim, *(strides or (0, 0, 0)),
+                             _ptr(k_scale), _ptr(v_scale))
+
+
+class KvBatch:
+    """The sequences of a step (wpcg_kv_batch): device arrays kv_len int32[n_seq],
+    table int32[n_seq][table_stride] and q_start int32[n_seq + 1] (None: one
+    row each), whose contents may change between the calls, within the
+    bounds n_rows, max_q and max_kv."""
+
+    def __init__(self, n_seq: int, n_rows: int, kv_len, table, table_stride: int, max_kv: int, max_q: int = 1,
+                 q_start=None):
+        self.kv_len, self.table, self.q_start = kv_len, table, q_start
+        self.desc = _KvBatch(n_seq, n_rows, max_q, max_kv, table_stride, _ptr(q_start), _ptr(kv_len), _ptr(table))
+
+
+class KvAppend:
+    """Head norm, rotation and store of a batch's new rows (wpcg_kv_append).
+    Strides are elements between rows; 0 = packed."""
+
+    def __init__(self, ctx: Context, kv: PagedKv, batch: KvBatch, n_heads: int, dtype: int = DTYPE_F32,
+                 q_out_dtype: int = DTYPE_F32, q_norm=None, k_norm=None, eps: float = 1e-6, frequencies=None,
+                 q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, q_out_stride: int = 0):
+        self.ctx, self.kv, self.batch = ctx, kv, batch
+        self._keep = (q_norm, k_norm, frequencies)
+        self.desc = _KvRows(None, None, None, dtype, q_out_dtype, n_heads, q_stride, k_stride, v_stride, q_out_stride,
+                            None, _ptr(q_norm), _ptr(k_norm), _ptr(frequencies), eps)
+        self._refs = (C.byref(kv.desc), C.byref(batch.desc), C.byref(self.desc))
+
+    def run(self, q, k, v, q_out, stream=None):
+        d = self.desc
+        d.q, d.k, d.v, d.q_out = _ptr(q), _ptr(k), _ptr(v), _ptr(q_out)
+        check(lib.wpcg_kv_append(self.ctx.h, *self._refs, stream))
+
+
+class PagedAttention:
+    """Attention of a batch's rows over their pages (wpcg_paged_attention),
+    with a workspace of its own: calls of one object must not overlap."""
+
+    def __init__(self, ctx: Context, kv: PagedKv, batch: KvBatch, n_heads: int, dtype: int = DTYPE_F32,
+                 scale: float | None = None, window: int = 0, sinks: int = 0, q_stride: int = 0,
+                 out_stride: int = 0):
+        self.ctx, self.kv, self.batch = ctx, kv, batch
+        if scale is None:
+            scale = float(kv.desc.head_dim) ** -0.5
+        self.desc = _Attention(None, None, dtype, n_heads, q_stride, out_stride, scale, window, sinks)
+        self._refs = (C.byref(kv.desc), C.byref(batch.desc), C.byref(self.desc))
+        n = C.c_uint64()
+        check(lib.wpcg_paged_attention_workspace(*self._refs, C.byref(n)))
+        self.workspace_bytes = n.value
+        self.workspace = ctx.alloc(n.value) if n.value else None
+
+    def run(self, q, out, stream=None):
+        d = self.desc
+        d.q, d.out = _ptr(q), _ptr(out)
+        check(lib.wpcg_paged_attention(self.ctx.h, *self._refs, _ptr(self.workspace), self.workspace_bytes, stream))
+
+
+class DraftVerify:
+    """Verification of drafts by sampling (wpcg_draft_verify), with a
+    workspace of its own: calls of one object must not overlap."""
+
+    def __init__(self, ctx: Context, n_seq: int, n_rows: int, max_rows: int, vocab: int, q_start=None,
+                 temperature=None, logits_stride: int = 0, draft_stride: int = 0):
+        self.ctx = ctx
+        self._keep = (q_start, temperature)
+        self.desc = _Draft(n_seq, n_rows, max_rows, vocab, _ptr(q_start), None, logits_stride, None, draft_stride,
+                           None, None, None, _ptr(temperature), None, None)
+        self._ref = C.byref(self.desc)
+        n = C.c_uint64()
+        check(lib.wpcg_draft_verify_workspace(self._ref, C.byref(n)))
+        self.workspace_bytes = n.value
+        self.workspace = ctx.alloc(n.value) if n.value else None
+
+    def run(self, logits, tokens, u, u_next, accepted, out, draft_probs=None, stream=None):
+        d = self.desc
+        d.logits, d.tokens, d.u, d.u_next = _ptr(logits), _ptr(tokens), _ptr(u), _ptr(u_next)
+        d.accepted, d.out, d.draft_probs = _ptr(accepted), _ptr(out), _ptr(draft_probs)
+        check(lib.wpcg_draft_verify(self.ctx.h, self._ref, _ptr(self.workspace), self.workspace_bytes, stream))
 
 
 # ------------------------------------------------------------------ encoder
