@@ -4,22 +4,24 @@
 // Every key and value is read once for the query heads of its group, and with
 // one to a few rows that is all there is to do: the memory is the bound (two
 // flops a byte and query head). So the kernel is built to keep loads in
-// flight. Nothing is staged: a wave loads 32 tokens' keys and values straight
-// into the matrix cores' operand layout, 16 bytes a lane, and the next tile's
-// keys are on their way while this tile's softmax runs. A wave owns every
-// fourth tile of the workgroup's chunk, with a running maximum and sum of its
-// own; the four are put together through LDS at the end.
+// flight. Keys and values are not staged: a wave loads 32 tokens of them
+// straight into the matrix cores' operand layout, 16 bytes a lane, and the
+// next tile's keys are on their way while this tile's softmax runs. A wave owns
+// every eighth tile of the workgroup's chunk, with a running maximum and sum
+// of its own; the eight are put together through LDS at the end.
 //
-// Layout. Columns are (row, query head) pairs, 16 a workgroup: lane l holds
-// column l % 16 throughout, lane group g = l / 16. With keys as the A operand
-// (16 tokens) and queries as B, the scores S^T leave lane (column, g) the
-// tokens 4g .. 4g+3 of a 16-token half. That is what the second product needs
-// as its B operand already: a contraction may take its terms in any order, so
-// V^T's A operand just takes tokens 4g .. 4g+3 of both halves in lane group
-// g too, and the terms never leave their lane. The running maximum, the sum
-// and the rescaling factor are one number a lane. V^T needs one dimension's
-// eight tokens side by side: a lane loads D/16 dimensions of eight tokens
-// and transposes them in registers, one byte permute per two values.
+// Layout. Columns are (row, query head) pairs, 16 or 32 a workgroup: lane l
+// holds column l % 16 throughout (and column 16 + l % 16), lane group g =
+// l / 16. With keys as the A operand (16 tokens) and queries as B, the scores
+// S^T leave lane (column, g) the tokens 4g .. 4g+3 of a 16-token half. That is
+// what the second product needs as its B operand already: a contraction may
+// take its terms in any order, so V^T's A operand just takes tokens 4g .. 4g+3
+// of both halves in lane group g too, and the terms never leave their lane.
+// The running maximum, the sum and the rescaling factor are one number a lane
+// and column. V^T needs one dimension's eight tokens side by side: a lane loads
+// D/16 dimensions of eight tokens and transposes them in registers, one byte
+// permute per two values. The queries' operands stay in LDS, where all waves
+// read them (three bf16 terms of F32 queries would take 96 registers).
 //
 // Precision. With BF16 queries the products are bf16 x bf16 (keys, values and
 // queries exact), the softmax's terms rounded to bf16 for the second: half a
@@ -31,9 +33,10 @@
 namespace wpcg {
 namespace {
 
-constexpr int WAVES = 4;
+constexpr int WAVES = ATTN_FEW_WAVES;
 constexpr int THREADS = 64 * WAVES;
-constexpr int TILE = ATTN_FEW_TILE, COLS = ATTN_FEW_COLS;
+constexpr int TILE = ATTN_FEW_TILE;
+constexpr int SLOTS = 4;  // waves whose outputs lie in LDS at a time
 
 // Keys of 16 tokens as A fragments. BF16 and E4M3: D/32 fragments of 32
 // dimensions; lane (token, g) holds dimensions key_dim(f, g) + 0..7. F32:
@@ -116,14 +119,14 @@ struct Values {
     }
 };
 
-// acc[j] += A_j B over the tile's 32 tokens, A_j being dimension n*DV + j of
-// the values, for NT bf16 terms of B. ODD: what is not finite in A is kept out
-// of the products and added to the columns of `see` (1.0 where the column sees
-// the token) alone; three more products count the +inf, -inf and NaN a column
-// sees.
-template <int D, int CT, int NT, bool ODD>
-__device__ __forceinline__ void add_values(const Values<D, CT>& v, const pbf16x8 (&b)[NT], pf32x4 (&acc)[D / 16],
-                                           pbf16x8 see)
+// acc[.][j] += A_j B over the tile's 32 tokens, A_j being dimension n*DV + j of
+// the values, for NT bf16 terms of B in each of NB column blocks. ODD: what is
+// not finite in A is kept out of the products and added to the columns of
+// `see` (1.0 where the column sees the token) alone; three more products count
+// the +inf, -inf and NaN a column sees.
+template <int D, int CT, int NB, int NT, bool ODD>
+__device__ __forceinline__ void add_values(const Values<D, CT>& v, const pbf16x8 (&b)[NB][NT], pf32x4 (&acc)[NB][D / 16],
+                                           const pbf16x8 (&see)[NB])
 {
 #pragma unroll
     for (int i = 0; i < D / 32; i++) {
@@ -145,12 +148,14 @@ __device__ __forceinline__ void add_values(const Values<D, CT>& v, const pbf16x8
                 for (int x = 0; x < 8; x++) is[x] = bf16_is(t[x], kind);
                 const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const pf32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(side(is, e), see, (pf32x4){}, 0, 0, 0);
+                for (int e = 0; e < 2; e++)
 #pragma unroll
-                    for (int y = 0; y < 4; y++)
-                        if (n[y] > 0.0f) acc[2 * i + e][y] += add;
-                }
+                    for (int n = 0; n < NB; n++) {
+                        const pf32x4 k = __builtin_amdgcn_mfma_f32_16x16x32_bf16(side(is, e), see[n], (pf32x4){}, 0, 0, 0);
+#pragma unroll
+                        for (int y = 0; y < 4; y++)
+                            if (k[y] > 0.0f) acc[n][2 * i + e][y] += add;
+                    }
             }
 #pragma unroll
             for (int x = 0; x < 8; x++) t[x] = bf16_finite(t[x]);
@@ -159,21 +164,26 @@ __device__ __forceinline__ void add_values(const Values<D, CT>& v, const pbf16x8
         for (int e = 0; e < 2; e++) {
             const pbf16x8 a = side(t, e);
 #pragma unroll
-            for (int n = NT - 1; n >= 0; n--)  // small terms first
-                acc[2 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[n], acc[2 * i + e], 0, 0, 0);
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int k = NT - 1; k >= 0; k--)  // small terms first
+                    acc[n][2 * i + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[n][k], acc[n][2 * i + e], 0, 0, 0);
         }
     }
 }
 
-template <int D, int CT, bool QF32>
+template <int D, int CT, bool QF32, int NB>
 __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
 {
     constexpr bool F32MM = CT == CT_F32;  // the fp32 matrix cores
     constexpr int NT = QF32 ? 3 : 1;      // bf16 terms of q and of the softmax's terms
     constexpr int DV = D / 16;
     constexpr int ES = ct_size<CT>();
-    __shared__ float s_o[WAVES][COLS][D + 4];
+    constexpr int COLS = 16 * NB;
+    constexpr int QF = F32MM ? D / 16 : D / 32, QT = F32MM ? 1 : NT;  // q's fragments and their terms
+    __shared__ __attribute__((aligned(16))) float s_o[SLOTS][COLS][D + 4];
     __shared__ float s_ml[WAVES][COLS][2];
+    __shared__ pu32x4 s_q[NB][QF][QT][64];
 
     // block -> (column block, chunk, sequence and head); the heads of a
     // sequence are neighbours
@@ -184,57 +194,20 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
     const SeqRows sq = seq_rows(p.b, seq);
     const int cols = sq.n * p.group;  // of this sequence and head
     if (cb * COLS >= cols) return;
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int col = cb * COLS + c;
-    const bool live = col < cols;
-    const int row = live ? col / p.group : 0;
-    const int head = kvh * p.group + (live ? col % p.group : 0);
     const int len = sq.bad ? 0 : sq.len;
     const int pos0 = len - sq.n;  // position of the sequence's row 0
-    const int first = cb * COLS / p.group, last = min(cols, (cb + 1) * COLS) - 1;
-    const SeenTiles<TILE> seen = seen_tiles<TILE>(pos0 + first, pos0 + last / p.group, p.window, p.sinks);
+    const int first = cb * COLS / p.group, last = (min(cols, (cb + 1) * COLS) - 1) / p.group;
+    const SeenTiles<TILE> seen = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks);
     const int v0 = split * p.chunk, v1 = min(v0 + p.chunk, seen.total());
     if (v0 >= v1 && split > 0) return;
-    const int pos = pos0 + row;
     // tokens that every column of the block sees: no mask there
     const int all_hi = pos0 + first + 1;
-    const int all_lo = p.window > 0 ? pos0 + last / p.group - p.window + 1 : 0;
-
-    // q as B fragments, in the keys' order of dimensions
-    const uint64_t q_at = (uint64_t)(sq.a + row) * p.q_row + (uint64_t)head * D;
-    constexpr int QF = F32MM ? 1 : D / 32, QW = F32MM ? D / 16 : 1;
-    pbf16x8 qb[QF][NT];
-    pf32x4 qf[QW];
-    if constexpr (F32MM) {
+    const int all_lo = p.window > 0 ? pos0 + last - p.window + 1 : 0;
+    int pos[NB];  // of this lane's columns
 #pragma unroll
-        for (int f = 0; f < QW; f++)
-            qf[f] = live ? *(const pf32x4*)((const float*)p.q + q_at + key_dim<CT>(f, g)) : (pf32x4){};
-    } else {
-#pragma unroll
-        for (int f = 0; f < QF; f++) {
-            const int d = key_dim<CT>(f, g);
-            if constexpr (QF32) {
-                pf32x4 a = {}, b = {};
-                if (live) {
-                    a = *(const pf32x4*)((const float*)p.q + q_at + d);
-                    b = *(const pf32x4*)((const float*)p.q + q_at + d + 4);
-                }
-                uint32_t t[4][3];
-                split3(a[0], a[1], t[0]);
-                split3(a[2], a[3], t[1]);
-                split3(b[0], b[1], t[2]);
-                split3(b[2], b[3], t[3]);
-#pragma unroll
-                for (int n = 0; n < 3; n++)
-                    qb[f][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
-            } else {
-                const pu32x4 w = live ? *(const pu32x4*)((const uint16_t*)p.q + q_at + d) : (pu32x4){};
-                qb[f][0] = __builtin_bit_cast(pbf16x8, w);
-            }
-        }
-    }
-    const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
+    for (int n = 0; n < NB; n++) pos[n] = pos0 + min(cb * COLS + 16 * n + c, cols - 1) / p.group;
 
     const uint8_t* const kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
     const uint8_t* const vp = (const uint8_t*)p.v + (uint64_t)kvh * p.head_stride * ES;
@@ -257,18 +230,53 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
 
     Keys<D, CT> K[2];
     Values<D, CT> V;
-    pf32x4 acc[DV] = {};
-    float m = -INFINITY, l = 0.0f;
-
     int vt = v0 + wave;
     uint64_t at[2] = {0, 0};
     if (vt < v1) {
         const int t0 = seen.tile(vt) * TILE;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            at[h] = place(t0 + 16 * h);
-            K[h].load(kp + at[h] + (uint64_t)c * token_bytes, g);
+        for (int h = 0; h < 2; h++) at[h] = place(t0 + 16 * h);
+#pragma unroll
+        for (int h = 0; h < 2; h++) K[h].load(kp + at[h] + (uint64_t)c * token_bytes, g);
+    }
+
+    // q as B fragments in LDS, in the keys' order of dimensions: fragment f of
+    // column block n by wave (n QF + f) % WAVES
+#pragma unroll
+    for (int x = 0; x < NB * QF; x++) {
+        if (x % WAVES != wave) continue;
+        const int n = x / QF, f = x % QF, col = cb * COLS + 16 * n + c;
+        const bool live = col < cols;
+        const uint64_t q_at = live ? (uint64_t)(sq.a + col / p.group) * p.q_row +
+                                         (uint64_t)(kvh * p.group + col % p.group) * D + key_dim<CT>(f, g) : 0;
+        if constexpr (F32MM) {
+            s_q[n][f][0][lane] = live ? *(const pu32x4*)((const float*)p.q + q_at) : (pu32x4){};
+        } else if constexpr (QF32) {
+            pf32x4 a = {}, b = {};
+            if (live) {
+                a = *(const pf32x4*)((const float*)p.q + q_at);
+                b = *(const pf32x4*)((const float*)p.q + q_at + 4);
+            }
+            uint32_t t[4][3];
+            split3(a[0], a[1], t[0]);
+            split3(a[2], a[3], t[1]);
+            split3(b[0], b[1], t[2]);
+            split3(b[2], b[3], t[3]);
+#pragma unroll
+            for (int k = 0; k < 3; k++) s_q[n][f][k][lane] = (pu32x4){t[0][k], t[1][k], t[2][k], t[3][k]};
+        } else {
+            s_q[n][f][0][lane] = live ? *(const pu32x4*)((const uint16_t*)p.q + q_at) : (pu32x4){};
         }
+    }
+    const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
+    __syncthreads();
+
+    pf32x4 acc[NB][DV] = {};
+    float m[NB], l[NB];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
     }
     for (; vt < v1; vt += WAVES) {
         const int t0 = seen.tile(vt) * TILE;
@@ -281,22 +289,32 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
             next[0] = place(t1);
             next[1] = place(t1 + 16);
         }
+        asm volatile("" ::: "memory");  // q's fragments are read again, not kept in registers
         // scores
-        pf32x4 s[2] = {};
+        pf32x4 s[NB][2] = {};
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int n = 0; n < NB; n++) {
             if constexpr (F32MM) {
 #pragma unroll
-                for (int f = 0; f < QW; f++)
+                for (int f = 0; f < QF; f++) {
+                    const pf32x4 q = __builtin_bit_cast(pf32x4, s_q[n][f][0][lane]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(K[h].w[f][e]), qf[f][e], s[h], 0, 0, 0);
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            s[n][h] =
+                                __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(K[h].w[f][e]), q[e], s[n][h], 0, 0, 0);
+                }
             } else {
 #pragma unroll
-                for (int n = NT - 1; n >= 0; n--)
+                for (int k = NT - 1; k >= 0; k--)  // small terms first
 #pragma unroll
-                    for (int f = 0; f < QF; f++)
-                        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K[h].frag(f), qb[f][n], s[h], 0, 0, 0);
+                    for (int f = 0; f < QF; f++) {
+                        const pbf16x8 q = __builtin_bit_cast(pbf16x8, s_q[n][f][k][lane]);
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K[h].frag(f), q, s[n][h], 0, 0, 0);
+                    }
             }
         }
         if (vt + WAVES < v1) {
@@ -309,29 +327,34 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
         const bool whole = t0 + TILE <= all_hi && t0 >= all_lo;
         if (!whole) {
 #pragma unroll
-            for (int x = 0; x < 8; x++) {
-                const int t = t0 + 16 * (x / 4) + 4 * g + x % 4;
-                if (!row_sees(pos, t, p.window, p.sinks)) s[x / 4][x % 4] = -INFINITY;
-            }
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const int t = t0 + 16 * (x / 4) + 4 * g + x % 4;
+                    if (!row_sees(pos[n], t, p.window, p.sinks)) s[n][x / 4][x % 4] = -INFINITY;
+                }
         }
         // running maximum and terms
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = max_x16_32(top) * sc;
-        const float now = fmaxf(m, top);
-        const float base = now == -INFINITY ? 0.0f : now;
-        if (__any(now > m)) {
-            const float f = exp2_fast(m - base);
-            l *= f;
+        float e[NB][8];
 #pragma unroll
-            for (int j = 0; j < DV; j++) acc[j] *= f;
-            m = now;
-        }
-        float e[8];
+        for (int n = 0; n < NB; n++) {
+            float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                              fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+            top = max_x16_32(top) * sc;
+            const float now = fmaxf(m[n], top);
+            const float base = now == -INFINITY ? 0.0f : now;
+            if (__any(now > m[n])) {
+                const float f = exp2_fast(m[n] - base);
+                l[n] *= f;
 #pragma unroll
-        for (int x = 0; x < 8; x++) {
-            e[x] = exp2_fast(fmaf(s[x / 4][x % 4], sc, -base));
-            l += e[x];
+                for (int j = 0; j < DV; j++) acc[n][j] *= f;
+                m[n] = now;
+            }
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                e[n][x] = exp2_fast(fmaf(s[n][x / 4][x % 4], sc, -base));
+                l[n] += e[n][x];
+            }
         }
         // what a masked token's value holds stays out: tokens that no column
         // sees are cleared, and values that are not finite and that only some
@@ -349,21 +372,24 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
                 for (int kind = 0; kind < 3; kind++) {
                     const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
 #pragma unroll
-                    for (int j = 0; j < DV; j++) {
-                        pf32x4 n = {};
+                    for (int n = 0; n < NB; n++)
 #pragma unroll
-                        for (int x = 0; x < 8; x++) {
-                            const int t = t0 + 16 * (x / 4) + 4 * g + x % 4;
-                            const uint32_t w = V.w[x][j];
-                            const bool hit = kind == 0 ? w == 0x7f800000u : kind == 1 ? w == 0xff800000u
-                                                                                    : (w & 0x7fffffffu) > 0x7f800000u;
-                            n = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                hit ? 1.0f : 0.0f, row_sees(pos, t, p.window, p.sinks) ? 1.0f : 0.0f, n, 0, 0, 0);
+                        for (int j = 0; j < DV; j++) {
+                            pf32x4 k = {};
+#pragma unroll
+                            for (int x = 0; x < 8; x++) {
+                                const int t = t0 + 16 * (x / 4) + 4 * g + x % 4;
+                                const uint32_t w = V.w[x][j];
+                                const bool hit = kind == 0   ? w == 0x7f800000u
+                                                 : kind == 1 ? w == 0xff800000u
+                                                             : (w & 0x7fffffffu) > 0x7f800000u;
+                                k = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    hit ? 1.0f : 0.0f, row_sees(pos[n], t, p.window, p.sinks) ? 1.0f : 0.0f, k, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (k[i] > 0.0f) acc[n][j][i] += add;
                         }
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (n[i] > 0.0f) acc[j][i] += add;
-                    }
                 }
 #pragma unroll
                 for (int x = 0; x < 8; x++)
@@ -372,97 +398,132 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
                         if ((V.w[x][j] & 0x7f800000u) == 0x7f800000u) V.w[x][j] = 0;
             }
 #pragma unroll
-            for (int x = 0; x < 8; x++)
+            for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int j = 0; j < DV; j++)
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(V.w[x][j]), e[x], acc[j], 0, 0, 0);
+                for (int x = 0; x < 8; x++)
+#pragma unroll
+                    for (int j = 0; j < DV; j++)
+                        acc[n][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(V.w[x][j]), e[n][x], acc[n][j],
+                                                                         0, 0, 0);
         } else {
-            pbf16x8 b[NT];
-            if constexpr (QF32) {
-                uint32_t t[4][3];
+            pbf16x8 b[NB][NT], see[NB];
 #pragma unroll
-                for (int x = 0; x < 4; x++) split3(e[2 * x], e[2 * x + 1], t[x]);
+            for (int n = 0; n < NB; n++) {
+                if constexpr (QF32) {
+                    uint32_t t[4][3];
 #pragma unroll
-                for (int n = 0; n < 3; n++)
-                    b[n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
-            } else {
-                pu32x4 t;
+                    for (int x = 0; x < 4; x++) split3(e[n][2 * x], e[n][2 * x + 1], t[x]);
 #pragma unroll
-                for (int x = 0; x < 4; x++) t[x] = pk_bf16_rne(e[2 * x], e[2 * x + 1]);
-                b[0] = __builtin_bit_cast(pbf16x8, t);
+                    for (int k = 0; k < 3; k++)
+                        b[n][k] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][k], t[1][k], t[2][k], t[3][k]});
+                } else {
+                    pu32x4 t;
+#pragma unroll
+                    for (int x = 0; x < 4; x++) t[x] = pk_bf16_rne(e[n][2 * x], e[n][2 * x + 1]);
+                    b[n][0] = __builtin_bit_cast(pbf16x8, t);
+                }
             }
             if (odd) {
-                pu32x4 see;
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int t = t0 + 16 * (x / 2) + 4 * g + 2 * x % 4;
-                    see[x] = (row_sees(pos, t, p.window, p.sinks) ? 0x3f80u : 0u) |
-                             (row_sees(pos, t + 1, p.window, p.sinks) ? 0x3f800000u : 0u);
+                for (int n = 0; n < NB; n++) {
+                    pu32x4 w;
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const int t = t0 + 16 * (x / 2) + 4 * g + 2 * x % 4;
+                        w[x] = (row_sees(pos[n], t, p.window, p.sinks) ? 0x3f80u : 0u) |
+                               (row_sees(pos[n], t + 1, p.window, p.sinks) ? 0x3f800000u : 0u);
+                    }
+                    see[n] = __builtin_bit_cast(pbf16x8, w);
                 }
-                add_values<D, CT, NT, true>(V, b, acc, __builtin_bit_cast(pbf16x8, see));
+                add_values<D, CT, NB, NT, true>(V, b, acc, see);
             } else {
-                add_values<D, CT, NT, false>(V, b, acc, pbf16x8{});
+                add_values<D, CT, NB, NT, false>(V, b, acc, see);
             }
         }
     }
-    l = sum_x16_32(l);
-    if (__any(fault)) l = __builtin_nanf("");
 
-    // the four waves' parts together; a lane's D/4 outputs are dimensions
-    // (4g + i) * DV + j of column c
-    if (g == 0) {
-        s_ml[wave][c][0] = m;
-        s_ml[wave][c][1] = l;
-    }
-    __syncthreads();
-    float top = s_ml[0][c][0];
+    // the waves' parts together; a lane's outputs are dimensions
+    // (4g + i) * DV + j of its columns
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) top = fmaxf(top, s_ml[w][c][0]);
-    const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
-#pragma unroll
-    for (int j = 0; j < DV; j++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) s_o[wave][c][(4 * g + i) * DV + j] = f == 0.0f ? 0.0f : acc[j][i] * f;
-    __syncthreads();
-
-    // thread -> column tid / 16, DV dimensions
-    const int oc = (int)threadIdx.x / 16, od = (int)threadIdx.x % 16 * DV;
-    const int ocol = cb * COLS + oc;
-    if (ocol >= cols) return;
-    float om = s_ml[0][oc][0], ol = 0.0f;
-#pragma unroll
-    for (int w = 1; w < WAVES; w++) om = fmaxf(om, s_ml[w][oc][0]);
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) {
-        const float wm = s_ml[w][oc][0], wl = s_ml[w][oc][1];
-        ol += wm == -INFINITY ? (wl != wl ? wl : 0.0f) : wl * exp2_fast(wm - om);
-    }
-    float o[DV];
-#pragma unroll
-    for (int j = 0; j < DV; j++) {
-        o[j] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) o[j] += s_o[w][oc][od + j];
-    }
-    const int orow = ocol / p.group, ohead = kvh * p.group + ocol % p.group;
-    if (p.splits > 1) {
-        const uint64_t slot = ((uint64_t)split * p.b.n_rows + sq.a + orow) * p.n_heads + ohead;
-#pragma unroll
-        for (int j = 0; j < DV; j += 4)
-            *(pf32x4*)(p.part_o + slot * D + od + j) = (pf32x4){o[j], o[j + 1], o[j + 2], o[j + 3]};
-        if (od == 0) {
-            p.part_ml[slot * 2] = om;
-            p.part_ml[slot * 2 + 1] = ol;
+    for (int n = 0; n < NB; n++) {
+        l[n] = sum_x16_32(l[n]);
+        if (__any(fault)) l[n] = __builtin_nanf("");
+        if (g == 0) {
+            s_ml[wave][16 * n + c][0] = m[n];
+            s_ml[wave][16 * n + c][1] = l[n];
         }
-        return;
     }
-    attn_store<DV, QF32>(p, sq, orow, ohead, od, D, o, ol, p.v_scale ? p.v_scale[kvh] : 1.0f);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+        float top = s_ml[0][16 * n + c][0];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) top = fmaxf(top, s_ml[w][16 * n + c][0]);
+        const float f = m[n] == -INFINITY ? 0.0f : exp2_fast(m[n] - top);
+#pragma unroll
+        for (int j = 0; j < DV; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[n][j][i] = f == 0.0f ? 0.0f : acc[n][j][i] * f;
+    }
+#pragma unroll
+    for (int r = 0; r < WAVES / SLOTS; r++) {
+        if (wave / SLOTS == r) {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < DV; j += 4) {
+                        pf32x4* o = (pf32x4*)&s_o[wave % SLOTS][16 * n + c][(4 * g + i) * DV + j];
+                        const pf32x4 v = {acc[n][j][i], acc[n][j + 1][i], acc[n][j + 2][i], acc[n][j + 3][i]};
+                        *o = r ? *o + v : v;
+                    }
+        }
+        __syncthreads();
+    }
+
+    // thread -> column, four dimensions
+    constexpr int PER = D / 4;
+    for (int x = (int)threadIdx.x; x < COLS * PER; x += THREADS) {
+        const int oc = x / PER, od = x % PER * 4;
+        const int ocol = cb * COLS + oc;
+        if (ocol >= cols) break;
+        float om = s_ml[0][oc][0], ol = 0.0f;
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) om = fmaxf(om, s_ml[w][oc][0]);
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float wm = s_ml[w][oc][0], wl = s_ml[w][oc][1];
+            ol += wm == -INFINITY ? (wl != wl ? wl : 0.0f) : wl * exp2_fast(wm - om);
+        }
+        pf32x4 o = *(const pf32x4*)&s_o[0][oc][od];
+#pragma unroll
+        for (int w = 1; w < SLOTS; w++) o += *(const pf32x4*)&s_o[w][oc][od];
+        const int orow = ocol / p.group, ohead = kvh * p.group + ocol % p.group;
+        if (p.splits > 1) {
+            const uint64_t slot = ((uint64_t)split * p.b.n_rows + sq.a + orow) * p.n_heads + ohead;
+            *(pf32x4*)(p.part_o + slot * D + od) = o;
+            if (od == 0) {
+                p.part_ml[slot * 2] = om;
+                p.part_ml[slot * 2 + 1] = ol;
+            }
+        } else {
+            const float r[4] = {o[0], o[1], o[2], o[3]};
+            attn_store<4, QF32>(p, sq, orow, ohead, od, D, r, ol, p.v_scale ? p.v_scale[kvh] : 1.0f);
+        }
+    }
 }
 
 template <int D, int CT, bool QF32>
 void go(const PagedAttnArgs& p, unsigned blocks, hipStream_t s)
 {
-    k_attn_few<D, CT, QF32><<<dim3(blocks), dim3(THREADS), 0, s>>>(p);
+    if constexpr (CT != CT_F32) {
+        if (p.cols == 2 * ATTN_FEW_COLS) {
+            k_attn_few<D, CT, QF32, 2><<<dim3(blocks), dim3(THREADS), 0, s>>>(p);
+            return;
+        }
+    }
+    k_attn_few<D, CT, QF32, 1><<<dim3(blocks), dim3(THREADS), 0, s>>>(p);
 }
 
 template <int D>
@@ -479,65 +540,82 @@ void go_types(const PagedAttnArgs& p, int q_dtype, int cache_dtype, unsigned blo
 }
 
 // ---- the chunks' states joined -------------------------------------------------
-// A workgroup per (row, query head): out = sum_i 2^(m_i - M) o_i / sum_i
-// 2^(m_i - M) l_i over the chunks that the row's workgroup had, in an order
-// that depends on their number alone. Four chunks are read at a time.
-template <int D, bool QF32, bool MANY>
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that the
+// row's workgroup had, in an order that depends on the call's bounds alone.
+// PAR groups of D/4 threads share a (row, query head): one where the chunks
+// are few, so that many rows have few threads each, eight where a long
+// sequence has many.
+template <int D, bool QF32, int TILE_, int PAR>
 __global__ __launch_bounds__(256) void k_attn_join(PagedAttnArgs p)
 {
-    constexpr int COLS_ = MANY ? ATTN_MANY_COLS : ATTN_FEW_COLS;
-    constexpr int TILE_ = MANY ? ATTN_MANY_TILE : ATTN_FEW_TILE;
-    constexpr int TH = D / 4, PAR = 256 / TH;  // threads of a chunk, chunks at a time
-    __shared__ float s_o[PAR][D];
-    __shared__ float s_l[PAR], s_red[4];
-    const int head = (int)(blockIdx.x % (unsigned)p.n_heads), rest = (int)(blockIdx.x / (unsigned)p.n_heads);
-    const int seq = rest % p.b.n_seq, row = rest / p.b.n_seq;
-    const SeqRows sq = seq_rows(p.b, seq);
-    if (row >= sq.n) return;
-    const int kvh = head / p.group;
-    const int cols = sq.n * p.group, cb = (row * p.group + head % p.group) / COLS_;
-    const int len = sq.bad ? 0 : sq.len, pos0 = len - sq.n;
-    const int first = cb * COLS_ / p.group, last = (min(cols, (cb + 1) * COLS_) - 1) / p.group;
-    const int tiles = seen_tiles<TILE_>(pos0 + first, pos0 + last, p.window, p.sinks).total();
-    const int n = max(1, (tiles + p.chunk - 1) / p.chunk);
+    constexpr int TH = D / 4, PER = 256 / (TH * PAR);
+    __shared__ float s_o[PAR][PER][D];
+    __shared__ float s_ml[PAR][PER][2];
     const int tid = (int)threadIdx.x;
-    const uint64_t slot0 = (uint64_t)(sq.a + row) * p.n_heads + head;
-    const uint64_t step = (uint64_t)p.b.n_rows * p.n_heads;
-
-    float m = -INFINITY;
-    for (int i = tid; i < n; i += 256) m = fmaxf(m, p.part_ml[(slot0 + i * step) * 2]);
-    m = max_x16_32(m);
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-    if ((tid & 63) == 0) s_red[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const float base = m == -INFINITY ? 0.0f : m;
-
-    const int part = tid / TH, d = tid % TH * 4;
-    float l = 0.0f;
+    const int part = tid / TH % PAR, mine = tid / (TH * PAR), d = tid % TH * 4;
+    const uint64_t x = (uint64_t)blockIdx.x * PER + mine;
+    const int head = (int)(x % (unsigned)p.n_heads);
+    const uint64_t rest = x / (unsigned)p.n_heads;
+    const int row = (int)(rest / (unsigned)p.b.n_seq), seq = (int)(rest % (unsigned)p.b.n_seq);
+    SeqRows sq = {};
+    if (row < p.b.max_q) sq = seq_rows(p.b, seq);
+    const bool live = row < sq.n;
+    float m = -INFINITY, l = 0.0f;
     pf32x4 o = {};
-    for (int i = part; i < n; i += PAR) {
-        const uint64_t slot = slot0 + i * step;
-        const float f = exp2_fast(p.part_ml[slot * 2] - base);
-        const float li = p.part_ml[slot * 2 + 1];
-        const pf32x4 oi = *(const pf32x4*)(p.part_o + slot * D + d);
-        l += f == 0.0f && li == li ? 0.0f : li * f;
-        if (f != 0.0f) o += oi * f;
+    if (live) {
+        const int cols = sq.n * p.group, cb = (row * p.group + head % p.group) / p.cols;
+        const int len = sq.bad ? 0 : sq.len, pos0 = len - sq.n;
+        const int first = cb * p.cols / p.group, last = (min(cols, (cb + 1) * p.cols) - 1) / p.group;
+        const int tiles = seen_tiles<TILE_>(pos0 + first, pos0 + last, p.window, p.sinks).total();
+        const int n = max(1, (tiles + p.chunk - 1) / p.chunk);
+        const uint64_t slot0 = (uint64_t)(sq.a + row) * p.n_heads + head;
+        const uint64_t step = (uint64_t)p.b.n_rows * p.n_heads;
+        for (int i = part; i < n; i += PAR) m = fmaxf(m, p.part_ml[(slot0 + i * step) * 2]);
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+        for (int i = part; i < n; i += PAR) {
+            const uint64_t slot = slot0 + i * step;
+            const float f = exp2_fast(p.part_ml[slot * 2] - base);
+            const float li = p.part_ml[slot * 2 + 1];
+            const pf32x4 oi = *(const pf32x4*)(p.part_o + slot * D + d);
+            l += f == 0.0f && li == li ? 0.0f : li * f;
+            if (f != 0.0f) o += oi * f;
+        }
     }
-    *(pf32x4*)&s_o[part][d] = o;
-    if (d == 0) s_l[part] = l;
-    __syncthreads();
-    // sums over the parts, in their order
-    if (part != 0) return;
-    float lt = 0.0f, out[4] = {};
+    if constexpr (PAR > 1) {
+        *(pf32x4*)&s_o[part][mine][d] = o;
+        if (d == 0) {
+            s_ml[part][mine][0] = m;
+            s_ml[part][mine][1] = l;
+        }
+        __syncthreads();
+        if (part != 0) return;
+        float top = m;
 #pragma unroll
-    for (int i = 0; i < PAR; i++) {
-        lt += s_l[i];
+        for (int i = 1; i < PAR; i++) top = fmaxf(top, s_ml[i][mine][0]);
+        o = (pf32x4){};
+        l = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) out[j] += s_o[i][d + j];
+        for (int i = 0; i < PAR; i++) {  // in their order
+            const float mi = s_ml[i][mine][0], li = s_ml[i][mine][1];
+            const float f = mi == -INFINITY ? 0.0f : exp2_fast(mi - top);
+            l += f == 0.0f && li == li ? 0.0f : li * f;
+            if (f != 0.0f) o += *(const pf32x4*)&s_o[i][mine][d] * f;
+        }
     }
-    attn_store<4, QF32>(p, sq, row, head, d, D, out, lt, p.v_scale ? p.v_scale[kvh] : 1.0f);
+    if (!live) return;
+    const float r[4] = {o[0], o[1], o[2], o[3]};
+    attn_store<4, QF32>(p, sq, row, head, d, D, r, l, p.v_scale ? p.v_scale[head / p.group] : 1.0f);
+}
+
+template <int D, bool QF32, int TILE_>
+void join(const PagedAttnArgs& p, hipStream_t s)
+{
+    constexpr int MANY = 8;
+    const uint64_t all = (uint64_t)p.b.n_seq * p.b.max_q * p.n_heads;
+    const auto blocks = [&](int par) { return dim3((unsigned)((all * (D / 4) * par + 255) / 256)); };
+    if (p.splits > 4) k_attn_join<D, QF32, TILE_, MANY><<<blocks(MANY), dim3(256), 0, s>>>(p);
+    else k_attn_join<D, QF32, TILE_, 1><<<blocks(1), dim3(256), 0, s>>>(p);
 }
 
 }  // namespace
@@ -553,21 +631,15 @@ hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, in
 
 hipError_t launch_attn_join(const PagedAttnArgs& p, int head_dim, int q_dtype, bool many, hipStream_t s)
 {
-    const uint64_t blocks = (uint64_t)p.b.n_seq * p.b.max_q * p.n_heads;
-    if (blocks == 0) return hipSuccess;
-    const dim3 grid((unsigned)blocks), block(256);
+    if ((uint64_t)p.b.n_seq * p.b.max_q == 0) return hipSuccess;
     const bool f32 = q_dtype == WPCG_DTYPE_F32;
-#define WPCG_JOIN(D, F, M) \
-    if (head_dim == D && f32 == F && many == M) k_attn_join<D, F, M><<<grid, block, 0, s>>>(p)
-    WPCG_JOIN(64, false, false);
-    WPCG_JOIN(64, true, false);
-    WPCG_JOIN(128, false, false);
-    WPCG_JOIN(128, true, false);
-    WPCG_JOIN(64, false, true);
-    WPCG_JOIN(64, true, true);
-    WPCG_JOIN(128, false, true);
-    WPCG_JOIN(128, true, true);
-#undef WPCG_JOIN
+    if (many) {
+        if (head_dim == 128) f32 ? join<128, true, ATTN_MANY_TILE>(p, s) : join<128, false, ATTN_MANY_TILE>(p, s);
+        else f32 ? join<64, true, ATTN_MANY_TILE>(p, s) : join<64, false, ATTN_MANY_TILE>(p, s);
+    } else {
+        if (head_dim == 128) f32 ? join<128, true, ATTN_FEW_TILE>(p, s) : join<128, false, ATTN_FEW_TILE>(p, s);
+        else f32 ? join<64, true, ATTN_FEW_TILE>(p, s) : join<64, false, ATTN_FEW_TILE>(p, s);
+    }
     return hipGetLastError();
 }
 

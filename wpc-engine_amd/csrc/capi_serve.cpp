@@ -94,26 +94,25 @@ int check_pointers(const wpcg_kv_pages* kv, const wpcg_kv_batch* b)
 
 struct Plan {
     bool many;
-    int col_blocks, chunk, splits;
+    int cols, col_blocks, chunk, splits;
     uint64_t bytes;
 };
 
 // Which kernel, and how many workgroups share a sequence's tokens.
 //
-// Few rows: up to FEW_BLOCKS column blocks of 16, each reading the keys and
-// values again.
-//
-// A batch is split over the tokens until it has about TARGET workgroups, in
-// chunks of at least the given tiles: a shorter chunk pays more for its state
-// than it gains. The bounds stand in for the lengths, which only the device
-// knows; a shorter sequence just has fewer chunks.
+// A batch is split over the tokens until it has about `target` workgroups, in
+// chunks of at least `least` tiles: a shorter chunk pays more for its state and
+// the second launch than it gains. The bounds stand in for the lengths, which
+// only the device knows; a shorter sequence just has fewer chunks.
 int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attention* a, Plan* out)
 {
     const int64_t group = a->n_heads / kv->n_kv_heads, cols = (int64_t)b.max_q * group;
-    constexpr int64_t FEW_COLS = 2 * ATTN_FEW_COLS;
     Plan p;
-    p.many = cols > FEW_COLS;
-    const int64_t cw = p.many ? ATTN_MANY_COLS : ATTN_FEW_COLS, tw = p.many ? ATTN_MANY_TILE : ATTN_FEW_TILE;
+    p.many = cols > 2 * ATTN_FEW_COLS;
+    // (over an F32 cache the wider form's registers do not suffice)
+    p.cols = p.many ? ATTN_MANY_COLS
+             : cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
+    const int64_t cw = p.cols, tw = p.many ? ATTN_MANY_TILE : ATTN_FEW_TILE;
     const int64_t blocks = (cols + cw - 1) / cw;
     // tiles that a column block can see
     int64_t tiles = (b.max_kv + tw - 1) / tw;
@@ -124,7 +123,7 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
         tiles = std::min(tiles, seen);
     }
     const int64_t base = (int64_t)b.n_seq * kv->n_kv_heads * blocks;
-    const int64_t target = p.many ? 512 : 1024, least = p.many ? 8 : 4;
+    const int64_t target = 512, least = p.many ? 8 : 2 * ATTN_FEW_WAVES;
     int64_t chunk = tiles;
     if (base > 0 && base < target) {
         const int64_t want = (target + base - 1) / base;
@@ -152,14 +151,7 @@ int check_attention(const wpcg_kv_pages* kv, const wpcg_attention* a)
     return WPCG_OK;
 }
 
-// ids of a chunk of a row's logits: short ones while the rows are few, so
-// that a single sequence's five rows still have a few hundred workgroups
-int draft_chunk(const wpcg_draft* d)
-{
-    return (uint64_t)d->n_rows * ((d->vocab + 8191) / 8192) >= 1024 ? 8192 : 2048;
-}
-
-int check_draft(const wpcg_draft* d, int* chunk, int* chunks, uint64_t* bytes)
+int check_draft(const wpcg_draft* d, int* chunks, uint64_t* bytes)
 {
     if (!d) return fail(WPCG_E_ARG, "null argument");
     if (d->vocab == 0 || d->vocab > INT_BOUND) return fail(WPCG_E_ARG, "vocab out of range");
@@ -173,12 +165,11 @@ int check_draft(const wpcg_draft* d, int* chunk, int* chunks, uint64_t* bytes)
     if ((d->logits_stride && d->logits_stride < d->vocab) || (d->draft_stride && d->draft_stride < d->vocab))
         return fail(WPCG_E_SHAPE, "row stride shorter than the row");
     if (d->logits_stride >> 40 || d->draft_stride >> 40) return fail(WPCG_E_ARG, "row stride too large");
-    *chunk = draft_chunk(d);
-    *chunks = (int)((d->vocab + *chunk - 1) / *chunk);
+    *chunks = (int)((d->vocab + DRAFT_CHUNK - 1) / DRAFT_CHUNK);
     if ((uint64_t)std::max(d->n_rows, d->n_seq) * *chunks >= 1u << 31)
         return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
     *bytes = (uint64_t)d->n_rows * *chunks * sizeof(DraftPart) + (uint64_t)d->n_seq * *chunks * sizeof(double) +
-             (uint64_t)d->n_seq * sizeof(DraftChoice);
+             (uint64_t)d->n_seq * sizeof(DraftDone);
     return WPCG_OK;
 }
 
@@ -300,6 +291,7 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
     a.scale = (float)((double)att->scale * 1.4426950408889634);
     a.window = (int)std::min<uint64_t>(att->window, INT_BOUND);
     a.sinks = (int)std::min<uint64_t>(att->sinks, INT_BOUND);
+    a.cols = plan.cols;
     a.col_blocks = plan.col_blocks;
     a.chunk = plan.chunk;
     a.splits = plan.splits;
@@ -316,15 +308,15 @@ int wpcg_draft_verify_workspace(const wpcg_draft* d, uint64_t* bytes)
 {
     if (!bytes) return fail(WPCG_E_ARG, "null output");
     *bytes = 0;
-    int chunk, chunks;
-    return check_draft(d, &chunk, &chunks, bytes);
+    int chunks;
+    return check_draft(d, &chunks, bytes);
 }
 
 int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream)
 {
     DraftArgs a{};
     uint64_t bytes = 0;
-    if (int rc = check_draft(d, &a.chunk, &a.chunks, &bytes)) return rc;
+    if (int rc = check_draft(d, &a.chunks, &bytes)) return rc;
     if (d->n_seq == 0) return check_ctx(ctx);
     if (!d->accepted_dev) return fail(WPCG_E_ARG, "null argument");
     if (d->n_rows > 0) {
@@ -351,8 +343,9 @@ int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t
     a.accepted = d->accepted_dev;
     a.out = d->out_dev;
     a.part = (DraftPart*)ws_dev;
-    a.choice = (DraftChoice*)(a.part + (uint64_t)d->n_rows * a.chunks);
-    a.rest = (double*)(a.choice + d->n_seq);
+    a.rest = (double*)(a.part + (uint64_t)d->n_rows * a.chunks);
+    a.done = (DraftDone*)(a.rest + (uint64_t)d->n_seq * a.chunks);
+    a.vec = aligned(a.logits) && a.logits_row % 4 == 0 && aligned(a.probs) && a.probs_row % 4 == 0;
     WPCG_HIP(launch_draft_verify(a, pick(ctx, stream)));
     return WPCG_OK;
 }

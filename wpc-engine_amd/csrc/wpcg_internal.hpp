@@ -493,14 +493,14 @@ struct KvAppendArgs {
 hipError_t launch_kv_append(const KvAppendArgs& p, int head_dim, bool bf16, hipStream_t s);
 // Attention over pages. A column is a (row, query head) pair: column c of a
 // sequence's key-value head is row c / group, query head c % group of its
-// group. The kernel for few rows takes ATTN_FEW_COLS columns a workgroup,
-// that for many ATTN_MANY_COLS; each reads a chunk of `chunk` tiles
+// group. The kernel for few rows takes ATTN_FEW_COLS columns a workgroup, or
+// twice as many, that for many ATTN_MANY_COLS; each reads a chunk of `chunk` tiles
 // (ATTN_FEW_TILE, ATTN_MANY_TILE tokens) of those its columns see, the chunks
 // are `splits` at most. With splits > 1 chunk i leaves a column's
 // unnormalised output (fp32) at part_o[(i * n_rows + row) * n_heads + head]
 // (head_dim values) and its maximum (of the scores times log2 e) and sum of
 // terms at part_ml [same][2], and launch_attn_join puts them together.
-constexpr int ATTN_FEW_COLS = 16, ATTN_FEW_TILE = 32;
+constexpr int ATTN_FEW_COLS = 16, ATTN_FEW_TILE = 32, ATTN_FEW_WAVES = 8;
 constexpr int ATTN_MANY_COLS = 128, ATTN_MANY_TILE = 64;
 struct PagedAttnArgs {
     PagedBatch b;
@@ -512,7 +512,7 @@ struct PagedAttnArgs {
     int n_heads, n_kv, group;
     float scale;  // times log2 e
     int window, sinks;
-    int col_blocks;  // of a sequence's key-value head
+    int cols, col_blocks;  // columns of a workgroup; blocks of them of a sequence's key-value head
     int chunk, splits;
     float *part_o, *part_ml;
 };
@@ -522,30 +522,29 @@ hipError_t launch_attn_join(const PagedAttnArgs& p, int head_dim, int q_dtype, b
 
 // ---- verification of drafts (draft.hip) -------------------------------------
 // A chunk's state of a row: sum of exp((x - max) / T), the largest logit and
-// its first place; and what was decided for a sequence: Z and M of the row the
-// next token comes from, its first largest logit, the accepted drafts.
+// (greedy rows) its first place; and a sequence's count of finished workgroups.
+constexpr int DRAFT_CHUNK = 2048;  // ids
 struct DraftPart {
     double sum;
     float max;
     int at;
 };
-struct DraftChoice {
-    double z;
-    float m;
-    int at, accepted, pad;
+struct DraftDone {
+    int done, pad;
 };
 struct DraftArgs {
     int n_seq, n_rows, max_rows, vocab;
-    int chunk, chunks;  // ids of a chunk, chunks of a row
+    int chunks;  // of a row
+    int vec;     // rows of logits and probs start on 16 bytes
     const int32_t* q_start;
     const float *logits, *probs;  // probs may be null
     uint64_t logits_row, probs_row;
     const uint32_t* tokens;
     const float *u, *u_next, *temperature;
     int32_t *accepted, *out;
-    DraftPart* part;      // [n_rows][chunks]
-    double* rest;         // [n_seq][chunks]
-    DraftChoice* choice;  // [n_seq]
+    DraftPart* part;    // [n_rows][chunks]
+    double* rest;       // [n_seq][chunks]
+    DraftDone* done;    // [n_seq]
 };
 hipError_t launch_draft_verify(const DraftArgs& p, hipStream_t s);
 
