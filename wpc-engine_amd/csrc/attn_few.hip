@@ -52,10 +52,11 @@ template <int D, int CT>
 struct Keys {
     static constexpr int LOADS = D * ct_size<CT>() / 64;  // of 16 bytes
     pu32x4 w[LOADS];
-    __device__ __forceinline__ void load(const uint8_t* row, int g)  // row: the lane's token
+    // half: the half tile's place (uniform), at: the lane's token and g
+    __device__ __forceinline__ void load(const uint8_t* half, uint32_t at)
     {
 #pragma unroll
-        for (int i = 0; i < LOADS; i++) w[i] = *(const pu32x4*)(row + i * 64 + g * 16);
+        for (int i = 0; i < LOADS; i++) w[i] = *(const pu32x4*)(half + at + i * 64);
     }
     __device__ __forceinline__ pbf16x8 frag(int f) const  // not F32
     {
@@ -73,9 +74,10 @@ struct Values {
     static constexpr int DV = D / 16;
     static constexpr int WORDS = DV * ct_size<CT>() / 4;  // of one token
     uint32_t w[8][WORDS];
-    __device__ __forceinline__ void load(int x, const uint8_t* row, int n)
+    // half: the half tile's place (uniform), at: the lane's token and dimensions
+    __device__ __forceinline__ void load(int x, const uint8_t* half, uint32_t at)
     {
-        const uint8_t* p = row + n * DV * ct_size<CT>();
+        const uint8_t* p = half + at;
         if constexpr (WORDS >= 4) {
 #pragma unroll
             for (int i = 0; i < WORDS / 4; i++) {
@@ -91,10 +93,10 @@ struct Values {
             w[x][0] = *(const uint32_t*)p;
         }
     }
-    __device__ __forceinline__ void clear(int x)
+    __device__ __forceinline__ void keep(int x, bool it)
     {
 #pragma unroll
-        for (int i = 0; i < WORDS; i++) w[x][i] = 0;
+        for (int i = 0; i < WORDS; i++) w[x][i] = it ? w[x][i] : 0u;
     }
     // bf16 pair of dimensions 2 i, 2 i + 1 of token x (not F32)
     __device__ __forceinline__ uint32_t pair(int x, int i) const
@@ -212,62 +214,86 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
     const uint8_t* const kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
     const uint8_t* const vp = (const uint8_t*)p.v + (uint64_t)kvh * p.head_stride * ES;
     const int32_t* const table = p.b.table + (uint64_t)seq * p.b.table_stride;
-    const uint64_t page_bytes = p.page_stride * ES, token_bytes = p.token_stride * ES;
+    const uint64_t page_bytes = p.page_stride * ES;
+    const uint32_t token_bytes = (uint32_t)(p.token_stride * ES);  // a page's tokens span less than 2^31 bytes
+    const uint32_t k_at = c * token_bytes + g * 16, v_at = 4 * g * token_bytes + c * DV * ES;
 
-    // a half tile's place in the pages (elements from the head's start); false
-    // where it needs a page that is none. Halves that no row sees read page 0
-    // unlooked at: they are masked.
-    bool fault = false;
-    const auto place = [&](int t0) -> uint64_t {
-        if (!seen.any(t0, t0 + 16)) return 0;
-        const uint32_t id = (uint32_t)table[t0 >> p.b.page_shift];
-        if (id >= p.b.n_pages) {
-            fault = true;
-            return 0;
+    // q as B fragments for LDS, in the keys' order of dimensions: fragment f of
+    // column block n by wave (n QF + f) % WAVES
+    constexpr int QX = (NB * QF + WAVES - 1) / WAVES;  // of a wave
+    pu32x4 qa[QX], qz[QX];
+#pragma unroll
+    for (int i = 0; i < QX; i++) {
+        const int x = i * WAVES + wave, n = x / QF, f = x % QF, col = cb * COLS + 16 * n + c;
+        qa[i] = qz[i] = (pu32x4){};
+        if (x < NB * QF && col < cols) {
+            const uint64_t q_at = (uint64_t)(sq.a + col / p.group) * p.q_row +
+                                  (uint64_t)(kvh * p.group + col % p.group) * D + key_dim<CT>(f, g);
+            if constexpr (QF32) {
+                qa[i] = *(const pu32x4*)((const float*)p.q + q_at);
+                if (!F32MM) qz[i] = *(const pu32x4*)((const float*)p.q + q_at + 4);
+            } else {
+                qa[i] = *(const pu32x4*)((const uint16_t*)p.q + q_at);
+            }
         }
-        return (uint64_t)id * page_bytes + (uint64_t)(t0 & (p.b.page_size - 1)) * token_bytes;
+    }
+
+    // The places in the pages of the wave's next 32 tiles, a half tile a lane:
+    // lane i has half i % 2 of tile v + WAVES * (i / 2). Halves that no row
+    // sees read page 0 unlooked at: they are masked. (Looked up tile by tile,
+    // every lookup waited for all the loads before it: 66 us instead of 55 for
+    // 131072 tokens of E4M3, 32 / 8 heads.)
+    bool fault = false;
+    uint32_t place_lo = 0, place_hi = 0;
+    const auto look_up = [&](int v) {
+        v += WAVES * (lane / 2);
+        const int t0 = seen.tile(v) * TILE + 16 * (lane % 2);
+        uint64_t at = 0;
+        if (v < v1 && seen.any(t0, t0 + 16)) {
+            const uint32_t id = (uint32_t)table[t0 >> p.b.page_shift];
+            if (id >= p.b.n_pages) fault = true;
+            else at = (uint64_t)id * page_bytes + (uint64_t)((t0 & (p.b.page_size - 1)) * token_bytes);
+        }
+        place_lo = (uint32_t)at;
+        place_hi = (uint32_t)(at >> 32);
+    };
+    const auto place = [&](int tile, int half) -> uint64_t {
+        const int i = 2 * tile + half;
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place_hi, i) << 32 |
+               (uint32_t)__builtin_amdgcn_readlane((int)place_lo, i);
     };
 
     Keys<D, CT> K[2];
     Values<D, CT> V;
-    int vt = v0 + wave;
+    int vt = v0 + wave, turn = 0;
     uint64_t at[2] = {0, 0};
     if (vt < v1) {
-        const int t0 = seen.tile(vt) * TILE;
+        look_up(vt);
 #pragma unroll
-        for (int h = 0; h < 2; h++) at[h] = place(t0 + 16 * h);
+        for (int h = 0; h < 2; h++) {
+            at[h] = place(0, h);
+            K[h].load(kp + at[h], k_at);
+        }
 #pragma unroll
-        for (int h = 0; h < 2; h++) K[h].load(kp + at[h] + (uint64_t)c * token_bytes, g);
+        for (int x = 0; x < 8; x++) V.load(x, vp + at[x / 4], v_at + (x % 4) * token_bytes);
     }
-
-    // q as B fragments in LDS, in the keys' order of dimensions: fragment f of
-    // column block n by wave (n QF + f) % WAVES
 #pragma unroll
-    for (int x = 0; x < NB * QF; x++) {
-        if (x % WAVES != wave) continue;
-        const int n = x / QF, f = x % QF, col = cb * COLS + 16 * n + c;
-        const bool live = col < cols;
-        const uint64_t q_at = live ? (uint64_t)(sq.a + col / p.group) * p.q_row +
-                                         (uint64_t)(kvh * p.group + col % p.group) * D + key_dim<CT>(f, g) : 0;
-        if constexpr (F32MM) {
-            s_q[n][f][0][lane] = live ? *(const pu32x4*)((const float*)p.q + q_at) : (pu32x4){};
-        } else if constexpr (QF32) {
-            pf32x4 a = {}, b = {};
-            if (live) {
-                a = *(const pf32x4*)((const float*)p.q + q_at);
-                b = *(const pf32x4*)((const float*)p.q + q_at + 4);
-            }
+    for (int i = 0; i < QX; i++) {
+        const int x = i * WAVES + wave, n = x / QF, f = x % QF;
+        if (x >= NB * QF) break;
+        if constexpr (QF32 && !F32MM) {
             uint32_t t[4][3];
-            split3(a[0], a[1], t[0]);
-            split3(a[2], a[3], t[1]);
-            split3(b[0], b[1], t[2]);
-            split3(b[2], b[3], t[3]);
+            split3(__uint_as_float(qa[i][0]), __uint_as_float(qa[i][1]), t[0]);
+            split3(__uint_as_float(qa[i][2]), __uint_as_float(qa[i][3]), t[1]);
+            split3(__uint_as_float(qz[i][0]), __uint_as_float(qz[i][1]), t[2]);
+            split3(__uint_as_float(qz[i][2]), __uint_as_float(qz[i][3]), t[3]);
 #pragma unroll
             for (int k = 0; k < 3; k++) s_q[n][f][k][lane] = (pu32x4){t[0][k], t[1][k], t[2][k], t[3][k]};
         } else {
-            s_q[n][f][0][lane] = live ? *(const pu32x4*)((const uint16_t*)p.q + q_at) : (pu32x4){};
+            s_q[n][f][0][lane] = qa[i];
         }
     }
+
     const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
     __syncthreads();
 
@@ -280,16 +306,11 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
     }
     for (; vt < v1; vt += WAVES) {
         const int t0 = seen.tile(vt) * TILE;
-#pragma unroll
-        for (int x = 0; x < 8; x++)
-            V.load(x, vp + at[x / 4] + (uint64_t)(4 * g + x % 4) * token_bytes, c);
-        uint64_t next[2] = {0, 0};
-        if (vt + WAVES < v1) {
-            const int t1 = seen.tile(vt + WAVES) * TILE;
-            next[0] = place(t1);
-            next[1] = place(t1 + 16);
-        }
-        asm volatile("" ::: "memory");  // q's fragments are read again, not kept in registers
+        const bool more = vt + WAVES < v1;
+        turn = (turn + 1) % 32;
+        if (turn == 0 && more) look_up(vt + WAVES);
+        int again = lane;  // q's fragments are read anew, not kept in registers
+        asm volatile("" : "+v"(again));
         // scores
         pf32x4 s[NB][2] = {};
 #pragma unroll
@@ -297,7 +318,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
             if constexpr (F32MM) {
 #pragma unroll
                 for (int f = 0; f < QF; f++) {
-                    const pf32x4 q = __builtin_bit_cast(pf32x4, s_q[n][f][0][lane]);
+                    const pf32x4 q = __builtin_bit_cast(pf32x4, s_q[n][f][0][again]);
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -310,19 +331,20 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
                 for (int k = NT - 1; k >= 0; k--)  // small terms first
 #pragma unroll
                     for (int f = 0; f < QF; f++) {
-                        const pbf16x8 q = __builtin_bit_cast(pbf16x8, s_q[n][f][k][lane]);
+                        const pbf16x8 q = __builtin_bit_cast(pbf16x8, s_q[n][f][k][again]);
 #pragma unroll
                         for (int h = 0; h < 2; h++)
                             s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(K[h].frag(f), q, s[n][h], 0, 0, 0);
                     }
             }
         }
-        if (vt + WAVES < v1) {
+        // the next keys; behind the last tile, one address for all lanes, so
+        // that the number of loads in flight is known at every wait
 #pragma unroll
-            for (int h = 0; h < 2; h++) K[h].load(kp + next[h] + (uint64_t)c * token_bytes, g);
+        for (int h = 0; h < 2; h++) {
+            at[h] = more ? place(turn, h) : 0;
+            K[h].load(kp + at[h], more ? k_at : 0);
         }
-        at[0] = next[0];
-        at[1] = next[1];
         // mask
         const bool whole = t0 + TILE <= all_hi && t0 >= all_lo;
         if (!whole) {
@@ -363,7 +385,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
         if (!whole) {
 #pragma unroll
             for (int x = 0; x < 8; x++)
-                if (!seen.some(t0 + 16 * (x / 4) + 4 * g + x % 4)) V.clear(x);
+                V.keep(x, seen.some(t0 + 16 * (x / 4) + 4 * g + x % 4));
             odd = __any(V.odd());
         }
         if constexpr (F32MM) {
@@ -440,6 +462,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
                 add_values<D, CT, NB, NT, false>(V, b, acc, see);
             }
         }
+#pragma unroll
+        for (int x = 0; x < 8; x++)
+            V.load(x, vp + at[x / 4], more ? v_at + (x % 4) * token_bytes : 0);
     }
 
     // the waves' parts together; a lane's outputs are dimensions
@@ -570,16 +595,32 @@ __global__ __launch_bounds__(256) void k_attn_join(PagedAttnArgs p)
         const int n = max(1, (tiles + p.chunk - 1) / p.chunk);
         const uint64_t slot0 = (uint64_t)(sq.a + row) * p.n_heads + head;
         const uint64_t step = (uint64_t)p.b.n_rows * p.n_heads;
-        for (int i = part; i < n; i += PAR) m = fmaxf(m, p.part_ml[(slot0 + i * step) * 2]);
-        const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll 4
-        for (int i = part; i < n; i += PAR) {
-            const uint64_t slot = slot0 + i * step;
-            const float f = exp2_fast(p.part_ml[slot * 2] - base);
-            const float li = p.part_ml[slot * 2 + 1];
-            const pf32x4 oi = *(const pf32x4*)(p.part_o + slot * D + d);
-            l += f == 0.0f && li == li ? 0.0f : li * f;
-            if (f != 0.0f) o += oi * f;
+        // eight chunks' states in flight at a time
+        for (int i0 = part; i0 < n; i0 += 8 * PAR) {
+            float mi[8], li[8];
+            pf32x4 oi[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int i = i0 + j * PAR;
+                const uint64_t slot = slot0 + (uint64_t)(i < n ? i : part) * step;
+                mi[j] = i < n ? p.part_ml[slot * 2] : -INFINITY;
+                li[j] = i < n ? p.part_ml[slot * 2 + 1] : 0.0f;
+                oi[j] = *(const pf32x4*)(p.part_o + slot * D + d);
+            }
+            float now = m;
+#pragma unroll
+            for (int j = 0; j < 8; j++) now = fmaxf(now, mi[j]);
+            const float base = now == -INFINITY ? 0.0f : now;
+            const float old = exp2_fast(m - base);
+            l *= old;
+            o *= old;
+            m = now;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float f = exp2_fast(mi[j] - base);
+                l += f == 0.0f && li[j] == li[j] ? 0.0f : li[j] * f;
+                if (f != 0.0f) o += oi[j] * f;
+            }
         }
     }
     if constexpr (PAR > 1) {

@@ -61,6 +61,8 @@ int check_pages(const wpcg_kv_pages* kv, Pages* s)
         if (x * es % 16 != 0) return fail(WPCG_E_SHAPE, "a page stride is not a multiple of 16 bytes");
         if (x >> 40) return fail(WPCG_E_ARG, "a page stride is too large");
     }
+    // (a token's place in its page is a 32-bit offset in the kernels)
+    if (s->token * es * kv->page_size >> 31) return fail(WPCG_E_ARG, "a page stride is too large");
     return WPCG_OK;
 }
 
@@ -123,7 +125,7 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
         tiles = std::min(tiles, seen);
     }
     const int64_t base = (int64_t)b.n_seq * kv->n_kv_heads * blocks;
-    const int64_t target = 512, least = p.many ? 8 : 2 * ATTN_FEW_WAVES;
+    const int64_t target = p.many ? 512 : 256, least = p.many ? 8 : 2 * ATTN_FEW_WAVES;
     int64_t chunk = tiles;
     if (base > 0 && base < target) {
         const int64_t want = (target + base - 1) / base;
