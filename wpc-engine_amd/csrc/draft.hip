@@ -14,9 +14,7 @@
 // the drafter's row), so memory bounds a batch, and launch latency a single
 // sequence. Exponentials, sums and comparisons are fp64: a draft that is as
 // good as its target leaves differences p - q far below p, and the running
-// sums of 10^5 weights decide which id they pass at. The exponential is the
-// Taylor polynomial of degree 10 on +-ln(2)/2 (next term 2.2e-13), times a
-// power of two.
+// sums of 10^5 weights decide which id they pass at.
 #include "paged.h"
 #include "wave.h"
 
@@ -26,23 +24,26 @@ namespace {
 constexpr int THREADS = 256, CHUNK = DRAFT_CHUNK;
 static_assert(CHUNK == 8 * THREADS, "pick: eight ids a thread");
 
-// 2^y; 0 below the normal numbers, NaN for NaN
+// 2^y for y <= 0 (or NaN): y = n + f, n the whole number that adding 1.5 * 2^52
+// leaves in the low bits, the polynomial of degree 8 through 2^f at the nine
+// Chebyshev points of +-1/2 (within 1.1e-12 of it there), n added to its
+// exponent. 0 below 2^-1000.
 __device__ __forceinline__ double exp2_d(double y)
 {
-    const double n = rint(y);
-    const double z = (y - n) * 0.6931471805599453;
-    double r = 1.0 / 3628800;
-    r = fma(r, z, 1.0 / 362880);
-    r = fma(r, z, 1.0 / 40320);
-    r = fma(r, z, 1.0 / 5040);
-    r = fma(r, z, 1.0 / 720);
-    r = fma(r, z, 1.0 / 120);
-    r = fma(r, z, 1.0 / 24);
-    r = fma(r, z, 1.0 / 6);
-    r = fma(r, z, 0.5);
-    r = fma(r, z, 1.0);
-    r = fma(r, z, 1.0);
-    return y < -1000.0 ? 0.0 : ldexp(r, (int)n);
+    const double t = y + 6755399441055744.0;
+    const double f = y - (t - 6755399441055744.0);
+    double r = 1.3255224878668817e-06;
+    r = fma(r, f, 1.5310079402249296e-05);
+    r = fma(r, f, 0.00015403455852453838);
+    r = fma(r, f, 0.0013333450568000645);
+    r = fma(r, f, 0.009618129159402558);
+    r = fma(r, f, 0.05550410941205933);
+    r = fma(r, f, 0.2402265069581299);
+    r = fma(r, f, 0.6931471805459335);
+    r = fma(r, f, 1.0);
+    const uint64_t n = (uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, t) << 52;
+    r = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, r) + n);
+    return y < -1000.0 ? 0.0 : r;
 }
 
 struct Rows {
@@ -119,17 +120,21 @@ struct Chunk {
     __device__ __forceinline__ void load(const float* x, int c0, int vocab, bool vec, float none)
     {
         const int lane = (int)threadIdx.x & 63;
+        // one way for the whole wave, and no load behind a condition: a lane
+        // that skips one would have to wait for those before it
+        if (vec && c0 + CHUNK <= vocab) {
 #pragma unroll
-        for (int i = 0; i < CHUNK / 256; i++) {
-            const int at = c0 + 256 * i + 4 * lane;
-            if (vec && at + 4 <= vocab) {
-                const pf32x4 w = *(const pf32x4*)(x + at);
+            for (int i = 0; i < CHUNK / 256; i++) {
+                const pf32x4 w = *(const pf32x4*)(x + c0 + 256 * i + 4 * lane);
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[4 * i + j] = w[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[4 * i + j] = at + j < vocab ? x[at + j] : none;
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CHUNK / 64; i++) v[i] = x[min(c0 + 256 * (i / 4) + 4 * lane + i % 4, vocab - 1)];
+#pragma unroll
+            for (int i = 0; i < CHUNK / 64; i++)
+                if (c0 + 256 * (i / 4) + 4 * lane + i % 4 >= vocab) v[i] = none;
         }
     }
 };
@@ -140,16 +145,16 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
     const int row = (int)(blockIdx.x / (unsigned)groups);
     const int chunk = (int)(blockIdx.x % (unsigned)groups) * 4 + ((int)threadIdx.x >> 6);
     const int lane = (int)threadIdx.x & 63;
+    if (chunk >= p.chunks) return;
+    // the values are on their way while the row's sequence is looked for
+    Chunk c;
+    c.load(p.logits + (uint64_t)row * p.logits_row, chunk * CHUNK, p.vocab, p.vec, -INFINITY);
     const int s = draft_seq(p, row);
     if (s >= p.n_seq) return;
     const Rows q = draft_rows(p, s);
     if (row < q.a || row >= q.a + q.n) return;
     if (row == q.a && chunk == 0 && lane == 0) p.done[s].done = 0;
-    if (chunk >= p.chunks) return;
     const double rate = draft_rate(p, s);
-    const float* x = p.logits + (uint64_t)row * p.logits_row;
-    Chunk c;
-    c.load(x, chunk * CHUNK, p.vocab, p.vec, -INFINITY);
     float best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < CHUNK / 64; i++) best = fmaxf(best, c.v[i]);
@@ -157,9 +162,9 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
     int at = 0x7fffffff;
     double sum = 0.0;
     if (rate > 0.0) {
-        const double base = best == -INFINITY ? 0.0 : (double)best;
+        const double base = best == -INFINITY ? 0.0 : -(double)best * rate;
 #pragma unroll
-        for (int i = 0; i < CHUNK / 64; i++) sum += exp2_d(((double)c.v[i] - base) * rate);
+        for (int i = 0; i < CHUNK / 64; i++) sum += exp2_d(fma((double)c.v[i], rate, base));
         sum = wave_sum_d(sum);
     } else {
 #pragma unroll
@@ -171,8 +176,8 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
     if (lane == 0) p.part[(uint64_t)row * p.chunks + chunk] = DraftPart{sum, best, best == -INFINITY ? 0x7fffffff : at};
 }
 
-// M and Z of a row (Z = sum of 2^((x - M) rate)), by a wave; at: the first
-// largest logit
+// M and Z of a row (Z = sum of 2^((x - M) rate)), by 32 lanes; at: the first
+// largest logit (greedy)
 struct RowState {
     double z;
     float m;
@@ -180,22 +185,38 @@ struct RowState {
 };
 __device__ __forceinline__ RowState row_state(const DraftArgs& p, int row, double rate)
 {
+    constexpr int AHEAD = 4;  // states in flight
     const DraftPart* part = p.part + (uint64_t)row * p.chunks;
+    const int l = (int)threadIdx.x & 31;
     float m = -INFINITY;
     int at = 0x7fffffff;
-    for (int i = (int)threadIdx.x & 63; i < p.chunks; i += 64) larger(m, at, part[i].max, part[i].at);
+    double z = 0.0;
+    for (int i0 = l; i0 < p.chunks; i0 += 32 * AHEAD) {
+        DraftPart c[AHEAD];
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
+        for (int j = 0; j < AHEAD; j++) c[j] = part[min(i0 + 32 * j, p.chunks - 1)];
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++)
+            if (i0 + 32 * j >= p.chunks) c[j] = DraftPart{0.0, -INFINITY, 0x7fffffff};
+        const float old = m;
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) larger(m, at, c[j].max, c[j].at);
+        const auto to_m = [&](float v) { return v == -INFINITY ? 1.0 : exp2_d(((double)v - (double)m) * rate); };
+        z *= to_m(old);
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) z += c[j].sum * to_m(c[j].max);
+    }
+    const float mine = m;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
         const float v = __shfl_xor(m, d);
         const int j = __shfl_xor(at, d);
         larger(m, at, v, j);
     }
-    double z = 0.0;
-    for (int i = (int)threadIdx.x & 63; i < p.chunks; i += 64) {
-        const float v = part[i].max;
-        z += part[i].sum * (v == -INFINITY ? 1.0 : exp2_d(((double)v - (double)m) * rate));
-    }
-    return {wave_sum_d(z), m, at};
+    z *= mine == -INFINITY ? 1.0 : exp2_d(((double)mine - (double)m) * rate);
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) z += __shfl_xor(z, d);
+    return {z, m, at};
 }
 
 // The row that a sequence's next token comes from.
@@ -206,22 +227,21 @@ struct Choice {
 };
 __device__ __forceinline__ Choice choose(const DraftArgs& p, int s, const Rows& q, double rate, RowState* s_st, int* s_ok)
 {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    for (int i = wave; i < q.n; i += 4) {
-        const RowState st = row_state(p, q.a + i, rate);
+    // half a wave a row, so that the first eight rows' loads go out together
+    for (int i = (int)threadIdx.x / 32; i < q.n; i += THREADS / 32) {
+        const uint64_t r = (uint64_t)(q.a + i);
+        const bool drafted = i + 1 < q.n;
+        const uint32_t d = p.tokens[drafted ? r + 1 : r];
+        const float u = drafted ? p.u[r] : 0.0f;
+        const bool inside = drafted && d < (uint32_t)p.vocab;
+        const uint64_t at = inside ? d : 0;
+        const float x = p.logits[r * p.logits_row + at];
+        const float w = p.probs && drafted ? p.probs[r * p.probs_row + at] : 1.0f;
+        const RowState st = row_state(p, (int)r, rate);
         int ok = 0;
-        if (i + 1 < q.n) {
-            const uint32_t d = p.tokens[q.a + i + 1];
-            if (rate == 0.0) {
-                ok = st.m > -INFINITY && d == (uint32_t)st.at;
-            } else if (d < (uint32_t)p.vocab) {
-                const uint64_t r = (uint64_t)(q.a + i);
-                const double e = exp2_d(((double)p.logits[r * p.logits_row + d] - (double)st.m) * rate);
-                const double w = p.probs ? (double)p.probs[r * p.probs_row + d] : 1.0;
-                ok = (double)p.u[q.a + i] * w < e / st.z;
-            }
-        }
-        if (lane == 0) {
+        if (rate == 0.0) ok = drafted && st.m > -INFINITY && d == (uint32_t)st.at;
+        else if (inside) ok = (double)u * (double)w < exp2_d(((double)x - (double)st.m) * rate) / st.z;
+        if ((threadIdx.x & 31) == 0) {
             s_st[i] = st;
             s_ok[i] = ok;
         }
@@ -238,7 +258,7 @@ __device__ __forceinline__ Choice choose(const DraftArgs& p, int s, const Rows& 
 // Z times an id's weight in the row, from its logit x and the drafter's q
 __device__ __forceinline__ double weight(float x, float q, const RowState& st, double rate, bool rest)
 {
-    const double e = exp2_d(((double)x - (double)st.m) * rate);
+    const double e = exp2_d(fma((double)x, rate, -(double)st.m * rate));
     if (!rest) return e;
     const double w = e - (double)q * st.z;
     return w > 0.0 || w != w ? w : 0.0;
@@ -262,6 +282,7 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
     __shared__ double s_s[4], s_before;
     __shared__ int s_at, s_id, s_last, s_last_id;
     const int tid = (int)threadIdx.x;
+    const double u = (double)p.u_next[s];
     bool rest = c.rest;
     const auto of_chunk = [&](int i) {
         if (rest) return __hip_atomic_load(&p.rest[(uint64_t)s * p.chunks + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -271,22 +292,22 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
     // a thread's run of chunks
     const int run = (p.chunks + THREADS - 1) / THREADS;
     const int j0 = min(tid * run, p.chunks), j1 = min(j0 + run, p.chunks);
-    double before, total;
+    double before, total, last = 0.0;
     for (int turn = 0; turn < 2; turn++) {
         double sum = 0.0;
-        for (int i = j0; i < j1; i++) sum += of_chunk(i);
+        for (int i = j0; i < j1; i++) sum += last = of_chunk(i);
         before = block_before(sum, s_s, total);
         if (total > 0.0 || !rest) break;
         rest = false;  // nothing is left of p - q: the row's own weights
     }
-    const double want = (double)p.u_next[s] * total;
+    const double want = u * total;
     if (tid == 0) {
         s_at = s_id = 0x7fffffff;
         s_last = s_last_id = -1;
     }
     __syncthreads();
     for (int i = j0; i < j1; i++) {
-        const double w = of_chunk(i);
+        const double w = run == 1 ? last : of_chunk(i);
         if (w > 0.0) atomicMax(&s_last, i);  // of use where rounding leaves none
         if (before + w > want) {
             atomicMin(&s_at, i);
@@ -302,27 +323,30 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
     // ids 8 t .. 8 t + 7 of the chunk
     const int i0 = chunk * CHUNK + 8 * tid;
     double w[8], sum = 0.0, all;
+    float x[8], q[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const int i = i0 + j;
-        w[j] = 0.0;
-        if (i < p.vocab) {
-            const float q = p.probs ? (rest ? p.probs[(uint64_t)row * p.probs_row + i] : 0.0f) : i == draft ? 1.0f : 0.0f;
-            w[j] = weight(p.logits[(uint64_t)row * p.logits_row + i], q, c.st, rate, rest);
-        }
+        const uint64_t i = (uint64_t)min(i0 + j, p.vocab - 1);
+        x[j] = p.logits[(uint64_t)row * p.logits_row + i];
+        q[j] = p.probs && rest ? p.probs[(uint64_t)row * p.probs_row + i] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        if (!p.probs && i0 + j == draft) q[j] = 1.0f;
+        w[j] = i0 + j < p.vocab ? weight(x[j], q[j], c.st, rate, rest) : 0.0;
         sum += w[j];
     }
     double t = block_before(sum, s_s, all);
     t += s_before;
-    int first = 0x7fffffff, last = -1;
+    int first = 0x7fffffff, final = -1;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         t += w[j];
-        if (w[j] > 0.0) last = i0 + j;
+        if (w[j] > 0.0) final = i0 + j;
         if (!end && t > want && first == 0x7fffffff) first = i0 + j;
     }
     if (first != 0x7fffffff) atomicMin(&s_id, first);
-    if (last >= 0) atomicMax(&s_last_id, last);
+    if (final >= 0) atomicMax(&s_last_id, final);
     __syncthreads();
     return s_id != 0x7fffffff ? s_id : s_last_id;
 }
@@ -343,6 +367,7 @@ __global__ __launch_bounds__(THREADS) void k_draft_choose(DraftArgs p)
     const double rate = draft_rate(p, s);
     const Choice c = choose(p, s, q, rate, s_st, s_ok);
     const int row = q.a + c.accepted, draft = c.rest ? (int)p.tokens[row + 1] : -1;
+    const int shown = tid < c.accepted ? (int)p.tokens[q.a + tid + 1] : -1;  // at most 64 rows
     int token = -1;
     if (rate == 0.0) {
         if (group != 0) return;
@@ -360,16 +385,22 @@ __global__ __launch_bounds__(THREADS) void k_draft_choose(DraftArgs p)
 #pragma unroll
                 for (int i = 0; i < CHUNK / 64; i++) sum += weight(x.v[i], r.v[i], c.st, rate, true);
                 sum = wave_sum_d(sum);
-                if ((tid & 63) == 0)
-                    __hip_atomic_store(&p.rest[(uint64_t)s * p.chunks + chunk], sum, __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT);
+                // Handed over by an exchange, which is performed at the
+                // device's coherence point and returns only then; the empty
+                // asm waits for it. So every part of this workgroup is there
+                // before its count, and the last one's coherent loads find
+                // them; no cache is written back or invalidated for it.
+                if ((tid & 63) == 0) {
+                    const uint64_t was = __hip_atomic_exchange((uint64_t*)p.rest + (uint64_t)s * p.chunks + chunk,
+                                                               __builtin_bit_cast(uint64_t, sum), __ATOMIC_RELAXED,
+                                                               __HIP_MEMORY_SCOPE_AGENT);
+                    asm volatile("" ::"v"(was));
+                }
             }
             // the last of the sequence's workgroups goes on
             __syncthreads();
-            if (tid == 0) {
-                __threadfence();
-                s_done = __hip_atomic_fetch_add(&p.done[s].done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-            }
+            if (tid == 0)
+                s_done = __hip_atomic_fetch_add(&p.done[s].done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (s_done != groups - 1) return;
         } else if (group != 0) {
@@ -377,8 +408,7 @@ __global__ __launch_bounds__(THREADS) void k_draft_choose(DraftArgs p)
         }
         token = pick(p, s, row, c, rate, draft);
     }
-    for (int i = tid; i < q.n; i += THREADS)
-        p.out[q.a + i] = i < c.accepted ? (int)p.tokens[q.a + i + 1] : i == c.accepted ? token : -1;
+    if (tid < q.n) p.out[q.a + tid] = tid == c.accepted ? token : shown;
     if (tid == 0) p.accepted[s] = c.accepted;
 }
 
