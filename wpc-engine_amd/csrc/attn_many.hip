@@ -15,9 +15,8 @@
 // is the second product's B operand as it stands if V^T's A operand takes its
 // tokens in the same order. So the softmax's terms stay in their lane, the
 // maximum needs one lane exchange, and the rescaling factor is one number a
-// lane. Keys go to LDS in 16-byte pieces [8 dimensions][token], the token
-// index XORed with the piece's so that neither the writes (along a row) nor
-// the reads (along tokens) meet in a bank; values are transposed in registers
+// lane. Keys go to LDS in rows padded by 16 bytes, so that neither the writes
+// (along a row) nor the reads (along tokens) meet in a bank; values are transposed in registers
 // by byte permutes on their way to LDS and lie in the order the operand is
 // read, 1 KiB a wave without conflicts. The next tile's loads are in flight
 // during the products.
@@ -41,7 +40,7 @@ struct Shape {
     static constexpr int NBUF = NK == 1 ? 2 : 1;     // tiles in LDS
     static constexpr int CW = CT == CT_F32 ? 4 : 8;  // dimensions of a value load
     static constexpr int NCH = D / CW;
-    static constexpr int PLANE = TILE * D;           // bf16 elements of one term of a tile
+    static constexpr int KEYS = TILE * (D + 8), VALUES = TILE * D;  // bf16 elements of one term of a tile in LDS
     static constexpr int KT = 16 * (D / 8) / 64;     // key pieces of a lane and tile
     static constexpr int VT = (4 * NCH + 63) / 64;   // value pieces (4 tokens) of a lane and tile
 };
@@ -56,8 +55,9 @@ struct Carried {
     uint32_t v[S::VT][4][VW];
 };
 template <int W>
-__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p)
+__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* base, uint32_t at)  // base: uniform
 {
+    const uint8_t* p = base + at;
     if constexpr (W >= 4) {
 #pragma unroll
         for (int i = 0; i < W; i += 4) {
@@ -73,8 +73,20 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p)
     }
 }
 
-// Place of the 16-byte piece (dimensions 8c .. 8c+7, token t) of a tile's keys.
-__device__ __forceinline__ int key_at(int c, int t) { return (c * TILE + (t ^ (c & 15))) * 8; }
+// Whether a word of a cache holds a value that is not finite.
+template <int CT>
+__device__ __forceinline__ bool word_odd(uint32_t w)
+{
+    if constexpr (CT == CT_F32) return (w & 0x7f800000u) == 0x7f800000u;
+    else if constexpr (CT == CT_BF16) return bf16_odd(w);
+    else return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;  // NaN alone: 0x7f
+}
+
+// Place of the 16-byte piece (dimensions 8c .. 8c+7, token t) of a tile's keys:
+// rows of D + 8 elements, an odd number of pieces, so that sixteen tokens'
+// pieces lie in different banks, and every read is one base and a constant.
+template <int D>
+__device__ __forceinline__ int key_at(int c, int t) { return t * (D + 8) + c * 8; }
 // Place of slot (h, p) of 16-token group j of its values: the eight tokens
 // 16j + 4h + 0..3 and 16j + 8 + 4h + 0..3 of dimension CW * (p % NCH) + p / NCH.
 template <int D>
@@ -104,8 +116,8 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
     using S = Shape<D, CT, QF32>;
     constexpr int ES = ct_size<CT>();
     constexpr int CW = S::CW, NCH = S::NCH;
-    __shared__ __attribute__((aligned(16))) uint16_t s_k[S::NBUF][S::NK][S::PLANE];
-    __shared__ __attribute__((aligned(16))) uint16_t s_v[S::NBUF][S::NK][S::PLANE];
+    __shared__ __attribute__((aligned(16))) uint16_t s_k[S::NBUF][S::NK][S::KEYS];
+    __shared__ __attribute__((aligned(16))) uint16_t s_v[S::NBUF][S::NK][S::VALUES];
     __shared__ int s_odd[S::NBUF][WAVES], s_fault[WAVES];
 
     // block -> (column block, chunk, sequence and head): the blocks of a head
@@ -172,23 +184,35 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
     const uint8_t* const kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
     const uint8_t* const vp = (const uint8_t*)p.v + (uint64_t)kvh * p.head_stride * ES;
     const int32_t* const table = p.b.table + (uint64_t)seq * p.b.table_stride;
-    const uint64_t page_bytes = p.page_stride * ES, token_bytes = p.token_stride * ES;
+    const uint64_t page_bytes = p.page_stride * ES;
+    const uint32_t token_bytes = (uint32_t)(p.token_stride * ES);  // a page's tokens span less than 2^31 bytes
     bool fault = false;
 
-    // wave w brings in tokens 16 w .. 16 w + 15 of a tile
+    // wave w brings in tokens 16 w .. 16 w + 15 of a tile. Their places in the
+    // pages are looked up 64 tiles at a time, a tile a lane; where no row sees
+    // them page 0 is read unlooked at.
     Carried<D, CT> in;
-    const auto fetch = [&](int vt) {
-        const int t0 = __builtin_amdgcn_readfirstlane(seen.tile(vt) * TILE + 16 * wave);
+    uint32_t place_lo = 0, place_hi = 0;
+    const auto look_up = [&](int vt) {
+        const int t0 = seen.tile(vt + lane) * TILE + 16 * wave;
         uint64_t at = 0;
-        if (seen.any(t0, t0 + 16)) {
+        if (vt + lane < v1 && seen.any(t0, t0 + 16)) {
             const uint32_t id = (uint32_t)table[t0 >> p.b.page_shift];
             if (id >= p.b.n_pages) fault = true;
-            else at = (uint64_t)id * page_bytes + (uint64_t)(t0 & (p.b.page_size - 1)) * token_bytes;
+            else at = (uint64_t)id * page_bytes + (uint64_t)((t0 & (p.b.page_size - 1)) * token_bytes);
         }
+        place_lo = (uint32_t)at;
+        place_hi = (uint32_t)(at >> 32);
+    };
+    const auto fetch = [&](int vt) {
+        const int turn = (vt - v0) % 64;
+        if (turn == 0) look_up(vt);
+        const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place_hi, turn) << 32 |
+                            (uint32_t)__builtin_amdgcn_readlane((int)place_lo, turn);
 #pragma unroll
         for (int i = 0; i < S::KT; i++) {
             const int x = lane + 64 * i;
-            load_words(in.k[i], kp + at + (uint64_t)(x / (D / 8)) * token_bytes + x % (D / 8) * 8 * ES);
+            load_words(in.k[i], kp + at, x / (D / 8) * token_bytes + x % (D / 8) * 8 * ES);
         }
 #pragma unroll
         for (int i = 0; i < S::VT; i++) {
@@ -197,7 +221,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
                 const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
 #pragma unroll
                 for (int y = 0; y < 4; y++)
-                    load_words(in.v[i][y], vp + at + (uint64_t)(8 * xh + 4 * vh + y) * token_bytes + n * CW * ES);
+                    load_words(in.v[i][y], vp + at, (8 * xh + 4 * vh + y) * token_bytes + n * CW * ES);
             }
         }
     };
@@ -207,7 +231,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
 #pragma unroll
         for (int i = 0; i < S::KT; i++) {
             const int x = lane + 64 * i;
-            const int at = key_at(x % (D / 8), 16 * wave + x / (D / 8));
+            const int at = key_at<D>(x % (D / 8), 16 * wave + x / (D / 8));
             if constexpr (CT == CT_F32) {
                 uint32_t t[4][3];
 #pragma unroll
@@ -223,15 +247,29 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
                                                       e4m3_bf16<false>(in.k[i][1]), e4m3_bf16<true>(in.k[i][1])};
             }
         }
-        bool odd = false;
+        if (!whole) {  // tokens that no column sees hold anything
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < S::VT; i++) {
+                const int x = lane + 64 * i, xh = x / NCH % 2, vh = x / (2 * NCH);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const bool some = seen.some(t0 + 16 * wave + 8 * xh + 4 * vh + k);
+#pragma unroll
+                    for (int y = 0; y < Carried<D, CT>::VW; y++) {
+                        in.v[i][k][y] = some ? in.v[i][k][y] : 0u;
+                        odd |= word_odd<CT>(in.v[i][k][y]);
+                    }
+                }
+            }
+            odd = __any(odd && lane < 4 * NCH);
+            if (lane == 0) s_odd[buf][wave] = odd;
+        }
 #pragma unroll
         for (int i = 0; i < S::VT; i++) {
             const int x = lane + 64 * i;
             if (4 * NCH % 64 == 0 || x < 4 * NCH) {
                 const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
-                bool some[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) some[k] = whole || seen.some(t0 + 16 * wave + 8 * xh + 4 * vh + k);
 #pragma unroll
                 for (int y = 0; y < CW / 2; y++) {
                     // bf16 pairs of dimensions 2 y, 2 y + 1 of the four tokens
@@ -245,15 +283,6 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
                         else
                             t[k][0] = y % 2 ? e4m3_bf16<true>(in.v[i][k][y / 2]) : e4m3_bf16<false>(in.v[i][k][y / 2]);
                     }
-                    if (!whole) {  // tokens that no column sees hold anything
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-#pragma unroll
-                            for (int e = 0; e < S::NK; e++) {
-                                t[k][e] = some[k] ? t[k][e] : 0u;
-                                odd |= bf16_odd(t[k][e]);
-                            }
-                    }
 #pragma unroll
                     for (int e = 0; e < S::NK; e++) {
                         const pu32x2 lo = {__builtin_amdgcn_perm(t[1][e], t[0][e], 0x05040100u),
@@ -266,12 +295,13 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
                 }
             }
         }
-        odd = __any(odd);
-        if (lane == 0) s_odd[buf][wave] = odd;
     };
 
     pf32x16 acc[D / 32] = {};
     float m = -INFINITY, l = 0.0f;
+    // q is there: else its first use in the loop would wait, every time
+    // around, for all loads in flight
+    __builtin_amdgcn_s_waitcnt(0);
     if (v0 < v1) fetch(v0);
     for (int vt = v0; vt < v1; vt++) {
         const int buf = (vt - v0) % S::NBUF;
@@ -280,7 +310,8 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
         __syncthreads();
         if (vt + 1 < v1) fetch(vt + 1);
         const int t0 = seen.tile(vt) * TILE;
-        if (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3]) {
+        const bool all = t0 + TILE <= all_hi && t0 >= all_lo;  // every column sees every token
+        if (!all && (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3])) {
             // values that are not finite: added to the columns that see their
             // token (products with ones count the +inf, -inf and NaN a column
             // sees), and zeros for the products below
@@ -316,7 +347,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
                 }
             }
             __syncthreads();
-            for (int i = (int)threadIdx.x; i < S::NK * S::PLANE / 2; i += THREADS) {
+            for (int i = (int)threadIdx.x; i < S::NK * S::VALUES / 2; i += THREADS) {
                 uint32_t* w = (uint32_t*)&s_v[buf][0][0] + i;
                 *w = bf16_finite(*w);
             }
@@ -324,17 +355,38 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
         }
         if (!active || !wseen.any(t0, t0 + TILE)) continue;
 
+        // Operands come from LDS a group ahead of the products that take
+        // them: four fragments of keys (half a group's products hide the
+        // reads of the next), then a 16-token group's of the values.
+        constexpr int KG = 2 * D / 64, VF = D / 32;  // groups of keys, fragments of a group of values
+        pbf16x8 frag[2][4][S::NK];
+        const auto load_keys = [&](int x) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < S::NK; e++)
+                    frag[x & 1][i][e] =
+                        *(const pbf16x8*)&s_k[buf][e][key_at<D>(2 * (4 * x % (D / 16) + i) + h, 32 * (4 * x / (D / 16)) + c)];
+        };
+        const auto load_values = [&](int j) {
+#pragma unroll
+            for (int d = 0; d < VF; d++)
+#pragma unroll
+                for (int e = 0; e < S::NK; e++)
+                    frag[j & 1][d][e] = *(const pbf16x8*)&s_v[buf][e][value_at<D>(j, 0, 32 * d) + lane * 8];
+        };
         // scores of two 32-token halves
         pf32x16 s[2] = {};
+        load_keys(0);
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int x = 0; x < KG; x++) {
+            if (x + 1 < KG) load_keys(x + 1);
+            else load_values(0);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int f = 0; f < D / 16; f++) {
-                pbf16x8 k[S::NK];
-#pragma unroll
-                for (int e = 0; e < S::NK; e++) k[e] = *(const pbf16x8*)&s_k[buf][e][key_at(2 * f + h, 32 * u + c)];
-                s[u] = mul_terms(k, qb[f], s[u]);
-            }
+            for (int i = 0; i < 4; i++)
+                s[4 * x / (D / 16)] = mul_terms(frag[x & 1][i], qb[4 * x % (D / 16) + i], s[4 * x / (D / 16)]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         const bool whole = t0 + TILE <= w_hi && t0 >= w_lo;
         if (!whole) {
@@ -352,9 +404,11 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
         top = max_x32(top) * sc;
-        const float now = fmaxf(m, top);
-        const float base = now == -INFINITY ? 0.0f : now;
-        if (__any(now > m)) {
+        // The maximum is followed only when it has grown by more than 2^8:
+        // terms up to 256 are as exact, and the rescaling (an operation per
+        // output register) is seldom needed.
+        if (__any(top > m + 8.0f)) {
+            const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
             // (what a first tile's infinities left in acc is kept)
             const float f = m == -INFINITY ? 1.0f : exp2_fast(m - base);
             l *= f;
@@ -362,15 +416,14 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
             for (int d = 0; d < D / 32; d++) acc[d] *= f;
             m = now;
         }
-        pbf16x8 b[4][S::NQ];
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
+        const float base = m == -INFINITY ? 0.0f : m;
+        pbf16x8 b[2][S::NQ];
+        const auto terms = [&](int j) {
             float e[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 e[i] = exp2_fast(fmaf(s[j / 2][8 * (j % 2) + i], sc, -base));
-                sum += e[i];
+                l += e[i];
             }
             if constexpr (QF32) {
                 uint32_t t[4][3];
@@ -378,23 +431,26 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
                 for (int i = 0; i < 4; i++) split3(e[2 * i], e[2 * i + 1], t[i]);
 #pragma unroll
                 for (int n = 0; n < 3; n++)
-                    b[j][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
+                    b[j & 1][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
             } else {
-                b[j][0] = __builtin_bit_cast(pbf16x8, (pu32x4){pk_bf16_rne(e[0], e[1]), pk_bf16_rne(e[2], e[3]),
-                                                               pk_bf16_rne(e[4], e[5]), pk_bf16_rne(e[6], e[7])});
+                b[j & 1][0] = __builtin_bit_cast(pbf16x8, (pu32x4){pk_bf16_rne(e[0], e[1]), pk_bf16_rne(e[2], e[3]),
+                                                                   pk_bf16_rne(e[4], e[5]), pk_bf16_rne(e[6], e[7])});
             }
-        }
-        l += sum;
+        };
+        terms(0);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
+            if (j < 3) load_values(j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (j < 3) terms(j + 1);
 #pragma unroll
-            for (int d = 0; d < D / 32; d++) {
-                pbf16x8 v[S::NK];
-#pragma unroll
-                for (int e = 0; e < S::NK; e++)
-                    v[e] = *(const pbf16x8*)&s_v[buf][e][value_at<D>(j, 0, 32 * d) + lane * 8];
-                acc[d] = mul_terms(v, b[j], acc[d]);
+            for (int d = 0; d < VF; d++) {
+                acc[d] = mul_terms(frag[j & 1][d], b[j & 1], acc[d]);
+                // a product, then a share of the next group's exponentials
+                __builtin_amdgcn_sched_group_barrier(0x8, S::NK * S::NQ > 3 ? 6 : S::NQ, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, QF32 ? 24 : 7, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     if (lane == 0) s_fault[wave] = 0;
