@@ -29,9 +29,7 @@
 namespace wpcg {
 namespace {
 
-constexpr int WAVES = 4;
-constexpr int THREADS = 64 * WAVES;
-constexpr int TILE = ATTN_MANY_TILE, COLS = ATTN_MANY_COLS;
+constexpr int TILE = ATTN_MANY_TILE;
 
 template <int D, int CT, bool QF32>
 struct Shape {
@@ -95,6 +93,335 @@ __device__ __forceinline__ int value_at(int j, int h, int p)
     return ((j * (D / 32) + p / 32) * 64 + h * 32 + p % 32) * 8;
 }
 
+// What brings tiles from the pages to LDS, in registers on the way: of four
+// waves, wave w the tokens 16 w .. 16 w + 15, of eight the first four their
+// keys and the others their values. Their places in the pages are looked up 64
+// tiles at a time, a tile a lane; where no row sees them page 0 is read
+// unlooked at.
+template <int D, int CT, int WAVES>
+struct Stage {
+    using S = Shape<D, CT, true>;
+    static constexpr int ES = ct_size<CT>(), CW = S::CW, NCH = S::NCH, NK = S::NK;
+    Carried<D, CT> in;
+    SeenTiles<TILE> seen;  // of the block's columns
+    int v0, v1;            // its tiles
+    int all_hi, all_lo;    // tokens that every column sees
+    const uint8_t *kp, *vp;
+    const int32_t* table;
+    uint64_t page_bytes;
+    uint32_t token_bytes;  // a page's tokens span less than 2^31 bytes
+    uint32_t n_pages;
+    int page_shift, page_size;
+    int lane, wave;     // wave: which 16 tokens
+    bool keys, values;  // what this wave brings
+    uint32_t place_lo = 0, place_hi = 0;
+    bool fault = false;
+
+    __device__ __forceinline__ Stage(const PagedAttnArgs& p, int seq, int kvh, const SeenTiles<TILE>& s, int a, int b,
+                                     int hi, int lo)
+        : seen(s), v0(a), v1(b), all_hi(hi), all_lo(lo)
+    {
+        kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
+        vp = (const uint8_t*)p.v + (uint64_t)kvh * p.head_stride * ES;
+        table = p.b.table + (uint64_t)seq * p.b.table_stride;
+        page_bytes = p.page_stride * ES;
+        token_bytes = (uint32_t)(p.token_stride * ES);
+        n_pages = p.b.n_pages;
+        page_shift = p.b.page_shift;
+        page_size = p.b.page_size;
+        lane = (int)threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        keys = WAVES == 4 || wave < 4;
+        values = WAVES == 4 || wave >= 4;
+        wave &= 3;
+    }
+    __device__ __forceinline__ bool whole(int vt) const  // no column's mask touches the tile
+    {
+        const int t0 = seen.tile(vt) * TILE;
+        return t0 + TILE <= all_hi && t0 >= all_lo;
+    }
+    __device__ __forceinline__ void look_up(int vt)
+    {
+        const int t0 = seen.tile(vt + lane) * TILE + 16 * wave;
+        uint64_t at = 0;
+        if (vt + lane < v1 && seen.any(t0, t0 + 16)) {
+            const uint32_t id = (uint32_t)table[t0 >> page_shift];
+            if (id >= n_pages) fault = true;
+            else at = (uint64_t)id * page_bytes + (uint64_t)((t0 & (page_size - 1)) * token_bytes);
+        }
+        place_lo = (uint32_t)at;
+        place_hi = (uint32_t)(at >> 32);
+    }
+    // tile vt to registers; tiles come in their order
+    __device__ __forceinline__ void fetch(int vt)
+    {
+        const int turn = (vt - v0) % 64;
+        if (turn == 0) look_up(vt);
+        const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place_hi, turn) << 32 |
+                            (uint32_t)__builtin_amdgcn_readlane((int)place_lo, turn);
+        if (keys)
+#pragma unroll
+        for (int i = 0; i < S::KT; i++) {
+            const int x = lane + 64 * i;
+            load_words(in.k[i], kp + at, x / (D / 8) * token_bytes + x % (D / 8) * 8 * ES);
+        }
+        if (values)
+#pragma unroll
+        for (int i = 0; i < S::VT; i++) {
+            const int x = lane + 64 * i;
+            if (4 * NCH % 64 == 0 || x < 4 * NCH) {
+                const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    load_words(in.v[i][y], vp + at, (8 * xh + 4 * vh + y) * token_bytes + n * CW * ES);
+            }
+        }
+    }
+    // Values of tokens that no column sees, which hold anything, become zeros;
+    // whether some of the others are not finite. For tiles that are not whole.
+    __device__ __forceinline__ bool clean(int vt)
+    {
+        const int t0 = seen.tile(vt) * TILE;
+        bool odd = false;
+        if (!values) return false;
+#pragma unroll
+        for (int i = 0; i < S::VT; i++) {
+            const int x = lane + 64 * i, xh = x / NCH % 2, vh = x / (2 * NCH);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool some = seen.some(t0 + 16 * wave + 8 * xh + 4 * vh + k);
+#pragma unroll
+                for (int y = 0; y < Carried<D, CT>::VW; y++) {
+                    in.v[i][k][y] = some ? in.v[i][k][y] : 0u;
+                    odd |= word_odd<CT>(in.v[i][k][y]);
+                }
+            }
+        }
+        return __any(odd && lane < 4 * NCH);
+    }
+    // registers to LDS: keys [NK][KEYS], values [NK][VALUES]
+    __device__ __forceinline__ void put(uint16_t* k_to, uint16_t* v_to) const
+    {
+        if (keys)
+#pragma unroll
+        for (int i = 0; i < S::KT; i++) {
+            const int x = lane + 64 * i;
+            uint16_t* to = k_to + key_at<D>(x % (D / 8), 16 * wave + x / (D / 8));
+            if constexpr (CT == CT_F32) {
+                uint32_t t[4][3];
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    split3(__uint_as_float(in.k[i][2 * y]), __uint_as_float(in.k[i][2 * y + 1]), t[y]);
+#pragma unroll
+                for (int n = 0; n < 3; n++) *(pu32x4*)(to + n * S::KEYS) = (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]};
+            } else if constexpr (CT == CT_BF16) {
+                *(pu32x4*)to = (pu32x4){in.k[i][0], in.k[i][1], in.k[i][2], in.k[i][3]};
+            } else {
+                *(pu32x4*)to = (pu32x4){e4m3_bf16<false>(in.k[i][0]), e4m3_bf16<true>(in.k[i][0]),
+                                        e4m3_bf16<false>(in.k[i][1]), e4m3_bf16<true>(in.k[i][1])};
+            }
+        }
+        if (values)
+#pragma unroll
+        for (int i = 0; i < S::VT; i++) {
+            const int x = lane + 64 * i;
+            if (4 * NCH % 64 == 0 || x < 4 * NCH) {
+                const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
+#pragma unroll
+                for (int y = 0; y < CW / 2; y++) {
+                    // bf16 pairs of dimensions 2 y, 2 y + 1 of the four tokens
+                    uint32_t t[4][NK];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if constexpr (CT == CT_F32)
+                            split3(__uint_as_float(in.v[i][k][2 * y]), __uint_as_float(in.v[i][k][2 * y + 1]), t[k]);
+                        else if constexpr (CT == CT_BF16)
+                            t[k][0] = in.v[i][k][y];
+                        else
+                            t[k][0] = y % 2 ? e4m3_bf16<true>(in.v[i][k][y / 2]) : e4m3_bf16<false>(in.v[i][k][y / 2]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < NK; e++) {
+                        uint16_t* to = v_to + e * S::VALUES + 4 * xh;
+                        *(pu32x2*)(to + value_at<D>(wave, vh, 2 * y * NCH + n)) =
+                            (pu32x2){__builtin_amdgcn_perm(t[1][e], t[0][e], 0x05040100u),
+                                     __builtin_amdgcn_perm(t[3][e], t[2][e], 0x05040100u)};
+                        *(pu32x2*)(to + value_at<D>(wave, vh, (2 * y + 1) * NCH + n)) =
+                            (pu32x2){__builtin_amdgcn_perm(t[1][e], t[0][e], 0x07060302u),
+                                     __builtin_amdgcn_perm(t[3][e], t[2][e], 0x07060302u)};
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Values of a tile that are not finite, added to the columns that see their
+// token (products with ones count the +inf, -inf and NaN a column sees).
+template <int D, int NK>
+__device__ __forceinline__ void add_odd(const PagedAttnArgs& p, const uint16_t* values, int t0, int pos,
+                                        pf32x16 (&acc)[D / 32])
+{
+    const int lane = (int)threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++) {
+#pragma unroll 1
+        for (int j = 0; j < 4; j++) {
+            pu32x4 see;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int t = t0 + 16 * j + 8 * (i / 2) + 4 * h + 2 * i % 4;
+                see[i] = (row_sees(pos, t, p.window, p.sinks) ? 0x3f80u : 0u) |
+                         (row_sees(pos, t + 1, p.window, p.sinks) ? 0x3f800000u : 0u);
+            }
+#pragma unroll 1
+            for (int kind = 0; kind < 3; kind++) {
+                pf32x16 n = {};
+#pragma unroll
+                for (int e = 0; e < NK; e++) {
+                    const pu32x4 w = *(const pu32x4*)(values + e * TILE * D + value_at<D>(j, 0, 32 * d) + lane * 8);
+                    const pu32x4 is = {bf16_is(w[0], kind), bf16_is(w[1], kind), bf16_is(w[2], kind), bf16_is(w[3], kind)};
+                    n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pbf16x8, is),
+                                                                __builtin_bit_cast(pbf16x8, see), n, 0, 0, 0);
+                }
+                const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (n[i] > 0.0f) acc[d][i] += add;
+            }
+        }
+    }
+}
+// ... and zeros in their place; words: the values' 32-bit words.
+__device__ __forceinline__ void clear_odd(uint16_t* values, int words)
+{
+    for (int i = (int)threadIdx.x; i < words; i += (int)blockDim.x) {
+        uint32_t* w = (uint32_t*)values + i;
+        *w = bf16_finite(*w);
+    }
+}
+
+// A column's maximum followed: only when it has grown by more than 2^8, for
+// terms up to 256 are as exact and the rescaling (an operation per output
+// register) is seldom needed. The exponent's base.
+template <int N>
+__device__ __forceinline__ float follow(float top, float& m, float& l, pf32x16 (&acc)[N])
+{
+    if (__any(top > m + 8.0f)) {
+        const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
+        // (what a first tile's infinities left in acc is kept)
+        const float f = m == -INFINITY ? 1.0f : exp2_fast(m - base);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < N; d++) acc[d] *= f;
+        m = now;
+    }
+    return m == -INFINITY ? 0.0f : m;
+}
+// Scores of tokens that the column's row does not see: with o the token's
+// place behind this lane's first one and `behind` the row's, it sees those of
+// 0 <= behind - o < window (one unsigned comparison) and of o < sinks.
+__device__ __forceinline__ void mask(const PagedAttnArgs& p, int t0, int pos, pf32x16 (&s)[2])
+{
+    const int lane0 = t0 + 4 * (((int)threadIdx.x & 63) >> 5);
+    const uint32_t window = p.window > 0 ? (uint32_t)p.window : 0x7fffffffu;
+    uint32_t behind = (uint32_t)(pos - lane0);
+    int sinks = p.window > 0 ? min(p.sinks, pos + 1) - lane0 : 0;
+    asm volatile("" : "+v"(behind), "+v"(sinks));
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int o = 32 * u + 8 * (i / 4) + i % 4;
+            s[u][i] = behind - (uint32_t)o < window || o < sinks ? s[u][i] : -INFINITY;
+        }
+}
+__device__ __forceinline__ float top_of(const pf32x16 (&s)[2])
+{
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
+    return max_x32(top);
+}
+// q of a column as B fragments: lane (column, h) holds dimensions 16 f + 8 h + 0..7
+template <int D, int NQ>
+__device__ __forceinline__ void load_q(const PagedAttnArgs& p, uint64_t at, bool live, pbf16x8 (&qb)[D / 16][NQ])
+{
+#pragma unroll
+    for (int f = 0; f < D / 16; f++) {
+        if constexpr (NQ == 3) {
+            pf32x4 a = {}, b = {};
+            if (live) {
+                a = *(const pf32x4*)((const float*)p.q + at + 16 * f);
+                b = *(const pf32x4*)((const float*)p.q + at + 16 * f + 4);
+            }
+            uint32_t t[4][3];
+            split3(a[0], a[1], t[0]);
+            split3(a[2], a[3], t[1]);
+            split3(b[0], b[1], t[2]);
+            split3(b[2], b[3], t[3]);
+#pragma unroll
+            for (int n = 0; n < 3; n++)
+                qb[f][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
+        } else {
+            qb[f][0] =
+                __builtin_bit_cast(pbf16x8, live ? *(const pu32x4*)((const uint16_t*)p.q + at + 16 * f) : (pu32x4){});
+        }
+    }
+}
+// Eight terms of a column (scores from s[i0] on) as a B fragment, added to l.
+template <int NQ>
+__device__ __forceinline__ void terms(const pf32x16& s, int i0, float sc, float base, float& l, pbf16x8 (&b)[NQ])
+{
+    float e[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        e[i] = exp2_fast(fmaf(s[i0 + i], sc, -base));
+        l += e[i];
+    }
+    if constexpr (NQ == 3) {
+        uint32_t t[4][3];
+#pragma unroll
+        for (int i = 0; i < 4; i++) split3(e[2 * i], e[2 * i + 1], t[i]);
+#pragma unroll
+        for (int n = 0; n < 3; n++) b[n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
+    } else {
+        b[0] = __builtin_bit_cast(pbf16x8, (pu32x4){pk_bf16_rne(e[0], e[1]), pk_bf16_rne(e[2], e[3]),
+                                                    pk_bf16_rne(e[4], e[5]), pk_bf16_rne(e[6], e[7])});
+    }
+}
+// A column's output, or its part of it.
+template <int D, int CW, bool QF32>
+__device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& sq, int split, int row, int head, float m,
+                                        float l, const pf32x16 (&acc)[D / 32], float v_scale)
+{
+    constexpr int NCH = D / CW;
+    const int h = ((int)threadIdx.x & 63) >> 5;
+    const uint64_t slot = ((uint64_t)split * p.b.n_rows + sq.a + row) * p.n_heads + head;
+#pragma unroll
+    for (int a0 = 0; a0 < NCH / 8; a0++)
+#pragma unroll
+        for (int b0 = 0; b0 < 4; b0++) {
+            float o[CW];
+#pragma unroll
+            for (int j = 0; j < CW; j++) o[j] = acc[j * NCH / 32][4 * (j * NCH % 32 / 8 + a0) + b0];
+            const int d = CW * (8 * a0 + 4 * h + b0);
+            if (p.splits > 1) {
+#pragma unroll
+                for (int j = 0; j < CW; j += 4)
+                    *(pf32x4*)(p.part_o + slot * D + d + j) = (pf32x4){o[j], o[j + 1], o[j + 2], o[j + 3]};
+            } else {
+                attn_store<CW, QF32>(p, sq, row, head, d, D, o, l, v_scale);
+            }
+        }
+    if (p.splits > 1 && h == 0) {
+        p.part_ml[slot * 2] = m;
+        p.part_ml[slot * 2 + 1] = l;
+    }
+}
+
 // acc += a b over their bf16 terms, small products first; of two three-term
 // numbers the products below 2^-24 of the first are left out.
 template <int NA, int NB>
@@ -110,15 +437,18 @@ __device__ __forceinline__ pf32x16 mul_terms(const pbf16x8 (&a)[NA], const pbf16
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], acc, 0, 0, 0);
 }
 
-template <int D, int CT, bool QF32>
-__global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p)
+// Two waves a SIMD (F32 queries: one), so that one's exponentials run beside
+// the other's products: two workgroups of four waves a CU, or one of eight
+// where there are columns enough, which brings in each tile once for 256 of
+// them.
+template <int D, int CT, bool QF32, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p)
 {
+    constexpr int COLS = 32 * WAVES;
     using S = Shape<D, CT, QF32>;
-    constexpr int ES = ct_size<CT>();
-    constexpr int CW = S::CW, NCH = S::NCH;
     __shared__ __attribute__((aligned(16))) uint16_t s_k[S::NBUF][S::NK][S::KEYS];
     __shared__ __attribute__((aligned(16))) uint16_t s_v[S::NBUF][S::NK][S::VALUES];
-    __shared__ int s_odd[S::NBUF][WAVES], s_fault[WAVES];
+    __shared__ int s_odd[S::NBUF][4], s_fault;
 
     // block -> (column block, chunk, sequence and head): the blocks of a head
     // are `pairs` apart, so that with a multiple of 8 pairs they run on one
@@ -138,8 +468,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
     const SeenTiles<TILE> seen = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks);
     const int v0 = split * p.chunk, v1 = min(v0 + p.chunk, seen.total());
     if (v0 >= v1 && split > 0) return;
-    const int all_hi = pos0 + first + 1;
-    const int all_lo = p.window > 0 ? pos0 + last - p.window + 1 : 0;
+    Stage<D, CT, WAVES> stage(p, seq, kvh, seen, v0, v1, pos0 + first + 1, p.window > 0 ? pos0 + last - p.window + 1 : 0);
 
     // the wave's columns
     const int w0 = cb * COLS + 32 * wave;
@@ -152,205 +481,34 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
     const SeenTiles<TILE> wseen = seen_tiles<TILE>(pos0 + wfirst, pos0 + wlast, p.window, p.sinks);
     const int w_hi = pos0 + wfirst + 1;
     const int w_lo = p.window > 0 ? pos0 + wlast - p.window + 1 : 0;
-
-    // q as B fragments: lane (column, h) holds dimensions 16 f + 8 h + 0..7
     pbf16x8 qb[D / 16][S::NQ];
-    {
-        const uint64_t at = (uint64_t)(sq.a + row) * p.q_row + (uint64_t)head * D + 8 * h;
-#pragma unroll
-        for (int f = 0; f < D / 16; f++) {
-            if constexpr (QF32) {
-                pf32x4 a = {}, b = {};
-                if (live) {
-                    a = *(const pf32x4*)((const float*)p.q + at + 16 * f);
-                    b = *(const pf32x4*)((const float*)p.q + at + 16 * f + 4);
-                }
-                uint32_t t[4][3];
-                split3(a[0], a[1], t[0]);
-                split3(a[2], a[3], t[1]);
-                split3(b[0], b[1], t[2]);
-                split3(b[2], b[3], t[3]);
-#pragma unroll
-                for (int n = 0; n < 3; n++)
-                    qb[f][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
-            } else {
-                qb[f][0] = __builtin_bit_cast(
-                    pbf16x8, live ? *(const pu32x4*)((const uint16_t*)p.q + at + 16 * f) : (pu32x4){});
-            }
-        }
-    }
+    load_q<D, S::NQ>(p, (uint64_t)(sq.a + row) * p.q_row + (uint64_t)head * D + 8 * h, live, qb);
     const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
-
-    const uint8_t* const kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
-    const uint8_t* const vp = (const uint8_t*)p.v + (uint64_t)kvh * p.head_stride * ES;
-    const int32_t* const table = p.b.table + (uint64_t)seq * p.b.table_stride;
-    const uint64_t page_bytes = p.page_stride * ES;
-    const uint32_t token_bytes = (uint32_t)(p.token_stride * ES);  // a page's tokens span less than 2^31 bytes
-    bool fault = false;
-
-    // wave w brings in tokens 16 w .. 16 w + 15 of a tile. Their places in the
-    // pages are looked up 64 tiles at a time, a tile a lane; where no row sees
-    // them page 0 is read unlooked at.
-    Carried<D, CT> in;
-    uint32_t place_lo = 0, place_hi = 0;
-    const auto look_up = [&](int vt) {
-        const int t0 = seen.tile(vt + lane) * TILE + 16 * wave;
-        uint64_t at = 0;
-        if (vt + lane < v1 && seen.any(t0, t0 + 16)) {
-            const uint32_t id = (uint32_t)table[t0 >> p.b.page_shift];
-            if (id >= p.b.n_pages) fault = true;
-            else at = (uint64_t)id * page_bytes + (uint64_t)((t0 & (p.b.page_size - 1)) * token_bytes);
-        }
-        place_lo = (uint32_t)at;
-        place_hi = (uint32_t)(at >> 32);
-    };
-    const auto fetch = [&](int vt) {
-        const int turn = (vt - v0) % 64;
-        if (turn == 0) look_up(vt);
-        const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place_hi, turn) << 32 |
-                            (uint32_t)__builtin_amdgcn_readlane((int)place_lo, turn);
-#pragma unroll
-        for (int i = 0; i < S::KT; i++) {
-            const int x = lane + 64 * i;
-            load_words(in.k[i], kp + at, x / (D / 8) * token_bytes + x % (D / 8) * 8 * ES);
-        }
-#pragma unroll
-        for (int i = 0; i < S::VT; i++) {
-            const int x = lane + 64 * i;
-            if (4 * NCH % 64 == 0 || x < 4 * NCH) {
-                const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
-#pragma unroll
-                for (int y = 0; y < 4; y++)
-                    load_words(in.v[i][y], vp + at, (8 * xh + 4 * vh + y) * token_bytes + n * CW * ES);
-            }
-        }
-    };
-    const auto put = [&](int vt, int buf) {
-        const int t0 = seen.tile(vt) * TILE;
-        const bool whole = t0 + TILE <= all_hi && t0 >= all_lo;
-#pragma unroll
-        for (int i = 0; i < S::KT; i++) {
-            const int x = lane + 64 * i;
-            const int at = key_at<D>(x % (D / 8), 16 * wave + x / (D / 8));
-            if constexpr (CT == CT_F32) {
-                uint32_t t[4][3];
-#pragma unroll
-                for (int y = 0; y < 4; y++)
-                    split3(__uint_as_float(in.k[i][2 * y]), __uint_as_float(in.k[i][2 * y + 1]), t[y]);
-#pragma unroll
-                for (int n = 0; n < 3; n++)
-                    *(pu32x4*)&s_k[buf][n][at] = (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]};
-            } else if constexpr (CT == CT_BF16) {
-                *(pu32x4*)&s_k[buf][0][at] = (pu32x4){in.k[i][0], in.k[i][1], in.k[i][2], in.k[i][3]};
-            } else {
-                *(pu32x4*)&s_k[buf][0][at] = (pu32x4){e4m3_bf16<false>(in.k[i][0]), e4m3_bf16<true>(in.k[i][0]),
-                                                      e4m3_bf16<false>(in.k[i][1]), e4m3_bf16<true>(in.k[i][1])};
-            }
-        }
-        if (!whole) {  // tokens that no column sees hold anything
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < S::VT; i++) {
-                const int x = lane + 64 * i, xh = x / NCH % 2, vh = x / (2 * NCH);
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const bool some = seen.some(t0 + 16 * wave + 8 * xh + 4 * vh + k);
-#pragma unroll
-                    for (int y = 0; y < Carried<D, CT>::VW; y++) {
-                        in.v[i][k][y] = some ? in.v[i][k][y] : 0u;
-                        odd |= word_odd<CT>(in.v[i][k][y]);
-                    }
-                }
-            }
-            odd = __any(odd && lane < 4 * NCH);
-            if (lane == 0) s_odd[buf][wave] = odd;
-        }
-#pragma unroll
-        for (int i = 0; i < S::VT; i++) {
-            const int x = lane + 64 * i;
-            if (4 * NCH % 64 == 0 || x < 4 * NCH) {
-                const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
-#pragma unroll
-                for (int y = 0; y < CW / 2; y++) {
-                    // bf16 pairs of dimensions 2 y, 2 y + 1 of the four tokens
-                    uint32_t t[4][S::NK];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if constexpr (CT == CT_F32)
-                            split3(__uint_as_float(in.v[i][k][2 * y]), __uint_as_float(in.v[i][k][2 * y + 1]), t[k]);
-                        else if constexpr (CT == CT_BF16)
-                            t[k][0] = in.v[i][k][y];
-                        else
-                            t[k][0] = y % 2 ? e4m3_bf16<true>(in.v[i][k][y / 2]) : e4m3_bf16<false>(in.v[i][k][y / 2]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < S::NK; e++) {
-                        const pu32x2 lo = {__builtin_amdgcn_perm(t[1][e], t[0][e], 0x05040100u),
-                                           __builtin_amdgcn_perm(t[3][e], t[2][e], 0x05040100u)};
-                        const pu32x2 hi = {__builtin_amdgcn_perm(t[1][e], t[0][e], 0x07060302u),
-                                           __builtin_amdgcn_perm(t[3][e], t[2][e], 0x07060302u)};
-                        *(pu32x2*)&s_v[buf][e][value_at<D>(wave, vh, 2 * y * NCH + n) + 4 * xh] = lo;
-                        *(pu32x2*)&s_v[buf][e][value_at<D>(wave, vh, (2 * y + 1) * NCH + n) + 4 * xh] = hi;
-                    }
-                }
-            }
-        }
-    };
 
     pf32x16 acc[D / 32] = {};
     float m = -INFINITY, l = 0.0f;
+    if (threadIdx.x == 0) s_fault = 0;  // (read behind the last barrier, written behind the first)
+    __syncthreads();
     // q is there: else its first use in the loop would wait, every time
     // around, for all loads in flight
     __builtin_amdgcn_s_waitcnt(0);
-    if (v0 < v1) fetch(v0);
+    if (v0 < v1) stage.fetch(v0);
     for (int vt = v0; vt < v1; vt++) {
         const int buf = (vt - v0) % S::NBUF;
+        const bool all = stage.whole(vt);
         if (S::NBUF == 1 && vt > v0) __syncthreads();  // the tile before is read
-        put(vt, buf);
+        if (!all) {
+            const bool odd = stage.clean(vt);
+            if (lane == 0 && stage.values) s_odd[buf][stage.wave] = odd;
+        }
+        stage.put(&s_k[buf][0][0], &s_v[buf][0][0]);
         __syncthreads();
-        if (vt + 1 < v1) fetch(vt + 1);
+        if (vt + 1 < v1) stage.fetch(vt + 1);
         const int t0 = seen.tile(vt) * TILE;
-        const bool all = t0 + TILE <= all_hi && t0 >= all_lo;  // every column sees every token
         if (!all && (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3])) {
-            // values that are not finite: added to the columns that see their
-            // token (products with ones count the +inf, -inf and NaN a column
-            // sees), and zeros for the products below
-            if (active) {
-#pragma unroll
-                for (int d = 0; d < D / 32; d++) {
-#pragma unroll 1
-                    for (int j = 0; j < 4; j++) {
-                        pu32x4 see;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int t = t0 + 16 * j + 8 * (i / 2) + 4 * h + 2 * i % 4;
-                            see[i] = (row_sees(pos, t, p.window, p.sinks) ? 0x3f80u : 0u) |
-                                     (row_sees(pos, t + 1, p.window, p.sinks) ? 0x3f800000u : 0u);
-                        }
-#pragma unroll 1
-                        for (int kind = 0; kind < 3; kind++) {
-                            pf32x16 n = {};
-#pragma unroll
-                            for (int e = 0; e < S::NK; e++) {
-                                const pu32x4 w = *(const pu32x4*)&s_v[buf][e][value_at<D>(j, 0, 32 * d) + lane * 8];
-                                const pu32x4 is = {bf16_is(w[0], kind), bf16_is(w[1], kind), bf16_is(w[2], kind),
-                                                   bf16_is(w[3], kind)};
-                                n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pbf16x8, is),
-                                                                            __builtin_bit_cast(pbf16x8, see), n, 0, 0, 0);
-                            }
-                            const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
-#pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                if (n[i] > 0.0f) acc[d][i] += add;
-                        }
-                    }
-                }
-            }
+            if (active) add_odd<D, S::NK>(p, &s_v[buf][0][0], t0, pos, acc);
             __syncthreads();
-            for (int i = (int)threadIdx.x; i < S::NK * S::VALUES / 2; i += THREADS) {
-                uint32_t* w = (uint32_t*)&s_v[buf][0][0] + i;
-                *w = bf16_finite(*w);
-            }
+            clear_odd(&s_v[buf][0][0], S::NK * S::VALUES / 2);
             __syncthreads();
         }
         if (!active || !wseen.any(t0, t0 + TILE)) continue;
@@ -378,6 +536,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
         // scores of two 32-token halves
         pf32x16 s[2] = {};
         load_keys(0);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int x = 0; x < KG; x++) {
             if (x + 1 < KG) load_keys(x + 1);
@@ -388,61 +547,16 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
                 s[4 * x / (D / 16)] = mul_terms(frag[x & 1][i], qb[4 * x % (D / 16) + i], s[4 * x / (D / 16)]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        const bool whole = t0 + TILE <= w_hi && t0 >= w_lo;
-        if (!whole) {
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int t = t0 + 32 * u + 8 * (i / 4) + 4 * h + i % 4;
-                    if (!row_sees(pos, t, p.window, p.sinks)) s[u][i] = -INFINITY;
-                }
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, s[u][i]);
-        top = max_x32(top) * sc;
-        // The maximum is followed only when it has grown by more than 2^8:
-        // terms up to 256 are as exact, and the rescaling (an operation per
-        // output register) is seldom needed.
-        if (__any(top > m + 8.0f)) {
-            const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
-            // (what a first tile's infinities left in acc is kept)
-            const float f = m == -INFINITY ? 1.0f : exp2_fast(m - base);
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < D / 32; d++) acc[d] *= f;
-            m = now;
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
+        __builtin_amdgcn_s_setprio(0);
+        if (t0 + TILE > w_hi || t0 < w_lo) mask(p, t0, pos, s);
+        const float base = follow(top_of(s) * sc, m, l, acc);
         pbf16x8 b[2][S::NQ];
-        const auto terms = [&](int j) {
-            float e[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                e[i] = exp2_fast(fmaf(s[j / 2][8 * (j % 2) + i], sc, -base));
-                l += e[i];
-            }
-            if constexpr (QF32) {
-                uint32_t t[4][3];
-#pragma unroll
-                for (int i = 0; i < 4; i++) split3(e[2 * i], e[2 * i + 1], t[i]);
-#pragma unroll
-                for (int n = 0; n < 3; n++)
-                    b[j & 1][n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
-            } else {
-                b[j & 1][0] = __builtin_bit_cast(pbf16x8, (pu32x4){pk_bf16_rne(e[0], e[1]), pk_bf16_rne(e[2], e[3]),
-                                                                   pk_bf16_rne(e[4], e[5]), pk_bf16_rne(e[6], e[7])});
-            }
-        };
-        terms(0);
+        terms<S::NQ>(s[0], 0, sc, base, l, b[0]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (j < 3) load_values(j + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (j < 3) terms(j + 1);
+            if (j < 3) terms<S::NQ>(s[(j + 1) / 2], 8 * ((j + 1) % 2), sc, base, l, b[(j + 1) & 1]);
 #pragma unroll
             for (int d = 0; d < VF; d++) {
                 acc[d] = mul_terms(frag[j & 1][d], b[j & 1], acc[d]);
@@ -453,41 +567,24 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_many(PagedAttnAr
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if (lane == 0) s_fault[wave] = 0;
-    if (__any(fault) && lane == 0) s_fault[wave] = 1;
+    if (stage.fault) s_fault = 1;
     __syncthreads();
     if (!live) return;
     l = sum_x32(l);
-    if (s_fault[0] | s_fault[1] | s_fault[2] | s_fault[3]) l = __builtin_nanf("");
-
-    const float v_scale = p.v_scale ? p.v_scale[kvh] : 1.0f;
-    const uint64_t slot = ((uint64_t)split * p.b.n_rows + sq.a + row) * p.n_heads + head;
-#pragma unroll
-    for (int a0 = 0; a0 < NCH / 8; a0++)
-#pragma unroll
-        for (int b0 = 0; b0 < 4; b0++) {
-            float o[CW];
-#pragma unroll
-            for (int j = 0; j < CW; j++) o[j] = acc[j * NCH / 32][4 * (j * NCH % 32 / 8 + a0) + b0];
-            const int d = CW * (8 * a0 + 4 * h + b0);
-            if (p.splits > 1) {
-#pragma unroll
-                for (int j = 0; j < CW; j += 4)
-                    *(pf32x4*)(p.part_o + slot * D + d + j) = (pf32x4){o[j], o[j + 1], o[j + 2], o[j + 3]};
-            } else {
-                attn_store<CW, QF32>(p, sq, row, head, d, D, o, l, v_scale);
-            }
-        }
-    if (p.splits > 1 && h == 0) {
-        p.part_ml[slot * 2] = m;
-        p.part_ml[slot * 2 + 1] = l;
-    }
+    if (s_fault) l = __builtin_nanf("");
+    put_out<D, S::CW, QF32>(p, sq, split, row, head, m, l, acc, p.v_scale ? p.v_scale[kvh] : 1.0f);
 }
 
 template <int D, int CT, bool QF32>
 void go(const PagedAttnArgs& p, unsigned blocks, hipStream_t s)
 {
-    k_attn_many<D, CT, QF32><<<dim3(blocks), dim3(THREADS), 0, s>>>(p);
+    if constexpr (!QF32) {
+        if (p.cols == 2 * ATTN_MANY_COLS) {
+            k_attn_many<D, CT, QF32, 8><<<dim3(blocks), dim3(512), 0, s>>>(p);
+            return;
+        }
+    }
+    k_attn_many<D, CT, QF32, 4><<<dim3(blocks), dim3(256), 0, s>>>(p);
 }
 
 template <int D>

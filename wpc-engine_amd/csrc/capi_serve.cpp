@@ -10,6 +10,7 @@
 namespace wpcg {
 namespace {
 
+constexpr int64_t CUS = 256;  // of an MI355X
 constexpr uint64_t INT_BOUND = 1u << 30;  // of rows, tokens, heads: sums of two stay ints
 
 uint64_t type_size(int dtype) { return dtype == WPCG_DTYPE_F32 ? 4 : dtype == WPCG_DTYPE_BF16 ? 2 : 1; }
@@ -100,38 +101,60 @@ struct Plan {
     uint64_t bytes;
 };
 
-// Which kernel, and how many workgroups share a sequence's tokens.
-//
-// A batch is split over the tokens until it has about `target` workgroups, in
-// chunks of at least `least` tiles: a shorter chunk pays more for its state and
-// the second launch than it gains. The bounds stand in for the lengths, which
-// only the device knows; a shorter sequence just has fewer chunks.
+// Which kernel, and how many workgroups share a sequence's tokens. The bounds
+// stand in for the lengths, which only the device knows; a shorter sequence
+// just has fewer chunks.
 int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attention* a, Plan* out)
 {
     const int64_t group = a->n_heads / kv->n_kv_heads, cols = (int64_t)b.max_q * group;
+    const int64_t pairs = (int64_t)b.n_seq * kv->n_kv_heads;
     Plan p;
     p.many = cols > 2 * ATTN_FEW_COLS;
-    // (over an F32 cache the wider form's registers do not suffice)
-    p.cols = p.many ? ATTN_MANY_COLS
-             : cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
-    const int64_t cw = p.cols, tw = p.many ? ATTN_MANY_TILE : ATTN_FEW_TILE;
-    const int64_t blocks = (cols + cw - 1) / cw;
-    // tiles that a column block can see
-    int64_t tiles = (b.max_kv + tw - 1) / tw;
-    if (a->window > 0) {
+    const int64_t tw = p.many ? ATTN_MANY_TILE : ATTN_FEW_TILE;
+    // tiles that a block of cw columns can see
+    const auto tiles_of = [&](int64_t cw) {
+        const int64_t all = (b.max_kv + tw - 1) / tw;
+        if (a->window == 0) return all;
         const int64_t rows = std::min<int64_t>(b.max_q, cw / group + 2);
         const int64_t seen = (std::min<int64_t>(a->sinks, b.max_kv) + tw - 1) / tw +
                              ((int64_t)std::min<uint64_t>(a->window, INT_BOUND) + rows + tw - 1) / tw + 1;
-        tiles = std::min(tiles, seen);
+        return std::min(all, seen);
+    };
+    if (p.many) {
+        // 256 columns a workgroup where that leaves every CU one and the tiles
+        // are many: a prompt of 4096 took 149 us so, 158 with 128 columns; with
+        // 18 tiles a block (a window of 1024) 238 us against 232, for a CU's
+        // one workgroup starts and ends alone.
+        const int64_t wide = 2 * ATTN_MANY_COLS;
+        p.cols = a->dtype == WPCG_DTYPE_BF16 && tiles_of(wide) >= 32 && pairs * ((cols + wide - 1) / wide) >= CUS
+                     ? wide : ATTN_MANY_COLS;
+    } else {
+        // (over an F32 cache the wider form's registers do not suffice)
+        p.cols = cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
     }
-    const int64_t base = (int64_t)b.n_seq * kv->n_kv_heads * blocks;
-    const int64_t target = p.many ? 512 : 256, least = p.many ? 8 : 2 * ATTN_FEW_WAVES;
-    int64_t chunk = tiles;
-    if (base > 0 && base < target) {
-        const int64_t want = (target + base - 1) / base;
-        chunk = std::max(least, (tiles + want - 1) / want);
-    }
-    p.chunk = (int)std::max<int64_t>(1, chunk);
+    const int64_t blocks = (cols + p.cols - 1) / p.cols, base = pairs * blocks, tiles = tiles_of(p.cols);
+    // The cheapest split by this estimate, in microseconds: workgroups run in
+    // rounds of those the chip holds; each has 4 us of start and end and its
+    // tiles, and a split one a second launch of 5 us. A tile of the few-row
+    // kernel takes what its bytes take at 20 GB/s, a CU's share of the memory's
+    // rate, and about what it gets with half of them idle too (64000 tokens of
+    // BF16 on 128 workgroups: 100 us, 2.6 TB/s; on 256: 53 us); of the many-row
+    // kernel what its products take.
+    const double bytes = 2.0 * tw * kv->head_dim * type_size(kv->dtype);
+    const bool two = p.many && p.cols == ATTN_MANY_COLS && a->dtype == WPCG_DTYPE_BF16;  // workgroups on a CU
+    const int64_t room = two ? 2 * CUS : CUS;
+    const double many_tile = (a->dtype == WPCG_DTYPE_BF16 ? 2.4 : kv->dtype == WPCG_DTYPE_F32 ? 6.0 : 3.5) *
+                             (kv->head_dim / 128.0);
+    const auto cost = [&](int64_t s) {
+        const int64_t all = base * s, rounds = (all + room - 1) / room;
+        const double tile = p.many ? many_tile : bytes / 20480.0;
+        return rounds * (4.0 + (double)((tiles + s - 1) / s) * tile) + (s > 1 ? 5.0 : 0.0);
+    };
+    const int64_t least = p.many ? 2 : ATTN_FEW_WAVES;  // tiles of a chunk
+    int64_t best = 1;
+    for (int64_t s = 2; base > 0 && s <= tiles / least && base * s <= 4 * room; s++)
+        if (cost(s) < cost(best)) best = s;
+    p.chunk = (int)std::max<int64_t>(1, (tiles + best - 1) / best);
     p.splits = (int)std::max<int64_t>(1, (tiles + p.chunk - 1) / p.chunk);
     p.col_blocks = (int)std::max<int64_t>(1, blocks);
     if (base * p.splits >= (int64_t)1 << 31 || (uint64_t)b.n_seq * b.max_q * a->n_heads >= 1u << 31)
