@@ -60,13 +60,13 @@ class Paged:
     NaN, and the device objects over them. order: "head" packs [page][head]
     [token][dim], "token" [page][token][head][dim] with some padding."""
 
-    def __init__(self, ctx, rng, dtype, hkv, d, page, kv_len, order="head", scales=False, spare=3, values=True):
+    def __init__(self, ctx, rng, dtype, hkv, d, page, kv_len, order="head", scales=False, spare=3, values=True, width=0):
         self.ctx, self.dtype, self.hkv, self.d, self.page = ctx, dtype, hkv, d, page
         self.kv_len = list(kv_len)
         need = [-(-n // page) for n in self.kv_len]
         self.n_pages = sum(need) + spare
         ids = rng.permutation(self.n_pages).astype(np.int32)
-        self.table = np.full((len(need), max(max(need), 1) + 1), -7, np.int32)
+        self.table = np.full((len(need), max(max(need) + 1, 2, width)), -7, np.int32)
         at = 0
         for s, n in enumerate(need):
             self.table[s, :n] = ids[at:at + n]

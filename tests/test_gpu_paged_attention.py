@@ -122,6 +122,55 @@ def test_split_and_joined(ctx, q_dtype, dtype, rows, lens, heads, hkv, window):
 
 
 @pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("rows,heads,hkv,d,window", [(1, 8, 2, 128, 0), (1, 4, 4, 64, 0), (5, 8, 2, 128, 0),
+                                                     (3, 7, 1, 64, 2000), (2, 8, 2, 128, 40000)])
+def test_tiles_dealt_out(ctx, q_dtype, dtype, rows, heads, hkv, d, window):
+    """Sequences that may be long by the call's bounds (a million tokens) have
+    their tiles dealt out evenly, whatever their lengths are: some of several
+    workgroups, some many to one, some of no token or fewer than rows."""
+    print(f"[gpu] dealt: {q_dtype}/{dtype} rows {rows} {heads}/{hkv}x{d} window {window}", flush=True)
+    rng = np.random.default_rng(rows + heads + d + q_dtype + 10 * dtype)
+    lens = [3000, 5, 0, 517, 1024, 33, 2100, rows, 512, 511, 1, 1500, 16, 640, 2, 900, 64, 100, 31, 32, 260, 700, 4, 48]
+    n = len(lens)
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 16, lens, scales=dtype == E4M3, width=62500).upload()
+    nr = [rows] * n
+    nr[4], nr[9] = 1, max(1, rows - 1)
+    q = R.encode(rng.standard_normal((sum(nr), heads, d)) * 1.5, q_dtype)
+    b = pg.batch(nr, max_kv=1000000, max_q=rows)
+    got, op = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, 20)
+    assert op.workspace_bytes > 0
+    want, bound = expected(pg, q, nr, heads, q_dtype, 0.09, window, 20)
+    check(got, want, bound)
+    again, _ = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, 20)
+    assert np.array_equal(got.view(np.uint64), again.view(np.uint64))
+    # a page that is none in one sequence, a length that is none in another
+    pg.table[0, 100] = pg.n_pages + 1
+    pg.d_table.write(pg.table)
+    pg.d_len.write(np.array(lens[:3] + [-1] + lens[4:], np.int32))
+    got, _ = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, 20)
+    at = np.cumsum([0] + nr)
+    if window != 2000:  # (which hides the page)
+        assert np.isnan(got[:at[1]]).all()
+    assert np.isnan(got[at[3]:at[4]]).all()
+    check(got[at[1]:at[3]], want[at[1]:at[3]], bound[at[1]:at[3]])
+    check(got[at[4]:], want[at[4]:], bound[at[4]:])
+
+
+@pytest.mark.parametrize("n,rows", [(700, 1), (2048, 2), (2049, 1)])
+def test_more_sequences_than_threads(ctx, n, rows):
+    """Dealt out over several rounds of a workgroup's threads; one sequence more
+    than that takes, each with workgroups of its own again."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(0, 40, n)]
+    lens[5], lens[n - 1] = 900, 1300
+    pg = R.Paged(ctx, rng, BF16, 1, 64, 16, lens, width=6250).upload()
+    q = R.encode(rng.standard_normal((n * rows, 2, 64)), BF16)
+    got, op = run(ctx, pg, pg.batch([rows] * n, max_kv=100000), q, 2, BF16, 0.125)
+    assert (op.workspace_bytes > 0) == (n <= 2048)
+    check(got, *expected(pg, q, [rows] * n, 2, BF16, 0.125, 0, 0))
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
 @pytest.mark.parametrize("rows", [2, 30])
 def test_infinite_values_reach_only_rows_that_see_them(ctx, q_dtype, dtype, rows):
     """The last token's values hold NaN (and infinities where the type has

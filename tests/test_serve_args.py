@@ -158,19 +158,25 @@ def workspace(kv, b, a):
 
 
 def test_attention_workspace():
-    """None while the batch fills the GPU or is short; else every part of every
-    row and head, and a smaller one, none or an unaligned one is refused."""
+    """None for short sequences, a state of every column or row and head for each
+    part; too small a one, none or an unaligned one is refused."""
     assert workspace(pages(), batch(), attention()) == 0
     long = batch(max_kv=100000, table_stride=6250)
-    n = workspace(pages(), long, attention())
-    part = 5 * 8 * 130 * 4
+    n, part = workspace(pages(), long, attention()), 3 * 2 * 16 * 130 * 4
     assert n > 0 and n % part == 0
     refused(attend(pages(), long, attention(), n=n - 1), E_ARG, "bytes of workspace")
     refused(attend(pages(), long, attention(), ws=None, n=0), E_ARG, "bytes of workspace")
     refused(attend(pages(), long, attention(), ws=AT + 4, n=n), E_ARG, "aligned")
     refused(attend(pages(), long, attention(), n=n), E_ARG, "null context")
-    # a window bounds the parts
-    assert workspace(pages(), long, attention(window=64)) <= 2 * part
+    # many sequences that may be long: the same whatever the lengths are
+    many = [batch(max_kv=k, table_stride=k // 16, n_rows=n, n_seq=n, max_q=1) for k, n in ((100000, 200), (200000, 300))]
+    assert len({workspace(pages(), b, attention()) for b in many}) == 1
+    # a window bounds what there is to share
+    assert workspace(pages(), long, attention(window=64)) == 0
+    rows = batch(max_kv=100000, table_stride=6250, n_seq=1, n_rows=40, max_q=40)
+    n, part = workspace(pages(), rows, attention()), 40 * 8 * 130 * 4
+    assert n > 0 and n % part == 0
+    refused(attend(pages(), rows, attention(), n=n - 1), E_ARG, "bytes of workspace")
     assert wpcg.lib.wpcg_paged_attention_workspace(ref(pages()), ref(batch()), ref(attention()), None) == E_ARG
 
 

@@ -600,14 +600,70 @@ void go_types(const PagedAttnArgs& p, int q_dtype, int cache_dtype, unsigned blo
     }
 }
 
+// ---- the chunks' states joined -------------------------------------------------
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that the
+// row's workgroup had, in their order; D/4 threads a (row, query head).
+template <int D, bool QF32>
+__global__ __launch_bounds__(256) void k_attn_many_join(PagedAttnArgs p)
+{
+    constexpr int TH = D / 4, PER = 256 / TH;
+    const int tid = (int)threadIdx.x, d = tid % TH * 4;
+    const uint64_t x = (uint64_t)blockIdx.x * PER + tid / TH;
+    const int head = (int)(x % (unsigned)p.n_heads);
+    const uint64_t rest = x / (unsigned)p.n_heads;
+    const int row = (int)(rest / (unsigned)p.b.n_seq), seq = (int)(rest % (unsigned)p.b.n_seq);
+    if (row >= p.b.max_q) return;
+    const SeqRows sq = seq_rows(p.b, seq);
+    if (row >= sq.n) return;
+    const int cols = sq.n * p.group, cb = (row * p.group + head % p.group) / p.cols;
+    const int len = sq.bad ? 0 : sq.len, pos0 = len - sq.n;
+    const int first = cb * p.cols / p.group, last = (min(cols, (cb + 1) * p.cols) - 1) / p.group;
+    const int tiles = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks).total();
+    const int n = max(1, (tiles + p.chunk - 1) / p.chunk);
+    const uint64_t slot0 = (uint64_t)(sq.a + row) * p.n_heads + head;
+    const uint64_t step = (uint64_t)p.b.n_rows * p.n_heads;
+    float m = -INFINITY, l = 0.0f;
+    pf32x4 o = {};
+    for (int i0 = 0; i0 < n; i0 += 4) {  // four in flight
+        float mi[4], li[4];
+        pf32x4 oi[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint64_t slot = slot0 + (uint64_t)min(i0 + j, n - 1) * step;
+            mi[j] = p.part_ml[slot * 2];
+            li[j] = p.part_ml[slot * 2 + 1];
+            oi[j] = *(const pf32x4*)(p.part_o + slot * D + d);
+            if (i0 + j >= n) {
+                mi[j] = -INFINITY;
+                li[j] = 0.0f;
+            }
+        }
+        add_parts<4>(m, l, o, mi, li, oi);
+    }
+    const float r[4] = {o[0], o[1], o[2], o[3]};
+    attn_store<4, QF32>(p, sq, row, head, d, D, r, l, p.v_scale ? p.v_scale[head / p.group] : 1.0f);
+}
+template <int D, bool QF32>
+void join(const PagedAttnArgs& p, hipStream_t s)
+{
+    const uint64_t all = (uint64_t)p.b.n_seq * p.b.max_q * p.n_heads;
+    k_attn_many_join<D, QF32><<<dim3((unsigned)((all * (D / 4) + 255) / 256)), dim3(256), 0, s>>>(p);
+}
+
 }  // namespace
 
 hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s)
 {
     const uint64_t blocks = (uint64_t)p.b.n_seq * p.n_kv * p.col_blocks * p.splits;
     if (blocks == 0) return hipSuccess;
-    if (head_dim == 128) go_types<128>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
-    else go_types<64>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
+    const bool f32 = q_dtype == WPCG_DTYPE_F32;
+    if (head_dim == 128) {
+        go_types<128>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
+        if (p.splits > 1) f32 ? join<128, true>(p, s) : join<128, false>(p, s);
+    } else {
+        go_types<64>(p, q_dtype, cache_dtype, (unsigned)blocks, s);
+        if (p.splits > 1) f32 ? join<64, true>(p, s) : join<64, false>(p, s);
+    }
     return hipGetLastError();
 }
 

@@ -97,7 +97,8 @@ int check_pointers(const wpcg_kv_pages* kv, const wpcg_kv_batch* b)
 
 struct Plan {
     bool many;
-    int cols, col_blocks, chunk, splits;
+    int cols, col_blocks, blocks, chunk, splits;
+    uint64_t parts;  // columns whose states the workspace holds
     uint64_t bytes;
 };
 
@@ -140,14 +141,13 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
     // rate, and about what it gets with half of them idle too (64000 tokens of
     // BF16 on 128 workgroups: 100 us, 2.6 TB/s; on 256: 53 us); of the many-row
     // kernel what its products take.
-    const double bytes = 2.0 * tw * kv->head_dim * type_size(kv->dtype);
     const bool two = p.many && p.cols == ATTN_MANY_COLS && a->dtype == WPCG_DTYPE_BF16;  // workgroups on a CU
     const int64_t room = two ? 2 * CUS : CUS;
-    const double many_tile = (a->dtype == WPCG_DTYPE_BF16 ? 2.4 : kv->dtype == WPCG_DTYPE_F32 ? 6.0 : 3.5) *
-                             (kv->head_dim / 128.0);
+    const double tile = p.many ? (a->dtype == WPCG_DTYPE_BF16 ? 2.4 : kv->dtype == WPCG_DTYPE_F32 ? 6.0 : 3.5) *
+                                     (kv->head_dim / 128.0)
+                               : 2.0 * tw * kv->head_dim * type_size(kv->dtype) / 20480.0;
     const auto cost = [&](int64_t s) {
-        const int64_t all = base * s, rounds = (all + room - 1) / room;
-        const double tile = p.many ? many_tile : bytes / 20480.0;
+        const int64_t rounds = (base * s + room - 1) / room;
         return rounds * (4.0 + (double)((tiles + s - 1) / s) * tile) + (s > 1 ? 5.0 : 0.0);
     };
     const int64_t least = p.many ? 2 : ATTN_FEW_WAVES;  // tiles of a chunk
@@ -156,10 +156,23 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
         if (cost(s) < cost(best)) best = s;
     p.chunk = (int)std::max<int64_t>(1, (tiles + best - 1) / best);
     p.splits = (int)std::max<int64_t>(1, (tiles + p.chunk - 1) / p.chunk);
+    p.blocks = 0;
+    p.parts = p.splits == 1 ? 0 : p.many ? (uint64_t)p.splits * b.n_rows * a->n_heads : (uint64_t)p.splits * base * p.cols;
+    // A chunk that long may be one sequence's alone while the others' are
+    // empty, for the bounds do not tell: all tiles are dealt out evenly
+    // instead. (63 sequences of 500 tokens and one of 100000, 32 / 4 heads: 1028
+    // us with a workgroup a sequence and head, 79 so. It costs a few us more
+    // where the lengths are less unlike: 64 sequences of 512 to 4096 tokens 67
+    // and 75 us.)
+    if (!p.many && p.chunk * tile > 130.0 && b.n_seq <= ATTN_DEAL_SEQS && base * tiles < (int64_t)1 << 30) {
+        p.blocks = CUS;
+        p.parts = 2 * CUS * p.cols;
+        p.splits = 1;
+    }
     p.col_blocks = (int)std::max<int64_t>(1, blocks);
     if (base * p.splits >= (int64_t)1 << 31 || (uint64_t)b.n_seq * b.max_q * a->n_heads >= 1u << 31)
         return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
-    p.bytes = p.splits > 1 ? (uint64_t)p.splits * b.n_rows * a->n_heads * (kv->head_dim + 2) * sizeof(float) : 0;
+    p.bytes = p.parts * (kv->head_dim + 2) * sizeof(float) + p.blocks * sizeof(AttnEnd);
     *out = p;
     return WPCG_OK;
 }
@@ -318,14 +331,15 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
     a.sinks = (int)std::min<uint64_t>(att->sinks, INT_BOUND);
     a.cols = plan.cols;
     a.col_blocks = plan.col_blocks;
+    a.blocks = plan.blocks;
     a.chunk = plan.chunk;
     a.splits = plan.splits;
     a.part_o = (float*)ws_dev;
-    a.part_ml = a.part_o + (uint64_t)plan.splits * a.b.n_rows * a.n_heads * kv->head_dim;
+    a.part_ml = a.part_o + plan.parts * kv->head_dim;
+    a.ends = (AttnEnd*)(a.part_ml + plan.parts * 2);
     const hipStream_t s = pick(ctx, stream);
     const int d = (int)kv->head_dim;
     WPCG_HIP(plan.many ? launch_attn_many(a, d, att->dtype, kv->dtype, s) : launch_attn_few(a, d, att->dtype, kv->dtype, s));
-    if (plan.splits > 1) WPCG_HIP(launch_attn_join(a, d, att->dtype, plan.many, s));
     return WPCG_OK;
 }
 

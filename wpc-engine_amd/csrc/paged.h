@@ -163,6 +163,28 @@ __device__ __forceinline__ bool bf16_odd(uint32_t w)  // either half not finite
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
+// A column's state (maximum, sum, four outputs) with N parts' states added in
+// their order; a part that saw nothing has maximum -inf, one that met a page
+// that is none the sum NaN.
+template <int N>
+__device__ __forceinline__ void add_parts(float& m, float& l, pf32x4& o, const float (&mi)[N], const float (&li)[N],
+                                          const pf32x4 (&oi)[N])
+{
+    float now = m;
+#pragma unroll
+    for (int j = 0; j < N; j++) now = fmaxf(now, mi[j]);
+    const float base = now == -INFINITY ? 0.0f : now;
+    const float old = exp2_fast(m - base);
+    l *= old;
+    o *= old;
+    m = now;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const float f = exp2_fast(mi[j] - base);
+        l += f == 0.0f && li[j] == li[j] ? 0.0f : li[j] * f;
+        if (f != 0.0f) o += oi[j] * f;
+    }
+}
 // N consecutive outputs of a column, from dimension d on: o / l times the
 // values' scale; zeros for a row that sees nothing, NaN where its sequence's
 // length is none.

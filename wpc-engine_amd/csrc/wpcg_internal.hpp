@@ -494,14 +494,28 @@ hipError_t launch_kv_append(const KvAppendArgs& p, int head_dim, bool bf16, hipS
 // Attention over pages. A column is a (row, query head) pair: column c of a
 // sequence's key-value head is row c / group, query head c % group of its
 // group. The kernel for few rows takes ATTN_FEW_COLS columns a workgroup, or
-// twice as many, that for many ATTN_MANY_COLS; each reads a chunk of `chunk` tiles
-// (ATTN_FEW_TILE, ATTN_MANY_TILE tokens) of those its columns see, the chunks
-// are `splits` at most. With splits > 1 chunk i leaves a column's
-// unnormalised output (fp32) at part_o[(i * n_rows + row) * n_heads + head]
-// (head_dim values) and its maximum (of the scores times log2 e) and sum of
-// terms at part_ml [same][2], and launch_attn_join puts them together.
+// twice as many, that for many ATTN_MANY_COLS or twice as many, over tiles of
+// ATTN_FEW_TILE, ATTN_MANY_TILE tokens.
+//
+// A workgroup reads a chunk of `chunk` tiles of those its columns see, the
+// chunks are `splits` at most. With splits > 1 chunk i leaves a column's state
+// (unnormalised output, maximum of the scores times log2 e, sum of terms; fp32)
+// in part_o (head_dim values a state) and part_ml (two): few rows at
+// ((i * n_seq * n_kv + sequence's head) * col_blocks + column block) * cols +
+// column, many rows at (i * n_rows + row) * n_heads + head.
+//
+// Few rows, blocks > 0: that many workgroups share all tiles evenly (at least
+// ATTN_SHARE_MIN each; at most ATTN_DEAL_SEQS sequences) instead; the states of
+// items that several have parts of are at [2 blocks][cols], and ends [blocks]
+// tells which item a workgroup's first part ends.
 constexpr int ATTN_FEW_COLS = 16, ATTN_FEW_TILE = 32, ATTN_FEW_WAVES = 8;
+constexpr int ATTN_SHARE_MIN = 16, ATTN_DEAL_SEQS = 2048;
 constexpr int ATTN_MANY_COLS = 128, ATTN_MANY_TILE = 64;
+struct AttnEnd {
+    int seq, kvh, cb;  // seq -1: none
+    int first;         // the workgroup of its first part
+    int second;        // which of that one's parts
+};
 struct PagedAttnArgs {
     PagedBatch b;
     const void *q, *k, *v;
@@ -513,12 +527,12 @@ struct PagedAttnArgs {
     float scale;  // times log2 e
     int window, sinks;
     int cols, col_blocks;  // columns of a workgroup; blocks of them of a sequence's key-value head
-    int chunk, splits;
+    int chunk, splits, blocks;
     float *part_o, *part_ml;
+    AttnEnd* ends;
 };
 hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
-hipError_t launch_attn_join(const PagedAttnArgs& p, int head_dim, int q_dtype, bool many, hipStream_t s);
 
 // ---- verification of drafts (draft.hip) -------------------------------------
 // A chunk's state of a row: sum of exp((x - max) / T), the largest logit and
