@@ -459,6 +459,18 @@ int wpcg_model_set_prefill(wpcg_model* m, int enabled);
  * reference counterpart. */
 #define WPCG_VERIFY_MAX 64
 int wpcg_model_verify(wpcg_model* m, const uint32_t* tokens, uint32_t n, uint32_t* argmax, float* logits);
+/* The same by sampling: accepted receives the number of drafts kept and out
+ * (n ids) the kept drafts, the next token, then -1, by wpcg_draft_verify's
+ * rule over the rows' logits; the kept tokens are distributed as the model's
+ * own samples at this temperature. draft_probs: n - 1 rows of vocab floats,
+ * what each draft was drawn from (null: chosen outright); u: n - 1 uniform
+ * numbers in [0, 1) (may be null if n is 1), u_next one more; temperature not
+ * above 0: greedy. All arrays are the host's. The position moves on by n, as
+ * with wpcg_model_verify: the kept tokens' cache entries end at the former
+ * position + 1 + accepted, where wpcg_model_set_position takes it before the
+ * next token is fed. No reference counterpart. */
+int wpcg_model_verify_sampled(wpcg_model* m, const uint32_t* tokens, uint32_t n, const float* draft_probs,
+                              const float* u, float u_next, float temperature, uint32_t* accepted, int32_t* out);
 /* Move the position back to pos (<= the current one): later cache entries
  * are ignored and overwritten by the next steps. No reference counterpart. */
 int wpcg_model_set_position(wpcg_model* m, uint32_t pos);
@@ -501,7 +513,8 @@ int wpcg_model_debug_read(wpcg_model* m, int which, float* out, uint64_t n);
  * WPCG_DTYPE_E4M3 (8 bits: 1 sign, 4 exponent, 3 mantissa, largest value 448;
  * the value a byte stands for is its own times its head's scale). Limits:
  * head_dim 64 or 128 (else E_UNSUPPORTED); page_size a power of two in
- * 16..256; pointers and strides multiples of 16 bytes; scales positive.
+ * 16..256; pointers and strides multiples of 16 bytes; page_size token strides
+ * shorter than 2^31 bytes; scales positive.
  *
  * A batch's rows are numbered through: sequence s owns rows q_start[s] ..
  * q_start[s+1]-1 (q_start null: sequence s is row s alone), the newest tokens
@@ -514,7 +527,9 @@ int wpcg_model_debug_read(wpcg_model* m, int which, float* out, uint64_t n);
  * out; one whose kv_len is not in 0..max_kv, or that needs a page whose id is
  * not in 0..n_pages-1, gets NaN in its output rows and nothing is stored for
  * the tokens concerned. A sequence longer in rows than in tokens (kv_len < n)
- * has rows before position 0; they append nothing and see nothing. */
+ * has rows before position 0; they append nothing and see nothing. Row ranges
+ * that overlap (q_start falls somewhere) leave it open whose result the shared
+ * rows hold. */
 #define WPCG_DTYPE_E4M3 3
 typedef struct wpcg_kv_pages_s {
     void* k_dev;
@@ -575,9 +590,11 @@ int wpcg_kv_append(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* 
  * cache (an F32 cache is E_UNSUPPORTED) and rounds the softmax's terms to
  * bf16 before they meet V. Sums and softmax statistics are fp32. One pass over
  * the pages with a running maximum; long sequences are split over workgroups
- * and joined by a second launch. How a batch is split depends on the batch's
- * bounds (n_seq, max_q, max_kv), not on what the arrays hold; the same call
- * gives the same bits.
+ * and joined by a second launch. Whether and into how many parts a batch is
+ * split depends on its bounds (n_seq, n_rows, max_q, max_kv); batches that may
+ * hold a few very long sequences among short ones deal their tiles out by the
+ * lengths, so that there a sequence's last bits may depend on the others'
+ * lengths. The same call on the same arrays gives the same bits.
  * ws_dev: device memory of at least wpcg_paged_attention_workspace bytes
  * (16-byte aligned; may be null if that is 0), whose contents are nothing
  * before or after the call. Calls that may overlap need one each, also as
@@ -609,14 +626,15 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  *   last row's (all accepted) from p_r: the lowest id whose running sum of
  *   weights passes u_next[s] times their total (where p_r - q_r leaves no
  *   weight at all: from p_r).
- * A temperature not above 0 (null: all 1) is greedy: a draft is accepted while it is the
- * first largest logit, which also is the next token. accepted[s] receives the
+ * A temperature not above 0 (null: all 1) is greedy: a draft is accepted while
+ * it is the first largest logit, which also is the next token. accepted[s] receives the
  * number of accepted drafts, out the rows' tokens: the accepted drafts, the
  * next token, then -1. Probabilities, running sums and comparisons are fp64;
  * u and u_next are in [0, 1). A row without any weight (NaN, or no logit
  * above -inf) accepts nothing and gives next token -1; a draft id outside the
- * vocabulary is rejected; a sequence whose row range is empty, longer than max_rows or not within n_rows gets
- * accepted = -1 and none of its out is written. vocab <= 2^30, max_rows <=
+ * vocabulary is rejected; a sequence whose row range is empty, longer than
+ * max_rows or not within n_rows gets accepted = -1 and none of its out is
+ * written. vocab <= 2^30, max_rows <=
  * WPCG_DRAFT_MAX. Workspace and streams as for wpcg_paged_attention. */
 #define WPCG_DRAFT_MAX 64
 typedef struct wpcg_draft_s {

@@ -83,6 +83,8 @@ BAD_PAGES = [
     (dict(page_stride=1 << 20, head_stride=2048), E_SHAPE, "shorter"),
     (dict(page_stride=1 << 20, head_stride=2048, token_stride=132), E_SHAPE, "16 bytes"),
     (dict(page_stride=1 << 45, head_stride=2048, token_stride=128), E_ARG, "too large"),
+    # 16 tokens of a page 2^31 bytes apart in all: places in a page are 32-bit offsets
+    (dict(page_stride=1 << 32, head_stride=128, token_stride=1 << 26), E_ARG, "too large"),
     (dict(k=None), E_ARG, "null"), (dict(v=None), E_ARG, "null"), (dict(k=AT + 8), E_ARG, "aligned"),
 ]
 
@@ -101,6 +103,13 @@ def test_pages(kw, code, text):
 def test_batches(kw, code, text):
     refused(append(pages(), batch(**kw), rows()), code, text)
     refused(attend(pages(), batch(**kw), attention()), code, text)
+
+
+def test_model_verification():
+    a = np.zeros(4, np.uint32)
+    n = C.c_uint32()
+    at = a.ctypes.data_as(C.c_void_p)
+    refused(wpcg.lib.wpcg_model_verify_sampled(None, at, 4, None, at, 0.5, 1.0, C.byref(n), at), E_ARG, "null")
 
 
 def test_null_descriptions():

@@ -31,7 +31,7 @@ struct Layer {
 // most cap of them).
 struct Prefill {
     uint32_t cap = 0;
-    std::vector<void*> allocs;  // everything below but vlogits and vids
+    std::vector<void*> allocs;  // everything below down to dxs
     float *x = nullptr, *xn = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *attn = nullptr;
     float *g = nullptr, *u = nullptr;           // dense MLP [cap][inter]
     float *r = nullptr, *w = nullptr;           // router logits [cap][E], weights [cap][top_k]
@@ -46,6 +46,8 @@ struct Prefill {
     float* dxs = nullptr;
     float* vlogits = nullptr;  // verification: [WPCG_VERIFY_MAX][vocab], made on first use
     uint32_t* vids = nullptr;  // [WPCG_VERIFY_MAX]
+    float* draft_probs = nullptr;  // sampled verification: [WPCG_VERIFY_MAX - 1][vocab], made on first use
+    void* draft = nullptr;         // its other arrays and workspace
 };
 
 }  // namespace
@@ -673,6 +675,20 @@ int prefill_run(wpcg_model* m, uint32_t pos0, uint32_t n, uint32_t n_prompt)
     return WPCG_OK;
 }
 
+// The verification's logit rows and argmaxes.
+int make_verify(wpcg_model* m)
+{
+    Prefill& P = m->pf;
+    if (P.vlogits) return WPCG_OK;
+    if (!P.vids) {  // (the small one may be left from a call that could not have the other)
+        WPCG_HIP(hipMalloc(&P.vids, WPCG_VERIFY_MAX * 4));
+        m->allocs.push_back(P.vids);
+    }
+    WPCG_HIP(hipMalloc(&P.vlogits, (size_t)WPCG_VERIFY_MAX * m->cfg.vocab * 4));
+    m->allocs.push_back(P.vlogits);
+    return WPCG_OK;
+}
+
 // FAST verification of tokens[pos0 .. pos0+n-1] (n <= WPCG_VERIFY_MAX <= cap,
 // one pass): every row's logits (final norm, head as one batched GEMM) and
 // argmax; the position ends at pos0 + n.
@@ -682,14 +698,7 @@ int verify_run(wpcg_model* m, uint32_t pos0, uint32_t n)
     const wpcg_model_config& c = m->cfg;
     Prefill& P = m->pf;
     hipStream_t s = m->ctx->stream;
-    if (!P.vlogits) {
-        if (!P.vids) {  // (the small one may be left from a call that could not have the other)
-            WPCG_HIP(hipMalloc(&P.vids, WPCG_VERIFY_MAX * 4));
-            m->allocs.push_back(P.vids);
-        }
-        WPCG_HIP(hipMalloc(&P.vlogits, (size_t)WPCG_VERIFY_MAX * c.vocab * 4));
-        m->allocs.push_back(P.vlogits);
-    }
+    if (int rc = make_verify(m)) return rc;
     if (int rc = prefill_pass(m, pos0, n, s)) return rc;
     wpcg_linear* head = logits_head(m);
     WPCG_HIP(launch_rms_pack_rows(P.x, m->final_norm, (int)n, (int)c.hidden, c.eps, P.xf, P.xsum, s));
@@ -1223,6 +1232,81 @@ int wpcg_model_verify(wpcg_model* m, const uint32_t* tokens, uint32_t n, uint32_
         argmax[i] = m->hst.last;
     }
     m->hst_ok = true;
+    return WPCG_OK;
+}
+
+int wpcg_model_verify_sampled(wpcg_model* m, const uint32_t* tokens, uint32_t n, const float* draft_probs,
+                              const float* u, float u_next, float temperature, uint32_t* accepted, int32_t* out)
+{
+    if (!m || !tokens || !accepted || !out || (n > 1 && !u)) return fail(WPCG_E_ARG, "null argument");
+    if (n == 0 || n > WPCG_VERIFY_MAX) return fail(WPCG_E_ARG, "verify takes 1.." + std::to_string(WPCG_VERIFY_MAX) + " tokens");
+    for (uint32_t i = 0; i < n; i++)
+        if (tokens[i] >= m->cfg.vocab) return fail(WPCG_E_ARG, "token id out of range");
+    for (uint32_t i = 0; i < n; i++) {
+        const float v = i + 1 < n ? u[i] : u_next;
+        if (!(v >= 0.f && v < 1.f)) return fail(WPCG_E_ARG, "uniform numbers must be in [0, 1)");
+    }
+    if (int rc = ready(m)) return rc;
+    hipStream_t s = m->ctx->stream;
+    const size_t V = m->cfg.vocab;
+    if (int rc = host_state(m)) return rc;
+    DecodeState st = m->hst;
+    if ((uint64_t)st.pos + n > m->cfg.max_pos) return fail(WPCG_E_ARG, "KV cache full (max_pos reached)");
+    const uint32_t pos0 = st.pos;
+    if (int rc = make_verify(m)) return rc;
+    // what the decision reads beside the logits, for WPCG_VERIFY_MAX rows:
+    // tokens, u, u_next, temperature; accepted, out; then its workspace
+    wpcg_draft d{};
+    d.n_seq = 1;
+    d.n_rows = d.max_rows = WPCG_VERIFY_MAX;
+    d.vocab = (uint32_t)V;
+    uint64_t ws = 0;
+    if (int rc = wpcg_draft_verify_workspace(&d, &ws)) return rc;
+    constexpr size_t WORDS = 4 * WPCG_VERIFY_MAX;  // (a multiple of 16 bytes)
+    Prefill& P = m->pf;
+    if (!P.draft) {
+        WPCG_HIP(hipMalloc(&P.draft, WORDS * 4 + ws));
+        m->allocs.push_back(P.draft);
+    }
+    if (draft_probs && n > 1 && !P.draft_probs) {
+        WPCG_HIP(hipMalloc(&P.draft_probs, (size_t)(WPCG_VERIFY_MAX - 1) * V * 4));
+        m->allocs.push_back(P.draft_probs);
+    }
+    uint32_t words[WORDS] = {};
+    std::memcpy(words, tokens, n * 4);
+    if (n > 1) std::memcpy(words + WPCG_VERIFY_MAX, u, (n - 1) * 4);
+    std::memcpy(words + 2 * WPCG_VERIFY_MAX, &u_next, 4);
+    std::memcpy(words + 2 * WPCG_VERIFY_MAX + 1, &temperature, 4);
+    uint32_t* w = (uint32_t*)P.draft;
+    WPCG_HIP(hipMemcpyAsync(w, words, sizeof words, hipMemcpyHostToDevice, s));
+    if (draft_probs && n > 1)
+        WPCG_HIP(hipMemcpyAsync(P.draft_probs, draft_probs, (size_t)(n - 1) * V * 4, hipMemcpyHostToDevice, s));
+    WPCG_HIP(hipStreamSynchronize(s));  // `words` and the caller's arrays are read
+    st.n_prompt = 0xffffffffu;
+    if (int rc = put_state(m, st, tokens, n)) return rc;
+    m->hst_ok = false;
+    if (m->mode == WPCG_MODE_FAST && m->use_prefill && prefill_ok(m)) {
+        if (int rc = verify_run(m, pos0, n)) return rc;
+    } else {
+        for (uint32_t i = 0; i < n; i++) {
+            if (int rc = run_step(m, pos0 + i)) return rc;
+            WPCG_HIP(launch_copy_words(P.vlogits + i * V, m->logits, (uint32_t)V, s));
+        }
+    }
+    d.n_rows = d.max_rows = n;
+    d.logits_dev = P.vlogits;
+    d.draft_probs_dev = draft_probs && n > 1 ? P.draft_probs : nullptr;
+    d.tokens_dev = w;
+    d.u_dev = (const float*)w + WPCG_VERIFY_MAX;
+    d.u_next_dev = (const float*)w + 2 * WPCG_VERIFY_MAX;
+    d.temperature_dev = d.u_next_dev + 1;
+    d.out_dev = (int32_t*)w + 3 * WPCG_VERIFY_MAX;
+    d.accepted_dev = (int32_t*)w + 2 * WPCG_VERIFY_MAX + 2;
+    if (int rc = wpcg_draft_verify(m->ctx, &d, w + WORDS, ws, s)) return rc;
+    WPCG_HIP(hipMemcpyAsync(words, w, sizeof words, hipMemcpyDeviceToHost, s));
+    if (int rc = take_state(m, nullptr)) return rc;  // waits for the stream
+    *accepted = words[2 * WPCG_VERIFY_MAX + 2];
+    std::memcpy(out, words + 3 * WPCG_VERIFY_MAX, n * 4);
     return WPCG_OK;
 }
 

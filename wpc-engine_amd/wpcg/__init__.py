@@ -125,6 +125,8 @@ _SIGS = {
     "wpcg_model_prefill": (C.c_int, [_p, _p, C.c_uint32, _p, C.POINTER(C.c_uint32)]),
     "wpcg_model_set_prefill": (C.c_int, [_p, C.c_int]),
     "wpcg_model_verify": (C.c_int, [_p, _p, C.c_uint32, _p, _p]),
+    "wpcg_model_verify_sampled": (C.c_int, [_p, _p, C.c_uint32, _p, _p, C.c_float, C.c_float,
+                                            C.POINTER(C.c_uint32), _p]),
     "wpcg_model_set_position": (C.c_int, [_p, C.c_uint32]),
     "wpcg_model_debug_read": (C.c_int, [_p, C.c_int, _p, _u64]),
     "wpcg_rms_norm": (C.c_int, [_p, _p, _p, C.c_uint32, C.c_float, _p, C.c_int, _p]),
@@ -1087,6 +1089,23 @@ class Model:
         check(lib.wpcg_model_verify(self.h, _np_ptr(t), t.size, _np_ptr(ids),
                                     None if logits is None else _np_ptr(logits)))
         return ids, logits
+
+    def verify_sampled(self, tokens, u, u_next: float, draft_probs=None, temperature: float = 1.0):
+        """(number of drafts kept, int32[n]: the kept drafts, the next token, then -1)"""
+        t = np.ascontiguousarray(tokens, np.uint32)
+        u = np.ascontiguousarray(u, np.float32)
+        if u.size != max(t.size, 1) - 1:
+            raise ValueError(f"{t.size} tokens need {max(t.size, 1) - 1} uniform numbers, not {u.size}")
+        if draft_probs is not None:
+            draft_probs = np.ascontiguousarray(draft_probs, np.float32)
+            if draft_probs.shape != (u.size, self.cfg.vocab):
+                raise ValueError(f"draft_probs must be {(u.size, self.cfg.vocab)}, not {draft_probs.shape}")
+        n = C.c_uint32()
+        out = np.empty(t.size, np.int32)
+        check(lib.wpcg_model_verify_sampled(self.h, _np_ptr(t), t.size,
+                                            None if draft_probs is None else _np_ptr(draft_probs),
+                                            _np_ptr(u), u_next, temperature, C.byref(n), _np_ptr(out)))
+        return n.value, out
 
     def set_position(self, pos: int):
         check(lib.wpcg_model_set_position(self.h, pos))
