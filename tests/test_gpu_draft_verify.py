@@ -128,6 +128,24 @@ def test_masked_ties_and_rows_without_weight(ctx):
     assert (acc[3], out[9]) == (0, -1) and (acc[4], out[12]) == (0, -1) and (acc[5], out[15]) == (0, -1)
 
 
+def test_low_temperatures_and_large_logits(ctx):
+    """(x - max) / T is taken as a difference first: logits around 300 at
+    temperatures down to the smallest float."""
+    rng = np.random.default_rng(8)
+    c = case(rng, [3] * 7, 3001, temperature=[1, 1e-3, 1e-6, 1e-12, 1e-20, 1e-38, 1e-45])
+    c["logits"] += np.float32(300)
+    lg = c["logits"]
+    lg[4:8, 1000:1006] = lg[4:8].max(-1, keepdims=True) + np.float32(0.001) * np.arange(6, dtype=np.float32)
+    lg[8:12, 500] = lg[8:12, 77] = lg[8:12].max(-1) + 1  # equal ones share the weight at any temperature
+    lg[16:20, 2999] = lg[16:20, 5] = lg[16:20].max(-1) + 1
+    for s in range(1, 7):  # drafts that are likely there
+        c["tokens"][4 * s + 1:4 * s + 3] = lg[4 * s:4 * s + 2].argmax(-1)
+    acc, out = run(ctx, c)
+    wa, wo = want(c)
+    assert np.array_equal(acc, wa) and np.array_equal(out, wo)
+    assert acc[1:].min() >= 1
+
+
 def test_bounds_of_u_next(ctx):
     """0 takes the first id with weight, the largest float below 1 the last ones."""
     rng = np.random.default_rng(5)

@@ -24,14 +24,15 @@ namespace {
 constexpr int THREADS = 256, CHUNK = DRAFT_CHUNK;
 static_assert(CHUNK == 8 * THREADS, "pick: eight ids a thread");
 
-// 2^y for y <= 0 (or NaN): y = n + f, n the whole number that adding 1.5 * 2^52
-// leaves in the low bits, the polynomial of degree 8 through 2^f at the nine
-// Chebyshev points of +-1/2 (within 1.1e-12 of it there), n added to its
-// exponent. 0 below 2^-1000.
-__device__ __forceinline__ double exp2_d(double y)
+// 2^(x rate) for x <= 0 (or NaN), a difference of two logits: x rate = n + f, n
+// the whole number that adding 1.5 * 2^52 leaves in the low bits, the
+// polynomial of degree 8 through 2^f at the nine Chebyshev points of +-1/2
+// (within 1.1e-12 of it there), n added to its exponent. 0 below 2^-1000.
+__device__ __forceinline__ double exp2_d(double x, double rate)
 {
-    const double t = y + 6755399441055744.0;
-    const double f = y - (t - 6755399441055744.0);
+    const double t = fma(x, rate, 6755399441055744.0);
+    const double whole = t - 6755399441055744.0;
+    const double f = fma(x, rate, -whole);
     double r = 1.3255224878668817e-06;
     r = fma(r, f, 1.5310079402249296e-05);
     r = fma(r, f, 0.00015403455852453838);
@@ -43,7 +44,7 @@ __device__ __forceinline__ double exp2_d(double y)
     r = fma(r, f, 1.0);
     const uint64_t n = (uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, t) << 52;
     r = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, r) + n);
-    return y < -1000.0 ? 0.0 : r;
+    return whole < -1000.0 ? 0.0 : r;
 }
 
 struct Rows {
@@ -162,9 +163,9 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
     int at = 0x7fffffff;
     double sum = 0.0;
     if (rate > 0.0) {
-        const double base = best == -INFINITY ? 0.0 : -(double)best * rate;
+        const double base = best == -INFINITY ? 0.0 : (double)best;
 #pragma unroll
-        for (int i = 0; i < CHUNK / 64; i++) sum += exp2_d(fma((double)c.v[i], rate, base));
+        for (int i = 0; i < CHUNK / 64; i++) sum += exp2_d((double)c.v[i] - base, rate);
         sum = wave_sum_d(sum);
     } else {
 #pragma unroll
@@ -201,7 +202,7 @@ __device__ __forceinline__ RowState row_state(const DraftArgs& p, int row, doubl
         const float old = m;
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) larger(m, at, c[j].max, c[j].at);
-        const auto to_m = [&](float v) { return v == -INFINITY ? 1.0 : exp2_d(((double)v - (double)m) * rate); };
+        const auto to_m = [&](float v) { return v == -INFINITY ? 1.0 : exp2_d((double)v - (double)m, rate); };
         z *= to_m(old);
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) z += c[j].sum * to_m(c[j].max);
@@ -213,7 +214,7 @@ __device__ __forceinline__ RowState row_state(const DraftArgs& p, int row, doubl
         const int j = __shfl_xor(at, d);
         larger(m, at, v, j);
     }
-    z *= mine == -INFINITY ? 1.0 : exp2_d(((double)mine - (double)m) * rate);
+    z *= mine == -INFINITY ? 1.0 : exp2_d((double)mine - (double)m, rate);
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) z += __shfl_xor(z, d);
     return {z, m, at};
@@ -240,7 +241,7 @@ __device__ __forceinline__ Choice choose(const DraftArgs& p, int s, const Rows& 
         const RowState st = row_state(p, (int)r, rate);
         int ok = 0;
         if (rate == 0.0) ok = drafted && st.m > -INFINITY && d == (uint32_t)st.at;
-        else if (inside) ok = (double)u * (double)w < exp2_d(((double)x - (double)st.m) * rate) / st.z;
+        else if (inside) ok = (double)u * (double)w < exp2_d((double)x - (double)st.m, rate) / st.z;
         if ((threadIdx.x & 31) == 0) {
             s_st[i] = st;
             s_ok[i] = ok;
@@ -258,7 +259,7 @@ __device__ __forceinline__ Choice choose(const DraftArgs& p, int s, const Rows& 
 // Z times an id's weight in the row, from its logit x and the drafter's q
 __device__ __forceinline__ double weight(float x, float q, const RowState& st, double rate, bool rest)
 {
-    const double e = exp2_d(fma((double)x, rate, -(double)st.m * rate));
+    const double e = exp2_d((double)x - (double)st.m, rate);
     if (!rest) return e;
     const double w = e - (double)q * st.z;
     return w > 0.0 || w != w ? w : 0.0;
@@ -287,7 +288,7 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
     const auto of_chunk = [&](int i) {
         if (rest) return __hip_atomic_load(&p.rest[(uint64_t)s * p.chunks + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const DraftPart& part = p.part[(uint64_t)row * p.chunks + i];
-        return part.max == -INFINITY ? 0.0 : part.sum * exp2_d(((double)part.max - (double)c.st.m) * rate);
+        return part.max == -INFINITY ? 0.0 : part.sum * exp2_d((double)part.max - (double)c.st.m, rate);
     };
     // a thread's run of chunks
     const int run = (p.chunks + THREADS - 1) / THREADS;
