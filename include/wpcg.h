@@ -524,12 +524,13 @@ int wpcg_model_debug_read(wpcg_model* m, int which, float* out, uint64_t n);
  * them. Rows of no sequence are left as they were. Nothing outside the
  * arrays is read or written whatever the device arrays hold: a sequence whose
  * row range is not within 0..n_rows, in order and at most max_q long is left
- * out; one whose kv_len is not in 0..max_kv, or that needs a page whose id is
- * not in 0..n_pages-1, gets NaN in its output rows and nothing is stored for
- * the tokens concerned. A sequence longer in rows than in tokens (kv_len < n)
- * has rows before position 0; they append nothing and see nothing. Row ranges
- * that overlap (q_start falls somewhere) leave it open whose result the shared
- * rows hold. */
+ * out; one whose kv_len is not in 0..max_kv gets NaN in its output rows and
+ * stores nothing; a page whose id is not in 0..n_pages-1 gives NaN in the rows
+ * that need it (attention: maybe in the sequence's others too) and stores
+ * nothing of them. A sequence longer in rows than in tokens (kv_len < n)
+ * has rows before position 0; they append nothing and see nothing. Where
+ * q_start falls from one sequence to the next, which sequences are left out
+ * and whose results shared rows hold is open. */
 #define WPCG_DTYPE_E4M3 3
 typedef struct wpcg_kv_pages_s {
     void* k_dev;
@@ -584,7 +585,9 @@ int wpcg_kv_append(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* 
  * t < sinks (the first tokens stay visible). A row that sees nothing gives
  * zeros; what the cache holds at tokens a row does not see (NaN, infinities)
  * does not reach it, and pages whose tokens no row sees are not looked at, so
- * a window's old pages may be given away and their ids be anything.
+ * a window's old pages may be given away and their ids be anything. Keys,
+ * values and queries that are not finite may make outputs of the rows that do
+ * see them infinite or NaN. Single tokens, drafts and prompts may share a call.
  * q and out are rows of dtype F32 or BF16 (0 strides = packed). An F32 q keeps
  * fp32 accuracy whatever the cache holds; a BF16 q goes with a BF16 or E4M3
  * cache (an F32 cache is E_UNSUPPORTED) and rounds the softmax's terms to
@@ -627,14 +630,15 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  *   weights passes u_next[s] times their total (where p_r - q_r leaves no
  *   weight at all: from p_r).
  * A temperature not above 0 (null: all 1) is greedy: a draft is accepted while
- * it is the first largest logit, which also is the next token. accepted[s] receives the
- * number of accepted drafts, out the rows' tokens: the accepted drafts, the
- * next token, then -1. Probabilities, running sums and comparisons are fp64;
- * u and u_next are in [0, 1). A row without any weight (NaN, or no logit
- * above -inf) accepts nothing and gives next token -1; a draft id outside the
- * vocabulary is rejected; a sequence whose row range is empty, longer than
- * max_rows or not within n_rows gets accepted = -1 and none of its out is
- * written. vocab <= 2^30, max_rows <=
+ * it is the first largest logit, which also is the next token. accepted[s]
+ * receives the number of accepted drafts, out the rows' tokens: the accepted
+ * drafts, the next token, then -1. Probabilities, running sums and comparisons
+ * are fp64; u and u_next are in [0, 1). A row without any weight (NaN, +inf, or
+ * no logit above -inf; greedy rows pass NaN over) accepts nothing and gives
+ * next token -1; where the drafter's row leaves no weight or NaN, p_r is taken;
+ * a draft id outside the vocabulary is rejected; a sequence whose row range is
+ * empty, longer than max_rows or not within n_rows gets accepted = -1 and none
+ * of its out is written (q_start must not fall). vocab <= 2^30, max_rows <=
  * WPCG_DRAFT_MAX. Workspace and streams as for wpcg_paged_attention. */
 #define WPCG_DRAFT_MAX 64
 typedef struct wpcg_draft_s {

@@ -122,6 +122,45 @@ def test_split_and_joined(ctx, q_dtype, dtype, rows, lens, heads, hkv, window):
 
 
 @pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("singles,prompts,lens,heads,hkv,window", [
+    (5, [70, 9, 8, 0, 33], (1, 400), 8, 2, 0), (70, [200, 5], (20, 300), 8, 2, 60), (150, [300], (1, 90), 4, 4, 0),
+    (3, [90], (2000, 6000), 8, 2, 0), (6, [20, 150, 1], (10, 700), 20, 1, 0), (4, [40], (10, 700), 64, 1, 0)])
+@pytest.mark.parametrize("max_kv", [None, 6500, 1000000])
+def test_prompts_among_single_tokens(ctx, q_dtype, dtype, singles, prompts, lens, heads, hkv, window, max_kv):
+    """A batch's short and long row ranges are two kernels' work where it may be
+    long: around the border (32 columns: 8 rows of 4 heads and 9), more sequences than a wave
+    looks through at once, long sequences of few rows beside a prompt, groups
+    of 20 and of 64 heads (none of its rows is the few-row kernel's); a bad
+    length and a bad page in either part, rows of no sequence as they were."""
+    print(f"[gpu] mixed: {q_dtype}/{dtype} {singles} + {prompts} {heads}/{hkv} window {window}", flush=True)
+    rng = np.random.default_rng(singles + heads + q_dtype + 10 * dtype)
+    rows = [1] * singles + prompts
+    order = rng.permutation(len(rows))
+    rows = [rows[i] for i in order]
+    kv = [int(x) + r for x, r in zip(rng.integers(*lens, len(rows)), rows)]
+    pg = R.Paged(ctx, rng, dtype, hkv, 64, 16, kv, scales=dtype == E4M3, width=(max_kv or 0) // 16 + 1).upload()
+    n = sum(rows)
+    q = R.encode(rng.standard_normal((n + 7, heads, 64)) * 1.5, q_dtype)
+    batch = pg.batch(rows, n_rows=n + 7, max_kv=max_kv)
+    want, bound = expected(pg, q[:n], rows, heads, q_dtype, 0.125, window, 9)
+    got, op = run(ctx, pg, batch, q, heads, q_dtype, 0.125, window, 9)
+    fill = R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]
+    check(got[:n], want, bound)
+    assert (got[n:] == fill).all()
+    at = np.cumsum([0] + rows)
+    one, many = rows.index(1), int(np.argmax(rows))
+    pg.table[many, kv[many] // 16 - 1] = -3  # the prompt's last whole page, which its last row sees
+    pg.d_table.write(pg.table)
+    pg.d_len.write(np.array([-1 if s == one else m for s, m in enumerate(kv)], np.int32))
+    got, _ = run(ctx, pg, batch, q, heads, q_dtype, 0.125, window, 9)
+    assert np.isnan(got[at[one]]).all() and np.isnan(got[at[many + 1] - 1]).all()
+    for s in range(len(rows)):
+        if s not in (one, many) and rows[s]:
+            part = slice(at[s], at[s + 1])
+            check(got[part], want[part], bound[part])
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
 @pytest.mark.parametrize("rows,heads,hkv,d,window", [(1, 8, 2, 128, 0), (1, 4, 4, 64, 0), (5, 8, 2, 128, 0),
                                                      (3, 7, 1, 64, 2000), (2, 8, 2, 128, 40000)])
 def test_tiles_dealt_out(ctx, q_dtype, dtype, rows, heads, hkv, d, window):

@@ -158,6 +158,12 @@ def test_too_many_workgroups():
     refused(attend(pages(), batch(n_seq=1 << 20, n_rows=1 << 30, max_q=1 << 20), attention()), E_UNSUPPORTED, "workgroups")
     refused(append(pages(n_kv_heads=64), batch(n_rows=1 << 30), rows(n_heads=64)), E_UNSUPPORTED, "workgroups")
     refused(verify(draft(n_rows=1 << 25, vocab=1 << 20)), E_UNSUPPORTED, "workgroups")
+    # a launch's threads have to fit 32 bits: 256 a workgroup, one for a row or chunk
+    refused(append(pages(), batch(n_rows=1 << 24), rows()), E_UNSUPPORTED, "workgroups")
+    refused(append(pages(), batch(n_rows=(1 << 24) - 1), rows()), E_ARG, "null context")
+    refused(verify(draft(n_rows=1 << 24)), E_UNSUPPORTED, "workgroups")
+    refused(attend(pages(), batch(n_seq=1 << 22, n_rows=1 << 22, max_q=1), attention()), E_UNSUPPORTED, "workgroups")
+    refused(attend(pages(), batch(n_seq=1 << 21, n_rows=1 << 21, max_q=1), attention()), E_ARG, "null context")
 
 
 def workspace(kv, b, a):

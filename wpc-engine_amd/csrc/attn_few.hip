@@ -566,14 +566,14 @@ __global__ __launch_bounds__(THREADS, 2) void k_attn_few(PagedAttnArgs p)
     const int v0 = split * p.chunk, v1 = min(v0 + p.chunk, seen.total());
     if (v0 >= v1 && split > 0) return;
     const uint64_t part = (((uint64_t)split * pairs + pair) * p.col_blocks + cb) * COLS;
-    const bool whole = p.splits == 1;
+    const bool whole = p.splits == 1 || seen.total() <= p.chunk;
     attend<D, CT, QF32, NB>(p, sh, sq, seq, pair % p.n_kv, cb, seen, v0, v1, whole ? nullptr : p.part_o + part * D,
                             whole ? nullptr : p.part_ml + part * 2);
 }
 
 // Joins the chunks: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over
-// those that the row's workgroups had, in an order that depends on the call's
-// bounds alone. PAR groups of D/4 threads share a (row, query head): one where
+// those that the row's workgroups had (where one had all it wrote the outputs),
+// in an order that depends on the call's bounds alone. PAR groups of D/4 threads share a (row, query head): one where
 // the chunks are few, eight where they are many.
 template <int D, bool QF32, int PAR>
 __global__ __launch_bounds__(256) void k_attn_few_join(PagedAttnArgs p)
@@ -589,7 +589,7 @@ __global__ __launch_bounds__(256) void k_attn_few_join(PagedAttnArgs p)
     const int row = (int)(rest / (unsigned)p.b.n_seq), seq = (int)(rest % (unsigned)p.b.n_seq);
     SeqRows sq = {};
     if (row < p.b.max_q) sq = seq_rows(p.b, seq);
-    const bool live = row < sq.n;
+    bool live = row < sq.n;
     float m = -INFINITY, l = 0.0f;
     pf32x4 o = {};
     if (live) {
@@ -597,7 +597,8 @@ __global__ __launch_bounds__(256) void k_attn_few_join(PagedAttnArgs p)
         const int cols = sq.n * p.group, pos0 = (sq.bad ? 0 : sq.len) - sq.n;
         const int first = cb * p.cols / p.group, last = (min(cols, (cb + 1) * p.cols) - 1) / p.group;
         const int tiles = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks).total();
-        const int n = max(1, (tiles + p.chunk - 1) / p.chunk);
+        live = tiles > p.chunk;
+        const int n = live ? (tiles + p.chunk - 1) / p.chunk : 0;
         const uint64_t step = (uint64_t)p.b.n_seq * p.n_kv * p.col_blocks * p.cols;
         const uint64_t at0 = ((uint64_t)(seq * p.n_kv + kvh) * p.col_blocks + cb) * p.cols + col % p.cols;
         for (int i0 = part; i0 < n; i0 += 8 * PAR) {  // eight in flight

@@ -394,8 +394,8 @@ __device__ __forceinline__ void terms(const pf32x16& s, int i0, float sc, float 
 }
 // A column's output, or its part of it.
 template <int D, int CW, bool QF32>
-__device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& sq, int split, int row, int head, float m,
-                                        float l, const pf32x16 (&acc)[D / 32], float v_scale)
+__device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& sq, bool part, int split, int row, int head,
+                                        float m, float l, const pf32x16 (&acc)[D / 32], float v_scale)
 {
     constexpr int NCH = D / CW;
     const int h = ((int)threadIdx.x & 63) >> 5;
@@ -408,7 +408,7 @@ __device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& s
 #pragma unroll
             for (int j = 0; j < CW; j++) o[j] = acc[j * NCH / 32][4 * (j * NCH % 32 / 8 + a0) + b0];
             const int d = CW * (8 * a0 + 4 * h + b0);
-            if (p.splits > 1) {
+            if (part) {
 #pragma unroll
                 for (int j = 0; j < CW; j += 4)
                     *(pf32x4*)(p.part_o + slot * D + d + j) = (pf32x4){o[j], o[j + 1], o[j + 2], o[j + 3]};
@@ -416,7 +416,7 @@ __device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& s
                 attn_store<CW, QF32>(p, sq, row, head, d, D, o, l, v_scale);
             }
         }
-    if (p.splits > 1 && h == 0) {
+    if (part && h == 0) {
         p.part_ml[slot * 2] = m;
         p.part_ml[slot * 2 + 1] = l;
     }
@@ -437,6 +437,36 @@ __device__ __forceinline__ pf32x16 mul_terms(const pbf16x8 (&a)[NA], const pbf16
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], acc, 0, 0, 0);
 }
 
+// Column block `at` of all the sequences' ones, laid end to end: first those of
+// sequences with several, the last, which sees most, foremost. Every wave looks
+// by itself, 64 sequences at a time.
+template <int COLS>
+__device__ __forceinline__ bool find_block(const PagedAttnArgs& p, int at, int& seq, int& cb)
+{
+    const int lane = (int)threadIdx.x & 63;
+    for (int pass = 0; pass < 2; pass++)
+        for (int s0 = 0; s0 < p.b.n_seq; s0 += 64) {
+            const int s = s0 + lane;
+            int v = s < p.b.n_seq ? (seq_rows(p.b, s).n * p.group + COLS - 1) / COLS : 0;
+            if ((v > 1) != (pass == 0)) v = 0;
+            int t = v;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int u = __shfl_up(t, d);
+                if (lane >= d) t += u;
+            }
+            const uint64_t behind = __ballot(t > at);
+            if (behind) {
+                const int l = __builtin_ctzll(behind);
+                seq = s0 + l;
+                cb = __builtin_amdgcn_readlane(t, l) - 1 - at;
+                return true;
+            }
+            at -= __builtin_amdgcn_readlane(t, 63);
+        }
+    return false;
+}
+
 // Two waves a SIMD (F32 queries: one), so that one's exponentials run beside
 // the other's products: two workgroups of four waves a CU, or one of eight
 // where there are columns enough, which brings in each tile once for 256 of
@@ -450,13 +480,23 @@ __global__ __launch_bounds__(64 * WAVES, QF32 ? 1 : 2) void k_attn_many(PagedAtt
     __shared__ __attribute__((aligned(16))) uint16_t s_v[S::NBUF][S::NK][S::VALUES];
     __shared__ int s_odd[S::NBUF][4], s_fault;
 
-    // block -> (column block, chunk, sequence and head): the blocks of a head
+    // workgroup -> column block, chunk, sequence and head: the blocks of a head
     // are `pairs` apart, so that with a multiple of 8 pairs they run on one
     // die and share its L2; the last column blocks, which see most, come first
-    const int pairs = p.b.n_seq * p.n_kv;
-    const int pair = (int)(blockIdx.x % (unsigned)pairs), rest = (int)(blockIdx.x / (unsigned)pairs);
-    const int split = rest % p.splits, cb = p.col_blocks - 1 - rest / p.splits;
-    const int seq = pair / p.n_kv, kvh = pair % p.n_kv;
+    int seq, kvh, cb, split;
+    if (p.blocks == 0) {
+        const int pairs = p.b.n_seq * p.n_kv;
+        const int pair = (int)(blockIdx.x % (unsigned)pairs), rest = (int)(blockIdx.x / (unsigned)pairs);
+        split = rest % p.splits;
+        cb = p.col_blocks - 1 - rest / p.splits;
+        seq = pair / p.n_kv;
+        kvh = pair % p.n_kv;
+    } else {
+        const int rest = (int)(blockIdx.x / (unsigned)p.n_kv);
+        split = rest % p.splits;
+        kvh = (int)(blockIdx.x % (unsigned)p.n_kv);
+        if (!find_block<COLS>(p, rest / p.splits, seq, cb)) return;
+    }
     const SeqRows sq = seq_rows(p.b, seq);
     const int cols = sq.n * p.group;
     if (cb * COLS >= cols) return;
@@ -572,7 +612,7 @@ __global__ __launch_bounds__(64 * WAVES, QF32 ? 1 : 2) void k_attn_many(PagedAtt
     if (!live) return;
     l = sum_x32(l);
     if (s_fault) l = __builtin_nanf("");
-    put_out<D, S::CW, QF32>(p, sq, split, row, head, m, l, acc, p.v_scale ? p.v_scale[kvh] : 1.0f);
+    put_out<D, S::CW, QF32>(p, sq, p.splits > 1 && seen.total() > p.chunk, split, row, head, m, l, acc, p.v_scale ? p.v_scale[kvh] : 1.0f);
 }
 
 template <int D, int CT, bool QF32>
@@ -602,7 +642,8 @@ void go_types(const PagedAttnArgs& p, int q_dtype, int cache_dtype, unsigned blo
 
 // ---- the chunks' states joined -------------------------------------------------
 // out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the chunks that the
-// row's workgroup had, in their order; D/4 threads a (row, query head).
+// row's workgroups had (where one had all it wrote the outputs), in their order;
+// D/4 threads a (row, query head).
 template <int D, bool QF32>
 __global__ __launch_bounds__(256) void k_attn_many_join(PagedAttnArgs p)
 {
@@ -610,16 +651,24 @@ __global__ __launch_bounds__(256) void k_attn_many_join(PagedAttnArgs p)
     const int tid = (int)threadIdx.x, d = tid % TH * 4;
     const uint64_t x = (uint64_t)blockIdx.x * PER + tid / TH;
     const int head = (int)(x % (unsigned)p.n_heads);
-    const uint64_t rest = x / (unsigned)p.n_heads;
-    const int row = (int)(rest / (unsigned)p.b.n_seq), seq = (int)(rest % (unsigned)p.b.n_seq);
-    if (row >= p.b.max_q) return;
-    const SeqRows sq = seq_rows(p.b, seq);
-    if (row >= sq.n) return;
+    const uint64_t at = x / (unsigned)p.n_heads;
+    if (at >= (uint64_t)p.b.n_rows) return;
+    // the row's sequence: the last one that starts at or before it
+    int lo = 0, hi = p.b.n_seq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if ((p.b.q_start ? p.b.q_start[mid] : mid) <= (int)at) lo = mid;
+        else hi = mid - 1;
+    }
+    const SeqRows sq = seq_rows(p.b, lo);
+    const int row = (int)at - sq.a;
+    if (row < 0 || row >= sq.n) return;
     const int cols = sq.n * p.group, cb = (row * p.group + head % p.group) / p.cols;
     const int len = sq.bad ? 0 : sq.len, pos0 = len - sq.n;
     const int first = cb * p.cols / p.group, last = (min(cols, (cb + 1) * p.cols) - 1) / p.group;
     const int tiles = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks).total();
-    const int n = max(1, (tiles + p.chunk - 1) / p.chunk);
+    if (tiles <= p.chunk) return;
+    const int n = (tiles + p.chunk - 1) / p.chunk;
     const uint64_t slot0 = (uint64_t)(sq.a + row) * p.n_heads + head;
     const uint64_t step = (uint64_t)p.b.n_rows * p.n_heads;
     float m = -INFINITY, l = 0.0f;
@@ -646,7 +695,7 @@ __global__ __launch_bounds__(256) void k_attn_many_join(PagedAttnArgs p)
 template <int D, bool QF32>
 void join(const PagedAttnArgs& p, hipStream_t s)
 {
-    const uint64_t all = (uint64_t)p.b.n_seq * p.b.max_q * p.n_heads;
+    const uint64_t all = (uint64_t)p.b.n_rows * p.n_heads;
     k_attn_many_join<D, QF32><<<dim3((unsigned)((all * (D / 4) + 255) / 256)), dim3(256), 0, s>>>(p);
 }
 
@@ -654,7 +703,8 @@ void join(const PagedAttnArgs& p, hipStream_t s)
 
 hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s)
 {
-    const uint64_t blocks = (uint64_t)p.b.n_seq * p.n_kv * p.col_blocks * p.splits;
+    const uint64_t blocks =
+        (p.blocks ? (uint64_t)p.blocks : (uint64_t)p.b.n_seq * p.col_blocks) * p.n_kv * p.splits;
     if (blocks == 0) return hipSuccess;
     const bool f32 = q_dtype == WPCG_DTYPE_F32;
     if (head_dim == 128) {

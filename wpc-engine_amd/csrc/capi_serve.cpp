@@ -12,6 +12,7 @@ namespace {
 
 constexpr int64_t CUS = 256;  // of an MI355X
 constexpr uint64_t INT_BOUND = 1u << 30;  // of rows, tokens, heads: sums of two stay ints
+constexpr int64_t GROUPS_256 = 1 << 24, GROUPS_512 = 1 << 23;  // workgroups of a launch: its threads fit 32 bits
 
 uint64_t type_size(int dtype) { return dtype == WPCG_DTYPE_F32 ? 4 : dtype == WPCG_DTYPE_BF16 ? 2 : 1; }
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -81,7 +82,7 @@ int check_batch(const wpcg_kv_batch* b, const wpcg_kv_pages* kv, PagedBatch* out
     }
     int shift = 0;
     while ((1u << shift) < kv->page_size) shift++;
-    *out = {(int)b->n_seq, (int)b->n_rows, (int)std::min(b->max_q, b->n_rows), (int)b->max_kv, kv->n_pages,
+    *out = {(int)b->n_seq, (int)b->n_rows, 0, (int)std::min(b->max_q, b->n_rows), (int)b->max_kv, kv->n_pages,
             (int)kv->page_size, shift, b->table_stride, b->q_start_dev, b->kv_len_dev, b->table_dev};
     return WPCG_OK;
 }
@@ -95,9 +96,12 @@ int check_pointers(const wpcg_kv_pages* kv, const wpcg_kv_batch* b)
     return WPCG_OK;
 }
 
+// One kernel's part of a call.
 struct Plan {
+    PagedBatch b;  // with the rows a sequence that it takes
     bool many;
     int cols, col_blocks, blocks, chunk, splits;
+    double us;       // of a workgroup's tiles, by estimate
     uint64_t parts;  // columns whose states the workspace holds
     uint64_t bytes;
 };
@@ -105,11 +109,16 @@ struct Plan {
 // Which kernel, and how many workgroups share a sequence's tokens. The bounds
 // stand in for the lengths, which only the device knows; a shorter sequence
 // just has fewer chunks.
-int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attention* a, Plan* out)
+int plan_kernel(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attention* a, Plan* out)
 {
     const int64_t group = a->n_heads / kv->n_kv_heads, cols = (int64_t)b.max_q * group;
-    const int64_t pairs = (int64_t)b.n_seq * kv->n_kv_heads;
+    // column blocks of all sequences together: each one's last may be a part of one
+    const auto all_blocks = [&](int64_t cw) {
+        const int64_t seqs = std::min<int64_t>(b.n_seq, b.n_rows / std::max(1, b.min_q));
+        return std::min(b.n_seq * ((cols + cw - 1) / cw), (int64_t)b.n_rows * group / cw + seqs);
+    };
     Plan p;
+    p.b = b;
     p.many = cols > 2 * ATTN_FEW_COLS;
     const int64_t tw = p.many ? ATTN_MANY_TILE : ATTN_FEW_TILE;
     // tiles that a block of cw columns can see
@@ -127,13 +136,19 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
         // 18 tiles a block (a window of 1024) 238 us against 232, for a CU's
         // one workgroup starts and ends alone.
         const int64_t wide = 2 * ATTN_MANY_COLS;
-        p.cols = a->dtype == WPCG_DTYPE_BF16 && tiles_of(wide) >= 32 && pairs * ((cols + wide - 1) / wide) >= CUS
+        p.cols = a->dtype == WPCG_DTYPE_BF16 && tiles_of(wide) >= 32 && kv->n_kv_heads * all_blocks(wide) >= CUS
                      ? wide : ATTN_MANY_COLS;
     } else {
         // (over an F32 cache the wider form's registers do not suffice)
         p.cols = cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
     }
-    const int64_t blocks = (cols + p.cols - 1) / p.cols, base = pairs * blocks, tiles = tiles_of(p.cols);
+    const int64_t blocks = (cols + p.cols - 1) / p.cols, tiles = tiles_of(p.cols);
+    // Workgroups of the many-row kernel look for their work where that saves
+    // half of them, for empty ones are not free: 255 sequences of 512 tokens
+    // with one new row each and a prompt of 1024, 32 / 8 heads, 223 us without,
+    // 154 so; 63 of 2048 and a prompt of 2048 282 and 170
+    const bool look = p.many && b.n_seq * blocks > 2 * all_blocks(p.cols);
+    const int64_t base = kv->n_kv_heads * (look ? all_blocks(p.cols) : b.n_seq * blocks);
     // The cheapest split by this estimate, in microseconds: workgroups run in
     // rounds of those the chip holds; each has 4 us of start and end and its
     // tiles, and a split one a second launch of 5 us. A tile of the few-row
@@ -151,12 +166,15 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
         return rounds * (4.0 + (double)((tiles + s - 1) / s) * tile) + (s > 1 ? 5.0 : 0.0);
     };
     const int64_t least = p.many ? 2 : ATTN_FEW_WAVES;  // tiles of a chunk
+    // (the many-row kernel's parts are of all n_rows, which may be a loose bound)
+    const int64_t room_parts = p.many && (int64_t)b.n_rows * a->n_heads > 1 << 20 ? 0 : 4 * room;
     int64_t best = 1;
-    for (int64_t s = 2; base > 0 && s <= tiles / least && base * s <= 4 * room; s++)
+    for (int64_t s = 2; base > 0 && s <= tiles / least && base * s <= room_parts; s++)
         if (cost(s) < cost(best)) best = s;
     p.chunk = (int)std::max<int64_t>(1, (tiles + best - 1) / best);
     p.splits = (int)std::max<int64_t>(1, (tiles + p.chunk - 1) / p.chunk);
-    p.blocks = 0;
+    p.us = p.chunk * tile;
+    p.blocks = look ? (int)all_blocks(p.cols) : 0;
     p.parts = p.splits == 1 ? 0 : p.many ? (uint64_t)p.splits * b.n_rows * a->n_heads : (uint64_t)p.splits * base * p.cols;
     // A chunk that long may be one sequence's alone while the others' are
     // empty, for the bounds do not tell: all tiles are dealt out evenly
@@ -164,18 +182,52 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
     // us with a workgroup a sequence and head, 79 so. It costs a few us more
     // where the lengths are less unlike: 64 sequences of 512 to 4096 tokens 67
     // and 75 us.)
-    if (!p.many && p.chunk * tile > 130.0 && b.n_seq <= ATTN_DEAL_SEQS && base * tiles < (int64_t)1 << 30) {
+    if (!p.many && p.us > 130.0 && b.n_seq <= ATTN_DEAL_SEQS && base * tiles < (int64_t)1 << 30) {
         p.blocks = CUS;
         p.parts = 2 * CUS * p.cols;
         p.splits = 1;
     }
     p.col_blocks = (int)std::max<int64_t>(1, blocks);
-    if (base * p.splits >= (int64_t)1 << 31 || (uint64_t)b.n_seq * b.max_q * a->n_heads >= 1u << 31)
+    // (a batch that is split has few workgroups, and its join few rows)
+    if (base * p.splits >= GROUPS_512)
         return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
-    p.bytes = p.parts * (kv->head_dim + 2) * sizeof(float) + p.blocks * sizeof(AttnEnd);
+    p.bytes = p.parts * (kv->head_dim + 2) * sizeof(float) + (p.many ? 0 : p.blocks * sizeof(AttnEnd));
     *out = p;
     return WPCG_OK;
 }
+
+struct Plans {
+    Plan part[2];
+    int n;
+    uint64_t bytes;  // they share the workspace: one runs behind the other
+};
+
+// A batch that may hold prompts and single tokens or drafts is two parts where
+// the tokens may be many: the few-row kernel shares a long sequence's tokens out
+// over the chip, the many-row one leaves them to a workgroup or few. Sequences
+// with one new row each beside one prompt, 32 / 8 heads, by the many-row kernel
+// alone and in two parts: 3 of 100000 tokens and a prompt of 2048 656 and 314
+// us, 63 of 4096 and 512 224 and 216, 63 of 2048 and 2048 (a workgroup's tiles
+// 77 us) 170 and 172.
+int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attention* a, Plans* out)
+{
+    out->n = 1;
+    if (int rc = plan_kernel(kv, b, a, &out->part[0])) return rc;
+    const int64_t few = 2 * ATTN_FEW_COLS / (a->n_heads / kv->n_kv_heads);  // rows that the few-row kernel takes
+    const int64_t all = (int64_t)b.n_seq * b.max_q;
+    if (out->part[0].many && few > 0 && b.n_seq > 1 && b.n_rows <= all - b.max_q + few && out->part[0].us > 100.0) {
+        PagedBatch part[2] = {b, b};
+        part[0].max_q = (int)few;
+        part[1].min_q = (int)few + 1;
+        out->n = 2;
+        for (int i = 0; i < 2; i++)
+            if (int rc = plan_kernel(kv, part[i], a, &out->part[i])) return rc;
+    }
+    out->bytes = 0;
+    for (int i = 0; i < out->n; i++) out->bytes = std::max(out->bytes, out->part[i].bytes);
+    return WPCG_OK;
+}
+
 
 int check_attention(const wpcg_kv_pages* kv, const wpcg_attention* a)
 {
@@ -204,7 +256,7 @@ int check_draft(const wpcg_draft* d, int* chunks, uint64_t* bytes)
         return fail(WPCG_E_SHAPE, "row stride shorter than the row");
     if (d->logits_stride >> 40 || d->draft_stride >> 40) return fail(WPCG_E_ARG, "row stride too large");
     *chunks = (int)((d->vocab + DRAFT_CHUNK - 1) / DRAFT_CHUNK);
-    if ((uint64_t)std::max(d->n_rows, d->n_seq) * *chunks >= 1u << 31)
+    if ((uint64_t)std::max(d->n_rows, d->n_seq) * ((*chunks + 3) / 4) >= (uint64_t)GROUPS_256)
         return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
     *bytes = (uint64_t)d->n_rows * *chunks * sizeof(DraftPart) + (uint64_t)d->n_seq * *chunks * sizeof(double) +
              (uint64_t)d->n_seq * sizeof(DraftDone);
@@ -245,7 +297,7 @@ int wpcg_kv_append(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* 
     a.n_kv = (int)kv->n_kv_heads;
     a.n_units = a.n_q + 2 * a.n_kv;
     const uint64_t per = 2048 / d;  // heads of a workgroup
-    if ((uint64_t)batch->n_rows * ((a.n_units + per - 1) / per) >= 1u << 31)
+    if ((uint64_t)batch->n_rows * ((a.n_units + per - 1) / per) >= (uint64_t)GROUPS_256)
         return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
     if (batch->n_seq == 0 || batch->n_rows == 0) return check_ctx(ctx);
     if (int rc = check_pointers(kv, batch)) return rc;
@@ -285,7 +337,7 @@ int wpcg_paged_attention_workspace(const wpcg_kv_pages* kv, const wpcg_kv_batch*
     PagedBatch b;
     if (int rc = check_batch(batch, kv, &b)) return rc;
     if (int rc = check_attention(kv, att)) return rc;
-    Plan plan;
+    Plans plan;
     if (int rc = plan_attention(kv, b, att, &plan)) return rc;
     *bytes = plan.bytes;
     return WPCG_OK;
@@ -302,7 +354,7 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
     const uint64_t width = (uint64_t)att->n_heads * kv->head_dim;
     if (int rc = row_stride(att->q_stride, width, att->dtype, &a.q_row)) return rc;
     if (int rc = row_stride(att->out_stride, width, att->dtype, &a.out_row)) return rc;
-    Plan plan;
+    Plans plan;
     if (int rc = plan_attention(kv, a.b, att, &plan)) return rc;
     if (batch->n_seq == 0 || batch->n_rows == 0) return check_ctx(ctx);
     if (int rc = check_pointers(kv, batch)) return rc;
@@ -329,17 +381,22 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
     a.scale = (float)((double)att->scale * 1.4426950408889634);
     a.window = (int)std::min<uint64_t>(att->window, INT_BOUND);
     a.sinks = (int)std::min<uint64_t>(att->sinks, INT_BOUND);
-    a.cols = plan.cols;
-    a.col_blocks = plan.col_blocks;
-    a.blocks = plan.blocks;
-    a.chunk = plan.chunk;
-    a.splits = plan.splits;
-    a.part_o = (float*)ws_dev;
-    a.part_ml = a.part_o + plan.parts * kv->head_dim;
-    a.ends = (AttnEnd*)(a.part_ml + plan.parts * 2);
     const hipStream_t s = pick(ctx, stream);
     const int d = (int)kv->head_dim;
-    WPCG_HIP(plan.many ? launch_attn_many(a, d, att->dtype, kv->dtype, s) : launch_attn_few(a, d, att->dtype, kv->dtype, s));
+    for (int i = 0; i < plan.n; i++) {
+        const Plan& p = plan.part[i];
+        a.b = p.b;
+        a.cols = p.cols;
+        a.col_blocks = p.col_blocks;
+        a.blocks = p.blocks;
+        a.chunk = p.chunk;
+        a.splits = p.splits;
+        a.part_o = (float*)ws_dev;
+        a.part_ml = a.part_o + p.parts * kv->head_dim;
+        a.ends = (AttnEnd*)(a.part_ml + p.parts * 2);
+        WPCG_HIP(p.many ? launch_attn_many(a, d, att->dtype, kv->dtype, s)
+                        : launch_attn_few(a, d, att->dtype, kv->dtype, s));
+    }
     return WPCG_OK;
 }
 

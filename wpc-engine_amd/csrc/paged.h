@@ -23,7 +23,7 @@ constexpr int ct_size() { return CT == CT_F32 ? 4 : CT == CT_BF16 ? 2 : 1; }
 
 // ---- the batch ---------------------------------------------------------------
 // Sequence s's rows [a, a + n) and tokens; n = 0: nothing to do for it (its row
-// range breaks the batch's bounds, or is empty). bad: the length is none.
+// range breaks the batch's bounds, or is empty, or is another kernel's). bad: the length is none.
 struct SeqRows {
     int a, n, len;
     bool bad;
@@ -33,7 +33,7 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedBatch& b, int s)
     SeqRows r;
     r.a = b.q_start ? b.q_start[s] : s;
     const int e = b.q_start ? b.q_start[s + 1] : s + 1;
-    const bool ok = r.a >= 0 && r.a <= e && e <= b.n_rows && e - r.a <= b.max_q;
+    const bool ok = r.a >= 0 && r.a <= e && e <= b.n_rows && e - r.a <= b.max_q && e - r.a >= b.min_q;
     r.n = ok ? e - r.a : 0;
     r.len = b.kv_len[s];
     r.bad = r.len < 0 || r.len > b.max_kv;

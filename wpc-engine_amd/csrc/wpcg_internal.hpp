@@ -472,7 +472,7 @@ hipError_t launch_argmax_rows(const float* logits, int n, int rows, uint32_t* ou
 // wpcg_kv_batch and the page geometry as the kernels take them; every bound
 // fits an int (capi_serve.cpp checks).
 struct PagedBatch {
-    int n_seq, n_rows, max_q, max_kv;
+    int n_seq, n_rows, min_q, max_q, max_kv;  // sequences of fewer or more rows are left out
     uint32_t n_pages;
     int page_size, page_shift;
     uint64_t table_stride;
@@ -508,6 +508,9 @@ hipError_t launch_kv_append(const KvAppendArgs& p, int head_dim, bool bf16, hipS
 // ATTN_SHARE_MIN each; at most ATTN_DEAL_SEQS sequences) instead; the states of
 // items that several have parts of are at [2 blocks][cols], and ends [blocks]
 // tells which item a workgroup's first part ends.
+//
+// Many rows, blocks > 0: that many workgroups a key-value head and chunk, which
+// look for their sequence and column block; else one for each.
 constexpr int ATTN_FEW_COLS = 16, ATTN_FEW_TILE = 32, ATTN_FEW_WAVES = 8;
 constexpr int ATTN_SHARE_MIN = 16, ATTN_DEAL_SEQS = 2048;
 constexpr int ATTN_MANY_COLS = 128, ATTN_MANY_TILE = 64;

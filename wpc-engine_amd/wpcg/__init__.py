@@ -832,7 +832,8 @@ class KvBatch:
 
 class KvAppend:
     """Head norm, rotation and store of a batch's new rows (wpcg_kv_append).
-    Strides are elements between rows; 0 = packed."""
+    Strides are elements between rows; 0 = packed. One thread at a time may
+    use an object."""
 
     def __init__(self, ctx: Context, kv: PagedKv, batch: KvBatch, n_heads: int, dtype: int = DTYPE_F32,
                  q_out_dtype: int = DTYPE_F32, q_norm=None, k_norm=None, eps: float = 1e-6, frequencies=None,
