@@ -161,9 +161,25 @@ int plan_kernel(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attenti
     const double tile = p.many ? (a->dtype == WPCG_DTYPE_BF16 ? 2.4 : kv->dtype == WPCG_DTYPE_F32 ? 6.0 : 3.5) *
                                      (kv->head_dim / 128.0)
                                : 2.0 * tw * kv->head_dim * type_size(kv->dtype) / 20480.0;
+    // Without a window a prompt's first blocks see fewest tiles and run last, so
+    // that where there are more workgroups than room the sum of their tiles
+    // counts (1500 rows in fp32 over BF16, 32 / 4 heads, 376 blocks of 1 to 24
+    // tiles: 129 us in equal rounds' split, 81 whole). The many-row kernel's
+    // parts are written and read again, at 4 TB/s.
+    const int64_t unseen = p.many && a->window == 0 ? std::max<int64_t>(0, b.max_q - p.cols / group) : 0;
+    const int64_t lowest = std::max<int64_t>(1, tiles - unseen / tw);
+    const double mean = (tiles + lowest) / 2.0;
     const auto cost = [&](int64_t s) {
-        const int64_t rounds = (base * s + room - 1) / room;
-        return rounds * (4.0 + (double)((tiles + s - 1) / s) * tile) + (s > 1 ? 5.0 : 0.0);
+        const int64_t chunk = (tiles + s - 1) / s;
+        // chunks of all blocks of 1 .. t tiles
+        const auto chunks = [&](int64_t t) { return (double)chunk * (t / chunk) * (t / chunk + 1) / 2 + (double)(t % chunk) * (t / chunk + 1); };
+        const double parts = (chunks(tiles) - chunks(lowest - 1)) / (tiles - lowest + 1);
+        double join = s > 1 ? 5.0 : 0.0;
+        if (p.many && s > 1) join += base * p.cols * parts * (kv->head_dim + 2) * 8.0 / 4e6;
+        if (unseen > 0 && base * parts > room)
+            return base * (parts * 4.0 + mean * tile) / room + 0.5 * (s == 1 ? lowest : chunk) * tile + join;
+        const int64_t rounds = ((int64_t)(base * parts) + room - 1) / room;
+        return rounds * (4.0 + chunk * tile) + join;
     };
     const int64_t least = p.many ? 2 : ATTN_FEW_WAVES;  // tiles of a chunk
     // (the many-row kernel's parts are of all n_rows, which may be a loose bound)
