@@ -74,25 +74,54 @@ __device__ __forceinline__ double draft_rate(const DraftArgs& p, int s)
     return t > 0.0f ? 1.4426950408889634 / (double)t : 0.0;
 }
 
+// Lane exchanges of doubles: 0 from lanes that there are none.
+constexpr int DPP_ROW_SHR = 0x110, DPP_WAVE_SHR1 = 0x138;  // from n lanes before, in a row of 16; of the wave
+template <int CTRL, int ROW_MASK = 0xF>
+__device__ __forceinline__ double dpp_d(double v)
+{
+    const uint64_t w = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)wave_dpp_i<CTRL, ROW_MASK>(0, (int)(uint32_t)w);
+    const uint32_t hi = (uint32_t)wave_dpp_i<CTRL, ROW_MASK>(0, (int)(w >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_d(double v, int lane)
+{
+    const uint64_t w = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)w, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Every lane: the sum over its row of 16 lanes.
+__device__ __forceinline__ double row_sum_d(double v)
+{
+    v += dpp_d<WDPP_XOR1>(v);
+    v += dpp_d<WDPP_XOR2>(v);
+    v += dpp_d<WDPP_HALF_MIRROR>(v);
+    return v + dpp_d<WDPP_MIRROR>(v);
+}
 __device__ __forceinline__ double wave_sum_d(double v)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
+    v = row_sum_d(v);
+    v += dpp_d<WDPP_BCAST15, 0xA>(v);
+    v += dpp_d<WDPP_BCAST31, 0xC>(v);
+    return lane_d(v, 63);
+}
+// The sums over the lanes up to this one.
+__device__ __forceinline__ double wave_scan_d(double v)
+{
+    v += dpp_d<DPP_ROW_SHR + 1>(v);
+    v += dpp_d<DPP_ROW_SHR + 2>(v);
+    v += dpp_d<DPP_ROW_SHR + 4>(v);
+    v += dpp_d<DPP_ROW_SHR + 8>(v);
+    v += dpp_d<WDPP_BCAST15, 0xA>(v);
+    return v + dpp_d<WDPP_BCAST31, 0xC>(v);
 }
 // The sum of v over the threads before this one, and over all in total; four
 // waves, s: four doubles.
 __device__ __forceinline__ double block_before(double v, double* s, double& total)
 {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    double t = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double u = __shfl_up(t, d);
-        if (lane >= d) t += u;
-    }
-    double before = __shfl_up(t, 1);
-    if (lane == 0) before = 0.0;
+    const double t = wave_scan_d(v), before = dpp_d<DPP_WAVE_SHR1>(t);
     if (lane == 63) s[wave] = t;
     __syncthreads();
     total = 0.0;
@@ -171,8 +200,7 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
 #pragma unroll
         for (int i = CHUNK / 64 - 1; i >= 0; i--)
             if (c.v[i] == best) at = chunk * CHUNK + 256 * (i / 4) + 4 * lane + i % 4;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) at = min(at, __shfl_xor(at, d));
+        at = ~wave_max_i(~at);
     }
     if (lane == 0) p.part[(uint64_t)row * p.chunks + chunk] = DraftPart{sum, best, best == -INFINITY ? 0x7fffffff : at};
 }
@@ -208,15 +236,23 @@ __device__ __forceinline__ RowState row_state(const DraftArgs& p, int row, doubl
         for (int j = 0; j < AHEAD; j++) z += c[j].sum * to_m(c[j].max);
     }
     const float mine = m;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const float v = __shfl_xor(m, d);
-        const int j = __shfl_xor(at, d);
-        larger(m, at, v, j);
-    }
+    larger(m, at, wave_dpp<WDPP_XOR1>(m, m), wave_dpp_i<WDPP_XOR1>(at, at));
+    larger(m, at, wave_dpp<WDPP_XOR2>(m, m), wave_dpp_i<WDPP_XOR2>(at, at));
+    larger(m, at, wave_dpp<WDPP_HALF_MIRROR>(m, m), wave_dpp_i<WDPP_HALF_MIRROR>(at, at));
+    larger(m, at, wave_dpp<WDPP_MIRROR>(m, m), wave_dpp_i<WDPP_MIRROR>(at, at));
+    // the rows of a half wave
+    const auto ms = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    const auto as = __builtin_amdgcn_permlane16_swap((uint32_t)at, (uint32_t)at, false, false);
+    m = __uint_as_float(ms[0]);
+    at = (int)as[0];
+    larger(m, at, __uint_as_float(ms[1]), (int)as[1]);
     z *= mine == -INFINITY ? 1.0 : exp2_d((double)mine - (double)m, rate);
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) z += __shfl_xor(z, d);
+    z = row_sum_d(z);
+    const uint64_t w = __builtin_bit_cast(uint64_t, z);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)w, (uint32_t)w, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(w >> 32), (uint32_t)(w >> 32), false, false);
+    z = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) +
+        __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
     return {z, m, at};
 }
 

@@ -64,4 +64,16 @@ __device__ __forceinline__ int wave_sum_i(int v)
     return __builtin_amdgcn_readlane(v, 63);
 }
 
+__device__ __forceinline__ int wave_max_i(int v)
+{
+    constexpr int LEAST = -0x7fffffff - 1;
+    v = max(v, wave_dpp_i<WDPP_XOR1>(LEAST, v));
+    v = max(v, wave_dpp_i<WDPP_XOR2>(LEAST, v));
+    v = max(v, wave_dpp_i<WDPP_HALF_MIRROR>(LEAST, v));
+    v = max(v, wave_dpp_i<WDPP_MIRROR>(LEAST, v));
+    v = max(v, wave_dpp_i<WDPP_BCAST15, 0xA>(LEAST, v));
+    v = max(v, wave_dpp_i<WDPP_BCAST31, 0xC>(LEAST, v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 }  // namespace wpcg
