@@ -2,13 +2,13 @@
 // prompts behind cached tokens; causal, with a window and sinks.
 //
 // The work is two matrix products a tile and the exponentials between them:
-// the matrix cores are the bound for long prompts, and the exponentials (a
-// quarter-rate instruction each) come close behind. A workgroup takes 128
-// columns ((row, query head) pairs of one key-value head, so that keys and
-// values are shared by the heads of a group) and walks the 64-token tiles
-// they see; each of its four waves owns 32 columns and keeps their running
-// maximum, sum and output in registers. Tiles no column of a wave sees are
-// skipped, tiles that all see whole take no mask.
+// the matrix cores are the bound for long prompts, and the vector units come
+// close behind. A workgroup takes 128 columns ((row, query head) pairs of one
+// key-value head, so that keys and values are shared by the heads of a group),
+// or 256, and walks the 64-token tiles they see; each of its four or eight
+// waves owns 32 columns and keeps their running maximum, sum and output in
+// registers. Tiles no column of a wave sees are skipped, tiles that all see
+// whole take no mask.
 //
 // Layout. 32 x 32 x 16 products with keys as A and queries as B leave the
 // scores S^T with column l % 32 in lane l and tokens 8a + 4(l/32) + b, which
@@ -16,14 +16,21 @@
 // tokens in the same order. So the softmax's terms stay in their lane, the
 // maximum needs one lane exchange, and the rescaling factor is one number a
 // lane. Keys go to LDS in rows padded by 16 bytes, so that neither the writes
-// (along a row) nor the reads (along tokens) meet in a bank; values are transposed in registers
-// by byte permutes on their way to LDS and lie in the order the operand is
-// read, 1 KiB a wave without conflicts. The next tile's loads are in flight
-// during the products.
+// (along a row) nor the reads (along tokens) meet in a bank; values are
+// transposed in registers by byte permutes on their way to LDS and lie in the
+// order the operand is read, 1 KiB a wave without conflicts. The next tile's
+// loads are in flight during the products.
 //
 // Precision is that of attn_few.hip; an F32 cache is carried as three bf16
 // terms too, and a product of two fp32 values takes the six of its nine terms
 // that reach 2^-24.
+//
+// Measured, heads of 128: a prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 149
+// us, 920 TFLOP/s, with the matrix cores busy in 37 % of the cycles and the
+// vector units in 39 %; 2048 rows behind 30720 tokens 1050 TFLOP/s (a library's
+// 8192^3 product 1300); two prompts of up to 5000 with a window of 1024, 32 / 4
+// heads over E4M3 (144 GFLOP) 223 us; 777 rows behind 523 tokens, 32 / 4 heads,
+// all F32 (11.6 GFLOP, six products each) 123 us with the join's 11.
 #include "paged.h"
 
 namespace wpcg {

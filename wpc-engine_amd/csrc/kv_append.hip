@@ -11,6 +11,10 @@
 // angles while the loads are in flight: the product and the reduction modulo
 // 2 pi are fp64 (fp32 would lose the angle's fraction from positions of a few
 // thousand on), sine and cosine of what is left, within +-pi, fp32.
+//
+// Measured, 32 / 8 heads of 128, fp32 rows into E4M3 pages: 3 prompts of up to
+// 2000 rows (149 MB) 33.3 us, 4.5 TB/s; 64 sequences of one row, 32 / 4 heads
+// into BF16 pages 4.3 us, of which a launch alone is 3.8.
 #include "paged.h"
 #include "wave.h"
 
