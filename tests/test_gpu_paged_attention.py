@@ -209,6 +209,57 @@ def test_more_sequences_than_threads(ctx, n, rows):
     check(got, *expected(pg, q, [rows] * n, 2, BF16, 0.125, 0, 0))
 
 
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("d,heads,hkv,window,sinks", [(64, 8, 2, 0, 0), (128, 8, 2, 0, 0), (128, 20, 4, 0, 0),
+                                                      (64, 8, 2, 2500, 3), (128, 8, 2, 2300, 70)])
+def test_long_prompts(ctx, dtype, d, heads, hkv, window, sinks):
+    """Batches that may hold long prompts with blocks enough for every CU take 256
+    columns a workgroup, two halves of it in turns: sequences of none, one, two,
+    three and many tiles, of rows for a part of a workgroup and for several, one
+    whose last token's values are not finite (twice in a row of tiles), a bad
+    length, a bad page; the same call gives the same bits."""
+    print(f"[gpu] long prompts: {dtype} {heads}/{hkv}x{d} window {window}", flush=True)
+    rng = np.random.default_rng(d + heads + window + dtype)
+    n = 300 // hkv
+    rows = [1] * n
+    kv = [int(x) for x in rng.integers(1, 9, n)]
+    for s, (r, m) in {3: (100, 100), 4: (70, 2600), 10: (33, 64), 11: (90, 129), 20: (130, 192), 21: (100, 193),
+                      30: (40, 500), 31: (9, 64), 40: (64, 65), 50: (20, 5), 60: (110, 900)}.items():
+        rows[s], kv[s] = r, m
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 16, kv, scales=dtype == E4M3, width=170)
+    # not finite: the last rows alone see them, the others' are masked
+    for at in (450, 499):
+        x = pg.real["v"][30][at] / pg.scale["v"][:, None]  # as stored
+        x[0, 7], x[0, 9] = np.nan, (np.nan if dtype == E4M3 else -np.inf)
+        pg.put("v", 30, R.encode(x, dtype)[None], [at])
+    pg.upload()
+    total = sum(rows)
+    q = R.encode(rng.standard_normal((total + 3, heads, d)) * 1.5, BF16)
+    batch = pg.batch(rows, n_rows=total + 3, max_kv=2700, max_q=256)
+    got, _ = run(ctx, pg, batch, q, heads, BF16, 0.1, window, sinks)
+    want, bound = expected(pg, q[:total], rows, heads, BF16, 0.1, window, sinks)
+    at = np.cumsum([0] + rows)
+    group = heads // hkv
+    odd = got[at[30]:at[31], :group][..., [7, 9]]
+    first = np.array([max(0, t - (500 - 40)) for t in (450, 499)])  # row from which a token is seen
+    assert np.isfinite(odd[:first[0]]).all() and not np.isfinite(odd[first[0]:]).any()
+    got[at[30] + first[0]:at[31], :group, [7, 9]] = want[at[30] + first[0]:at[31], :group, [7, 9]]
+    check(got[:total], want, bound)
+    fill = R.decode(np.full(1, 0x5A5A, np.uint16), BF16)[0]
+    assert (got[total:] == fill).all()
+    again, _ = run(ctx, pg, batch, q, heads, BF16, 0.1, window, sinks)
+    again[at[30] + first[0]:at[31], :group, [7, 9]] = want[at[30] + first[0]:at[31], :group, [7, 9]]
+    assert np.array_equal(got.view(np.uint64), again.view(np.uint64))
+    pg.table[60, 40] = pg.n_pages
+    pg.d_table.write(pg.table)
+    pg.d_len.write(np.array([2701 if s == 20 else m for s, m in enumerate(kv)], np.int32))
+    bad, _ = run(ctx, pg, batch, q, heads, BF16, 0.1, window, sinks)
+    assert np.isnan(bad[at[20]:at[21]]).all() and np.isnan(bad[at[61] - 1]).all()
+    for s in range(n):
+        if s not in (20, 30, 60):
+            assert np.array_equal(bad[at[s]:at[s + 1]], got[at[s]:at[s + 1]])
+
+
 @pytest.mark.parametrize("q_dtype,dtype", TYPES)
 @pytest.mark.parametrize("rows", [2, 30])
 def test_infinite_values_reach_only_rows_that_see_them(ctx, q_dtype, dtype, rows):
