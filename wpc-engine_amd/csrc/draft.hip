@@ -317,11 +317,58 @@ __device__ __forceinline__ void draft_chunk(Chunk& q, const DraftArgs& p, int ro
     }
 }
 
+// The first thread that found something: its number and running sum; and the
+// last thread's that has some weight. Numbers rise with the threads; MISSING or
+// -1 where there is none. s: of four waves.
+constexpr int MISSING = 0x7fffffff;
+struct Found {
+    int at, last;
+    double before;
+};
+__device__ __forceinline__ Found find_first(bool found, int at, double before, int last, Found* s)
+{
+    const uint64_t f = __ballot(found), w = __ballot(last >= 0);
+    Found r = {MISSING, -1, 0.0};
+    if (f) {
+        const int l = __builtin_ctzll(f);
+        r.at = __builtin_amdgcn_readlane(at, l);
+        r.before = lane_d(before, l);
+    }
+    if (w) r.last = __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(w));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = r;
+    __syncthreads();
+    r = s[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; i++) {
+        if (r.at == MISSING) {
+            r.at = s[i].at;
+            r.before = s[i].before;
+        }
+        r.last = max(r.last, s[i].last);
+    }
+    return r;
+}
+// Eight consecutive values of a row, i0 a multiple of 8; behind its end the last.
+__device__ __forceinline__ void load_eight(float (&v)[8], const float* x, int i0, int vocab, bool vec)
+{
+    if (vec && i0 + 8 <= vocab) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const pf32x4 w = *(const pf32x4*)(x + i0 + 4 * i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[4 * i + j] = w[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = x[min(i0 + j, vocab - 1)];
+    }
+}
+
 // The token of a sampled row: its chunks' weights, then the chunk's ids.
 __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double rate, int draft)
 {
-    __shared__ double s_s[4], s_before;
-    __shared__ int s_at, s_id, s_last, s_last_id;
+    __shared__ double s_s[4];
+    __shared__ Found s_chunk[4], s_id[4];
     const int tid = (int)threadIdx.x;
     const double u = (double)p.u_next[s];
     bool rest = c.rest;
@@ -333,44 +380,35 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
     // a thread's run of chunks
     const int run = (p.chunks + THREADS - 1) / THREADS;
     const int j0 = min(tid * run, p.chunks), j1 = min(j0 + run, p.chunks);
-    double before, total, last = 0.0;
+    double before, total, only = 0.0;
     for (int turn = 0; turn < 2; turn++) {
         double sum = 0.0;
-        for (int i = j0; i < j1; i++) sum += last = of_chunk(i);
+        for (int i = j0; i < j1; i++) sum += only = of_chunk(i);
         before = block_before(sum, s_s, total);
         if (total > 0.0 || !rest) break;
         rest = false;  // nothing is left of p - q: the row's own weights
     }
     const double want = u * total;
-    if (tid == 0) {
-        s_at = s_id = 0x7fffffff;
-        s_last = s_last_id = -1;
-    }
-    __syncthreads();
+    int at = MISSING, last = -1;  // last: of use where rounding leaves none
     for (int i = j0; i < j1; i++) {
-        const double w = run == 1 ? last : of_chunk(i);
-        if (w > 0.0) atomicMax(&s_last, i);  // of use where rounding leaves none
+        const double w = run == 1 ? only : of_chunk(i);
+        if (w > 0.0) last = i;
         if (before + w > want) {
-            atomicMin(&s_at, i);
+            at = i;
             break;
         }
         before += w;
     }
-    __syncthreads();
-    const int chunk = s_at != 0x7fffffff ? s_at : s_last;
+    const Found f = find_first(at != MISSING, at, before, last, s_chunk);
+    const bool end = f.at == MISSING;  // the last id with weight
+    const int chunk = end ? f.last : f.at;
     if (chunk < 0) return -1;
-    const bool end = s_at == 0x7fffffff;  // the last id with weight
-    if (tid == chunk / run) s_before = before;  // stopped at the chunk
     // ids 8 t .. 8 t + 7 of the chunk
     const int i0 = chunk * CHUNK + 8 * tid;
     double w[8], sum = 0.0, all;
-    float x[8], q[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint64_t i = (uint64_t)min(i0 + j, p.vocab - 1);
-        x[j] = p.logits[(uint64_t)row * p.logits_row + i];
-        q[j] = p.probs && rest ? p.probs[(uint64_t)row * p.probs_row + i] : 0.0f;
-    }
+    float x[8], q[8] = {};
+    load_eight(x, p.logits + (uint64_t)row * p.logits_row, i0, p.vocab, p.vec);
+    if (p.probs && rest) load_eight(q, p.probs + (uint64_t)row * p.probs_row, i0, p.vocab, p.vec);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         if (!p.probs && i0 + j == draft) q[j] = 1.0f;
@@ -378,18 +416,16 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
         sum += w[j];
     }
     double t = block_before(sum, s_s, all);
-    t += s_before;
-    int first = 0x7fffffff, final = -1;
+    t += f.before;
+    int first = MISSING, final = -1;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         t += w[j];
         if (w[j] > 0.0) final = i0 + j;
-        if (!end && t > want && first == 0x7fffffff) first = i0 + j;
+        if (!end && t > want && first == MISSING) first = i0 + j;
     }
-    if (first != 0x7fffffff) atomicMin(&s_id, first);
-    if (final >= 0) atomicMax(&s_last_id, final);
-    __syncthreads();
-    return s_id != 0x7fffffff ? s_id : s_last_id;
+    const Found id = find_first(first != MISSING, first, 0.0, final, s_id);
+    return id.at != MISSING ? id.at : id.last;
 }
 
 __global__ __launch_bounds__(THREADS) void k_draft_choose(DraftArgs p)
