@@ -16,9 +16,10 @@
 // good as its target leaves differences p - q far below p, and the running
 // sums of 10^5 weights decide which id they pass at.
 //
-// Measured at 151936 ids: 64 sequences with their drafts (260 MB) 74 us, the
-// first launch 44 (5.2 TB/s) and the second 31; one sequence with four drafts
-// 19.7 us, 4.3 and 17 of them, the second's ten dependent round trips.
+// Measured at 151936 ids: 64 sequences with their drafts (260 MB) 72 us, the
+// first launch 44 (5.2 TB/s) and the second 23; one sequence with four drafts
+// 14.7 us, 4.0 and 10.7 of them. (With LDS atomics in place of the ballots that
+// find the drawn id 19.7 us: 75 threads at one word took 2 to 3 us each time.)
 #include "paged.h"
 #include "wave.h"
 
