@@ -194,3 +194,24 @@ def test_captured(ctx):
         wa, wo = want(c)
         assert np.array_equal(acc.read(np.int32, 3), wa) and np.array_equal(out.read(np.int32, n), wo)
     del g
+
+
+def test_other_streams(ctx):
+    """Calls of two objects on streams of other contexts, at once."""
+    rng = np.random.default_rng(9)
+    c = case(rng, [4, 2, 3], 30000)
+    wa, wo = want(c)
+    dev = {k: ctx.upload(c[k]) for k in ("logits", "probs", "tokens", "u", "u_next", "t")}
+    q = ctx.upload(np.cumsum([0] + c["rows"]).astype(np.int32))
+    others = [wpcg.Context(0) for _ in range(2)]
+    n = len(wo)
+    ops = [wpcg.DraftVerify(ctx, 3, n, 5, 30000, q_start=q, temperature=dev["t"]) for _ in others]
+    accs, outs = ([ctx.alloc(4 * m) for _ in others] for m in (3, n))
+    for _ in range(20):
+        for o, op, acc, out in zip(others, ops, accs, outs):
+            op.run(dev["logits"], dev["tokens"], dev["u"], dev["u_next"], acc, out, draft_probs=dev["probs"],
+                   stream=o.stream)
+    for o, acc, out in zip(others, accs, outs):
+        o.sync()
+        assert np.array_equal(acc.read(np.int32, 3), wa) and np.array_equal(out.read(np.int32, n), wo)
+        o.close()

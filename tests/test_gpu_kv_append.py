@@ -218,3 +218,30 @@ def test_captured(ctx):
         got = pg.dv.read(np.uint32, pg.bits["v"].size)
         assert np.array_equal(got[pg.index(0, [n - 1])], v)
     del g
+
+
+def test_other_streams(ctx):
+    """Two batches of one layer's pages stored on streams of other contexts, at once."""
+    rng = np.random.default_rng(10)
+    d, lens = 128, [40, 25]
+    pg = R.Paged(ctx, rng, BF16, 2, d, 16, lens).upload()
+    others = [wpcg.Context(0) for _ in range(2)]
+    runs, keep = [], []
+    for s in range(2):  # all of a sequence's tokens
+        q, k, v = inputs(rng, lens[s], 4, 2, d, BF16)
+        dev = [ctx.upload(a) for a in (q, k, v)]
+        arrays = [ctx.upload(np.array(a, np.int32)) for a in ([0, lens[s]], [lens[s]], pg.table[s])]
+        batch = wpcg.KvBatch(1, lens[s], arrays[1], arrays[2], pg.table.shape[1], lens[s], max_q=lens[s],
+                             q_start=arrays[0])
+        runs.append((wpcg.KvAppend(ctx, pg.kv, batch, 4, BF16, BF16), dev, ctx.alloc(q.nbytes)))
+        keep.append((k, v, arrays))
+    for _ in range(20):
+        for o, (op, dev, out) in zip(others, runs):
+            op.run(*dev, out, stream=o.stream)
+    for o in others:
+        o.sync()
+        o.close()
+    for n, x in (("k", pg.dk), ("v", pg.dv)):
+        got = x.read(np.uint16, pg.bits[n].size)
+        for s in range(2):
+            assert np.array_equal(got[pg.index(s, np.arange(lens[s]))], keep[s][0 if n == "k" else 1])

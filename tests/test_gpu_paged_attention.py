@@ -408,6 +408,45 @@ def test_captured_graph_follows_the_lengths(ctx, rows):
     del g, g2
 
 
+@pytest.mark.parametrize("max_kv", [1200, 60000])
+def test_captured_graph_follows_the_row_ranges(ctx, max_kv):
+    """One graph of a batch that both kernels may have parts of (the longer
+    bound), replayed while sequences change from one new row to a prompt and
+    back, with eager calls of another object between."""
+    print(f"[gpu] graph of mixed rows, bound {max_kv}", flush=True)
+    rng = np.random.default_rng(max_kv)
+    full = [700, 90, 1100, 300, 64, 33]
+    pg = R.Paged(ctx, rng, BF16, 2, 128, 16, full, width=max_kv // 16).upload()
+    total = 320
+    batch = pg.batch([1] * 6, n_rows=total, max_kv=max_kv, max_q=250)
+    q = R.encode(rng.standard_normal((total, 8, 128)), BF16)
+    qd = ctx.upload(q)
+    outs = [ctx.alloc(q.nbytes) for _ in range(2)]
+    ops = [wpcg.PagedAttention(ctx, pg.kv, batch, 8, BF16, scale=0.09) for _ in range(2)]
+    g = ctx.capture(lambda: ops[0].run(qd, outs[0]))
+    kept = pg.real
+    for rows, lens in (([1, 90, 1, 200, 8, 9], full), ([250, 1, 0, 1, 64, 1], [250, 2, 0, 300, 64, 33]),
+                       ([1] * 6, full), ([9, 9, 9, 9, 9, 9], [700, 90, 1100, 300, 64, 5]),
+                       ([1, 90, 1, 200, 8, 9], full)):
+        pg.d_len.write(np.array(lens, np.int32))
+        pg.d_start.write(np.cumsum([0] + rows).astype(np.int32))
+        for o in outs:
+            o.write(np.full(q.size, 0xFFFF, np.uint16))
+        g.launch()
+        ops[1].run(qd, outs[1])
+        g.launch()
+        ctx.sync()
+        pg.kv_len = lens
+        pg.real = {n: [x[:m] for x, m in zip(kept[n], lens)] for n in "kv"}
+        n = sum(rows)
+        want, bound = expected(pg, q[:n], rows, 8, BF16, 0.09, 0, 0)
+        pg.real = kept
+        bits = [o.read(np.uint16, q.size).reshape(q.shape) for o in outs]
+        assert np.array_equal(bits[0], bits[1]) and (bits[0][n:] == 0xFFFF).all()
+        check(R.decode(bits[0][:n], BF16), want, bound)
+    del g
+
+
 def test_other_streams(ctx):
     """Calls of two objects on streams of other contexts, at once."""
     rng = np.random.default_rng(12)
