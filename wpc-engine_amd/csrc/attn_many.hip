@@ -25,13 +25,12 @@
 // terms too, and a product of two fp32 values takes the six of its nine terms
 // that reach 2^-24.
 //
-// Measured, heads of 128: a prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 149
-// us, 920 TFLOP/s, with the matrix cores busy in 37 % of the cycles and the
-// vector units in 39 %; the last 2048 rows of 32768 tokens 1050 TFLOP/s (a
-// library's 8192^3 product 1300); two prompts of up to 5000 with a window of
-// 1024, 32 / 4 heads over E4M3 (144 GFLOP) 223 us; 777 rows behind 523 tokens,
-// 32 / 4 heads, all F32 (11.6 GFLOP, six products each) 123 us with the join's
-// 11.
+// Measured, heads of 128: a prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 147
+// us, 935 TFLOP/s, with the matrix cores busy in 37 % of the cycles and the
+// vector units in 39 %; 2048 rows behind 30720 tokens 1050 TFLOP/s (a library's
+// 8192^3 product 1300); two prompts of up to 5000 with a window of 1024, 32 / 4
+// heads over E4M3 (144 GFLOP) 223 us; 777 rows behind 523 tokens, 32 / 4 heads,
+// all F32 (11.6 GFLOP, six products each) 123 us with the join's 11.
 #include "paged.h"
 
 namespace wpcg {
@@ -52,16 +51,18 @@ struct Shape {
 };
 
 // A tile on its way: what one lane carries of the 16 tokens that its wave
-// brings in.
-template <int D, int CT>
+// brings in, keys and values (BOTH) or one of them.
+template <int D, int CT, bool BOTH>
 struct Carried {
     using S = Shape<D, CT, true>;
     static constexpr int KW = 8 * ct_size<CT>() / 4, VW = S::CW * ct_size<CT>() / 4;  // words
-    uint32_t k[S::KT][KW];
-    uint32_t v[S::VT][4][VW];
+    static constexpr int KN = S::KT * KW, VN = S::VT * 4 * VW;
+    uint32_t w[BOTH ? KN + VN : KN > VN ? KN : VN];
+    __device__ __forceinline__ uint32_t& k(int i, int y) { return w[i * KW + y]; }
+    __device__ __forceinline__ uint32_t& v(int i, int x, int y) { return w[(BOTH ? KN : 0) + (i * 4 + x) * VW + y]; }
 };
 template <int W>
-__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* base, uint32_t at)  // base: uniform
+__device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* base, uint32_t at)  // base: uniform
 {
     const uint8_t* p = base + at;
     if constexpr (W >= 4) {
@@ -103,14 +104,15 @@ __device__ __forceinline__ int value_at(int j, int h, int p)
 
 // What brings tiles from the pages to LDS, in registers on the way: of four
 // waves, wave w the tokens 16 w .. 16 w + 15, of eight the first four their
-// keys and the others their values. Their places in the pages are looked up 64
+// values and the others their keys. Their places in the pages are looked up 64
 // tiles at a time, a tile a lane; where no row sees them page 0 is read
 // unlooked at.
 template <int D, int CT, int WAVES>
 struct Stage {
     using S = Shape<D, CT, true>;
     static constexpr int ES = ct_size<CT>(), CW = S::CW, NCH = S::NCH, NK = S::NK;
-    Carried<D, CT> in;
+    using C = Carried<D, CT, WAVES == 4>;
+    C in;
     SeenTiles<TILE> seen;  // of the block's columns
     int v0, v1;            // its tiles
     int all_hi, all_lo;    // tokens that every column sees
@@ -123,6 +125,7 @@ struct Stage {
     int lane, wave;     // wave: which 16 tokens
     bool keys, values;  // what this wave brings
     uint32_t place_lo = 0, place_hi = 0;
+    uint32_t offset[4];  // of eight waves: the lane's four pieces
     bool fault = false;
 
     __device__ __forceinline__ Stage(const PagedAttnArgs& p, int seq, int kvh, const SeenTiles<TILE>& s, int a, int b,
@@ -139,9 +142,19 @@ struct Stage {
         page_size = p.b.page_size;
         lane = (int)threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-        keys = WAVES == 4 || wave < 4;
-        values = WAVES == 4 || wave >= 4;
+        keys = WAVES == 4 || wave >= 4;
+        values = WAVES == 4 || wave < 4;
         wave &= 3;
+        if constexpr (WAVES == 8) {
+            static_assert(C::KW == C::VW && S::VT == 1 && S::KT <= 4, "four pieces of one size");
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                // (behind a head's last piece, the first ones again)
+                const int k = lane + 64 * (i % S::KT), v = lane % (4 * NCH);
+                const int token = keys ? k / (D / 8) : 8 * (v / NCH % 2) + 4 * (v / (2 * NCH)) + i;
+                offset[i] = token * token_bytes + (keys ? k % (D / 8) * 8 : v % NCH * CW) * ES;
+            }
+        }
     }
     __device__ __forceinline__ bool whole(int vt) const  // no column's mask touches the tile
     {
@@ -167,13 +180,23 @@ struct Stage {
         if (turn == 0) look_up(vt);
         const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place_hi, turn) << 32 |
                             (uint32_t)__builtin_amdgcn_readlane((int)place_lo, turn);
-        if (keys)
+        if constexpr (WAVES == 8) {
+            // keys or values by the same four loads: in two branches they would
+            // have registers of their own, and be waited for to be put together
+            const uint8_t* const from = (keys ? kp : vp) + at;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t o = offset[i];  // (32 bits, and not 64 made before the loop)
+                asm volatile("" : "+v"(o));
+                load_words<C::KW>(&in.w[i * C::KW], from, o);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < S::KT; i++) {
             const int x = lane + 64 * i;
-            load_words(in.k[i], kp + at, x / (D / 8) * token_bytes + x % (D / 8) * 8 * ES);
+            load_words<C::KW>(&in.k(i, 0), kp + at, x / (D / 8) * token_bytes + x % (D / 8) * 8 * ES);
         }
-        if (values)
 #pragma unroll
         for (int i = 0; i < S::VT; i++) {
             const int x = lane + 64 * i;
@@ -181,7 +204,7 @@ struct Stage {
                 const int n = x % NCH, xh = x / NCH % 2, vh = x / (2 * NCH);
 #pragma unroll
                 for (int y = 0; y < 4; y++)
-                    load_words(in.v[i][y], vp + at, (8 * xh + 4 * vh + y) * token_bytes + n * CW * ES);
+                    load_words<C::VW>(&in.v(i, y, 0), vp + at, (8 * xh + 4 * vh + y) * token_bytes + n * CW * ES);
             }
         }
     }
@@ -199,16 +222,16 @@ struct Stage {
             for (int k = 0; k < 4; k++) {
                 const bool some = seen.some(t0 + 16 * wave + 8 * xh + 4 * vh + k);
 #pragma unroll
-                for (int y = 0; y < Carried<D, CT>::VW; y++) {
-                    in.v[i][k][y] = some ? in.v[i][k][y] : 0u;
-                    odd |= word_odd<CT>(in.v[i][k][y]);
+                for (int y = 0; y < C::VW; y++) {
+                    in.v(i, k, y) = some ? in.v(i, k, y) : 0u;
+                    odd |= word_odd<CT>(in.v(i, k, y));
                 }
             }
         }
         return __any(odd && lane < 4 * NCH);
     }
     // registers to LDS: keys [NK][KEYS], values [NK][VALUES]
-    __device__ __forceinline__ void put(uint16_t* k_to, uint16_t* v_to) const
+    __device__ __forceinline__ void put(uint16_t* k_to, uint16_t* v_to)
     {
         if (keys)
 #pragma unroll
@@ -219,14 +242,14 @@ struct Stage {
                 uint32_t t[4][3];
 #pragma unroll
                 for (int y = 0; y < 4; y++)
-                    split3(__uint_as_float(in.k[i][2 * y]), __uint_as_float(in.k[i][2 * y + 1]), t[y]);
+                    split3(__uint_as_float(in.k(i, 2 * y)), __uint_as_float(in.k(i, 2 * y + 1)), t[y]);
 #pragma unroll
                 for (int n = 0; n < 3; n++) *(pu32x4*)(to + n * S::KEYS) = (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]};
             } else if constexpr (CT == CT_BF16) {
-                *(pu32x4*)to = (pu32x4){in.k[i][0], in.k[i][1], in.k[i][2], in.k[i][3]};
+                *(pu32x4*)to = (pu32x4){in.k(i, 0), in.k(i, 1), in.k(i, 2), in.k(i, 3)};
             } else {
-                *(pu32x4*)to = (pu32x4){e4m3_bf16<false>(in.k[i][0]), e4m3_bf16<true>(in.k[i][0]),
-                                        e4m3_bf16<false>(in.k[i][1]), e4m3_bf16<true>(in.k[i][1])};
+                *(pu32x4*)to = (pu32x4){e4m3_bf16<false>(in.k(i, 0)), e4m3_bf16<true>(in.k(i, 0)),
+                                        e4m3_bf16<false>(in.k(i, 1)), e4m3_bf16<true>(in.k(i, 1))};
             }
         }
         if (values)
@@ -242,11 +265,11 @@ struct Stage {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         if constexpr (CT == CT_F32)
-                            split3(__uint_as_float(in.v[i][k][2 * y]), __uint_as_float(in.v[i][k][2 * y + 1]), t[k]);
+                            split3(__uint_as_float(in.v(i, k, 2 * y)), __uint_as_float(in.v(i, k, 2 * y + 1)), t[k]);
                         else if constexpr (CT == CT_BF16)
-                            t[k][0] = in.v[i][k][y];
+                            t[k][0] = in.v(i, k, y);
                         else
-                            t[k][0] = y % 2 ? e4m3_bf16<true>(in.v[i][k][y / 2]) : e4m3_bf16<false>(in.v[i][k][y / 2]);
+                            t[k][0] = y % 2 ? e4m3_bf16<true>(in.v(i, k, y / 2)) : e4m3_bf16<false>(in.v(i, k, y / 2));
                     }
 #pragma unroll
                     for (int e = 0; e < NK; e++) {
@@ -265,9 +288,10 @@ struct Stage {
 };
 
 // Values of a tile that are not finite, added to the columns that see their
-// token (products with ones count the +inf, -inf and NaN a column sees).
+// token (products with ones count the +inf, -inf and NaN a column sees); in:
+// the 16-token groups that hold some.
 template <int D, int NK>
-__device__ __forceinline__ void add_odd(const PagedAttnArgs& p, const uint16_t* values, int t0, int pos,
+__device__ __forceinline__ void add_odd(const PagedAttnArgs& p, const uint16_t* values, const int* in, int t0, int pos,
                                         pf32x16 (&acc)[D / 32])
 {
     const int lane = (int)threadIdx.x & 63, h = lane >> 5;
@@ -275,6 +299,7 @@ __device__ __forceinline__ void add_odd(const PagedAttnArgs& p, const uint16_t* 
     for (int d = 0; d < D / 32; d++) {
 #pragma unroll 1
         for (int j = 0; j < 4; j++) {
+            if (!in[j]) continue;
             pu32x4 see;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -475,60 +500,92 @@ __device__ __forceinline__ bool find_block(const PagedAttnArgs& p, int at, int& 
     return false;
 }
 
-// Two waves a SIMD (F32 queries: one), so that one's exponentials run beside
-// the other's products: two workgroups of four waves a CU, or one of eight
-// where there are columns enough, which brings in each tile once for 256 of
-// them.
-template <int D, int CT, bool QF32, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p)
+// What a workgroup of COLS columns has to do.
+template <int COLS>
+struct Work {
+    int seq, kvh, cb, split, pos0, v0, v1, first, last;  // pos0: position of the sequence's row 0; rows first .. last
+    SeqRows sq;
+    SeenTiles<TILE> seen;
+    // false: nothing
+    __device__ __forceinline__ bool find(const PagedAttnArgs& p)
+    {
+        // workgroup -> column block, chunk, sequence and head: the blocks of a
+        // head are `pairs` apart, so that with a multiple of 8 pairs they run on
+        // one die and share its L2; the last column blocks, which see most, come
+        // first
+        if (p.blocks == 0) {
+            const int pairs = p.b.n_seq * p.n_kv;
+            const int pair = (int)(blockIdx.x % (unsigned)pairs), rest = (int)(blockIdx.x / (unsigned)pairs);
+            split = rest % p.splits;
+            cb = p.col_blocks - 1 - rest / p.splits;
+            seq = pair / p.n_kv;
+            kvh = pair % p.n_kv;
+        } else {
+            const int rest = (int)(blockIdx.x / (unsigned)p.n_kv);
+            split = rest % p.splits;
+            kvh = (int)(blockIdx.x % (unsigned)p.n_kv);
+            if (!find_block<COLS>(p, rest / p.splits, seq, cb)) return false;
+        }
+        sq = seq_rows(p.b, seq);
+        const int cols = sq.n * p.group;
+        if (cb * COLS >= cols) return false;
+        pos0 = (sq.bad ? 0 : sq.len) - sq.n;
+        first = cb * COLS / p.group;
+        last = (min(cols, (cb + 1) * COLS) - 1) / p.group;
+        seen = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks);
+        v0 = split * p.chunk;
+        v1 = min(v0 + p.chunk, seen.total());
+        return v0 < v1 || split == 0;
+    }
+    __device__ __forceinline__ int all_hi() const { return pos0 + first + 1; }
+    __device__ __forceinline__ int all_lo(const PagedAttnArgs& p) const
+    {
+        return p.window > 0 ? pos0 + last - p.window + 1 : 0;
+    }
+};
+// A wave's 32 columns from w0 on.
+struct Columns {
+    bool active, live;  // it has some; this lane's is one
+    int row, head, pos;
+    int hi, lo;  // tokens that all of them see
+    SeenTiles<TILE> seen;
+    template <int COLS>
+    __device__ __forceinline__ Columns(const PagedAttnArgs& p, const Work<COLS>& w, int w0)
+    {
+        const int cols = w.sq.n * p.group, col = w0 + ((int)threadIdx.x & 31);
+        active = w0 < cols;
+        live = col < cols;
+        row = live ? col / p.group : 0;
+        head = w.kvh * p.group + (live ? col % p.group : 0);
+        pos = w.pos0 + row;
+        const int first = active ? w0 / p.group : 0, last = active ? (min(cols, w0 + 32) - 1) / p.group : 0;
+        seen = seen_tiles<TILE>(w.pos0 + first, w.pos0 + last, p.window, p.sinks);
+        hi = w.pos0 + first + 1;
+        lo = p.window > 0 ? w.pos0 + last - p.window + 1 : 0;
+    }
+};
+
+// Two workgroups of four waves a CU (F32 queries: one).
+template <int D, int CT, bool QF32>
+__global__ __launch_bounds__(256, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p)
 {
-    constexpr int COLS = 32 * WAVES;
+    constexpr int COLS = ATTN_MANY_COLS;
     using S = Shape<D, CT, QF32>;
     __shared__ __attribute__((aligned(16))) uint16_t s_k[S::NBUF][S::NK][S::KEYS];
     __shared__ __attribute__((aligned(16))) uint16_t s_v[S::NBUF][S::NK][S::VALUES];
     __shared__ int s_odd[S::NBUF][4], s_fault;
 
-    // workgroup -> column block, chunk, sequence and head: the blocks of a head
-    // are `pairs` apart, so that with a multiple of 8 pairs they run on one
-    // die and share its L2; the last column blocks, which see most, come first
-    int seq, kvh, cb, split;
-    if (p.blocks == 0) {
-        const int pairs = p.b.n_seq * p.n_kv;
-        const int pair = (int)(blockIdx.x % (unsigned)pairs), rest = (int)(blockIdx.x / (unsigned)pairs);
-        split = rest % p.splits;
-        cb = p.col_blocks - 1 - rest / p.splits;
-        seq = pair / p.n_kv;
-        kvh = pair % p.n_kv;
-    } else {
-        const int rest = (int)(blockIdx.x / (unsigned)p.n_kv);
-        split = rest % p.splits;
-        kvh = (int)(blockIdx.x % (unsigned)p.n_kv);
-        if (!find_block<COLS>(p, rest / p.splits, seq, cb)) return;
-    }
-    const SeqRows sq = seq_rows(p.b, seq);
-    const int cols = sq.n * p.group;
-    if (cb * COLS >= cols) return;
+    Work<COLS> w;
+    if (!w.find(p)) return;
+    const SeqRows& sq = w.sq;
+    const SeenTiles<TILE>& seen = w.seen;
+    const int kvh = w.kvh, v0 = w.v0, v1 = w.v1;
+    Stage<D, CT, 4> stage(p, w.seq, kvh, seen, v0, v1, w.all_hi(), w.all_lo(p));
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     const int c = lane & 31, h = lane >> 5;
-    const int len = sq.bad ? 0 : sq.len;
-    const int pos0 = len - sq.n;
-    const int first = cb * COLS / p.group, last = (min(cols, (cb + 1) * COLS) - 1) / p.group;
-    const SeenTiles<TILE> seen = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks);
-    const int v0 = split * p.chunk, v1 = min(v0 + p.chunk, seen.total());
-    if (v0 >= v1 && split > 0) return;
-    Stage<D, CT, WAVES> stage(p, seq, kvh, seen, v0, v1, pos0 + first + 1, p.window > 0 ? pos0 + last - p.window + 1 : 0);
-
-    // the wave's columns
-    const int w0 = cb * COLS + 32 * wave;
-    const bool active = w0 < cols;
-    const int col = w0 + c;
-    const bool live = col < cols;
-    const int row = live ? col / p.group : 0, head = kvh * p.group + (live ? col % p.group : 0);
-    const int pos = pos0 + row;
-    const int wfirst = active ? w0 / p.group : 0, wlast = active ? (min(cols, w0 + 32) - 1) / p.group : 0;
-    const SeenTiles<TILE> wseen = seen_tiles<TILE>(pos0 + wfirst, pos0 + wlast, p.window, p.sinks);
-    const int w_hi = pos0 + wfirst + 1;
-    const int w_lo = p.window > 0 ? pos0 + wlast - p.window + 1 : 0;
+    const Columns my(p, w, w.cb * COLS + 32 * wave);
+    const bool active = my.active, live = my.live;
+    const int row = my.row, head = my.head, pos = my.pos;
     pbf16x8 qb[D / 16][S::NQ];
     load_q<D, S::NQ>(p, (uint64_t)(sq.a + row) * p.q_row + (uint64_t)head * D + 8 * h, live, qb);
     const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
@@ -554,12 +611,12 @@ __global__ __launch_bounds__(64 * WAVES, QF32 ? 1 : 2) void k_attn_many(PagedAtt
         if (vt + 1 < v1) stage.fetch(vt + 1);
         const int t0 = seen.tile(vt) * TILE;
         if (!all && (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3])) {
-            if (active) add_odd<D, S::NK>(p, &s_v[buf][0][0], t0, pos, acc);
+            if (active) add_odd<D, S::NK>(p, &s_v[buf][0][0], s_odd[buf], t0, pos, acc);
             __syncthreads();
             clear_odd(&s_v[buf][0][0], S::NK * S::VALUES / 2);
             __syncthreads();
         }
-        if (!active || !wseen.any(t0, t0 + TILE)) continue;
+        if (!active || !my.seen.any(t0, t0 + TILE)) continue;
 
         // Operands come from LDS a group ahead of the products that take
         // them: four fragments of keys (half a group's products hide the
@@ -596,7 +653,7 @@ __global__ __launch_bounds__(64 * WAVES, QF32 ? 1 : 2) void k_attn_many(PagedAtt
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
-        if (t0 + TILE > w_hi || t0 < w_lo) mask(p, t0, pos, s);
+        if (t0 + TILE > my.hi || t0 < my.lo) mask(p, t0, pos, s);
         const float base = follow(top_of(s) * sc, m, l, acc);
         pbf16x8 b[2][S::NQ];
         terms<S::NQ>(s[0], 0, sc, base, l, b[0]);
@@ -620,7 +677,118 @@ __global__ __launch_bounds__(64 * WAVES, QF32 ? 1 : 2) void k_attn_many(PagedAtt
     if (!live) return;
     l = sum_x32(l);
     if (s_fault) l = __builtin_nanf("");
-    put_out<D, S::CW, QF32>(p, sq, p.splits > 1 && seen.total() > p.chunk, split, row, head, m, l, acc, p.v_scale ? p.v_scale[kvh] : 1.0f);
+    put_out<D, S::CW, QF32>(p, sq, p.splits > 1 && seen.total() > p.chunk, w.split, row, head, m, l, acc, p.v_scale ? p.v_scale[kvh] : 1.0f);
+}
+
+// Prompts of BF16 queries with blocks enough: one workgroup of eight waves a CU,
+// which brings in each tile once for 256 columns, four waves its values and four
+// its keys. With half the registers for tiles on their way, operands are read
+// two groups ahead (a prompt of 4096 159 -> 154 us, a window of 1024 in BF16 256
+// -> 237 against two workgroups of four waves).
+template <int D, int CT>
+__global__ __launch_bounds__(512, 2) void k_attn_wide(PagedAttnArgs p)
+{
+    constexpr int COLS = 2 * ATTN_MANY_COLS;
+    using S = Shape<D, CT, false>;
+    __shared__ __attribute__((aligned(16))) uint16_t s_k[2][S::KEYS], s_v[2][S::VALUES];
+    __shared__ int s_odd[2][4], s_fault;
+    Work<COLS> w;
+    if (!w.find(p)) return;
+    const int kvh = w.kvh, v0 = w.v0, v1 = w.v1;
+    Stage<D, CT, 8> stage(p, w.seq, kvh, w.seen, v0, v1, w.all_hi(), w.all_lo(p));
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int c = lane & 31, h = lane >> 5;
+    const Columns my(p, w, w.cb * COLS + 32 * wave);
+    pbf16x8 qb[D / 16][1];
+    load_q<D, 1>(p, (uint64_t)(w.sq.a + my.row) * p.q_row + (uint64_t)my.head * D + 8 * h, my.live, qb);
+    const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
+
+    pf32x16 acc[D / 32] = {};
+    float m = -INFINITY, l = 0.0f;
+    if (threadIdx.x == 0) s_fault = 0;  // (read behind the last barrier, written behind the first)
+    __syncthreads();
+    __builtin_amdgcn_s_waitcnt(0);  // q is there, as in k_attn_many
+    if (v0 < v1) stage.fetch(v0);
+    for (int vt = v0; vt < v1; vt++) {
+        const int b = (vt - v0) & 1;
+        const bool all = stage.whole(vt);
+        if (!all) {
+            const bool odd = stage.clean(vt);
+            if (lane == 0 && stage.values) s_odd[b][stage.wave] = odd;
+        }
+        if (stage.values) stage.put(nullptr, s_v[b]);
+        else stage.put(s_k[b], nullptr);
+        __syncthreads();
+        if (vt + 1 < v1) stage.fetch(vt + 1);
+        const int t0 = w.seen.tile(vt) * TILE;
+        if (!all && (s_odd[b][0] | s_odd[b][1] | s_odd[b][2] | s_odd[b][3])) {
+            if (my.active) add_odd<D, 1>(p, s_v[b], s_odd[b], t0, my.pos, acc);
+            __syncthreads();
+            clear_odd(s_v[b], S::VALUES / 2);
+            __syncthreads();
+        }
+        if (!my.active || !my.seen.any(t0, t0 + TILE)) continue;
+
+        // Operands come from LDS in groups of four fragments, two groups ahead of
+        // the products that take them: keys, then values.
+        constexpr int KG = 2 * D / 64, VF = D / 32, GROUPS = KG + 4;
+        pbf16x8 frag[3][4];
+        const auto load = [&](int g) {
+            if (g < KG) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    frag[g % 3][i] =
+                        *(const pbf16x8*)&s_k[b][key_at<D>(2 * (4 * g % (D / 16) + i) + h, 32 * (4 * g / (D / 16)) + c)];
+            } else {
+#pragma unroll
+                for (int d = 0; d < VF; d++)
+                    frag[g % 3][d] = *(const pbf16x8*)&s_v[b][value_at<D>(g - KG, 0, 32 * d) + lane * 8];
+            }
+        };
+        pf32x16 s[2] = {};
+        load(0);
+        load(1);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int g = 0; g < KG; g++) {
+            load(g + 2);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                s[4 * g / (D / 16)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    frag[g % 3][i], qb[4 * g % (D / 16) + i][0], s[4 * g / (D / 16)], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (t0 + TILE > my.hi || t0 < my.lo) mask(p, t0, my.pos, s);
+        const float base = follow(top_of(s) * sc, m, l, acc);
+        pbf16x8 e[2][1];
+        terms<1>(s[0], 0, sc, base, l, e[0]);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int g = KG + j;
+            if (g + 2 < GROUPS) load(g + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            if (j < 3) terms<1>(s[(j + 1) / 2], 8 * ((j + 1) % 2), sc, base, l, e[(j + 1) & 1]);
+#pragma unroll
+            for (int d = 0; d < VF; d++) {
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[g % 3][d], e[j & 1][0], acc[d], 0, 0, 0);
+                // a product, then a share of the next group's exponentials
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 7, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    }
+    if (stage.fault) s_fault = 1;
+    __syncthreads();
+    if (!my.live) return;
+    l = sum_x32(l);
+    if (s_fault) l = __builtin_nanf("");
+    put_out<D, S::CW, false>(p, w.sq, p.splits > 1 && w.seen.total() > p.chunk, w.split, my.row, my.head, m, l, acc,
+                             p.v_scale ? p.v_scale[kvh] : 1.0f);
 }
 
 template <int D, int CT, bool QF32>
@@ -628,11 +796,11 @@ void go(const PagedAttnArgs& p, unsigned blocks, hipStream_t s)
 {
     if constexpr (!QF32) {
         if (p.cols == 2 * ATTN_MANY_COLS) {
-            k_attn_many<D, CT, QF32, 8><<<dim3(blocks), dim3(512), 0, s>>>(p);
+            k_attn_wide<D, CT><<<dim3(blocks), dim3(512), 0, s>>>(p);
             return;
         }
     }
-    k_attn_many<D, CT, QF32, 4><<<dim3(blocks), dim3(256), 0, s>>>(p);
+    k_attn_many<D, CT, QF32><<<dim3(blocks), dim3(256), 0, s>>>(p);
 }
 
 template <int D>
