@@ -95,6 +95,16 @@ def test_many_sequences_uniform_rows(ctx):
     assert len(set(acc.tolist())) == 4
 
 
+def test_many_ragged_sequences(ctx):
+    """More sequences than are looked at in one step."""
+    rng = np.random.default_rng(10)
+    c = case(rng, [int(x) for x in rng.integers(0, 5, 700)], 400)
+    acc, out = run(ctx, c, extra=5)
+    wa, wo = want(c)
+    assert np.array_equal(acc, wa) and np.array_equal(out[:len(wo)], wo) and (out[len(wo):] == 99).all()
+    assert set(acc.tolist()) == {0, 1, 2, 3, 4}
+
+
 def test_drafter_equal_to_the_target(ctx):
     """p = q to fp32: nearly every draft stands, and where one does not, the
     rest of p - q is rounding, compared in 64 bits."""

@@ -245,3 +245,29 @@ def test_other_streams(ctx):
         got = x.read(np.uint16, pg.bits[n].size)
         for s in range(2):
             assert np.array_equal(got[pg.index(s, np.arange(lens[s]))], keep[s][0 if n == "k" else 1])
+
+
+@pytest.mark.parametrize("n", [64, 65, 130, 4500])
+def test_many_sequences(ctx, n):
+    """A row's sequence is looked for in one, two and three steps; sequences
+    without rows between, rows behind the last."""
+    rng = np.random.default_rng(n)
+    rows = rng.integers(0, 4, n)
+    rows[0], rows[n - 1] = 0, 2
+    lens = [int(r) + int(x) for r, x in zip(rows, rng.integers(0, 20, n))]
+    pg = R.Paged(ctx, rng, F32, 1, 64, 16, lens).upload()
+    total = int(rows.sum())
+    batch = pg.batch(list(rows), n_rows=total + 3)
+    k, v = (R.encode(rng.standard_normal((total + 3, 1, 64)), F32) for _ in range(2))
+    op = wpcg.KvAppend(ctx, pg.kv, batch, 0, F32)
+    op.run(None, ctx.upload(k), ctx.upload(v), None)
+    ctx.sync()
+    for name, x, dev in (("k", k, pg.dk), ("v", v, pg.dv)):
+        want = pg.bits[name].copy()
+        at = 0
+        for s in range(n):
+            r = int(rows[s])
+            if r:
+                want[pg.index(s, np.arange(lens[s] - r, lens[s]))] = x[at:at + r]
+            at += r
+        assert np.array_equal(dev.read(np.uint32, want.size), want)

@@ -62,16 +62,6 @@ __device__ __forceinline__ Rows draft_rows(const DraftArgs& p, int s)
     const bool ok = a >= 0 && a < e && e <= p.n_rows && e - a <= p.max_rows;
     return {a, ok ? e - a : 0};
 }
-__device__ __forceinline__ int draft_seq(const DraftArgs& p, int r)
-{
-    if (!p.q_start) return r / p.max_rows;
-    int s = 0;
-    for (int i = 0; i < p.n_seq; i += 64) {
-        const int at = i + (int)(threadIdx.x & 63);
-        s += __popcll(__ballot(at < p.n_seq && p.q_start[at < p.n_seq ? at + 1 : 0] <= r));
-    }
-    return s;
-}
 // log2(e) / T, or 0: greedy
 __device__ __forceinline__ double draft_rate(const DraftArgs& p, int s)
 {
@@ -184,7 +174,7 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
     // the values are on their way while the row's sequence is looked for
     Chunk c;
     c.load(p.logits + (uint64_t)row * p.logits_row, chunk * CHUNK, p.vocab, p.vec, -INFINITY);
-    const int s = draft_seq(p, row);
+    const int s = p.q_start ? seq_of_row(p.q_start, p.n_seq, row) : row / p.max_rows;
     if (s >= p.n_seq) return;
     const Rows q = draft_rows(p, s);
     if (row < q.a || row >= q.a + q.n) return;

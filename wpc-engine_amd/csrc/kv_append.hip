@@ -63,19 +63,6 @@ __device__ __forceinline__ void store4(void* base, uint64_t at, int dtype, const
     }
 }
 
-// The sequence whose rows hold row r: how many of q_start[1..n_seq] are at
-// most r, counted 64 at a time by the wave.
-__device__ __forceinline__ int seq_of_row(const PagedBatch& b, int r)
-{
-    if (!b.q_start) return r;
-    int s = 0;
-    for (int i = 0; i < b.n_seq; i += 64) {
-        const int at = i + (int)(threadIdx.x & 63);
-        s += __popcll(__ballot(at < b.n_seq && b.q_start[at < b.n_seq ? at + 1 : 0] <= r));
-    }
-    return s;
-}
-
 template <int D, bool BF16>
 __global__ __launch_bounds__(THREADS) void k_kv_append(KvAppendArgs p)
 {
@@ -84,7 +71,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(KvAppendArgs p)
     __shared__ float2 turn[D / 2];
     const int groups = (p.n_units + HEADS - 1) / HEADS;
     const int r = (int)(blockIdx.x / (unsigned)groups);
-    const int s = seq_of_row(p.b, r);
+    const int s = p.b.q_start ? seq_of_row(p.b.q_start, p.b.n_seq, r) : r;
     if (s >= p.b.n_seq) return;
     const SeqRows q = seq_rows(p.b, s);
     if (r < q.a || r >= q.a + q.n) return;

@@ -40,6 +40,23 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedBatch& b, int s)
     return r;
 }
 
+// The sequence that holds row r: how many of start[1 .. n_seq], which rise, are
+// at most r. The wave looks at the ends of 64 groups of sequences at a time, of
+// one sequence each up to 64.
+__device__ __forceinline__ int seq_of_row(const int32_t* start, int n_seq, int r)
+{
+    int lo = 0;  // so many are
+    for (int left = n_seq; left > 0;) {
+        const int step = (left + 63) / 64, at = lo + ((int)(threadIdx.x & 63) + 1) * step;
+        const uint64_t most = __ballot(at <= lo + left && start[at <= lo + left ? at : 0] <= r);
+        const int groups = __popcll(most);
+        lo += groups * step;
+        // the next group's end is not, or lies behind the last
+        left = min(step - 1, left - groups * step);
+    }
+    return lo;
+}
+
 // The tokens that the rows at positions p0 .. p1 (p0 <= p1, p1 >= 0) see
 // together, as a list of TILE-token tiles: tiles [0, head) cover the sinks,
 // tiles [first, end) the rest. lo, hi: [lo, hi) and [0, sinks) are the tokens
