@@ -25,12 +25,12 @@
 // terms too, and a product of two fp32 values takes the six of its nine terms
 // that reach 2^-24.
 //
-// Measured, heads of 128: a prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 147
-// us, 935 TFLOP/s, with the matrix cores busy in 40 % of the cycles and the
+// Measured, heads of 128: a prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 146
+// us, 940 TFLOP/s, with the matrix cores busy in 40 % of the cycles and the
 // vector units in 42 %; 2048 rows behind 30720 tokens 1050 TFLOP/s (a library's
 // 8192^3 product 1300); two prompts of up to 5000 with a window of 1024, 32 / 4
-// heads over E4M3 (144 GFLOP) 223 us; 777 rows behind 523 tokens, 32 / 4 heads,
-// all F32 (11.6 GFLOP, six products each) 123 us with the join's 11.
+// heads over E4M3 (144 GFLOP) 226 us; 777 rows behind 523 tokens, 32 / 4 heads,
+// all F32 (11.6 GFLOP, six products each) 124 us with the join's 11.
 #include "paged.h"
 
 namespace wpcg {
@@ -288,10 +288,9 @@ struct Stage {
 };
 
 // Values of a tile that are not finite, added to the columns that see their
-// token (products with ones count the +inf, -inf and NaN a column sees); in:
-// the 16-token groups that hold some.
+// token (products with ones count the +inf, -inf and NaN a column sees).
 template <int D, int NK>
-__device__ __forceinline__ void add_odd(const PagedAttnArgs& p, const uint16_t* values, const int* in, int t0, int pos,
+__device__ __forceinline__ void add_odd(const PagedAttnArgs& p, const uint16_t* values, int t0, int pos,
                                         pf32x16 (&acc)[D / 32])
 {
     const int lane = (int)threadIdx.x & 63, h = lane >> 5;
@@ -299,7 +298,6 @@ __device__ __forceinline__ void add_odd(const PagedAttnArgs& p, const uint16_t* 
     for (int d = 0; d < D / 32; d++) {
 #pragma unroll 1
         for (int j = 0; j < 4; j++) {
-            if (!in[j]) continue;
             pu32x4 see;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -611,7 +609,7 @@ __global__ __launch_bounds__(256, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p
         if (vt + 1 < v1) stage.fetch(vt + 1);
         const int t0 = seen.tile(vt) * TILE;
         if (!all && (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3])) {
-            if (active) add_odd<D, S::NK>(p, &s_v[buf][0][0], s_odd[buf], t0, pos, acc);
+            if (active) add_odd<D, S::NK>(p, &s_v[buf][0][0], t0, pos, acc);
             __syncthreads();
             clear_odd(&s_v[buf][0][0], S::NK * S::VALUES / 2);
             __syncthreads();
@@ -722,7 +720,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_wide(PagedAttnArgs p)
         if (vt + 1 < v1) stage.fetch(vt + 1);
         const int t0 = w.seen.tile(vt) * TILE;
         if (!all && (s_odd[b][0] | s_odd[b][1] | s_odd[b][2] | s_odd[b][3])) {
-            if (my.active) add_odd<D, 1>(p, s_v[b], s_odd[b], t0, my.pos, acc);
+            if (my.active) add_odd<D, 1>(p, s_v[b], t0, my.pos, acc);
             __syncthreads();
             clear_odd(s_v[b], S::VALUES / 2);
             __syncthreads();

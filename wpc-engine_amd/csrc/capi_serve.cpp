@@ -132,12 +132,13 @@ int plan_kernel(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attenti
     };
     if (p.many) {
         // 256 columns a workgroup where that leaves every CU one and the tiles
-        // are some: two prompts of up to 5000 with a window of 1024 (18 tiles a
-        // block), 32 / 4 heads, BF16 256 us with 128 columns and 237 so, E4M3 241
-        // and 240; eight prompts of up to 1000, 32 / 8 heads, 115 and 107; below,
-        // a CU's one workgroup starts and ends alone.
-        const int64_t wide = 2 * ATTN_MANY_COLS;
-        p.cols = a->dtype == WPCG_DTYPE_BF16 && tiles_of(wide) >= 16 && kv->n_kv_heads * all_blocks(wide) >= CUS
+        // are some, more over E4M3, where the narrower form's registers suffice:
+        // two prompts of up to 5000 with a window of 1024 (18 tiles a block),
+        // 32 / 4 heads, BF16 256 us with 128 columns and 237 so, E4M3 225 and 231;
+        // a prompt of 4096, 32 / 8 heads, BF16 158 and 147; eight of up to 1000
+        // 115 and 107. Below, a CU's one workgroup starts and ends alone.
+        const int64_t wide = 2 * ATTN_MANY_COLS, some = kv->dtype == WPCG_DTYPE_E4M3 ? 32 : 16;
+        p.cols = a->dtype == WPCG_DTYPE_BF16 && tiles_of(wide) >= some && kv->n_kv_heads * all_blocks(wide) >= CUS
                      ? wide : ATTN_MANY_COLS;
     } else {
         // (over an F32 cache the wider form's registers do not suffice)
