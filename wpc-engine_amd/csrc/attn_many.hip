@@ -27,10 +27,11 @@
 //
 // Measured, heads of 128: a prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 146
 // us, 940 TFLOP/s, with the matrix cores busy in 40 % of the cycles and the
-// vector units in 42 %; 2048 rows behind 30720 tokens 1050 TFLOP/s (a library's
-// 8192^3 product 1300); two prompts of up to 5000 with a window of 1024, 32 / 4
-// heads over E4M3 (144 GFLOP) 226 us; 777 rows behind 523 tokens, 32 / 4 heads,
-// all F32 (11.6 GFLOP, six products each) 124 us with the join's 11.
+// vector units in 42 %; the last 2048 rows of 32768 tokens 1050 TFLOP/s (a
+// library's 8192^3 product 1300); two prompts of up to 5000 with a window of
+// 1024, 32 / 4 heads over E4M3 (144 GFLOP) 226 us; 777 rows behind 523 tokens,
+// 32 / 4 heads, all F32 (11.6 GFLOP, six products each) 124 us with the join's
+// 11.
 #include "paged.h"
 
 namespace wpcg {
