@@ -630,7 +630,8 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  *   weights passes u_next[s] times their total (where p_r - q_r leaves no
  *   weight at all: from p_r).
  * A temperature not above 0 (null: all 1) is greedy: a draft is accepted while
- * it is the first largest logit, which also is the next token. accepted[s]
+ * it is the first largest logit, which also is the next token; at +inf all ids
+ * with a logit above -inf are alike. accepted[s]
  * receives the number of accepted drafts, out the rows' tokens: the accepted
  * drafts, the next token, then -1. Probabilities, running sums and comparisons
  * are fp64; u and u_next are in [0, 1). A row without any weight (NaN, +inf, or

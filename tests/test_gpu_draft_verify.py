@@ -225,3 +225,49 @@ def test_other_streams(ctx):
         o.sync()
         assert np.array_equal(acc.read(np.int32, 3), wa) and np.array_equal(out.read(np.int32, n), wo)
         o.close()
+
+
+def test_infinite_temperature(ctx):
+    """softmax(logits / inf): every id whose logit is above -inf alike, and no
+    mark for greedy; sequences at other temperatures beside it."""
+    rng = np.random.default_rng(11)
+    inf = np.float32(np.inf)
+    for vocab in (7, 3000, 20011):
+        for with_probs in (True, False):
+            c = case(rng, [3, 0, 5, 2, 1, 4, 0, 2], vocab, temperature=[inf, inf, inf, 0, 1, inf, inf, inf])
+            c["u"][:4] = 0.5 / vocab  # below every p / q: drafts that were chosen outright pass too
+            acc, out = run(ctx, c, with_probs)
+            wa, wo = want(c, with_probs)
+            assert np.array_equal(acc, wa) and np.array_equal(out, wo), (vocab, with_probs)
+            assert acc[0] == 3
+
+
+def test_infinite_temperature_over_masked_ids(ctx):
+    """Ids at -inf have no weight at any temperature, all others one and the
+    same; rows of no weight, NaN or +inf accept nothing."""
+    rng = np.random.default_rng(12)
+    vocab, n = 5000, 12
+    c = case(rng, [0] * n + [1, 1], vocab, temperature=[np.inf] * (n + 2))
+    lg = c["logits"]
+    lg[:] *= 1e30
+    open_ids = [np.sort(rng.choice(vocab, int(k), replace=False)) for k in rng.integers(1, vocab, n + 2)]
+    open_ids[0], open_ids[1] = np.array([4321]), np.arange(vocab)
+    for r in range(n + 2):
+        row = r if r <= n else n + 2
+        keep = lg[row, open_ids[r]]
+        lg[row] = -np.inf
+        lg[row, open_ids[r]] = keep
+    lg[9], lg[10, 3], lg[11, 3] = -np.inf, np.nan, np.inf
+    # the drafts, chosen outright: an open id (probability 1 / k), a masked one
+    k = len(open_ids[n])
+    c["tokens"][n + 1], c["u"][n] = open_ids[n][k // 2], 0.9 / k
+    c["tokens"][n + 3], c["u"][n + 2] = np.setdiff1d(np.arange(vocab), open_ids[n + 1])[0], 0
+    acc, out = run(ctx, c, with_probs=False)
+    for r in range(9):
+        ids = open_ids[r]
+        at = float(c["u_next"][r]) * len(ids)
+        assert abs(at - round(at)) > 1e-6 and out[r] == ids[int(at)], r
+    assert (out[9:12] == -1).all() and (acc[9:12] == 0).all()
+    assert acc[n] == 1 and out[n] == c["tokens"][n + 1]
+    ids = open_ids[n + 1]
+    assert acc[n + 1] == 0 and out[n + 2] == ids[int(float(c["u_next"][n + 1]) * len(ids))] and out[n + 3] == -1

@@ -275,3 +275,17 @@ def test_model_verify_sampled(ctx, name, cfg, mode, seed):
     with pytest.raises(wpcg.WpcgError, match="full"):
         m.verify_sampled(np.zeros(17), np.zeros(16), 0.5)
     m.close()
+
+
+def test_model_verify_sampled_at_infinite_temperature(ctx):
+    """All ids alike: drafts chosen outright stand while u is below 1 / vocab."""
+    m = model(ctx, DENSE, tensors_of(DENSE, 24), wpcg.MODE_FAST)
+    V = DENSE["vocab"]
+    m.prefill(np.arange(9, dtype=np.uint32))
+    for u, kept in (([0.5 / V, 0.0005, 0.0011], 2), ([0.5, 0, 0], 0), ([0, 0, 0], 3)):
+        got, out = m.verify_sampled(np.array([3, 500, 1, 999]), u, 0.2505, temperature=np.inf)
+        m.set_position(9)
+        assert got == kept and out[:kept].tolist() == [500, 1, 999][:kept] and (out[kept + 1:] == -1).all()
+        # running sums of 1000 ones, of 999 without the rejected draft (500: behind the mark; 999)
+        assert out[kept] == 250
+    m.close()

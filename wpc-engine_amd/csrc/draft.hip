@@ -62,11 +62,12 @@ __device__ __forceinline__ Rows draft_rows(const DraftArgs& p, int s)
     const bool ok = a >= 0 && a < e && e <= p.n_rows && e - a <= p.max_rows;
     return {a, ok ? e - a : 0};
 }
-// log2(e) / T, or 0: greedy
+// log2(e) / T, or 0: greedy. For an infinite T 2^-1000: a difference of finite
+// logits times that is nothing beside 1, and one to -inf stays -inf.
 __device__ __forceinline__ double draft_rate(const DraftArgs& p, int s)
 {
     const float t = p.temperature ? p.temperature[s] : 1.0f;
-    return t > 0.0f ? 1.4426950408889634 / (double)t : 0.0;
+    return t > 0.0f ? fmax(1.4426950408889634 / (double)t, 0x1p-1000) : 0.0;
 }
 
 // Lane exchanges of doubles: 0 from lanes that there are none.
