@@ -271,3 +271,29 @@ def test_infinite_temperature_over_masked_ids(ctx):
     assert acc[n] == 1 and out[n] == c["tokens"][n + 1]
     ids = open_ids[n + 1]
     assert acc[n + 1] == 0 and out[n + 2] == ids[int(float(c["u_next"][n + 1]) * len(ids))] and out[n + 3] == -1
+
+
+@pytest.mark.parametrize("vocab,block,second", [(2048, 1000, 1024), (4096, 1500, 2048 + 300), (26 * 2048, 5 * 2048 + 11, 13 * 2048),
+                                                (600 * 2048, 3 * 2048, 333 * 2048)])
+@pytest.mark.parametrize("rest", [False, True])
+def test_the_drawn_id_has_weight(ctx, vocab, block, second, rest):
+    """Two equal blocks of weights and u_next at 1/2: the running sum meets the
+    mark where the first block ends, to rounding that depends on its order. Ids
+    without weight between the blocks (masked, or with p below q) are never
+    drawn: the last id of the first block or the first one of the second is."""
+    rng = np.random.default_rng(vocab + rest)
+    n = max(24, min(400, (1 << 23) // vocab))
+    rows = [2] * n if rest else [1] * n
+    total = sum(rows)
+    at = np.arange(0, total, rows[0])  # the rows that the next tokens come from
+    lg = np.full((total, vocab), 0.0 if rest else -np.inf, np.float32)
+    x = (rng.standard_normal((n, block)) * 3).astype(np.float32)
+    lg[at, :block] = lg[at, second:second + block] = x
+    probs = np.ones((total, vocab), np.float32)
+    probs[:, :block] = probs[:, second:second + block] = 0
+    c = {"rows": rows, "logits": lg, "probs": probs, "tokens": np.full(total, vocab - 1, np.uint32),
+         "u": np.full(total, np.nextafter(np.float32(1), np.float32(0))), "u_next": np.full(n, 0.5, np.float32),
+         "t": np.full(n, 1, np.float32)}
+    acc, out = run(ctx, c, with_probs=rest)
+    assert (acc == 0).all()
+    assert set(out[at].tolist()) <= {block - 1, second}

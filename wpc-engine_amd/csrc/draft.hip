@@ -311,7 +311,9 @@ __device__ __forceinline__ void draft_chunk(Chunk& q, const DraftArgs& p, int ro
 
 // The first thread that found something: its number and running sum; and the
 // last thread's that has some weight. Numbers rise with the threads; MISSING or
-// -1 where there is none. s: of four waves.
+// -1 where there is none. s: of four waves. A thread's running sum starts from
+// the scan and ends in its own order, so that the next one's start may be past
+// the mark where its end is not: only what has weight itself is found.
 constexpr int MISSING = 0x7fffffff;
 struct Found {
     int at, last;
@@ -384,10 +386,12 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
     int at = MISSING, last = -1;  // last: of use where rounding leaves none
     for (int i = j0; i < j1; i++) {
         const double w = run == 1 ? only : of_chunk(i);
-        if (w > 0.0) last = i;
-        if (before + w > want) {
-            at = i;
-            break;
+        if (w > 0.0) {
+            last = i;
+            if (before + w > want) {
+                at = i;
+                break;
+            }
         }
         before += w;
     }
@@ -413,8 +417,10 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         t += w[j];
-        if (w[j] > 0.0) final = i0 + j;
-        if (!end && t > want && first == MISSING) first = i0 + j;
+        if (w[j] > 0.0) {
+            final = i0 + j;
+            if (!end && t > want && first == MISSING) first = i0 + j;
+        }
     }
     const Found id = find_first(first != MISSING, first, 0.0, final, s_id);
     return id.at != MISSING ? id.at : id.last;
