@@ -297,3 +297,24 @@ def test_the_drawn_id_has_weight(ctx, vocab, block, second, rest):
     acc, out = run(ctx, c, with_probs=rest)
     assert (acc == 0).all()
     assert set(out[at].tolist()) <= {block - 1, second}
+
+
+def test_one_workspace_for_calls_in_a_row(ctx):
+    """Calls over other data one behind the other, without a wait between: the
+    parts and counts that a call leaves are none of the next one's."""
+    rng = np.random.default_rng(13)
+    cs = [case(rng, [4, 1, 0, 3] * 6, 21000, agree=1.5) for _ in range(5)]
+    n, k = len(cs[0]["tokens"]), len(cs[0]["rows"])
+    q = ctx.upload(np.cumsum([0] + cs[0]["rows"]).astype(np.int32))
+    op = wpcg.DraftVerify(ctx, k, n, 5, 21000, q_start=q)
+    dev = [{x: ctx.upload(c[x]) for x in ("logits", "probs", "tokens", "u", "u_next")} for c in cs]
+    order = [i for _ in range(4) for i in rng.permutation(5)]
+    outs = [(ctx.alloc(4 * k), ctx.alloc(4 * n)) for _ in order]
+    for i, (acc, out) in zip(order, outs):
+        d = dev[i]
+        op.run(d["logits"], d["tokens"], d["u"], d["u_next"], acc, out, draft_probs=d["probs"])
+    ctx.sync()
+    right = [want(c) for c in cs]
+    for i, (acc, out) in zip(order, outs):
+        assert np.array_equal(acc.read(np.int32, k), right[i][0]) and np.array_equal(out.read(np.int32, n), right[i][1])
+    assert min(min(a) for a, _ in right) == 0  # (drafts that fall: the parts are of use)

@@ -9,7 +9,11 @@
 //     weight of the row that the next token comes from, max(0, p - q). The
 //     sequence's last workgroup to finish finds the chunk in which the running
 //     sum passes u_next * total, then the place in it, and writes the results;
-//     the first launch has set the counter that it is known by.
+//     the first launch has set the counter that it is known by, and the parts
+//     to a mark that is none: a part is one atomic word, so that whoever reads
+//     another value has all of it, and no order between words is needed. (A
+//     release of the count writes the L2 back for every workgroup: 64 sequences
+//     68 and 102 us.)
 // Every logit is read once and one row of each sequence a second time (with
 // the drafter's row), so memory bounds a batch, and launch latency a single
 // sequence. Exponentials, sums and comparisons are fp64: a draft that is as
@@ -28,6 +32,9 @@ namespace {
 
 constexpr int THREADS = 256, CHUNK = DRAFT_CHUNK;
 static_assert(CHUNK == 8 * THREADS, "pick: eight ids a thread");
+// In `rest` until the chunk's sum is there, which is not negative. Who waits for
+// it has seen its workgroup's count, so that the store is on its way.
+constexpr double NO_SUM = -1.0;
 
 // 2^(x rate) for x <= 0 (or NaN), a difference of two logits: x rate = n + f, n
 // the whole number that adding 1.5 * 2^52 leaves in the low bits, the
@@ -165,13 +172,10 @@ struct Chunk {
     }
 };
 
-__global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
+// A chunk's state of a row, by a wave.
+__device__ __forceinline__ void chunk_state(const DraftArgs& p, int row, int chunk)
 {
-    const int groups = (p.chunks + 3) / 4;
-    const int row = (int)(blockIdx.x / (unsigned)groups);
-    const int chunk = (int)(blockIdx.x % (unsigned)groups) * 4 + ((int)threadIdx.x >> 6);
     const int lane = (int)threadIdx.x & 63;
-    if (chunk >= p.chunks) return;
     // the values are on their way while the row's sequence is looked for
     Chunk c;
     c.load(p.logits + (uint64_t)row * p.logits_row, chunk * CHUNK, p.vocab, p.vec, -INFINITY);
@@ -179,7 +183,6 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
     if (s >= p.n_seq) return;
     const Rows q = draft_rows(p, s);
     if (row < q.a || row >= q.a + q.n) return;
-    if (row == q.a && chunk == 0 && lane == 0) p.done[s].done = 0;
     const double rate = draft_rate(p, s);
     float best = -INFINITY;
 #pragma unroll
@@ -199,6 +202,24 @@ __global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
         at = ~wave_max_i(~at);
     }
     if (lane == 0) p.part[(uint64_t)row * p.chunks + chunk] = DraftPart{sum, best, best == -INFINITY ? 0x7fffffff : at};
+}
+
+__global__ __launch_bounds__(THREADS) void k_draft_stats(DraftArgs p)
+{
+    const int groups = (p.chunks + 3) / 4;
+    const int row = (int)(blockIdx.x / (unsigned)groups);
+    const int chunk = (int)(blockIdx.x % (unsigned)groups) * 4 + ((int)threadIdx.x >> 6);
+    if (chunk >= p.chunks) return;
+    chunk_state(p, row, chunk);
+    // The second launch's arrays made ready, of sequences without rows too. (At
+    // the end: behind these stores the loads above would not be scalar ones, and
+    // wait for the logits: 64 sequences 44 and 52 us.)
+    if ((threadIdx.x & 63) == 0) {
+        for (int s = row; s < p.n_seq; s += p.n_rows) {
+            p.rest[(uint64_t)s * p.chunks + chunk] = NO_SUM;
+            if (chunk == 0) p.done[s].done = 0;
+        }
+    }
 }
 
 // M and Z of a row (Z = sum of 2^((x - M) rate)), by 32 lanes; at: the first
@@ -367,7 +388,12 @@ __device__ int pick(const DraftArgs& p, int s, int row, const Choice& c, double 
     const double u = (double)p.u_next[s];
     bool rest = c.rest;
     const auto of_chunk = [&](int i) {
-        if (rest) return __hip_atomic_load(&p.rest[(uint64_t)s * p.chunks + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (rest) {
+            double w;
+            do w = __hip_atomic_load(&p.rest[(uint64_t)s * p.chunks + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            while (w == NO_SUM);
+            return w;
+        }
         const DraftPart& part = p.part[(uint64_t)row * p.chunks + i];
         return part.max == -INFINITY ? 0.0 : part.sum * exp2_d((double)part.max - (double)c.st.m, rate);
     };
@@ -460,17 +486,9 @@ __global__ __launch_bounds__(THREADS) void k_draft_choose(DraftArgs p)
 #pragma unroll
                 for (int i = 0; i < CHUNK / 64; i++) sum += weight(x.v[i], r.v[i], c.st, rate, true);
                 sum = wave_sum_d(sum);
-                // Handed over by an exchange, which is performed at the
-                // device's coherence point and returns only then; the empty
-                // asm waits for it. So every part of this workgroup is there
-                // before its count, and the last one's coherent loads find
-                // them; no cache is written back or invalidated for it.
-                if ((tid & 63) == 0) {
-                    const uint64_t was = __hip_atomic_exchange((uint64_t*)p.rest + (uint64_t)s * p.chunks + chunk,
-                                                               __builtin_bit_cast(uint64_t, sum), __ATOMIC_RELAXED,
-                                                               __HIP_MEMORY_SCOPE_AGENT);
-                    asm volatile("" ::"v"(was));
-                }
+                if ((tid & 63) == 0)
+                    __hip_atomic_store(&p.rest[(uint64_t)s * p.chunks + chunk], sum, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
             }
             // the last of the sequence's workgroups goes on
             __syncthreads();
