@@ -480,3 +480,24 @@ def test_nothing_to_do(ctx):
     pg.d_len.write(np.zeros(1, np.int32))
     got, _ = run(ctx, pg, batch, R.encode(rng.standard_normal((1, 1, 64)), BF16), 1, BF16, 0.125)
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("rows,lens,max_q,n_rows,heads,hkv,d", [([60], [9000], 64, 3000, 8, 2, 128),
+                                                                ([40, 0, 33, 1], [5000, 9, 3000, 2], 48, 900, 14, 2, 64)])
+def test_rows_far_below_their_bound(ctx, q_dtype, dtype, rows, lens, max_q, n_rows, heads, hkv, d):
+    """A batch that is split, n_rows a much looser bound than max_q of each
+    sequence: the parts are the sequences' own, the rows behind stay as they were."""
+    print(f"[gpu] loose rows: {q_dtype}/{dtype} rows {rows} of {n_rows}", flush=True)
+    rng = np.random.default_rng(n_rows + q_dtype + 10 * dtype)
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 16, lens, scales=dtype == E4M3).upload()
+    n = sum(rows)
+    q = np.zeros((n_rows, heads, d), R.BITS[q_dtype])
+    q[:n] = R.encode(rng.standard_normal((n, heads, d)) * 1.5, q_dtype)
+    b = pg.batch(rows, n_rows=n_rows, max_q=max_q)
+    got, op = run(ctx, pg, b, q, heads, q_dtype, 0.09)
+    part = len(rows) * max_q * heads * (d + 2) * 4
+    assert op.workspace_bytes >= 2 * part and op.workspace_bytes % part == 0
+    check(got[:n], *expected(pg, q[:n], rows, heads, q_dtype, 0.09, 0, 0))
+    fill = R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]
+    assert (got[n:] == fill).all()

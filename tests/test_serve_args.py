@@ -225,3 +225,29 @@ def test_frequencies():
     f = wpcg.rope_frequencies(1e6, 128)
     assert f.dtype == np.float64 and f.shape == (64,)
     assert f[0] == 1.0 and np.allclose(f[63], 1e6 ** (-126 / 128), rtol=1e-14)
+
+
+def test_workspace_under_loose_bounds():
+    """n_rows may be far above what the sequences can have: parts are of max_q
+    rows each then, and in any case of at most 2048 workgroups of 128 columns."""
+    def of(n_seq, n_rows, max_q, max_kv, heads, hkv, q=BF16, c=BF16, d=128, window=0):
+        kv = pages(n_kv_heads=hkv, head_dim=d, dtype=c)
+        b = batch(n_seq=n_seq, n_rows=n_rows, max_q=max_q, max_kv=max_kv, table_stride=max_kv // 16 + 1)
+        n = C.c_uint64(7)
+        a = attention(dtype=q, n_heads=heads, window=window)
+        rc = wpcg.lib.wpcg_paged_attention_workspace(ref(kv), ref(b), ref(a), C.byref(n))
+        assert rc == OK or (rc == E_UNSUPPORTED and "workgroups" in wpcg.last_error() and n.value == 0)
+        return n.value
+    for n_seq, max_q, max_kv, heads, hkv in ((1, 64, 131072, 32, 4), (8, 64, 4096, 32, 8), (3, 40, 60000, 8, 2)):
+        tight = of(n_seq, n_seq * max_q, max_q, max_kv, heads, hkv)
+        assert 0 < tight <= 2048 * 128 * 130 * 4
+        for n_rows in (n_seq * max_q + 1, 4000, 32768, 1 << 22):
+            assert of(n_seq, n_rows, max_q, max_kv, heads, hkv) == tight
+    rng = np.random.default_rng(1)
+    for _ in range(3000):
+        n_seq, n_rows, max_q, max_kv, window = (int(2 ** x) for x in rng.random(5) * [12, 22, 16, 20, 16])
+        hkv, group = int(rng.choice([1, 2, 4, 5, 8])), int(rng.choice([1, 2, 4, 7, 20, 64]))
+        q, c = [(BF16, BF16), (BF16, E4M3), (F32, F32), (F32, BF16)][int(rng.integers(4))]
+        d, window = int(rng.choice([64, 128])), window * int(rng.integers(2))
+        n = of(n_seq, n_rows, max_q, max_kv, hkv * group, hkv, q, c, d, window)
+        assert n <= 2048 * 128 * (d + 2) * 4, (n_seq, n_rows, max_q, max_kv, hkv, group, q, c, d, window, n)

@@ -426,12 +426,13 @@ __device__ __forceinline__ void terms(const pf32x16& s, int i0, float sc, float 
 }
 // A column's output, or its part of it.
 template <int D, int CW, bool QF32>
-__device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& sq, bool part, int split, int row, int head,
-                                        float m, float l, const pf32x16 (&acc)[D / 32], float v_scale)
+__device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& sq, int seq, bool part, int split, int row,
+                                        int head, float m, float l, const pf32x16 (&acc)[D / 32], float v_scale)
 {
     constexpr int NCH = D / CW;
     const int h = ((int)threadIdx.x & 63) >> 5;
-    const uint64_t slot = ((uint64_t)split * p.b.n_rows + sq.a + row) * p.n_heads + head;
+    const int first = p.part_seq ? seq * p.part_seq : sq.a;
+    const uint64_t slot = ((uint64_t)split * p.part_rows + first + row) * p.n_heads + head;
 #pragma unroll
     for (int a0 = 0; a0 < NCH / 8; a0++)
 #pragma unroll
@@ -676,7 +677,8 @@ __global__ __launch_bounds__(256, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p
     if (!live) return;
     l = sum_x32(l);
     if (s_fault) l = __builtin_nanf("");
-    put_out<D, S::CW, QF32>(p, sq, p.splits > 1 && seen.total() > p.chunk, w.split, row, head, m, l, acc, p.v_scale ? p.v_scale[kvh] : 1.0f);
+    put_out<D, S::CW, QF32>(p, sq, w.seq, p.splits > 1 && seen.total() > p.chunk, w.split, row, head, m, l, acc,
+                            p.v_scale ? p.v_scale[kvh] : 1.0f);
 }
 
 // Prompts of BF16 queries with blocks enough: one workgroup of eight waves a CU,
@@ -786,8 +788,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_wide(PagedAttnArgs p)
     if (!my.live) return;
     l = sum_x32(l);
     if (s_fault) l = __builtin_nanf("");
-    put_out<D, S::CW, false>(p, w.sq, p.splits > 1 && w.seen.total() > p.chunk, w.split, my.row, my.head, m, l, acc,
-                             p.v_scale ? p.v_scale[kvh] : 1.0f);
+    put_out<D, S::CW, false>(p, w.sq, w.seq, p.splits > 1 && w.seen.total() > p.chunk, w.split, my.row, my.head, m, l,
+                             acc, p.v_scale ? p.v_scale[kvh] : 1.0f);
 }
 
 template <int D, int CT, bool QF32>
@@ -826,17 +828,24 @@ __global__ __launch_bounds__(256) void k_attn_many_join(PagedAttnArgs p)
     const int tid = (int)threadIdx.x, d = tid % TH * 4;
     const uint64_t x = (uint64_t)blockIdx.x * PER + tid / TH;
     const int head = (int)(x % (unsigned)p.n_heads);
-    const uint64_t at = x / (unsigned)p.n_heads;
-    if (at >= (uint64_t)p.b.n_rows) return;
-    // the row's sequence: the last one that starts at or before it
-    int lo = 0, hi = p.b.n_seq - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if ((p.b.q_start ? p.b.q_start[mid] : mid) <= (int)at) lo = mid;
-        else hi = mid - 1;
+    const uint64_t at = x / (unsigned)p.n_heads;  // row of the parts
+    if (at >= (uint64_t)p.part_rows) return;
+    SeqRows sq;
+    int row;
+    if (p.part_seq) {
+        sq = seq_rows(p.b, (int)at / p.part_seq);
+        row = (int)at % p.part_seq;
+    } else {
+        // the row's sequence: the last one that starts at or before it
+        int lo = 0, hi = p.b.n_seq - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if ((p.b.q_start ? p.b.q_start[mid] : mid) <= (int)at) lo = mid;
+            else hi = mid - 1;
+        }
+        sq = seq_rows(p.b, lo);
+        row = (int)at - sq.a;
     }
-    const SeqRows sq = seq_rows(p.b, lo);
-    const int row = (int)at - sq.a;
     if (row < 0 || row >= sq.n) return;
     const int cols = sq.n * p.group, cb = (row * p.group + head % p.group) / p.cols;
     const int len = sq.bad ? 0 : sq.len, pos0 = len - sq.n;
@@ -844,8 +853,8 @@ __global__ __launch_bounds__(256) void k_attn_many_join(PagedAttnArgs p)
     const int tiles = seen_tiles<TILE>(pos0 + first, pos0 + last, p.window, p.sinks).total();
     if (tiles <= p.chunk) return;
     const int n = (tiles + p.chunk - 1) / p.chunk;
-    const uint64_t slot0 = (uint64_t)(sq.a + row) * p.n_heads + head;
-    const uint64_t step = (uint64_t)p.b.n_rows * p.n_heads;
+    const uint64_t slot0 = at * p.n_heads + head;
+    const uint64_t step = (uint64_t)p.part_rows * p.n_heads;
     float m = -INFINITY, l = 0.0f;
     pf32x4 o = {};
     for (int i0 = 0; i0 < n; i0 += 4) {  // four in flight
@@ -870,7 +879,7 @@ __global__ __launch_bounds__(256) void k_attn_many_join(PagedAttnArgs p)
 template <int D, bool QF32>
 void join(const PagedAttnArgs& p, hipStream_t s)
 {
-    const uint64_t all = (uint64_t)p.b.n_rows * p.n_heads;
+    const uint64_t all = (uint64_t)p.part_rows * p.n_heads;
     k_attn_many_join<D, QF32><<<dim3((unsigned)((all * (D / 4) + 255) / 256)), dim3(256), 0, s>>>(p);
 }
 

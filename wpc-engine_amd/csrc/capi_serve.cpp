@@ -100,7 +100,7 @@ int check_pointers(const wpcg_kv_pages* kv, const wpcg_kv_batch* b)
 struct Plan {
     PagedBatch b;  // with the rows a sequence that it takes
     bool many;
-    int cols, col_blocks, blocks, chunk, splits;
+    int cols, col_blocks, blocks, chunk, splits, part_rows, part_seq;
     double us;       // of a workgroup's tiles, by estimate
     uint64_t parts;  // columns whose states the workspace holds
     uint64_t bytes;
@@ -184,16 +184,21 @@ int plan_kernel(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attenti
         return rounds * (4.0 + chunk * tile) + join;
     };
     const int64_t least = p.many ? 2 : ATTN_FEW_WAVES;  // tiles of a chunk
-    // (the many-row kernel's parts are of all n_rows, which may be a loose bound)
-    const int64_t room_parts = p.many && (int64_t)b.n_rows * a->n_heads > 1 << 20 ? 0 : 4 * room;
     int64_t best = 1;
-    for (int64_t s = 2; base > 0 && s <= tiles / least && base * s <= room_parts; s++)
+    for (int64_t s = 2; base > 0 && s <= tiles / least && base * s <= 4 * room; s++)
         if (cost(s) < cost(best)) best = s;
     p.chunk = (int)std::max<int64_t>(1, (tiles + best - 1) / best);
     p.splits = (int)std::max<int64_t>(1, (tiles + p.chunk - 1) / p.chunk);
     p.us = p.chunk * tile;
     p.blocks = look ? (int)all_blocks(p.cols) : 0;
-    p.parts = p.splits == 1 ? 0 : p.many ? (uint64_t)p.splits * b.n_rows * a->n_heads : (uint64_t)p.splits * base * p.cols;
+    // Rows that the sequences can have: n_rows may be a looser bound. The blocks'
+    // columns are as many at least, so that parts are 4 * room * cols at most.
+    const int64_t seq_rows = (int64_t)b.n_seq * b.max_q;
+    p.part_seq = seq_rows < b.n_rows ? b.max_q : 0;
+    p.part_rows = (int)std::min<int64_t>(seq_rows, b.n_rows);
+    p.parts = p.splits == 1 ? 0
+              : p.many      ? (uint64_t)p.splits * p.part_rows * a->n_heads
+                            : (uint64_t)p.splits * base * p.cols;
     // A chunk that long may be one sequence's alone while the others' are
     // empty, for the bounds do not tell: all tiles are dealt out evenly
     // instead. (63 sequences of 500 tokens and one of 100000, 32 / 4 heads: 1028
@@ -409,6 +414,8 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
         a.blocks = p.blocks;
         a.chunk = p.chunk;
         a.splits = p.splits;
+        a.part_rows = p.part_rows;
+        a.part_seq = p.part_seq;
         a.part_o = (float*)ws_dev;
         a.part_ml = a.part_o + p.parts * kv->head_dim;
         a.ends = (AttnEnd*)(a.part_ml + p.parts * 2);

@@ -502,7 +502,9 @@ hipError_t launch_kv_append(const KvAppendArgs& p, int head_dim, bool bf16, hipS
 // (unnormalised output, maximum of the scores times log2 e, sum of terms; fp32)
 // in part_o (head_dim values a state) and part_ml (two): few rows at
 // ((i * n_seq * n_kv + sequence's head) * col_blocks + column block) * cols +
-// column, many rows at (i * n_rows + row) * n_heads + head.
+// column, many rows at (i * rows + row) * n_heads + head, where the rows are the
+// batch's, or, where n_rows is a looser bound than that, max_q of each sequence
+// (part_seq: max_q, else 0).
 //
 // Few rows, blocks > 0: that many workgroups share all tiles evenly (at least
 // ATTN_SHARE_MIN each; at most ATTN_DEAL_SEQS sequences) instead; the states of
@@ -531,6 +533,7 @@ struct PagedAttnArgs {
     int window, sinks;
     int cols, col_blocks;  // columns of a workgroup; blocks of them of a sequence's key-value head
     int chunk, splits, blocks;
+    int part_rows, part_seq;
     float *part_o, *part_ml;
     AttnEnd* ends;
 };
