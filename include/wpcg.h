@@ -608,7 +608,7 @@ typedef struct wpcg_attention_s {
     int32_t dtype;
     uint32_t n_heads;
     uint64_t q_stride, out_stride;
-    float scale;             /* > 0 */
+    float scale;             /* > 0, at most 2^127: finite times log2 e */
     uint32_t window, sinks;  /* 0: no window */
 } wpcg_attention;
 int wpcg_paged_attention_workspace(const wpcg_kv_pages* kv, const wpcg_kv_batch* batch,

@@ -251,3 +251,11 @@ def test_workspace_under_loose_bounds():
         d, window = int(rng.choice([64, 128])), window * int(rng.integers(2))
         n = of(n_seq, n_rows, max_q, max_kv, hkv * group, hkv, q, c, d, window)
         assert n <= 2048 * 128 * (d + 2) * 4, (n_seq, n_rows, max_q, max_kv, hkv, group, q, c, d, window, n)
+
+
+@pytest.mark.parametrize("scale,taken", [(2.0 ** 127, True), (2.3e38, True), (2.4e38, False), (3.4028235e38, False),
+                                         (1e-45, True)])
+def test_scales_at_the_ends_of_fp32(scale, taken):
+    """The kernels multiply by scale * log2 e in fp32."""
+    rc = attend(pages(), batch(), attention(scale=scale))
+    refused(rc, E_ARG, "null context" if taken else "scale")

@@ -251,6 +251,8 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
     return WPCG_OK;
 }
 
+// The scores' factor in base 2.
+float scale_log2(const wpcg_attention* a) { return (float)((double)a->scale * 1.4426950408889634); }
 
 int check_attention(const wpcg_kv_pages* kv, const wpcg_attention* a)
 {
@@ -260,7 +262,7 @@ int check_attention(const wpcg_kv_pages* kv, const wpcg_attention* a)
         return fail(WPCG_E_UNSUPPORTED, "BF16 queries take a BF16 or E4M3 cache");
     if (a->n_heads == 0 || a->n_heads > 65536 || a->n_heads % kv->n_kv_heads)
         return fail(WPCG_E_SHAPE, "n_heads is a multiple of n_kv_heads");
-    if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return fail(WPCG_E_ARG, "scale is positive");
+    if (!(a->scale > 0.0f) || !std::isfinite(scale_log2(a))) return fail(WPCG_E_ARG, "scale is positive, and finite times log2 e");
     return WPCG_OK;
 }
 
@@ -401,7 +403,7 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
     a.n_heads = (int)att->n_heads;
     a.n_kv = (int)kv->n_kv_heads;
     a.group = a.n_heads / a.n_kv;
-    a.scale = (float)((double)att->scale * 1.4426950408889634);
+    a.scale = scale_log2(att);
     a.window = (int)std::min<uint64_t>(att->window, INT_BOUND);
     a.sinks = (int)std::min<uint64_t>(att->sinks, INT_BOUND);
     const hipStream_t s = pick(ctx, stream);
