@@ -501,3 +501,91 @@ def test_rows_far_below_their_bound(ctx, q_dtype, dtype, rows, lens, max_q, n_ro
     check(got[:n], *expected(pg, q[:n], rows, heads, q_dtype, 0.09, 0, 0))
     fill = R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]
     assert (got[n:] == fill).all()
+
+
+def expected_rows(pg, q, rows, picked, q_dtype, scale, window, sinks):
+    """As `expected`, for the picked rows of every sequence alone."""
+    outs, bounds, at = [], [], 0
+    for s, n in enumerate(rows):
+        m, i = pg.kv_len[s], picked[s]
+        o, mag, reach = R.attention(R.decode(q[at + i], q_dtype), pg.real["k"][s], pg.real["v"][s], m - n + i, scale,
+                                    window, sinks)
+        outs.append(o)
+        bounds.append(R.attention_bound(o, mag, reach, pg.d, m, q_dtype))
+        at += n
+    return np.concatenate(outs), np.concatenate(bounds)
+
+
+# Prompts of 256 columns a workgroup, a workgroup for every column block: whole
+# (128 tiles, two look-ups of pages) and in parts that are joined, with and
+# without a window. parts: of each (row, query head).
+WIDE = [(64, [2050], [16384], 0, 0, 3), (128, [2050], [16384], 0, 0, 3), (64, [2050], [8192], 0, 0, 0),
+        (128, [1100, 1000], [12000, 4000], 5000, 70, 3), (128, [1000, 3, 900], [12000, 12000, 7001], 5000, 70, 2)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("d,rows,lens,window,sinks,parts", WIDE)
+def test_prompts_far_behind_in_a_sequence(ctx, dtype, d, rows, lens, window, sinks, parts):
+    """Some rows of every sequence against 64 bits; the same call gives the same
+    bits; a page that is none reaches the rows that see it and no other sequence."""
+    print(f"[gpu] far prompts: {dtype} {d} rows {rows} lens {lens} window {window}", flush=True)
+    rng = np.random.default_rng(d + sum(rows) + window + dtype)
+    heads, hkv = 32, 8
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 16, lens, scales=dtype == E4M3).upload()
+    n = sum(rows)
+    q = R.encode(rng.standard_normal((n, heads, d)) * 1.5, BF16)
+    b = pg.batch(rows)
+    got, op = run(ctx, pg, b, q, heads, BF16, 0.1, window, sinks)
+    # 256 columns: with 128 the parts would be others
+    assert op.workspace_bytes == parts * n * heads * (d + 2) * 4
+    at = np.cumsum([0] + rows)
+    picked = [np.unique([0, r - 1, *rng.integers(0, r, 8 // len(rows))]) for r in rows]
+    want, bound = expected_rows(pg, q, rows, picked, BF16, 0.1, window, sinks)
+    check(np.concatenate([got[a + i] for a, i in zip(at, picked)]), want, bound)
+    again, _ = run(ctx, pg, b, q, heads, BF16, 0.1, window, sinks)
+    assert np.array_equal(got.view(np.uint64), again.view(np.uint64))
+    t = lens[0] - rows[0] // 2  # a token of the first sequence's later rows
+    pg.table[0, t // 16] = pg.n_pages + 9
+    pg.d_table.write(pg.table)
+    bad, _ = run(ctx, pg, b, q, heads, BF16, 0.1, window, sinks)
+    first = t // 16 * 16 - (lens[0] - rows[0])  # the first row that sees the page
+    assert np.isnan(bad[first + 16:at[1]]).all()
+    assert np.array_equal(bad[at[1]:].view(np.uint64), got[at[1]:].view(np.uint64))
+    whole = first // 64 * 64  # (column blocks of 64 rows)
+    assert np.array_equal(bad[:whole].view(np.uint64), got[:whole].view(np.uint64))
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("rows,heads", [(2, 8), (5, 16)])
+def test_tiles_dealt_out_behind_a_window(ctx, q_dtype, dtype, rows, heads):
+    """Tiles dealt out by lists that leave a gap between sinks and window: the
+    lists are those of a sequence's rows together, sequences longer and shorter
+    than the window, sinks that meet it; ids of pages in the gap are anything."""
+    window, sinks = (12000, 6000)[dtype != E4M3], 300
+    print(f"[gpu] dealt, window: {q_dtype}/{dtype} rows {rows} heads {heads}", flush=True)
+    rng = np.random.default_rng(rows + q_dtype + 10 * dtype)
+    n, hkv, d = 130, 4, 128
+    lens = [int(x) + rows for x in rng.integers(0, 40, n)]
+    lens[3], lens[70], lens[71], lens[100], lens[129] = 2 * window + 77, window + 1, 0, window + 310, window - 5
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 16, lens, scales=dtype == E4M3, width=2500)
+    gap = (lens[3] - window) // 32  # a page in the gap's middle
+    pg.upload()
+    nr = [rows] * n
+    nr[50], nr[100] = 0, 1
+    q = R.encode(rng.standard_normal((sum(nr), heads, d)) * 1.5, q_dtype)
+    b = pg.batch(nr, max_kv=40000, max_q=rows)
+    keep = pg.table[3, gap]
+    pg.table[3, gap] = -3
+    pg.d_table.write(pg.table)
+    pg.table[3, gap] = keep
+    got, op = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, sinks)
+    cols = 32 if rows * heads // hkv > 16 and dtype != F32 else 16
+    assert op.workspace_bytes == 512 * cols * (d + 2) * 4 + 256 * 20
+    want, bound = expected(pg, q, nr, heads, q_dtype, 0.09, window, sinks)
+    check(got, want, bound)
+    at = np.cumsum([0] + nr)
+    pg.table[3, (lens[3] - 100) // 16] = pg.n_pages
+    pg.d_table.write(pg.table)
+    bad, _ = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, sinks)
+    assert np.isnan(bad[at[3]:at[4]]).all()
+    assert np.array_equal(np.delete(bad, range(at[3], at[4]), 0), np.delete(got, range(at[3], at[4]), 0))

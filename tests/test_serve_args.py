@@ -259,3 +259,26 @@ def test_scales_at_the_ends_of_fp32(scale, taken):
     """The kernels multiply by scale * log2 e in fp32."""
     rc = attend(pages(), batch(), attention(scale=scale))
     refused(rc, E_ARG, "null context" if taken else "scale")
+
+
+def test_plans_by_their_workspace():
+    """The parts that windowed batches are split in (none of them is too short
+    for a second one), in 128 and 256 columns a workgroup; and tiles dealt out
+    over 256 workgroups, with the table of ends behind their parts."""
+    def of(n_seq, n_rows, max_q, max_kv, heads, hkv, d, q, c, window, sinks):
+        kv = pages(n_kv_heads=hkv, head_dim=d, dtype=c)
+        b = batch(n_seq=n_seq, n_rows=n_rows, max_q=max_q, max_kv=max_kv, table_stride=max_kv // 16 + 1)
+        return workspace(kv, b, attention(dtype=q, n_heads=heads, window=window, sinks=sinks))
+    for q, c in ((BF16, BF16), (BF16, E4M3), (F32, F32), (F32, BF16), (F32, E4M3)):
+        assert of(2, 4, 2, 3001, 8, 2, 128, q, c, 700, 4) == 3 * 2 * 2 * 16 * 130 * 4
+        assert of(1, 65, 65, 4000, 4, 1, 128, q, c, 900, 4) == 6 * 65 * 4 * 130 * 4
+        window = 12000 if c == E4M3 else 6000
+        assert of(130, 260, 2, 40000, 8, 4, 128, q, c, window, 300) == 2 * 256 * 16 * 130 * 4 + 256 * 20
+        wide = 32 if c != F32 else 16
+        assert of(130, 650, 5, 40000, 16, 4, 128, q, c, window, 300) == 2 * 256 * wide * 130 * 4 + 256 * 20
+    for c in (BF16, E4M3):
+        for d, rows, lens, window, sinks, parts in (
+                (64, [2050], [16384], 0, 0, 3), (128, [2050], [16384], 0, 0, 3), (64, [2050], [8192], 0, 0, 0),
+                (128, [1100, 1000], [12000, 4000], 5000, 70, 3), (128, [1000, 3, 900], [12000, 12000, 7001], 5000, 70, 2)):
+            n = sum(rows)
+            assert of(len(rows), n, max(rows), max(lens), 32, 8, d, BF16, c, window, sinks) == parts * n * 32 * (d + 2) * 4
