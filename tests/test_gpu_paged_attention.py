@@ -589,3 +589,52 @@ def test_tiles_dealt_out_behind_a_window(ctx, q_dtype, dtype, rows, heads):
     bad, _ = run(ctx, pg, b, q, heads, q_dtype, 0.09, window, sinks)
     assert np.isnan(bad[at[3]:at[4]]).all()
     assert np.array_equal(np.delete(bad, range(at[3], at[4]), 0), np.delete(got, range(at[3], at[4]), 0))
+
+
+# Bounds of one batch for each way that a call's work is laid out: n_seq, n_rows,
+# max_q, max_kv, heads, hkv, d, q_dtype, dtype, window, sinks.
+LAYOUTS = [
+    (1, 5, 8, 1317, 2, 1, 64, F32, E4M3, 0, 0), (2, 24, 6, 1569, 4, 1, 64, F32, BF16, 0, 4),    # 16 and 32 columns in parts
+    (4, 24, 3, 40000, 64, 8, 64, F32, BF16, 0, 4),                                              # dealt out, 32 columns
+    (3, 54, 9, 531, 8, 1, 64, BF16, E4M3, 0, 0), (1, 12, 6, 585, 8, 1, 64, F32, BF16, 0, 0),    # parts under a loose n_rows
+    (5, 49, 98, 669, 7, 1, 64, F32, E4M3, 0, 0), (6, 8, 9, 783, 128, 2, 64, BF16, BF16, 0, 4),  # blocks looked for, in parts
+    (34, 68, 1, 8724, 512, 8, 64, BF16, E4M3, 0, 4), (59, 60, 35, 8139, 5, 5, 64, BF16, BF16, 0, 4),  # 256 columns in parts
+    (76, 81, 121, 7439, 28, 4, 64, BF16, E4M3, 0, 0), (76, 81, 121, 7439, 28, 4, 64, BF16, BF16, 6000, 100),  # ... looked for
+    (64, 71, 58, 3544, 8, 8, 64, BF16, E4M3, 0, 4),                                             # 256 columns, a grid, whole
+    (7, 8, 90, 9851, 28, 4, 128, F32, F32, 0, 0), (52, 86, 6, 7451, 14, 2, 64, F32, E4M3, 0, 4),  # from here on, few rows and
+    (95, 98, 5, 1834, 14, 2, 128, F32, BF16, 0, 4), (7, 30, 27, 20000, 32, 4, 64, BF16, BF16, 0, 4),  # many in two parts
+    (46, 80, 115, 3658, 8, 4, 128, BF16, BF16, 0, 4), (67, 70, 46, 1083, 8, 2, 128, F32, F32, 0, 0),
+    (9, 1611, 5695, 5695, 28, 4, 64, BF16, E4M3, 0, 4), (64, 70, 8, 4153, 100, 5, 64, F32, E4M3, 0, 0),
+    (87, 271, 7, 8682, 80, 4, 128, BF16, BF16, 0, 0), (89, 850, 65, 6249, 16, 4, 128, BF16, E4M3, 0, 4),
+    (86, 162, 21, 6564, 56, 8, 64, BF16, E4M3, 0, 0), (86, 162, 21, 6564, 56, 8, 64, BF16, BF16, 5000, 90),
+    (416, 418, 17, 5317, 40, 5, 64, BF16, BF16, 0, 0)]
+
+
+@pytest.mark.parametrize("n_seq,n_rows,max_q,max_kv,heads,hkv,d,q_dtype,dtype,window,sinks", LAYOUTS)
+def test_layouts(ctx, n_seq, n_rows, max_q, max_kv, heads, hkv, d, q_dtype, dtype, window, sinks):
+    """Ragged batches within the bounds, of which every way to lay a call out
+    over the chip is chosen for one: one sequence of the bound's length, the
+    others of any, some empty, some without rows, rows of no sequence."""
+    print(f"[gpu] layout: {n_seq} {n_rows} {max_q} {max_kv} {heads}/{hkv}x{d} {q_dtype}/{dtype}", flush=True)
+    rng = np.random.default_rng(n_seq + n_rows + heads + d + q_dtype + 10 * dtype + window)
+    left, rows = n_rows, []
+    for s in range(n_seq):  # a few long row ranges, the others short
+        most = min(max_q, max(0, left - (n_seq - s) // 2))
+        rows.append(int(rng.integers(1, max(1, most) + 1) if rng.random() < max(0.25, 5 / n_seq) else rng.integers(0, 2)))
+        rows[-1] = min(most, rows[-1])
+        left -= rows[-1]
+    # lengths: few long ones, for the references' sake, the rows at their ends
+    lens = [min(max_kv, r + int(max_kv ** rng.random()) - 1) if rng.random() < 0.9 else 0 for r in rows]
+    lens[int(np.argmax(rows))] = max_kv
+    pg = R.Paged(ctx, rng, dtype, hkv, d, 16, lens, scales=dtype == E4M3).upload()
+    n = sum(rows)
+    q = np.zeros((n_rows, heads, d), R.BITS[q_dtype])
+    q[:n] = R.encode(rng.standard_normal((n, heads, d)) * 1.5, q_dtype)
+    got, _ = run(ctx, pg, pg.batch(rows, n_rows=n_rows, max_kv=max_kv, max_q=max_q), q, heads, q_dtype, 0.1, window, sinks)
+    # the rows of the longest sequence by samples
+    picked = [np.arange(r) if r * m < 20000 else np.unique([0, r - 1, *rng.integers(0, r, 6)]) for r, m in zip(rows, lens)]
+    at = np.cumsum([0] + rows)
+    want, bound = expected_rows(pg, q[:n], rows, picked, q_dtype, 0.1, window, sinks)
+    check(np.concatenate([got[a + i] for a, i in zip(at, picked)]), want, bound)
+    fill = R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]
+    assert (got[n:] == fill).all()
