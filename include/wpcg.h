@@ -591,7 +591,9 @@ int wpcg_kv_append(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* 
  * q and out are rows of dtype F32 or BF16 (0 strides = packed). An F32 q keeps
  * fp32 accuracy whatever the cache holds; a BF16 q goes with a BF16 or E4M3
  * cache (an F32 cache is E_UNSUPPORTED) and rounds the softmax's terms to
- * bf16 before they meet V. Sums and softmax statistics are fp32. One pass over
+ * bf16 before they meet V. Sums and softmax statistics are fp32, and so is the sum
+ * of terms (up to 2^8) times values that is divided at the end: values of 2^128
+ * over 2^8 times the tokens may overflow it. One pass over
  * the pages with a running maximum; long sequences are split over workgroups
  * and joined by a second launch. Whether and into how many parts a batch is
  * split depends on its bounds (n_seq, n_rows, max_q, max_kv); batches that may
@@ -631,10 +633,11 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  *   weight at all: from p_r).
  * A temperature not above 0 (null: all 1) is greedy: a draft is accepted while
  * it is the first largest logit, which also is the next token; at +inf all ids
- * with a logit above -inf are alike. accepted[s]
- * receives the number of accepted drafts, out the rows' tokens: the accepted
- * drafts, the next token, then -1. Probabilities, running sums and comparisons
- * are fp64; u and u_next are in [0, 1). A row without any weight (NaN, +inf, or
+ * with a logit above -inf are alike. accepted[s] receives the number of accepted
+ * drafts, out the rows' tokens: the accepted drafts, the next token, then -1.
+ * Probabilities, running sums and comparisons are fp64, from exponentials that
+ * are right to 1.1e-12 of their value (0 below 2^-1000); an id without weight is
+ * never drawn. u and u_next are in [0, 1). A row without any weight (NaN, +inf, or
  * no logit above -inf; greedy rows pass NaN over) accepts nothing and gives
  * next token -1; where the drafter's row leaves no weight or NaN, p_r is taken;
  * a draft id outside the vocabulary is rejected; a sequence whose row range is

@@ -29,11 +29,11 @@
 // With F32 queries, q and the terms are carried as three bf16 each, exactly,
 // over a BF16 or E4M3 cache, and an F32 cache takes the fp32 matrix cores.
 //
-// Measured, heads of 128: 64 sequences of up to 4096 tokens, 32 / 4 heads, BF16
-// (310 MB) 68.7 us, 4.5 TB/s; one of 131072 tokens, 32 / 8 heads, F32 queries
-// over E4M3 (268 MB) 52.5 us, 5.1 TB/s, and 5.7 to join its chunks; 32 with a
-// window of 1024 (136 MB) 28.6 us; 16 of up to 6000 with five rows (227 MB) 59
-// and 5 us. A 1 GiB copy reaches 5.1 TB/s. One sequence of 300 tokens 10.4 us.
+// Measured, heads of 128, on one card: 64 sequences of up to 4096 tokens, 32 / 4
+// heads, BF16 (310 MB) 67.4 us, 4.6 TB/s; one of 131072 tokens, 32 / 8 heads, F32
+// queries over E4M3 (268 MB) 51 us, 5.2 TB/s, and 5.7 to join its chunks; 32 with a
+// window of 1024 (136 MB) 28.3 us; 16 of up to 6000 with five rows (227 MB) 57 and 5
+// us. A 1 GiB copy reaches 5.1 TB/s. One sequence of 300 tokens 10.4 us.
 #include "paged.h"
 
 namespace wpcg {

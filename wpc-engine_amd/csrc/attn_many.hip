@@ -25,13 +25,13 @@
 // terms too, and a product of two fp32 values takes the six of its nine terms
 // that reach 2^-24.
 //
-// Measured, heads of 128: a prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 146
-// us, 940 TFLOP/s, with the matrix cores busy in 40 % of the cycles and the
-// vector units in 42 %; the last 2048 rows of 32768 tokens 1050 TFLOP/s (a
-// library's 8192^3 product 1300); two prompts of up to 5000 with a window of
-// 1024, 32 / 4 heads over E4M3 (144 GFLOP) 226 us; 777 rows behind 523 tokens,
-// 32 / 4 heads, all F32 (11.6 GFLOP, six products each) 124 us with the join's
-// 11.
+// Measured, heads of 128, on one card (another one's prompts took 10 % more): a
+// prompt of 4096, 32 / 8 heads, BF16 (137 GFLOP) 142 us, 967 TFLOP/s, with the
+// matrix cores busy in 41 % of the cycles and the vector units in 42 %; two
+// prompts of up to 5000 with a window of 1024, 32 / 4 heads over E4M3 (144 GFLOP)
+// 222 us; 777 rows behind 523 tokens, 32 / 4 heads, all F32 (11.6 GFLOP, six
+// products each) 124 us with the join's 11. The last 2048 rows of 32768 tokens,
+// BF16, 1090 TFLOP/s (a library's 8192^3 product 1300).
 #include "paged.h"
 
 namespace wpcg {
@@ -684,8 +684,8 @@ __global__ __launch_bounds__(256, QF32 ? 1 : 2) void k_attn_many(PagedAttnArgs p
 // Prompts of BF16 queries with blocks enough: one workgroup of eight waves a CU,
 // which brings in each tile once for 256 columns, four waves its values and four
 // its keys. With half the registers for tiles on their way, operands are read
-// two groups ahead (a prompt of 4096 159 -> 154 us, a window of 1024 in BF16 256
-// -> 237 against two workgroups of four waves).
+// two groups ahead. plan_kernel has its times beside those of two workgroups of
+// four waves.
 template <int D, int CT>
 __global__ __launch_bounds__(512, 2) void k_attn_wide(PagedAttnArgs p)
 {

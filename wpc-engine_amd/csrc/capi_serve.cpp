@@ -131,12 +131,18 @@ int plan_kernel(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attenti
         return std::min(all, seen);
     };
     if (p.many) {
-        // 256 columns a workgroup where that leaves every CU one and the tiles
-        // are some, more over E4M3, where the narrower form's registers suffice:
-        // two prompts of up to 5000 with a window of 1024 (18 tiles a block),
-        // 32 / 4 heads, BF16 256 us with 128 columns and 237 so, E4M3 225 and 231;
-        // a prompt of 4096, 32 / 8 heads, BF16 158 and 147; eight of up to 1000
-        // 115 and 107. Below, a CU's one workgroup starts and ends alone.
+        // 256 columns a workgroup where that leaves every CU one and a block has
+        // tiles enough; over E4M3 more of them, where the narrower form's registers
+        // suffice. With 128 and 256 columns, us, one card, one run: two prompts of up
+        // to 5000, 32 / 4 heads, by the window:
+        //   window        256      512      1024     1500     2048     4000
+        //   tiles           7       11        19       26       35       66
+        //   BF16        132 125  170 159   249 231  309 294  381 359  553 512
+        //   E4M3        115 122  150 155   227 226  287 288  355 351  522 500
+        // 32 / 8 heads without one: a prompt of 4096 (64 tiles) BF16 167 and 156, E4M3
+        // 161 and 153; eight of up to 1000 (16 tiles) 111 and 105, 99 and 103; the
+        // last 2048 rows of 32768 tokens 1121 and 976, 1018 and 948. (BF16 with many
+        // blocks gains below its 16 tiles too.)
         const int64_t wide = 2 * ATTN_MANY_COLS, some = kv->dtype == WPCG_DTYPE_E4M3 ? 32 : 16;
         p.cols = a->dtype == WPCG_DTYPE_BF16 && tiles_of(wide) >= some && kv->n_kv_heads * all_blocks(wide) >= CUS
                      ? wide : ATTN_MANY_COLS;
@@ -204,7 +210,7 @@ int plan_kernel(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_attenti
     // instead. (63 sequences of 500 tokens and one of 100000, 32 / 4 heads: 1028
     // us with a workgroup a sequence and head, 79 so. It costs a few us more
     // where the lengths are less unlike: 64 sequences of 512 to 4096 tokens 67
-    // and 75 us.)
+    // and 75 us. The border between these was not looked for more closely.)
     if (!p.many && p.us > 130.0 && b.n_seq <= ATTN_DEAL_SEQS && base * tiles < (int64_t)1 << 30) {
         p.blocks = CUS;
         p.parts = 2 * CUS * p.cols;

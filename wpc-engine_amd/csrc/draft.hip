@@ -20,10 +20,11 @@
 // good as its target leaves differences p - q far below p, and the running
 // sums of 10^5 weights decide which id they pass at.
 //
-// Measured at 151936 ids: 64 sequences with their drafts (260 MB) 72 us, the
-// first launch 44 (5.2 TB/s) and the second 23; one sequence with four drafts
-// 14.7 us, 4.0 and 10.7 of them. (With LDS atomics in place of the ballots that
-// find the drawn id 19.7 us: 75 threads at one word took 2 to 3 us each time.)
+// Measured at 151936 ids, on four cards: 64 sequences with their drafts (260 MB)
+// 63 to 72 us, the first launch 44 (5.2 TB/s) and the second 23; one sequence
+// with four drafts 12.3 to 14.7 us, 4.1 and 10.4 of them. (With LDS atomics in
+// place of the ballots that find the drawn id 5 us more: 75 threads at one word
+// took 2 to 3 us each time.)
 #include "paged.h"
 #include "wave.h"
 
