@@ -591,15 +591,15 @@ int wpcg_kv_append(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* 
  * q and out are rows of dtype F32 or BF16 (0 strides = packed). An F32 q keeps
  * fp32 accuracy whatever the cache holds; a BF16 q goes with a BF16 or E4M3
  * cache (an F32 cache is E_UNSUPPORTED) and rounds the softmax's terms to
- * bf16 before they meet V. Sums and softmax statistics are fp32, and so is the sum
- * of terms (up to 2^8) times values that is divided at the end: values of 2^128
- * over 2^8 times the tokens may overflow it. One pass over
- * the pages with a running maximum; long sequences are split over workgroups
- * and joined by a second launch. Whether and into how many parts a batch is
- * split depends on its bounds (n_seq, n_rows, max_q, max_kv); batches that may
- * hold a few very long sequences among short ones deal their tiles out by the
- * lengths, so that there a sequence's last bits may depend on the others'
- * lengths. The same call on the same arrays gives the same bits.
+ * bf16 before they meet V. Sums and softmax statistics are fp32; the sum of terms
+ * (up to 2^8) times values is divided at the end, so that values above 2^120 over
+ * the number of tokens may overflow it. One pass over the pages with a running
+ * maximum; long sequences are split over workgroups and joined by a second launch.
+ * Whether and into how many parts a batch is split depends on its bounds (n_seq,
+ * n_rows, max_q, max_kv); batches that may hold a few very long sequences among
+ * short ones deal their tiles out by the lengths, so that there a sequence's last
+ * bits may depend on the others' lengths. The same call on the same arrays gives
+ * the same bits. A call whose bounds need 2^23 workgroups or more is E_UNSUPPORTED.
  * ws_dev: device memory of at least wpcg_paged_attention_workspace bytes
  * (16-byte aligned; may be null if that is 0), whose contents are nothing
  * before or after the call. Calls that may overlap need one each, also as

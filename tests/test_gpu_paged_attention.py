@@ -638,3 +638,20 @@ def test_layouts(ctx, n_seq, n_rows, max_q, max_kv, heads, hkv, d, q_dtype, dtyp
     check(np.concatenate([got[a + i] for a, i in zip(at, picked)]), want, bound)
     fill = R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]
     assert (got[n:] == fill).all()
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+def test_one_row_each_of_a_wide_group_in_parts(ctx, q_dtype, dtype):
+    """Groups of 40 query heads (the kernel for many rows), no row starts, more
+    rows than sequences: the parts are one row's of each sequence."""
+    print(f"[gpu] wide group, loose rows: {q_dtype}/{dtype}", flush=True)
+    rng = np.random.default_rng(q_dtype + 10 * dtype)
+    lens = [3000, 1, 700, 0, 64]
+    pg = R.Paged(ctx, rng, dtype, 2, 64, 16, lens, scales=dtype == E4M3).upload()
+    q = R.encode(rng.standard_normal((9, 80, 64)) * 1.5, q_dtype)
+    got, op = run(ctx, pg, pg.batch(None, n_rows=9), q, 80, q_dtype, 0.12)
+    part = 5 * 80 * 66 * 4
+    assert op.workspace_bytes >= 2 * part and op.workspace_bytes % part == 0
+    check(got[:5], *expected(pg, q[:5], [1] * 5, 80, q_dtype, 0.12, 0, 0))
+    fill = R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]
+    assert (got[5:] == fill).all()
