@@ -662,6 +662,44 @@ typedef struct wpcg_draft_s {
 int wpcg_draft_verify_workspace(const wpcg_draft* d, uint64_t* bytes);
 int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream);
 
+/* Log probabilities of given tokens, with what ranks and explains them, from rows
+ * of logits x (dtype F32 or BF16; row r at r * logits_stride elements, 0 =
+ * vocab): with p = softmax(x / temperature[r]) (null: 1)
+ *   logprob[r] = ln p(tokens[r])
+ *   rank[r]    = 1 + the ids that come before tokens[r]: those of a larger
+ *                logit, and of the same logit and a lower id
+ *   entropy[r] = -sum p ln p, in nats
+ *   top_ids[r], top_logprob[r] (top entries each): the first ids in that order
+ *                and their ln p
+ * Any output may be null; without logprob and rank tokens may be, too. Sums are
+ * fp32 over 32 ids and a wave, from exponentials right to 2^-22, and fp64 from
+ * there on; a token that is nearly certain keeps its log probability's digits. A
+ * temperature not above 0 is greedy: ln p is 0 for the first largest logit and
+ * -inf for the others, the entropy 0; at +inf all ids with a logit above -inf are
+ * alike. A token outside the vocabulary has log probability -inf and rank 0. An id
+ * whose logit is -inf or NaN is never listed: where fewer are left the last
+ * entries are id -1 and -inf. A row without a distribution (NaN or +inf in it, or
+ * no logit above -inf; greedy rows pass NaN over and take +inf as a value) has NaN
+ * in every probability and in the entropy; its ranks and ids are as said, the
+ * rank of a NaN logit 0. vocab <= 2^30, top <= WPCG_LOGPROB_TOP. Workspace and
+ * streams as for wpcg_paged_attention; no order in time changes a bit. */
+#define WPCG_LOGPROB_TOP 64
+typedef struct wpcg_logprob_s {
+    uint32_t n_rows, vocab, top;
+    int32_t dtype;
+    const void* logits_dev;
+    uint64_t logits_stride;
+    const float* temperature_dev; /* n_rows, or null */
+    const int32_t* tokens_dev;    /* n_rows, or null */
+    float* logprob_dev;           /* n_rows */
+    float* entropy_dev;           /* n_rows */
+    int32_t* rank_dev;            /* n_rows */
+    int32_t* top_ids_dev;         /* [n_rows][top] */
+    float* top_logprob_dev;       /* [n_rows][top] */
+} wpcg_logprob;
+int wpcg_logprobs_workspace(const wpcg_logprob* d, uint64_t* bytes);
+int wpcg_logprobs(wpcg_ctx* ctx, const wpcg_logprob* d, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream);
+
 /* ---- HIP graphs over the context stream (no reference counterpart) ----
  * wpcg_graph_begin starts capturing the context's stream; device calls with
  * stream NULL are then recorded instead of run, until wpcg_graph_end

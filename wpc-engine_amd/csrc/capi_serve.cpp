@@ -294,6 +294,24 @@ int check_draft(const wpcg_draft* d, int* chunks, uint64_t* bytes)
     return WPCG_OK;
 }
 
+int check_logprobs(const wpcg_logprob* d, int* chunks, uint64_t* part_bytes, uint64_t* bytes)
+{
+    if (!d) return fail(WPCG_E_ARG, "null argument");
+    if (int rc = check_rows_dtype(d->dtype)) return rc;
+    if (d->vocab == 0 || d->vocab > INT_BOUND) return fail(WPCG_E_ARG, "vocab out of range");
+    if (d->n_rows > INT_BOUND) return fail(WPCG_E_ARG, "batch bounds out of range");
+    if (d->top > WPCG_LOGPROB_TOP) return fail(WPCG_E_ARG, "top is at most " + std::to_string(WPCG_LOGPROB_TOP));
+    if (d->logits_stride && d->logits_stride < d->vocab) return fail(WPCG_E_SHAPE, "row stride shorter than the row");
+    if (d->logits_stride >> 40) return fail(WPCG_E_ARG, "row stride too large");
+    *chunks = (int)((d->vocab + LOGPROB_CHUNK - 1) / LOGPROB_CHUNK);
+    if ((uint64_t)d->n_rows * ((*chunks + 3) / 4) >= (uint64_t)GROUPS_256)
+        return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
+    const uint64_t all = (uint64_t)d->n_rows * *chunks;
+    *part_bytes = (all * sizeof(LogprobPart) + 15) / 16 * 16;
+    *bytes = *part_bytes + (d->top > 0 ? all * LOGPROB_SEGS * sizeof(float) : 0);
+    return WPCG_OK;
+}
+
 }  // namespace
 }  // namespace wpcg
 
@@ -476,6 +494,47 @@ int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t
     a.done = (DraftDone*)(a.rest + (uint64_t)d->n_seq * a.chunks);
     a.vec = aligned(a.logits) && a.logits_row % 4 == 0 && aligned(a.probs) && a.probs_row % 4 == 0;
     WPCG_HIP(launch_draft_verify(a, pick(ctx, stream)));
+    return WPCG_OK;
+}
+
+int wpcg_logprobs_workspace(const wpcg_logprob* d, uint64_t* bytes)
+{
+    if (!bytes) return fail(WPCG_E_ARG, "null output");
+    *bytes = 0;
+    int chunks;
+    uint64_t part = 0;
+    return check_logprobs(d, &chunks, &part, bytes);
+}
+
+int wpcg_logprobs(wpcg_ctx* ctx, const wpcg_logprob* d, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream)
+{
+    LogprobArgs a{};
+    uint64_t part = 0, bytes = 0;
+    if (int rc = check_logprobs(d, &a.chunks, &part, &bytes)) return rc;
+    if (d->n_rows == 0) return check_ctx(ctx);
+    if (!d->logits_dev || (!d->tokens_dev && (d->logprob_dev || d->rank_dev))) return fail(WPCG_E_ARG, "null argument");
+    if ((uintptr_t)d->logits_dev % type_size(d->dtype)) return fail(WPCG_E_ARG, "logits not aligned to their type");
+    if (!ws_dev || ws_bytes < bytes)
+        return fail(WPCG_E_ARG, "the call needs " + std::to_string(bytes) + " bytes of workspace");
+    if (!aligned(ws_dev)) return fail(WPCG_E_ARG, "workspace not aligned to 16 bytes");
+    if (int rc = check_ctx(ctx)) return rc;
+    a.n_rows = (int)d->n_rows;
+    a.vocab = (int)d->vocab;
+    a.top = d->top_ids_dev || d->top_logprob_dev ? (int)d->top : 0;
+    a.bf16 = d->dtype == WPCG_DTYPE_BF16;
+    a.logits = d->logits_dev;
+    a.row = d->logits_stride ? d->logits_stride : d->vocab;
+    a.vec = aligned(a.logits) && a.row * type_size(d->dtype) % 16 == 0;
+    a.temperature = d->temperature_dev;
+    a.tokens = d->tokens_dev;
+    a.logprob = d->logprob_dev;
+    a.entropy = d->entropy_dev;
+    a.rank = d->rank_dev;
+    a.top_ids = d->top_ids_dev;
+    a.top_logprob = d->top_logprob_dev;
+    a.part = (LogprobPart*)ws_dev;
+    a.seg = (float*)((uint8_t*)ws_dev + part);
+    WPCG_HIP(launch_logprobs(a, pick(ctx, stream)));
     return WPCG_OK;
 }
 

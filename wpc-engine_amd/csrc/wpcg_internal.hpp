@@ -568,6 +568,31 @@ struct DraftArgs {
 };
 hipError_t launch_draft_verify(const DraftArgs& p, hipStream_t s);
 
+// ---- log probabilities (logprob.hip) ------------------------------------------
+// A chunk's state of a row: its largest logit, the sum of e^t and of e^t t (t in
+// base 2, relative to that) over the others, how many reach it, and how many come
+// before the row's token.
+constexpr int LOGPROB_CHUNK = 2048;  // ids
+constexpr int LOGPROB_SEGS = LOGPROB_CHUNK / 64;  // their 64-id segments
+constexpr int LOGPROB_TOP = WPCG_LOGPROB_TOP;
+struct LogprobPart {
+    float max, z, s;
+    int tops, before;
+};
+struct LogprobArgs {
+    int n_rows, vocab, top, chunks;
+    int bf16, vec;  // vec: rows start on 16 bytes
+    const void* logits;
+    uint64_t row;
+    const float* temperature;
+    const int32_t* tokens;
+    float *logprob, *entropy, *top_logprob;
+    int32_t *rank, *top_ids;
+    LogprobPart* part;  // [n_rows][chunks]
+    float* seg;         // [n_rows][chunks][LOGPROB_SEGS] maxima, with top > 0
+};
+hipError_t launch_logprobs(const LogprobArgs& p, hipStream_t s);
+
 // ---- JSON DOM (json.cpp): safetensors headers, their index, config.json ----
 struct JsonValue {
     enum Kind { NUL, BOOL, NUM, STR, ARR, OBJ } kind = NUL;

@@ -150,6 +150,8 @@ _SIGS = {
     "wpcg_paged_attention": (C.c_int, [_p, _p, _p, _p, _p, _u64, _p]),
     "wpcg_draft_verify_workspace": (C.c_int, [_p, _u64p]),
     "wpcg_draft_verify": (C.c_int, [_p, _p, _p, _u64, _p]),
+    "wpcg_logprobs_workspace": (C.c_int, [_p, _u64p]),
+    "wpcg_logprobs": (C.c_int, [_p, _p, _p, _u64, _p]),
     "wpcg_graph_begin": (C.c_int, [_p]),
     "wpcg_graph_end": (C.c_int, [_p, _pp]),
     "wpcg_graph_launch": (C.c_int, [_p, _p]),
@@ -792,6 +794,12 @@ class _Draft(C.Structure):
                 ("tokens", _p), ("u", _p), ("u_next", _p), ("temperature", _p), ("accepted", _p), ("out", _p)]
 
 
+class _Logprob(C.Structure):
+    _fields_ = [("n_rows", C.c_uint32), ("vocab", C.c_uint32), ("top", C.c_uint32), ("dtype", C.c_int32),
+                ("logits", _p), ("logits_stride", _u64), ("temperature", _p), ("tokens", _p), ("logprob", _p),
+                ("entropy", _p), ("rank", _p), ("top_ids", _p), ("top_logprob", _p)]
+
+
 def rope_frequencies(theta: float, head_dim: int) -> np.ndarray:
     """theta^(-2i/head_dim), i < head_dim/2 (apply_rope, wpc-runtime/src/rope.rs:10-40)
     as the doubles that KvAppend takes."""
@@ -894,6 +902,30 @@ class DraftVerify:
         d.logits, d.tokens, d.u, d.u_next = _ptr(logits), _ptr(tokens), _ptr(u), _ptr(u_next)
         d.accepted, d.out, d.draft_probs = _ptr(accepted), _ptr(out), _ptr(draft_probs)
         check(lib.wpcg_draft_verify(self.ctx.h, self._ref, _ptr(self.workspace), self.workspace_bytes, stream))
+
+
+class LogProbs:
+    """Log probabilities of given tokens, rank, entropy and the `top` best ids
+    of rows of logits (wpcg_logprobs), with a workspace of its own: calls of one
+    object must not overlap."""
+
+    def __init__(self, ctx: Context, n_rows: int, vocab: int, top: int = 0, dtype: int = DTYPE_F32, temperature=None,
+                 logits_stride: int = 0):
+        self.ctx = ctx
+        self._keep = temperature
+        self.desc = _Logprob(n_rows, vocab, top, dtype, None, logits_stride, _ptr(temperature))
+        self._ref = C.byref(self.desc)
+        n = C.c_uint64()
+        check(lib.wpcg_logprobs_workspace(self._ref, C.byref(n)))
+        self.workspace_bytes = n.value
+        self.workspace = ctx.alloc(n.value) if n.value else None
+
+    def run(self, logits, tokens=None, logprob=None, entropy=None, rank=None, top_ids=None, top_logprob=None,
+            stream=None):
+        d = self.desc
+        d.logits, d.tokens, d.logprob, d.entropy = _ptr(logits), _ptr(tokens), _ptr(logprob), _ptr(entropy)
+        d.rank, d.top_ids, d.top_logprob = _ptr(rank), _ptr(top_ids), _ptr(top_logprob)
+        check(lib.wpcg_logprobs(self.ctx.h, self._ref, _ptr(self.workspace), self.workspace_bytes, stream))
 
 
 # ------------------------------------------------------------------ encoder
