@@ -662,6 +662,72 @@ typedef struct wpcg_draft_s {
 int wpcg_draft_verify_workspace(const wpcg_draft* d, uint64_t* bytes);
 int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream);
 
+/* Pages that sequences share: several answers to one prompt, beams, rejected
+ * drafts taken back, all on the device, so that a captured graph of these calls
+ * follows their arrays. A pool is the state of n_pages pages, the same in every
+ * layer: refs[p] counts the table entries that name page p (the host may add its
+ * own to hold a page; 0: free), row s of the table holds the pages of sequence s,
+ * whose first kv_len[s] tokens they store: ceil(kv_len / page_size) entries, -1
+ * where there is none (a window's old page); what lies behind them is nothing. A
+ * new pool is all zeros (and a table of anything).
+ *
+ * wpcg_kv_fork gives every sequence a new row: the first keep[s] tokens of the
+ * sequence parent[s] as it was before the call, and room for grow[s] more. parent
+ * null: itself; not in 0..n_seq-1: none, the sequence is freed (and may be begun
+ * anew by grow). keep null: all; at most what the parent has. grow null: `grow`
+ * for all; cut to what the table's row holds; kv_len[s] becomes keep + grow, the
+ * length that the append and the attention of the new tokens take. Whole pages
+ * are shared. The page that a row writes next, where it is begun (keep no
+ * multiple of page_size, and grow > 0), has to be its own: of the rows that would
+ * write into it the lowest keeps it if nothing else holds it, each other one gets
+ * a fresh page and an entry of copies, {page, fresh page, keep % page_size}, in
+ * the order of sequences. Fresh pages are the lowest free ones, pages that the
+ * call itself frees among them, in the order of sequences and places. With
+ * window > 0 pages that no row at position keep or later sees (as wpcg_attention
+ * has it, with sinks) are given back, and their entries are -1; a later keep
+ * must not reach back behind them. Entries that a row no longer has become -1.
+ * result: {free pages left, number of copies}; where pages are missing
+ * {-missing, 0}, and nothing else has changed. copies: [n_seq][3].
+ *
+ * wpcg_kv_compact moves pages to the front: the i-th page in use from above to
+ * the i-th free one from below, while that is lower and for at most max_copies;
+ * entries, counts and copies (page, new page, page_size) say so. result: {the
+ * last page in use + 1, number of moves}. A host that holds pages itself finds
+ * in copies where they went.
+ *
+ * wpcg_kv_copy then copies the listed pages' tokens, keys and values, in n_layers
+ * layers that differ in k_dev and v_dev alone: copies[i] = {from, to, tokens} for
+ * i < min(*n_copies, max_copies) (n_copies: result + 1). Ids outside the pages are
+ * passed over. A page that is copied to twice, or copied both from and to, holds
+ * one or the other; the lists above have none.
+ *
+ * refs, table and kv_len may hold anything; ids outside the pages are none, a
+ * length is cut to the row. Limits: n_pages <= 2^26, n_seq * table_stride <=
+ * 2^30, page_size as for wpcg_kv_pages. Workspace and streams as for
+ * wpcg_paged_attention. */
+typedef struct wpcg_kv_pool_s {
+    uint32_t n_pages, page_size, n_seq, table_stride;
+    int32_t* refs_dev;   /* n_pages */
+    int32_t* table_dev;  /* [n_seq][table_stride] */
+    int32_t* kv_len_dev; /* n_seq */
+} wpcg_kv_pool;
+typedef struct wpcg_kv_change_s {
+    const int32_t* parent_dev; /* n_seq each, or null */
+    const int32_t* keep_dev;
+    const int32_t* grow_dev;
+    uint32_t grow, window, sinks;
+    int32_t* copies_dev; /* [n_seq][3] */
+    int32_t* result_dev; /* 2 */
+} wpcg_kv_change;
+int wpcg_kv_fork_workspace(const wpcg_kv_pool* pool, uint64_t* bytes);
+int wpcg_kv_fork(wpcg_ctx* ctx, const wpcg_kv_pool* pool, const wpcg_kv_change* change, void* ws_dev,
+                 uint64_t ws_bytes, wpcg_stream stream);
+int wpcg_kv_compact_workspace(const wpcg_kv_pool* pool, uint64_t* bytes);
+int wpcg_kv_compact(wpcg_ctx* ctx, const wpcg_kv_pool* pool, uint32_t max_copies, int32_t* copies_dev,
+                    int32_t* result_dev, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream);
+int wpcg_kv_copy(wpcg_ctx* ctx, const wpcg_kv_pages* layers, uint32_t n_layers, const int32_t* copies_dev,
+                 const int32_t* n_copies_dev, uint32_t max_copies, wpcg_stream stream);
+
 /* Log probabilities of given tokens, with what ranks and explains them, from rows
  * of logits x (dtype F32 or BF16; row r at r * logits_stride elements, 0 =
  * vocab): with p = softmax(x / temperature[r]) (null: 1)

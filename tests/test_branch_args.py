@@ -63,3 +63,100 @@ def test_score_workspace():
     assert SCORE_WS(ref(scores(top=0)), C.byref(n)) == OK and n.value == 112
     assert SCORE_WS(ref(scores(top=65)), C.byref(n)) == E_ARG and n.value == 0
     assert SCORE_WS(ref(scores()), None) == E_ARG and SCORE_WS(None, C.byref(n)) == E_ARG
+
+
+# ---- pages ---------------------------------------------------------------------
+FORK, FORK_WS, COMPACT, COMPACT_WS, COPY = (getattr(wpcg.lib, "wpcg_kv_" + n) for n in (
+    "fork", "fork_workspace", "compact", "compact_workspace", "copy"))
+
+
+def pool(**kw):
+    a = dict(n_pages=100, page_size=16, n_seq=4, table_stride=20, refs=AT, table=AT, kv_len=AT)
+    a.update(kw)
+    return wpcg._KvPool(**a)
+
+
+def change(**kw):
+    a = dict(parent=AT, keep=AT, grow_each=AT, copies=AT, result=AT)
+    a.update(kw)
+    return wpcg._KvChange(**a)
+
+
+def pages(**kw):
+    a = dict(k=AT, v=AT, dtype=BF16, n_pages=10, page_size=16, n_kv_heads=2, head_dim=128)
+    a.update(kw)
+    return wpcg._KvPages(**a)
+
+
+def fork(p, c, ws=AT, n=1 << 40):
+    return FORK(None, ref(p), ref(c), ws, n, None)
+
+
+def compact(p, most=5, copies=AT, result=AT, ws=AT, n=1 << 40):
+    return COMPACT(None, ref(p), most, copies, result, ws, n, None)
+
+
+def copy(layers, copies=AT, n=AT, most=5):
+    return COPY(None, (wpcg._KvPages * len(layers))(*layers), len(layers), copies, n, most, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(page_size=8), E_SHAPE, "page_size"), (dict(page_size=48), E_SHAPE, "page_size"), (dict(n_pages=0), E_ARG, "n_pages"),
+    (dict(n_pages=(1 << 26) + 1), E_ARG, "n_pages"), (dict(table_stride=0), E_ARG, "table"),
+    (dict(n_seq=1 << 16, table_stride=1 << 15), E_ARG, "table"), (dict(table_stride=1 << 27), E_ARG, "table"),
+    (dict(n_seq=(1 << 30) + 1), E_ARG, "table"), (dict(n_seq=1 << 22, table_stride=1), E_UNSUPPORTED, "workgroups"),
+    (dict(refs=None), E_ARG, "null"), (dict(table=None), E_ARG, "null"), (dict(kv_len=None), E_ARG, "null"),
+])
+def test_pools(kw, code, text):
+    refused(fork(pool(**kw), change()), code, text)
+    refused(compact(pool(**kw)), code, text)
+
+
+def test_changes():
+    refused(fork(None, change()), E_ARG, "null")
+    refused(fork(pool(), None), E_ARG, "null")
+    for kw in (dict(copies=None), dict(result=None)):
+        refused(fork(pool(), change(**kw)), E_ARG, "null")
+        refused(compact(pool(), **kw), E_ARG, "null")
+    for p, c in ((pool(), change()), (pool(), change(parent=None, keep=None, grow_each=None, grow=1 << 31, window=1 << 31)),
+                 (pool(n_seq=0, table=None, kv_len=None), change(copies=None)), (pool(n_pages=1 << 26), change())):
+        refused(fork(p, c), E_ARG, "null context")
+    refused(compact(pool(), most=0, copies=None), E_ARG, "null context")
+    refused(compact(pool(n_seq=0, table=None, kv_len=None)), E_ARG, "null context")
+
+
+@pytest.mark.parametrize("query,call,words", [(FORK_WS, lambda *a: fork(pool(), change(), *a), 2 * 100 + 4 * 12 + 4 + 4 * 20 + 4 + 4),
+                                              (COMPACT_WS, lambda *a: compact(pool(), 5, AT, AT, *a), 3 * 100 + 4 + 4)])
+def test_pool_workspaces(query, call, words):
+    n = C.c_uint64()
+    assert query(ref(pool()), C.byref(n)) == OK and n.value == 4 * words
+    refused(call(AT, n.value - 1), E_ARG, "bytes of workspace")
+    refused(call(None, 0), E_ARG, "bytes of workspace")
+    refused(call(AT + 8, n.value), E_ARG, "aligned")
+    refused(call(AT, n.value), E_ARG, "null context")
+    assert query(ref(pool(n_pages=0)), C.byref(n)) == E_ARG and n.value == 0
+    assert query(ref(pool()), None) == E_ARG and query(None, C.byref(n)) == E_ARG
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(dtype=SPLIT), E_ARG, "F32, BF16 or E4M3"), (dict(head_dim=96), E_UNSUPPORTED, "head_dim"),
+    (dict(page_size=8), E_SHAPE, "page_size"), (dict(k=None), E_ARG, "null"), (dict(v=AT + 8), E_ARG, "aligned"),
+    (dict(n_pages=11), E_SHAPE, "different"), (dict(dtype=F32), E_SHAPE, "different"), (dict(n_kv_heads=4), E_SHAPE, "different"),
+    (dict(head_dim=64), E_SHAPE, "different"), (dict(page_size=32), E_SHAPE, "different"),
+    (dict(page_stride=4096, head_stride=128, token_stride=256), E_SHAPE, "different"),
+])
+def test_layers(kw, code, text):
+    refused(copy([pages(), pages(**kw)]), code, text)
+
+
+def test_copies():
+    # the packed order in other words is the same geometry
+    refused(copy([pages(), pages(page_stride=4096, head_stride=2048, token_stride=128)]), E_ARG, "null context")
+    refused(copy([pages()] * 200), E_ARG, "null context")
+    refused(copy([]), E_ARG, "null context")
+    refused(copy([pages()], most=0, copies=None, n=None), E_ARG, "null context")
+    refused(copy([pages()], copies=None), E_ARG, "null")
+    refused(copy([pages()], n=None), E_ARG, "null")
+    refused(copy([pages()], most=(1 << 26) + 1), E_ARG, "max_copies")
+    refused(COPY(None, None, 1, AT, AT, 1, None), E_ARG, "null")
+    refused(COPY(None, None, 65537, AT, AT, 1, None), E_ARG, "null")

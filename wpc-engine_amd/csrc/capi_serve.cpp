@@ -294,6 +294,71 @@ int check_draft(const wpcg_draft* d, int* chunks, uint64_t* bytes)
     return WPCG_OK;
 }
 
+// The blocks that pages are counted in, and what a call needs in device memory.
+int check_pool(const wpcg_kv_pool* p, PoolArgs* out, int* blocks)
+{
+    if (!p) return fail(WPCG_E_ARG, "null argument");
+    if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
+        return fail(WPCG_E_SHAPE, "page_size is a power of two in 16..256");
+    if (p->n_pages == 0 || p->n_pages > 1u << 26) return fail(WPCG_E_ARG, "n_pages out of range");
+    if (p->n_seq > INT_BOUND || p->table_stride == 0 || (uint64_t)p->n_seq * p->table_stride > INT_BOUND ||
+        (uint64_t)p->table_stride * p->page_size > INT_BOUND)
+        return fail(WPCG_E_ARG, "table out of range");
+    int shift = 0;
+    while ((1u << shift) < p->page_size) shift++;
+    *out = {(int)p->n_pages, (int)p->page_size, shift, (int)p->n_seq, (int)p->table_stride, p->refs_dev, p->table_dev,
+            p->kv_len_dev};
+    *blocks = (out->n_pages + POOL_BLOCK - 1) / POOL_BLOCK;
+    // workgroups of 1024 threads: a row's 1024 entries, a block of pages
+    if ((uint64_t)p->n_seq * ((p->table_stride + 1023) / 1024) + *blocks >= 1u << 22)
+        return fail(WPCG_E_UNSUPPORTED, "the pool needs too many workgroups");
+    return WPCG_OK;
+}
+int pool_ready(const wpcg_kv_pool* p, const void* result, const void* ws, uint64_t ws_bytes, uint64_t bytes)
+{
+    if (!p->refs_dev || (p->n_seq > 0 && (!p->table_dev || !p->kv_len_dev)) || !result)
+        return fail(WPCG_E_ARG, "null argument");
+    if (!ws || ws_bytes < bytes)
+        return fail(WPCG_E_ARG, "the call needs " + std::to_string(bytes) + " bytes of workspace");
+    if (!aligned(ws)) return fail(WPCG_E_ARG, "workspace not aligned to 16 bytes");
+    return WPCG_OK;
+}
+// The parts of a workspace, one behind the other.
+struct Parts {
+    uint8_t* at;
+    uint64_t used = 0;
+    template <class T>
+    T* take(uint64_t n)
+    {
+        T* r = (T*)(at + used);
+        used += (n * sizeof(T) + 15) / 16 * 16;
+        return r;
+    }
+};
+uint64_t fork_parts(ForkArgs* a, int blocks, void* ws)
+{
+    Parts w{(uint8_t*)ws};
+    a->blocks = blocks;
+    a->writers = w.take<ForkWriters>(a->p.n_pages);
+    a->rows = w.take<ForkRow>(a->p.n_seq);
+    a->tail = w.take<int>(a->p.n_seq);
+    a->kept = w.take<int>((uint64_t)a->p.n_seq * a->p.stride);
+    a->count = w.take<int>(blocks);
+    a->totals = w.take<int>(2);
+    return w.used;
+}
+uint64_t compact_parts(CompactArgs* a, int blocks, void* ws)
+{
+    Parts w{(uint8_t*)ws};
+    a->blocks = blocks;
+    a->count = w.take<int>(blocks);
+    a->total = w.take<int>(1);
+    a->rank = w.take<int>(a->p.n_pages);
+    a->used = w.take<int>(a->p.n_pages);
+    a->free = w.take<int>(a->p.n_pages);
+    return w.used;
+}
+
 int check_logprobs(const wpcg_logprob* d, int* chunks, uint64_t* part_bytes, uint64_t* bytes)
 {
     if (!d) return fail(WPCG_E_ARG, "null argument");
@@ -494,6 +559,112 @@ int wpcg_draft_verify(wpcg_ctx* ctx, const wpcg_draft* d, void* ws_dev, uint64_t
     a.done = (DraftDone*)(a.rest + (uint64_t)d->n_seq * a.chunks);
     a.vec = aligned(a.logits) && a.logits_row % 4 == 0 && aligned(a.probs) && a.probs_row % 4 == 0;
     WPCG_HIP(launch_draft_verify(a, pick(ctx, stream)));
+    return WPCG_OK;
+}
+
+int wpcg_kv_fork_workspace(const wpcg_kv_pool* pool, uint64_t* bytes)
+{
+    if (!bytes) return fail(WPCG_E_ARG, "null output");
+    *bytes = 0;
+    ForkArgs a{};
+    int blocks;
+    if (int rc = check_pool(pool, &a.p, &blocks)) return rc;
+    *bytes = fork_parts(&a, blocks, nullptr);
+    return WPCG_OK;
+}
+
+int wpcg_kv_fork(wpcg_ctx* ctx, const wpcg_kv_pool* pool, const wpcg_kv_change* c, void* ws_dev, uint64_t ws_bytes,
+                 wpcg_stream stream)
+{
+    ForkArgs a{};
+    int blocks;
+    if (int rc = check_pool(pool, &a.p, &blocks)) return rc;
+    if (!c) return fail(WPCG_E_ARG, "null argument");
+    if (int rc = pool_ready(pool, c->result_dev, ws_dev, ws_bytes, fork_parts(&a, blocks, ws_dev))) return rc;
+    if (pool->n_seq > 0 && !c->copies_dev) return fail(WPCG_E_ARG, "null argument");
+    if (int rc = check_ctx(ctx)) return rc;
+    a.parent = c->parent_dev;
+    a.keep = c->keep_dev;
+    a.grow = c->grow_dev;
+    a.grow_all = (int)std::min<uint64_t>(c->grow, INT_BOUND);
+    a.window = (int)std::min<uint64_t>(c->window, INT_BOUND);
+    a.sinks = (int)std::min<uint64_t>(c->sinks, INT_BOUND);
+    a.copies = c->copies_dev;
+    a.result = c->result_dev;
+    WPCG_HIP(launch_kv_fork(a, pick(ctx, stream)));
+    return WPCG_OK;
+}
+
+int wpcg_kv_compact_workspace(const wpcg_kv_pool* pool, uint64_t* bytes)
+{
+    if (!bytes) return fail(WPCG_E_ARG, "null output");
+    *bytes = 0;
+    CompactArgs a{};
+    int blocks;
+    if (int rc = check_pool(pool, &a.p, &blocks)) return rc;
+    *bytes = compact_parts(&a, blocks, nullptr);
+    return WPCG_OK;
+}
+
+int wpcg_kv_compact(wpcg_ctx* ctx, const wpcg_kv_pool* pool, uint32_t max_copies, int32_t* copies_dev,
+                    int32_t* result_dev, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream)
+{
+    CompactArgs a{};
+    int blocks;
+    if (int rc = check_pool(pool, &a.p, &blocks)) return rc;
+    if (int rc = pool_ready(pool, result_dev, ws_dev, ws_bytes, compact_parts(&a, blocks, ws_dev))) return rc;
+    if (max_copies > 0 && !copies_dev) return fail(WPCG_E_ARG, "null argument");
+    if (int rc = check_ctx(ctx)) return rc;
+    a.max_copies = (int)std::min<uint64_t>(max_copies, INT_BOUND);
+    a.copies = copies_dev;
+    a.result = result_dev;
+    WPCG_HIP(launch_kv_compact(a, pick(ctx, stream)));
+    return WPCG_OK;
+}
+
+int wpcg_kv_copy(wpcg_ctx* ctx, const wpcg_kv_pages* layers, uint32_t n_layers, const int32_t* copies_dev,
+                 const int32_t* n_copies_dev, uint32_t max_copies, wpcg_stream stream)
+{
+    if (n_layers > 0 && !layers) return fail(WPCG_E_ARG, "null pages");
+    if (n_layers > 65536) return fail(WPCG_E_ARG, "n_layers out of range");
+    if (max_copies > 1u << 26) return fail(WPCG_E_ARG, "max_copies out of range");
+    Pages st{};
+    for (uint32_t i = 0; i < n_layers; i++) {
+        const wpcg_kv_pages &l = layers[i], &o = layers[0];
+        Pages s;
+        if (int rc = check_pages(&l, &s)) return rc;
+        if (i == 0) st = s;
+        if (l.dtype != o.dtype || l.n_pages != o.n_pages || l.page_size != o.page_size || l.n_kv_heads != o.n_kv_heads ||
+            l.head_dim != o.head_dim || s.page != st.page || s.head != st.head || s.token != st.token)
+            return fail(WPCG_E_SHAPE, "layers of different pages");
+        if (!l.k_dev || !l.v_dev) return fail(WPCG_E_ARG, "null argument");
+        if (!aligned(l.k_dev) || !aligned(l.v_dev)) return fail(WPCG_E_ARG, "pages not aligned to 16 bytes");
+    }
+    if (n_layers == 0 || max_copies == 0) return check_ctx(ctx);
+    if (!copies_dev || !n_copies_dev) return fail(WPCG_E_ARG, "null argument");
+    if (int rc = check_ctx(ctx)) return rc;
+    const wpcg_kv_pages& kv = layers[0];
+    const uint64_t es = type_size(kv.dtype);
+    CopyArgs a{};
+    a.page_bytes = st.page * es;
+    a.head_bytes = st.head * es;
+    a.token_bytes = (uint32_t)(st.token * es);
+    a.heads = kv.n_kv_heads;
+    a.n_pages = (int)kv.n_pages;
+    a.page = (int)kv.page_size;
+    while ((16u << a.piece_shift) < kv.head_dim * es) a.piece_shift++;
+    a.max_copies = (int)max_copies;
+    a.copies = copies_dev;
+    a.n = n_copies_dev;
+    for (uint32_t l0 = 0; l0 < n_layers; l0 += COPY_LAYERS) {
+        const uint32_t n = std::min<uint32_t>(n_layers - l0, COPY_LAYERS);
+        for (uint32_t i = 0; i < n; i++) {
+            a.side[2 * i] = (uint8_t*)layers[l0 + i].k_dev;
+            a.side[2 * i + 1] = (uint8_t*)layers[l0 + i].v_dev;
+        }
+        a.units = 2 * n * a.heads;
+        WPCG_HIP(launch_kv_copy(a, pick(ctx, stream)));
+    }
     return WPCG_OK;
 }
 

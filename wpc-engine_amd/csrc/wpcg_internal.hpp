@@ -568,6 +568,57 @@ struct DraftArgs {
 };
 hipError_t launch_draft_verify(const DraftArgs& p, hipStream_t s);
 
+// ---- pages of a cache (kv_pool.hip) -----------------------------------------------
+constexpr int POOL_BLOCK = 4096;  // pages that a workgroup counts
+struct PoolArgs {
+    int n_pages, page, shift, n_seq, stride;
+    int32_t *refs, *table, *kv_len;
+};
+// A sequence's part of a fork, in pages and tokens.
+struct ForkRow {
+    int parent, keep, size;
+    int old_pages, kept_pages, pages;
+    int dead0, dead1;  // pages behind the window: none of them is kept
+    int from, base;    // its fresh pages: the first one's place in the row, and among all fresh pages
+    int copy, src;     // which copy the first of them is (-1: none), and of what page
+};
+struct ForkWriters {
+    int n, first;  // rows that write into a page next, the lowest of them
+};
+struct ForkArgs {
+    PoolArgs p;
+    const int32_t *parent, *keep, *grow;
+    int grow_all, window, sinks;
+    int32_t *copies, *result;
+    int blocks;            // of the pages
+    ForkWriters* writers;  // [n_pages], where a tail is
+    ForkRow* rows;         // [n_seq]
+    int *tail;             // [n_seq] the begun page that a row writes next, or -1
+    int *kept;             // [n_seq][stride] entries taken from other rows
+    int *count, *totals;   // [blocks] free pages; fresh pages and copies
+};
+hipError_t launch_kv_fork(const ForkArgs& a, hipStream_t s);
+struct CompactArgs {
+    PoolArgs p;
+    int max_copies;
+    int32_t *copies, *result;
+    int blocks, move_blocks;
+    int *count, *total;         // [blocks] pages in use; all of them
+    int *rank, *used, *free;    // [n_pages]
+};
+hipError_t launch_kv_compact(CompactArgs a, hipStream_t s);
+constexpr int COPY_LAYERS = 64;  // of a launch
+struct CopyArgs {
+    uint8_t* side[2 * COPY_LAYERS];  // keys and values of each layer
+    uint64_t page_bytes, head_bytes;
+    uint32_t token_bytes, heads, units;  // units: heads of a page in all layers, keys and values
+    int n_pages, page, piece_shift;      // 2^piece_shift pieces of 16 bytes a head's token
+    int max_copies, step_copies;
+    uint32_t step_units;  // of the waves in flight, whole copies and the rest
+    const int32_t *copies, *n;
+};
+hipError_t launch_kv_copy(CopyArgs a, hipStream_t s);
+
 // ---- log probabilities (logprob.hip) ------------------------------------------
 // A chunk's state of a row: its largest logit, the sum of e^t and of e^t t (t in
 // base 2, relative to that) over the others, how many reach it, and how many come

@@ -150,6 +150,11 @@ _SIGS = {
     "wpcg_paged_attention": (C.c_int, [_p, _p, _p, _p, _p, _u64, _p]),
     "wpcg_draft_verify_workspace": (C.c_int, [_p, _u64p]),
     "wpcg_draft_verify": (C.c_int, [_p, _p, _p, _u64, _p]),
+    "wpcg_kv_fork_workspace": (C.c_int, [_p, _u64p]),
+    "wpcg_kv_fork": (C.c_int, [_p, _p, _p, _p, _u64, _p]),
+    "wpcg_kv_compact_workspace": (C.c_int, [_p, _u64p]),
+    "wpcg_kv_compact": (C.c_int, [_p, _p, C.c_uint32, _p, _p, _p, _u64, _p]),
+    "wpcg_kv_copy": (C.c_int, [_p, _p, C.c_uint32, _p, _p, C.c_uint32, _p]),
     "wpcg_logprobs_workspace": (C.c_int, [_p, _u64p]),
     "wpcg_logprobs": (C.c_int, [_p, _p, _p, _u64, _p]),
     "wpcg_graph_begin": (C.c_int, [_p]),
@@ -794,6 +799,16 @@ class _Draft(C.Structure):
                 ("tokens", _p), ("u", _p), ("u_next", _p), ("temperature", _p), ("accepted", _p), ("out", _p)]
 
 
+class _KvPool(C.Structure):
+    _fields_ = [("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_seq", C.c_uint32), ("table_stride", C.c_uint32),
+                ("refs", _p), ("table", _p), ("kv_len", _p)]
+
+
+class _KvChange(C.Structure):
+    _fields_ = [("parent", _p), ("keep", _p), ("grow_each", _p), ("grow", C.c_uint32), ("window", C.c_uint32),
+                ("sinks", C.c_uint32), ("copies", _p), ("result", _p)]
+
+
 class _Logprob(C.Structure):
     _fields_ = [("n_rows", C.c_uint32), ("vocab", C.c_uint32), ("top", C.c_uint32), ("dtype", C.c_int32),
                 ("logits", _p), ("logits_stride", _u64), ("temperature", _p), ("tokens", _p), ("logprob", _p),
@@ -902,6 +917,76 @@ class DraftVerify:
         d.logits, d.tokens, d.u, d.u_next = _ptr(logits), _ptr(tokens), _ptr(u), _ptr(u_next)
         d.accepted, d.out, d.draft_probs = _ptr(accepted), _ptr(out), _ptr(draft_probs)
         check(lib.wpcg_draft_verify(self.ctx.h, self._ref, _ptr(self.workspace), self.workspace_bytes, stream))
+
+
+class KvPool:
+    """The pages' state that sequences share (wpcg_kv_pool): device arrays refs
+    int32[n_pages], table int32[n_seq][table_stride] and kv_len int32[n_seq], the
+    caller's (a KvBatch's table and lengths, say) or, where None, made empty."""
+
+    def __init__(self, ctx: Context, n_pages: int, page_size: int, n_seq: int, table_stride: int, refs=None, table=None,
+                 kv_len=None):
+        def made(b, n, value):
+            return ctx.upload(np.full(max(1, n), value, np.int32)) if b is None else b
+        self.ctx = ctx
+        self.refs, self.table = made(refs, n_pages, 0), made(table, n_seq * table_stride, -1)
+        self.kv_len = made(kv_len, n_seq, 0)
+        self.desc = _KvPool(n_pages, page_size, n_seq, table_stride, self.refs.ptr, self.table.ptr, self.kv_len.ptr)
+
+
+class KvFork:
+    """New rows for a pool's sequences (wpcg_kv_fork): parent, keep and grow_each
+    are device int32[n_seq] or None, grow the same for all; copies int32[n_seq][3]
+    and result int32[2] are written. Keeps its workspace: calls of one object
+    must not overlap."""
+
+    def __init__(self, ctx: Context, pool: KvPool, copies, result, parent=None, keep=None, grow: int = 0, grow_each=None,
+                 window: int = 0, sinks: int = 0):
+        self.ctx, self.pool = ctx, pool
+        self._keep = (copies, result, parent, keep, grow_each)
+        self.desc = _KvChange(_ptr(parent), _ptr(keep), _ptr(grow_each), grow, window, sinks, _ptr(copies), _ptr(result))
+        self._refs = (C.byref(pool.desc), C.byref(self.desc))
+        n = C.c_uint64()
+        check(lib.wpcg_kv_fork_workspace(self._refs[0], C.byref(n)))
+        self.workspace_bytes = n.value
+        self.workspace = ctx.alloc(n.value)
+
+    def run(self, stream=None):
+        check(lib.wpcg_kv_fork(self.ctx.h, *self._refs, _ptr(self.workspace), self.workspace_bytes, stream))
+
+
+class KvCompact:
+    """Moves a pool's pages in use to the front (wpcg_kv_compact), at most
+    max_copies of them a call; copies int32[max_copies][3] and result int32[2] are
+    written. Keeps its workspace: calls of one object must not overlap."""
+
+    def __init__(self, ctx: Context, pool: KvPool, copies, result, max_copies: int):
+        self.ctx, self.pool, self.copies, self.result, self.max_copies = ctx, pool, copies, result, max_copies
+        n = C.c_uint64()
+        check(lib.wpcg_kv_compact_workspace(C.byref(pool.desc), C.byref(n)))
+        self.workspace_bytes = n.value
+        self.workspace = ctx.alloc(n.value)
+
+    def run(self, stream=None):
+        check(lib.wpcg_kv_compact(self.ctx.h, C.byref(self.pool.desc), self.max_copies, _ptr(self.copies),
+                                  _ptr(self.result), _ptr(self.workspace), self.workspace_bytes, stream))
+
+
+class KvCopy:
+    """Copies the pages that a KvFork or KvCompact lists, in every layer
+    (wpcg_kv_copy): layers are PagedKv of one geometry, result is theirs."""
+
+    def __init__(self, ctx: Context, layers, copies, result, max_copies: int):
+        self.ctx, self.layers, self.max_copies = ctx, list(layers), max_copies
+        self._keep = (copies, result)
+        self.desc = (_KvPages * len(self.layers))(*(kv.desc for kv in self.layers))
+        self.copies = _ptr(copies)
+        at = _ptr(result)
+        self.n_copies = C.c_void_p((at.value if isinstance(at, C.c_void_p) else at) + 4)
+
+    def run(self, stream=None):
+        check(lib.wpcg_kv_copy(self.ctx.h, self.desc, len(self.layers), self.copies, self.n_copies, self.max_copies,
+                               stream))
 
 
 class LogProbs:
