@@ -618,6 +618,34 @@ int wpcg_paged_attention_workspace(const wpcg_kv_pages* kv, const wpcg_kv_batch*
 int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch,
                          const wpcg_attention* att, void* ws_dev, uint64_t ws_bytes, wpcg_stream stream);
 
+/* wpcg_paged_attention for a batch whose sequences come in groups that share
+ * their first tokens (answers to one prompt, beams, questions about one document):
+ * group g is sequences group_start[g] .. group_start[g+1]-1, and the first
+ * prefix_len[g] tokens of all of them are the same, so that their keys and values
+ * are read once for the group, from the pages of its first sequence. Tables,
+ * lengths and everything else are as for wpcg_paged_attention, which gives the
+ * same outputs within rounding: every sequence's row of the table lists all its
+ * pages, the shared ones among them (where a prefix ends inside a page, each
+ * sequence may have a copy of that page). A prefix is taken as far as max_prefix
+ * and the first sequence's length; sequences of no group, groups of one and
+ * groups whose numbers are not within the batch share nothing. Each sequence's
+ * rows come after its group's prefix as a rule, but need not. Work is shared out
+ * by the lengths, so that a sequence's last bits may depend on the others; the same call on the
+ * same arrays gives the same bits. Sharing is for single tokens and drafts: with
+ * more than 32 rows times query heads a key-value head, the call is
+ * wpcg_paged_attention itself. Where group_start falls, which group a sequence is
+ * of is open. Workspace and streams as for wpcg_paged_attention. */
+typedef struct wpcg_kv_prefix_s {
+    uint32_t n_groups, max_prefix;
+    const int32_t* group_start_dev; /* n_groups + 1 */
+    const int32_t* prefix_len_dev;  /* n_groups */
+} wpcg_kv_prefix;
+int wpcg_prefix_attention_workspace(const wpcg_kv_pages* kv, const wpcg_kv_batch* batch, const wpcg_kv_prefix* prefix,
+                                    const wpcg_attention* att, uint64_t* bytes);
+int wpcg_prefix_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch,
+                          const wpcg_kv_prefix* prefix, const wpcg_attention* att, void* ws_dev, uint64_t ws_bytes,
+                          wpcg_stream stream);
+
 /* Verification of drafted tokens by sampling, beside wpcg_model_verify's
  * greedy one: the accepted tokens are distributed as the target's own samples.
  * Sequence s owns rows q_start[s] .. q_start[s+1]-1 (q_start null: max_rows

@@ -160,3 +160,70 @@ def test_copies():
     refused(copy([pages()], most=(1 << 26) + 1), E_ARG, "max_copies")
     refused(COPY(None, None, 1, AT, AT, 1, None), E_ARG, "null")
     refused(COPY(None, None, 65537, AT, AT, 1, None), E_ARG, "null")
+
+
+# ---- attention over shared prefixes ----------------------------------------------
+ATTEND, ATTEND_WS = wpcg.lib.wpcg_prefix_attention, wpcg.lib.wpcg_prefix_attention_workspace
+
+
+def batch(**kw):
+    a = dict(n_seq=3, n_rows=5, max_q=3, max_kv=60, table_stride=4, q_start=AT, kv_len=AT, table=AT)
+    a.update(kw)
+    return wpcg._KvBatch(**a)
+
+
+def prefix(**kw):
+    a = dict(n_groups=2, max_prefix=50, group_start=AT, prefix_len=AT)
+    a.update(kw)
+    return wpcg._KvPrefix(**a)
+
+
+def attention(**kw):
+    a = dict(q=AT, out=AT, dtype=BF16, n_heads=8, scale=0.1)
+    a.update(kw)
+    return wpcg._Attention(**a)
+
+
+def attend(kv, b, x, a, ws=AT, n=1 << 40):
+    return ATTEND(None, ref(kv), ref(b), ref(x), ref(a), ws, n, None)
+
+
+def attend_ws(kv, b, x, a):
+    n = C.c_uint64(7)
+    rc = ATTEND_WS(ref(kv), ref(b), ref(x), ref(a), C.byref(n))
+    return n.value if rc == OK else rc
+
+
+def test_right_prefixes_end_at_the_context():
+    for x in (prefix(), prefix(n_groups=0, group_start=None, prefix_len=None), prefix(n_groups=3), prefix(n_groups=50),
+              prefix(max_prefix=0), prefix(max_prefix=1 << 30)):
+        for b in (batch(), batch(q_start=None, max_q=1), batch(n_seq=0), batch(n_rows=0), batch(max_q=5, n_rows=9)):
+            refused(attend(pages(), b, x, attention()), E_ARG, "null context")
+
+
+@pytest.mark.parametrize("kv,b,x,a,code,text", [
+    (None, {}, {}, {}, E_ARG, "null"), ({}, None, {}, {}, E_ARG, "null"), ({}, {}, None, {}, E_ARG, "null"),
+    ({}, {}, {}, None, E_ARG, "null"), ({}, {}, dict(group_start=None), {}, E_ARG, "null"),
+    ({}, {}, dict(prefix_len=None), {}, E_ARG, "null"), ({}, {}, dict(n_groups=(1 << 30) + 1), {}, E_ARG, "prefix bounds"),
+    ({}, {}, dict(max_prefix=(1 << 30) + 1), {}, E_ARG, "prefix bounds"), (dict(head_dim=96), {}, {}, {}, E_UNSUPPORTED, "head_dim"),
+    (dict(k=None), {}, {}, {}, E_ARG, "null"), ({}, dict(table_stride=3), {}, {}, E_SHAPE, "table"),
+    ({}, dict(q_start=None), {}, {}, E_ARG, "q_start"), ({}, {}, {}, dict(scale=0.0), E_ARG, "scale"),
+    ({}, {}, {}, dict(n_heads=9), E_SHAPE, "n_heads"), ({}, {}, {}, dict(out=AT + 2), E_ARG, "aligned"),
+    ({}, {}, {}, dict(q=None), E_ARG, "null"), ({}, {}, {}, dict(q_stride=8), E_SHAPE, "shorter"),
+    (dict(dtype=F32), {}, {}, {}, E_UNSUPPORTED, "BF16 queries"), ({}, dict(kv_len=None), {}, {}, E_ARG, "null"),
+])
+def test_prefix_refusals(kv, b, x, a, code, text):
+    made = [None if kw is None else f(**kw) for f, kw in ((pages, kv), (batch, b), (prefix, x), (attention, a))]
+    refused(attend(*made), code, text)
+
+
+def test_prefix_workspace():
+    n = attend_ws(pages(), batch(), prefix(), attention())
+    assert n > 0 and n % 4 == 0
+    refused(attend(pages(), batch(), prefix(), attention(), n=n - 1), E_ARG, "bytes of workspace")
+    refused(attend(pages(), batch(), prefix(), attention(), ws=None, n=0), E_ARG, "bytes of workspace")
+    refused(attend(pages(), batch(), prefix(), attention(), ws=AT + 4), E_ARG, "aligned")
+    # without sharing that of the plain call
+    for x in (prefix(n_groups=0), prefix(max_prefix=0), prefix(n_groups=3)):
+        assert attend_ws(pages(), batch(), x, attention()) == 0
+    assert ATTEND_WS(ref(pages()), ref(batch()), ref(prefix()), ref(attention()), None) == E_ARG

@@ -1,0 +1,301 @@
+"""GPU tests of wpcg_prefix_attention against a plain 64-bit implementation of each
+sequence by itself: groups of every size and prefix, types, head layouts, rows,
+windows that end in either part; lengths, groups and pages that are none; loose
+bounds, graphs, streams. Bounds are derived in serve_ref.attention_bound."""
+import numpy as np
+import pytest
+
+import serve_ref as R
+import wpcg
+from serve_ref import BF16, E4M3, F32
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [(BF16, BF16), (BF16, E4M3), (F32, F32), (F32, BF16), (F32, E4M3)]
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = wpcg.Context(0)
+    yield c
+    c.close()
+
+
+class Groups:
+    """A batch whose groups share: groups = [(prefix, [own tokens of each sequence])]."""
+
+    def __init__(self, ctx, rng, groups, dtype, hkv, d, page, order="head", width=0):
+        self.ctx, self.groups = ctx, groups
+        self.size = [len(own) for _, own in groups]
+        self.prefix = [p for p, _ in groups]
+        lens = [p + m for p, own in groups for m in own]
+        self.pg = pg = R.Paged(ctx, rng, dtype, hkv, d, page, lens, order=order, scales=dtype == E4M3, width=width)
+        self.start = np.cumsum([0] + self.size)
+        for g, (p, own) in enumerate(groups):
+            lead = self.start[g]
+            for s in range(lead + 1, self.start[g + 1]):
+                whole = p // page
+                pg.table[s, :whole] = pg.table[lead, :whole]
+                rest = np.arange(whole * page, p)
+                for n in "kv":
+                    pg.real[n][s][:p] = pg.real[n][lead][:p]
+                    if len(rest):
+                        pg.bits[n][pg.index(s, rest)] = pg.bits[n][pg.index(lead, rest)]
+        pg.upload()
+
+    def desc(self, max_prefix=None, start=None, prefix=None):
+        self.d_start = self.ctx.upload(np.asarray(self.start if start is None else start, np.int32))
+        prefix = self.prefix if prefix is None else prefix
+        self.d_prefix = self.ctx.upload(np.asarray(prefix, np.int32))
+        return wpcg.KvPrefix(len(prefix), self.d_start, self.d_prefix,
+                             max(max(self.prefix), 1) if max_prefix is None else max_prefix)
+
+
+def expected(pg, q, rows, q_dtype, scale, window, sinks):
+    outs, bounds = [], []
+    at = 0
+    for s, n in enumerate(rows):
+        m = pg.kv_len[s]
+        x = R.decode(q[at:at + n], q_dtype)
+        o, mag, reach = R.attention(x, pg.real["k"][s], pg.real["v"][s], np.arange(m - n, m), scale, window, sinks)
+        outs.append(o)
+        bounds.append(R.attention_bound(o, mag, reach, pg.d, m, q_dtype))
+        at += n
+    return np.concatenate(outs), np.concatenate(bounds)
+
+
+def check(got, want, bound):
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    off = np.abs(got - want) - bound
+    i = np.unravel_index(np.nanargmax(off), off.shape)
+    assert not (off > 0).any(), f"{(off > 0).sum()} of {off.size} off, worst {i}: {got[i]} for {want[i]} +- {bound[i]}"
+
+
+def run(ctx, pg, batch, prefix, q, heads, q_dtype, scale, window=0, sinks=0, stream=None):
+    rows = q.shape[0]
+    out = ctx.upload(np.full(rows * heads * pg.d * R.SIZE[q_dtype], 0x5A, np.uint8))
+    qd = ctx.upload(q)
+    op = wpcg.PrefixAttention(ctx, pg.kv, batch, prefix, heads, q_dtype, scale=scale, window=window, sinks=sinks)
+    if op.workspace is not None:
+        op.workspace.write(np.full(op.workspace_bytes, 0xFF, np.uint8))
+    op.run(qd, out, stream)
+    ctx.sync()
+    return R.decode(out.read(R.BITS[q_dtype], rows * heads * pg.d).reshape(rows, heads, pg.d), q_dtype)
+
+
+def one(ctx, rng, groups, q_dtype, dtype, hkv, heads, d, page, rows=1, window=0, sinks=0, order="head", null_start=False):
+    g = Groups(ctx, rng, groups, dtype, hkv, d, page, order)
+    n = len(g.pg.kv_len)
+    per = [rows] * n if np.isscalar(rows) else rows
+    q = R.encode(rng.standard_normal((sum(per), heads, d)) * 1.5, q_dtype)
+    scale = d ** -0.5
+    batch = g.pg.batch(None if null_start else per)
+    got = run(ctx, g.pg, batch, g.desc(), q, heads, q_dtype, scale, window, sinks)
+    want, bound = expected(g.pg, q, per, q_dtype, scale, window, sinks)
+    check(got, want, bound)
+    return g, batch, q, got, want, bound
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("d,heads,hkv", [(128, 8, 2), (64, 14, 2), (64, 3, 3), (128, 20, 1), (128, 32, 1), (128, 32, 4)])
+def test_one_row_each(ctx, q_dtype, dtype, d, heads, hkv):
+    """Groups of 4, 7, 1, 20, 32 and 8 query heads; of 2 to 40 sequences and of one;
+    prefixes of none, of parts of pages and of several chunks."""
+    print(f"[gpu] prefix {q_dtype}/{dtype} {heads}/{hkv}x{d}", flush=True)
+    rng = np.random.default_rng(d + heads + 10 * q_dtype + dtype)
+    groups = [(300, [1, 2, 40, 33, 7]), (64, [5, 5]), (17, [100]), (0, [3, 90]), (1, [1, 1, 1]), (129, list(range(1, 41))),
+              (16, [31, 32, 64])]
+    one(ctx, rng, groups, q_dtype, dtype, hkv, heads, d, 16)
+    one(ctx, rng, groups, q_dtype, dtype, hkv, heads, d, 16, null_start=True)
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("rows", [2, 5, 8])
+def test_drafts(ctx, q_dtype, dtype, rows):
+    """Several rows a sequence, ragged, one of them without any; prefixes that end
+    within the rows' own positions."""
+    print(f"[gpu] prefix drafts {q_dtype}/{dtype} rows {rows}", flush=True)
+    rng = np.random.default_rng(rows + 10 * q_dtype + dtype)
+    groups = [(200, [rows, rows + 1, 50, 90]), (33, [60, 8, 8]), (500, [20] * 9)]
+    per = [max(1, rows - i % 3) for i in range(16)]
+    per[5] = 0
+    one(ctx, rng, groups, q_dtype, dtype, 2, 8, 128, 32, rows=per, order="token")
+    # rows that begin before the prefix ends
+    one(ctx, rng, [(100, [1, 2, 0, 3]), (64, [0, 0])], q_dtype, dtype, 2, 8, 128, 16, rows=rows)
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 3), (33, 16), (64, 70), (100, 4), (150, 0), (400, 10), (5000, 4), (40, 250)])
+def test_windows(ctx, q_dtype, dtype, window, sinks):
+    """Windows that leave nothing of the prefix, some of it or all; sinks in it, up
+    to its end and beyond."""
+    print(f"[gpu] prefix window {q_dtype}/{dtype} {window} {sinks}", flush=True)
+    rng = np.random.default_rng(window + sinks + 10 * q_dtype + dtype)
+    groups = [(200, [3, 40, 130, 90]), (37, [120, 3, 8]), (300, [20] * 5), (10, [400, 5])]
+    one(ctx, rng, groups, q_dtype, dtype, 2, 8, 64, 16, rows=3, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+def test_long_prefixes(ctx, q_dtype, dtype):
+    """Several chunks and workgroups a prefix, own tokens of several too; the same
+    call gives the same bits."""
+    print(f"[gpu] prefix long {q_dtype}/{dtype}", flush=True)
+    rng = np.random.default_rng(3 + 10 * q_dtype + dtype)
+    groups = [(5000, [700, 3, 1500]), (900, [40, 1]), (2050, [9] * 12)]
+    g, batch, q, got, _, _ = one(ctx, rng, groups, q_dtype, dtype, 2, 4, 128, 64)
+    again = run(ctx, g.pg, batch, g.desc(), q, 4, q_dtype, 128 ** -0.5)
+    assert np.array_equal(got.view(np.uint64), again.view(np.uint64))
+
+
+@pytest.mark.parametrize("q_dtype,dtype", [(BF16, BF16), (F32, F32), (F32, E4M3)])
+def test_bounds_that_are_loose(ctx, q_dtype, dtype):
+    """More rows, tokens and prefix by the bounds than there are; rows of no
+    sequence as they were."""
+    rng = np.random.default_rng(4 + dtype)
+    g = Groups(ctx, rng, [(150, [4, 30, 9]), (20, [8, 8])], dtype, 2, 64, 16, width=7000)
+    q = R.encode(rng.standard_normal((5 + 20, 6, 64)), q_dtype)
+    batch = g.pg.batch([1] * 5, n_rows=25, max_kv=110000, max_q=3)
+    got = run(ctx, g.pg, batch, g.desc(max_prefix=100000), q, 6, q_dtype, 0.2)
+    check(got[:5], *expected(g.pg, q[:5], [1] * 5, q_dtype, 0.2, 0, 0))
+    assert (got[5:] == R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]).all()
+
+
+@pytest.mark.parametrize("q_dtype,dtype", [(BF16, BF16), (F32, BF16)])
+def test_groups_that_are_none(ctx, q_dtype, dtype):
+    """Groups whose numbers are out of bounds share nothing, a bound below the
+    prefix cuts it short, and there may be no groups at all."""
+    rng = np.random.default_rng(5)
+    g = Groups(ctx, rng, [(150, [4, 30, 9]), (70, [8, 8]), (33, [1, 2])], dtype, 2, 64, 16)
+    q = R.encode(rng.standard_normal((7, 8, 64)), q_dtype)
+    batch = g.pg.batch([1] * 7)
+    want = expected(g.pg, q, [1] * 7, q_dtype, 0.125, 0, 0)
+    for start, prefix, most in (([0, 3, 5, 7], [-5, 70, -2 ** 31], 150), ([0, 3, 5, 7], [150, 70, 33], 60),
+                                ([0, 3, 5, 7], [150, 70, 33], 0), ([-1, 3, 5, 7], [150, 70, 33], 150),
+                                ([0, 3, 5, 8], [150, 70, 33], 150), ([0, 3, 5, 2 ** 31 - 1], [150, 70, 33], 150),
+                                ([0, 3, 3, 5, 7], [150, 9, 70, 33], 150), ([1, 3, 4, 6], [150, 70, 0], 150),
+                                ([3, 5], [70], 150)):
+        check(run(ctx, g.pg, batch, g.desc(max_prefix=most, start=start, prefix=prefix), q, 8, q_dtype, 0.125), *want)
+    none = wpcg.KvPrefix(0, None, None, 100)
+    check(run(ctx, g.pg, batch, none, q, 8, q_dtype, 0.125), *want)
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+def test_lengths_and_pages_that_are_none(ctx, q_dtype, dtype):
+    """A length that is none, the first sequence's too; a page of the prefix that
+    is none reaches its group alone, one of a sequence's own that one alone."""
+    print(f"[gpu] prefix bad {q_dtype}/{dtype}", flush=True)
+    rng = np.random.default_rng(6 + dtype)
+    g, batch, q, _, want, bound = one(ctx, rng, [(150, [4, 30, 9]), (200, [8, 40, 20]), (33, [1, 2])], q_dtype, dtype, 2, 8, 64, 16)
+    pg, prefix = g.pg, g.desc()
+
+    def again(lens, table):
+        pg.d_len.write(np.asarray(lens, np.int32))
+        pg.d_table.write(table)
+        return run(ctx, pg, batch, prefix, q, 8, q_dtype, 0.125)
+    for bad in (-1, 10 ** 6, 2 ** 31 - 1, -2 ** 31):
+        for s in (0, 4):
+            got = again([bad if i == s else m for i, m in enumerate(pg.kv_len)], pg.table)
+            assert np.isnan(got[s]).all()
+            rest = [i for i in range(8) if i != s]
+            check(got[rest], want[rest], bound[rest])
+    table = pg.table.copy()
+    table[3:6, 2] = [pg.n_pages, -1, 2 ** 31 - 1]
+    got = again(pg.kv_len, table)
+    assert np.isnan(got[3:6]).all()
+    check(got[[0, 1, 2, 6, 7]], want[[0, 1, 2, 6, 7]], bound[[0, 1, 2, 6, 7]])
+    table = pg.table.copy()
+    table[1, 11] = -5
+    got = again(pg.kv_len, table)
+    assert np.isnan(got[1]).all()
+    check(got[[0, 2, 3, 4, 5, 6, 7]], want[[0, 2, 3, 4, 5, 6, 7]], bound[[0, 2, 3, 4, 5, 6, 7]])
+
+
+@pytest.mark.parametrize("q_dtype,dtype", [(BF16, BF16), (F32, F32), (F32, BF16)])
+def test_values_that_are_not_finite(ctx, q_dtype, dtype):
+    """NaN and infinities at tokens that a window hides from some rows reach those
+    that see them alone."""
+    rng = np.random.default_rng(7 + dtype)
+    g = Groups(ctx, rng, [(100, [3, 60, 90]), (64, [5, 80])], dtype, 1, 64, 16)
+    pg = g.pg
+    q = R.encode(rng.standard_normal((5, 4, 64)), q_dtype)
+    batch = pg.batch([1] * 5)
+    want, bound = expected(pg, q, [1] * 5, q_dtype, 0.125, 70, 2)
+    words = {F32: (0x7F800000, 0xFF800000, 0x7FC00000), BF16: (0x7F80, 0xFF80, 0x7FC0)}[dtype]
+    # the row of sequence 0 (103 tokens) sees the prefix from 33 on, those of 1 and 2 from 90 and not at all
+    for w in words:
+        for n in "kv":
+            x = pg.bits[n].copy()
+            x[pg.index(0, [60])] = w
+            (pg.dk if n == "k" else pg.dv).write(x)
+            got = run(ctx, pg, batch, g.desc(), q, 4, q_dtype, 0.125, 70, 2)
+            check(got[1:], want[1:], bound[1:])
+            assert not (np.abs(got[0] - want[0]) <= bound[0]).all()
+            (pg.dk if n == "k" else pg.dv).write(pg.bits[n])
+
+
+def test_prompts_are_plain(ctx):
+    """More than 32 rows times heads: the same bits as wpcg_paged_attention."""
+    rng = np.random.default_rng(8)
+    g = Groups(ctx, rng, [(90, [40, 40]), (33, [50, 70])], BF16, 2, 128, 16)
+    rows = [40, 30, 50, 1]
+    q = R.encode(rng.standard_normal((121, 8, 128)), BF16)
+    batch = g.pg.batch(rows)
+    got = run(ctx, g.pg, batch, g.desc(), q, 8, BF16, 0.1)
+    check(got, *expected(g.pg, q, rows, BF16, 0.1, 0, 0))
+    op = wpcg.PagedAttention(ctx, g.pg.kv, batch, 8, BF16, scale=0.1)
+    out = ctx.alloc(q.nbytes)
+    op.run(ctx.upload(q), out)
+    ctx.sync()
+    assert np.array_equal(R.decode(out.read(np.uint16, q.size).reshape(q.shape), BF16), got)
+
+
+def test_many_sequences(ctx):
+    """Groups laid out over more sequences than a workgroup has threads, and more
+    groups than a wave looks through at once."""
+    rng = np.random.default_rng(9)
+    groups = [(int(rng.integers(0, 90)), [int(x) for x in rng.integers(1, 40, rng.integers(1, 9))]) for _ in range(150)]
+    one(ctx, rng, groups, BF16, BF16, 1, 4, 64, 16)
+    one(ctx, rng, [(40, [2] * 600)], BF16, E4M3, 1, 4, 64, 16)
+    one(ctx, rng, [(70, [1 + i % 30 for i in range(1100)])], F32, BF16, 1, 2, 64, 16)
+
+
+def test_graphs_and_streams(ctx):
+    """Two captured calls in turn whose lengths, groups and queries change between
+    the replays, and the same bits from another stream."""
+    print("[gpu] prefix graphs", flush=True)
+    rng = np.random.default_rng(10)
+    made = []
+    for groups, dtype in (([(400, [60] * 7), (90, [60] * 3)], BF16), ([(64, [40] * 4)], F32)):
+        g = Groups(ctx, rng, groups, dtype, 2, 128, 16)
+        n = len(g.pg.kv_len)
+        batch, prefix = g.pg.batch([1] * n), g.desc()
+        q, out = ctx.alloc(n * 8 * 128 * R.SIZE[dtype]), ctx.alloc(n * 8 * 128 * R.SIZE[dtype])
+        op = wpcg.PrefixAttention(ctx, g.pg.kv, batch, prefix, 8, dtype, scale=0.1)
+        made.append((g, dtype, n, q, out, ctx.capture(lambda op=op, q=q, out=out: op.run(q, out)), op, batch))
+    whole = [list(m[0].pg.kv_len) for m in made]
+    for turn in range(5):
+        xs = []
+        for (g, dtype, n, q, out, graph, _, _), lens in zip(made, whole):
+            g.pg.kv_len = [m - int(rng.integers(0, 59 if dtype == BF16 else 39)) for m in lens]
+            g.pg.d_len.write(np.array(g.pg.kv_len, np.int32))
+            g.d_prefix.write(np.array([p - turn for p in g.prefix], np.int32))
+            x = R.encode(rng.standard_normal((n, 8, 128)), dtype)
+            q.write(x)
+            xs.append(x)
+            graph.launch()
+        ctx.sync()
+        for (g, dtype, n, _, out, _, _, _), x in zip(made, xs):
+            got = R.decode(out.read(R.BITS[dtype], x.size).reshape(x.shape), dtype)
+            real = {k: [v[:m] for v, m in zip(g.pg.real[k], g.pg.kv_len)] for k in "kv"}
+            outs = [R.attention(R.decode(x[s:s + 1], dtype), real["k"][s], real["v"][s], [g.pg.kv_len[s] - 1], 0.1, 0, 0)
+                    for s in range(n)]
+            bound = np.concatenate([R.attention_bound(*o, 128, g.pg.kv_len[s], dtype) for s, o in enumerate(outs)])
+            check(got, np.concatenate([o[0] for o in outs]), bound)
+    other = wpcg.Context(0)
+    g, dtype, n, q, out, graph, op, _ = made[0]
+    first = out.read(R.BITS[dtype], n * 8 * 128)
+    out.write(np.zeros_like(first))
+    op.run(q, out, other.stream)
+    other.sync()
+    assert np.array_equal(out.read(R.BITS[dtype], n * 8 * 128), first)
+    other.close()

@@ -257,6 +257,53 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
     return WPCG_OK;
 }
 
+// A batch whose groups share prefixes: how those are read, and the plans of the
+// batch without sharing, where that is what it takes.
+struct PrefixPlan {
+    bool shared;
+    Plans plain;
+    PrefixArgs args;  // chunks, splits, blocks and columns
+    uint64_t pre_parts, own_parts;
+    uint64_t bytes;
+};
+int plan_prefix(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_kv_prefix* x, const wpcg_attention* a,
+                PrefixPlan* out)
+{
+    PrefixPlan& o = *out;
+    o = {};
+    const int64_t group = a->n_heads / kv->n_kv_heads, cols = (int64_t)b.max_q * group;
+    const int64_t max_prefix = std::min<int64_t>(x->max_prefix, b.max_kv);
+    o.shared = b.n_rows > 0 && cols <= 2 * ATTN_FEW_COLS && x->n_groups > 0 && (int)x->n_groups < b.n_seq && max_prefix > 0;
+    if (!o.shared) {
+        if (int rc = plan_attention(kv, b, a, &o.plain)) return rc;
+        o.bytes = o.plain.bytes;
+        return WPCG_OK;
+    }
+    PrefixArgs& p = o.args;
+    p.n_groups = (int)x->n_groups;
+    p.max_prefix = (int)max_prefix;
+    const int64_t cw = ATTN_MANY_COLS, tiles = (max_prefix + ATTN_MANY_TILE - 1) / ATTN_MANY_TILE;
+    const int64_t blocks = std::min(x->n_groups * ((b.n_rows * group + cw - 1) / cw), b.n_rows * group / cw + x->n_groups);
+    const int64_t room = a->dtype == WPCG_DTYPE_BF16 ? 2 * CUS : CUS;
+    const int64_t splits = std::max<int64_t>(1, std::min(room / std::max<int64_t>(1, blocks * kv->n_kv_heads), tiles / 2));
+    p.chunk = (int)((tiles + splits - 1) / splits);
+    p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
+    p.blocks = (int)blocks;
+    const int64_t own = (b.max_kv + ATTN_FEW_TILE - 1) / ATTN_FEW_TILE;
+    p.a.cols = cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
+    p.a.col_blocks = (int)((cols + p.a.cols - 1) / p.a.cols);
+    p.a.chunk = (int)std::max<int64_t>(32, (own + 15) / 16);
+    p.a.splits = (int)((own + p.a.chunk - 1) / p.a.chunk);
+    p.a.part_rows = b.n_rows;
+    const int64_t items = (int64_t)b.n_seq * kv->n_kv_heads * p.a.col_blocks * p.a.splits;
+    if (items >= GROUPS_512 || blocks * kv->n_kv_heads * p.splits >= GROUPS_512)
+        return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
+    o.pre_parts = (uint64_t)p.splits * b.n_rows * a->n_heads;
+    o.own_parts = (uint64_t)items * p.a.cols;
+    o.bytes = (o.pre_parts + o.own_parts) * (kv->head_dim + 2) * sizeof(float);
+    return WPCG_OK;
+}
+
 // The scores' factor in base 2.
 float scale_log2(const wpcg_attention* a) { return (float)((double)a->scale * 1.4426950408889634); }
 
@@ -269,6 +316,73 @@ int check_attention(const wpcg_kv_pages* kv, const wpcg_attention* a)
     if (a->n_heads == 0 || a->n_heads > 65536 || a->n_heads % kv->n_kv_heads)
         return fail(WPCG_E_SHAPE, "n_heads is a multiple of n_kv_heads");
     if (!(a->scale > 0.0f) || !std::isfinite(scale_log2(a))) return fail(WPCG_E_ARG, "scale is positive, and finite times log2 e");
+    return WPCG_OK;
+}
+
+int check_prefix(const wpcg_kv_prefix* x)
+{
+    if (!x) return fail(WPCG_E_ARG, "null argument");
+    if (x->n_groups > INT_BOUND || x->max_prefix > INT_BOUND) return fail(WPCG_E_ARG, "prefix bounds out of range");
+    return WPCG_OK;
+}
+
+// What a call of attention has checked, without its plan and workspace.
+int attention_ready(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch, const wpcg_attention* att,
+                    uint64_t bytes, const void* ws, uint64_t ws_bytes)
+{
+    if (int rc = check_pointers(kv, batch)) return rc;
+    if (!att->q_dev || !att->out_dev) return fail(WPCG_E_ARG, "null argument");
+    if (!aligned(att->q_dev) || !aligned(att->out_dev)) return fail(WPCG_E_ARG, "rows not aligned to 16 bytes");
+    if (bytes) {
+        if (!ws || ws_bytes < bytes)
+            return fail(WPCG_E_ARG, "the call needs " + std::to_string(bytes) + " bytes of workspace");
+        if (!aligned(ws)) return fail(WPCG_E_ARG, "workspace not aligned to 16 bytes");
+    }
+    return check_ctx(ctx);
+}
+// A call's arguments for the kernels, without its plan; a.b is there.
+int attention_args(const wpcg_kv_pages* kv, const Pages& st, const wpcg_attention* att, PagedAttnArgs& a)
+{
+    const uint64_t width = (uint64_t)att->n_heads * kv->head_dim;
+    if (int rc = row_stride(att->q_stride, width, att->dtype, &a.q_row)) return rc;
+    if (int rc = row_stride(att->out_stride, width, att->dtype, &a.out_row)) return rc;
+    a.q = att->q_dev;
+    a.out = att->out_dev;
+    a.k = kv->k_dev;
+    a.v = kv->v_dev;
+    a.page_stride = st.page;
+    a.head_stride = st.head;
+    a.token_stride = st.token;
+    a.k_scale = kv->k_scale_dev;
+    a.v_scale = kv->v_scale_dev;
+    a.n_heads = (int)att->n_heads;
+    a.n_kv = (int)kv->n_kv_heads;
+    a.group = a.n_heads / a.n_kv;
+    a.scale = scale_log2(att);
+    a.window = (int)std::min<uint64_t>(att->window, INT_BOUND);
+    a.sinks = (int)std::min<uint64_t>(att->sinks, INT_BOUND);
+    return WPCG_OK;
+}
+int run_plans(PagedAttnArgs a, const Plans& plan, const wpcg_kv_pages* kv, const wpcg_attention* att, void* ws,
+              hipStream_t s)
+{
+    const int d = (int)kv->head_dim;
+    for (int i = 0; i < plan.n; i++) {
+        const Plan& p = plan.part[i];
+        a.b = p.b;
+        a.cols = p.cols;
+        a.col_blocks = p.col_blocks;
+        a.blocks = p.blocks;
+        a.chunk = p.chunk;
+        a.splits = p.splits;
+        a.part_rows = p.part_rows;
+        a.part_seq = p.part_seq;
+        a.part_o = (float*)ws;
+        a.part_ml = a.part_o + p.parts * kv->head_dim;
+        a.ends = (AttnEnd*)(a.part_ml + p.parts * 2);
+        WPCG_HIP(p.many ? launch_attn_many(a, d, att->dtype, kv->dtype, s)
+                        : launch_attn_few(a, d, att->dtype, kv->dtype, s));
+    }
     return WPCG_OK;
 }
 
@@ -465,54 +579,64 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
     PagedAttnArgs a{};
     if (int rc = check_batch(batch, kv, &a.b)) return rc;
     if (int rc = check_attention(kv, att)) return rc;
-    const uint64_t width = (uint64_t)att->n_heads * kv->head_dim;
-    if (int rc = row_stride(att->q_stride, width, att->dtype, &a.q_row)) return rc;
-    if (int rc = row_stride(att->out_stride, width, att->dtype, &a.out_row)) return rc;
+    if (int rc = attention_args(kv, st, att, a)) return rc;
     Plans plan;
     if (int rc = plan_attention(kv, a.b, att, &plan)) return rc;
     if (batch->n_seq == 0 || batch->n_rows == 0) return check_ctx(ctx);
-    if (int rc = check_pointers(kv, batch)) return rc;
-    if (!att->q_dev || !att->out_dev) return fail(WPCG_E_ARG, "null argument");
-    if (!aligned(att->q_dev) || !aligned(att->out_dev)) return fail(WPCG_E_ARG, "rows not aligned to 16 bytes");
-    if (plan.bytes) {
-        if (!ws_dev || ws_bytes < plan.bytes)
-            return fail(WPCG_E_ARG, "the call needs " + std::to_string(plan.bytes) + " bytes of workspace");
-        if (!aligned(ws_dev)) return fail(WPCG_E_ARG, "workspace not aligned to 16 bytes");
-    }
-    if (int rc = check_ctx(ctx)) return rc;
-    a.q = att->q_dev;
-    a.out = att->out_dev;
-    a.k = kv->k_dev;
-    a.v = kv->v_dev;
-    a.page_stride = st.page;
-    a.head_stride = st.head;
-    a.token_stride = st.token;
-    a.k_scale = kv->k_scale_dev;
-    a.v_scale = kv->v_scale_dev;
-    a.n_heads = (int)att->n_heads;
-    a.n_kv = (int)kv->n_kv_heads;
-    a.group = a.n_heads / a.n_kv;
-    a.scale = scale_log2(att);
-    a.window = (int)std::min<uint64_t>(att->window, INT_BOUND);
-    a.sinks = (int)std::min<uint64_t>(att->sinks, INT_BOUND);
+    if (int rc = attention_ready(ctx, kv, batch, att, plan.bytes, ws_dev, ws_bytes)) return rc;
+    return run_plans(a, plan, kv, att, ws_dev, pick(ctx, stream));
+}
+
+int wpcg_prefix_attention_workspace(const wpcg_kv_pages* kv, const wpcg_kv_batch* batch, const wpcg_kv_prefix* prefix,
+                                    const wpcg_attention* att, uint64_t* bytes)
+{
+    if (!bytes) return fail(WPCG_E_ARG, "null output");
+    *bytes = 0;
+    Pages st;
+    if (int rc = check_pages(kv, &st)) return rc;
+    PagedBatch b;
+    if (int rc = check_batch(batch, kv, &b)) return rc;
+    if (int rc = check_prefix(prefix)) return rc;
+    if (int rc = check_attention(kv, att)) return rc;
+    PrefixPlan plan;
+    if (int rc = plan_prefix(kv, b, prefix, att, &plan)) return rc;
+    *bytes = plan.bytes;
+    return WPCG_OK;
+}
+
+int wpcg_prefix_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_batch* batch,
+                          const wpcg_kv_prefix* prefix, const wpcg_attention* att, void* ws_dev, uint64_t ws_bytes,
+                          wpcg_stream stream)
+{
+    Pages st;
+    if (int rc = check_pages(kv, &st)) return rc;
+    PagedAttnArgs a{};
+    if (int rc = check_batch(batch, kv, &a.b)) return rc;
+    if (int rc = check_prefix(prefix)) return rc;
+    if (int rc = check_attention(kv, att)) return rc;
+    if (int rc = attention_args(kv, st, att, a)) return rc;
+    PrefixPlan plan;
+    if (int rc = plan_prefix(kv, a.b, prefix, att, &plan)) return rc;
+    if (batch->n_seq == 0 || batch->n_rows == 0) return check_ctx(ctx);
+    if (prefix->n_groups > 0 && (!prefix->group_start_dev || !prefix->prefix_len_dev))
+        return fail(WPCG_E_ARG, "null argument");
+    if (int rc = attention_ready(ctx, kv, batch, att, plan.bytes, ws_dev, ws_bytes)) return rc;
     const hipStream_t s = pick(ctx, stream);
-    const int d = (int)kv->head_dim;
-    for (int i = 0; i < plan.n; i++) {
-        const Plan& p = plan.part[i];
-        a.b = p.b;
-        a.cols = p.cols;
-        a.col_blocks = p.col_blocks;
-        a.blocks = p.blocks;
-        a.chunk = p.chunk;
-        a.splits = p.splits;
-        a.part_rows = p.part_rows;
-        a.part_seq = p.part_seq;
-        a.part_o = (float*)ws_dev;
-        a.part_ml = a.part_o + p.parts * kv->head_dim;
-        a.ends = (AttnEnd*)(a.part_ml + p.parts * 2);
-        WPCG_HIP(p.many ? launch_attn_many(a, d, att->dtype, kv->dtype, s)
-                        : launch_attn_few(a, d, att->dtype, kv->dtype, s));
-    }
+    if (!plan.shared) return run_plans(a, plan.plain, kv, att, ws_dev, s);
+    PrefixArgs& p = plan.args;
+    a.cols = p.a.cols;
+    a.col_blocks = p.a.col_blocks;
+    a.chunk = p.a.chunk;
+    a.splits = p.a.splits;
+    a.part_rows = p.a.part_rows;
+    a.part_o = (float*)ws_dev;
+    p.pre_o = a.part_o + plan.own_parts * kv->head_dim;
+    a.part_ml = p.pre_o + plan.pre_parts * kv->head_dim;
+    p.pre_ml = a.part_ml + plan.own_parts * 2;
+    p.a = a;
+    p.group_start = prefix->group_start_dev;
+    p.prefix_len = prefix->prefix_len_dev;
+    WPCG_HIP(launch_attn_prefix(p, (int)kv->head_dim, att->dtype, kv->dtype, s));
     return WPCG_OK;
 }
 

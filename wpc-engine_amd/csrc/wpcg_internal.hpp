@@ -540,6 +540,20 @@ struct PagedAttnArgs {
 hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 
+// Attention whose sequences share prefixes in groups (attn_prefix.hip): `a` has the
+// batch and the part of the sequences' own tokens, in parts as few rows leave them.
+// Prefixes are read in chunks of `chunk` many-row tiles, `splits` at most, by
+// `blocks` workgroups a key-value head and chunk, whose parts lie by row:
+// (i * n_rows + row) * n_heads + head.
+struct PrefixArgs {
+    PagedAttnArgs a;
+    int n_groups, max_prefix;
+    const int32_t *group_start, *prefix_len;
+    int chunk, splits, blocks;
+    float *pre_o, *pre_ml;
+};
+hipError_t launch_attn_prefix(const PrefixArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
+
 // ---- verification of drafts (draft.hip) -------------------------------------
 // A chunk's state of a row: sum of exp((x - max) / T), the largest logit and
 // (greedy rows) its first place; and a sequence's count of finished workgroups.

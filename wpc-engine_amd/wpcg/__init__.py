@@ -150,6 +150,8 @@ _SIGS = {
     "wpcg_paged_attention": (C.c_int, [_p, _p, _p, _p, _p, _u64, _p]),
     "wpcg_draft_verify_workspace": (C.c_int, [_p, _u64p]),
     "wpcg_draft_verify": (C.c_int, [_p, _p, _p, _u64, _p]),
+    "wpcg_prefix_attention_workspace": (C.c_int, [_p, _p, _p, _p, _u64p]),
+    "wpcg_prefix_attention": (C.c_int, [_p, _p, _p, _p, _p, _p, _u64, _p]),
     "wpcg_kv_fork_workspace": (C.c_int, [_p, _u64p]),
     "wpcg_kv_fork": (C.c_int, [_p, _p, _p, _p, _u64, _p]),
     "wpcg_kv_compact_workspace": (C.c_int, [_p, _u64p]),
@@ -799,6 +801,10 @@ class _Draft(C.Structure):
                 ("tokens", _p), ("u", _p), ("u_next", _p), ("temperature", _p), ("accepted", _p), ("out", _p)]
 
 
+class _KvPrefix(C.Structure):
+    _fields_ = [("n_groups", C.c_uint32), ("max_prefix", C.c_uint32), ("group_start", _p), ("prefix_len", _p)]
+
+
 class _KvPool(C.Structure):
     _fields_ = [("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_seq", C.c_uint32), ("table_stride", C.c_uint32),
                 ("refs", _p), ("table", _p), ("kv_len", _p)]
@@ -917,6 +923,41 @@ class DraftVerify:
         d.logits, d.tokens, d.u, d.u_next = _ptr(logits), _ptr(tokens), _ptr(u), _ptr(u_next)
         d.accepted, d.out, d.draft_probs = _ptr(accepted), _ptr(out), _ptr(draft_probs)
         check(lib.wpcg_draft_verify(self.ctx.h, self._ref, _ptr(self.workspace), self.workspace_bytes, stream))
+
+
+class KvPrefix:
+    """The groups of a batch whose sequences share their first tokens
+    (wpcg_kv_prefix): device arrays group_start int32[n_groups + 1] and prefix_len
+    int32[n_groups], whose contents may change between the calls; max_prefix
+    bounds the lengths."""
+
+    def __init__(self, n_groups: int, group_start, prefix_len, max_prefix: int):
+        self.group_start, self.prefix_len = group_start, prefix_len
+        self.desc = _KvPrefix(n_groups, max_prefix, _ptr(group_start), _ptr(prefix_len))
+
+
+class PrefixAttention:
+    """PagedAttention that reads a group's prefix once for its sequences
+    (wpcg_prefix_attention), with a workspace of its own: calls of one object
+    must not overlap."""
+
+    def __init__(self, ctx: Context, kv: PagedKv, batch: KvBatch, prefix: KvPrefix, n_heads: int, dtype: int = DTYPE_F32,
+                 scale: float | None = None, window: int = 0, sinks: int = 0, q_stride: int = 0,
+                 out_stride: int = 0):
+        self.ctx, self.kv, self.batch, self.prefix = ctx, kv, batch, prefix
+        if scale is None:
+            scale = float(kv.desc.head_dim) ** -0.5
+        self.desc = _Attention(None, None, dtype, n_heads, q_stride, out_stride, scale, window, sinks)
+        self._refs = (C.byref(kv.desc), C.byref(batch.desc), C.byref(prefix.desc), C.byref(self.desc))
+        n = C.c_uint64()
+        check(lib.wpcg_prefix_attention_workspace(*self._refs, C.byref(n)))
+        self.workspace_bytes = n.value
+        self.workspace = ctx.alloc(n.value) if n.value else None
+
+    def run(self, q, out, stream=None):
+        d = self.desc
+        d.q, d.out = _ptr(q), _ptr(out)
+        check(lib.wpcg_prefix_attention(self.ctx.h, *self._refs, _ptr(self.workspace), self.workspace_bytes, stream))
 
 
 class KvPool:
