@@ -259,6 +259,15 @@ def test_many_sequences(ctx):
     one(ctx, rng, [(70, [1 + i % 30 for i in range(1100)])], F32, BF16, 1, 2, 64, 16)
 
 
+@pytest.mark.parametrize("heads,hkv", [(4, 1), (3, 3), (10, 5), (8, 1)])
+def test_costs_that_are_rounded(ctx, heads, hkv):
+    """Prefixes of 1 to 12 tiles in few items, several groups behind each other."""
+    rng = np.random.default_rng(heads)
+    for most in (3, 6, 12):
+        groups = [(int(rng.integers(1, 32 * most)), [int(x) for x in rng.integers(1, 60, rng.integers(2, 5))]) for _ in range(12)]
+        one(ctx, rng, groups, BF16, BF16, hkv, heads, 64, 16)
+
+
 def test_graphs_and_streams(ctx):
     """Two captured calls in turn whose lengths, groups and queries change between
     the replays, and the same bits from another stream."""

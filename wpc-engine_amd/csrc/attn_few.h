@@ -11,7 +11,6 @@ namespace few {
 constexpr int WAVES = ATTN_FEW_WAVES;
 constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = ATTN_FEW_TILE;
-constexpr int SLOTS = 4;  // waves whose outputs lie in LDS at a time
 
 // Keys of 16 tokens as A fragments. BF16 and E4M3: D/32 fragments of 32
 // dimensions; lane (token, g) holds dimensions key_dim(f, g) + 0..7. F32:
@@ -155,9 +154,11 @@ __device__ __forceinline__ void add_values(const Values<D, CT>& v, const pbf16x8
     }
 }
 
-// What a workgroup shares.
-template <int D, int CT, bool QF32, int NB>
+// What a workgroup of W waves shares.
+template <int D, int CT, bool QF32, int NB, int W = ATTN_FEW_WAVES>
 struct Shared {
+    static constexpr int WAVES = W, THREADS = 64 * W;
+    static constexpr int SLOTS = W / 2;  // waves whose outputs lie in LDS at a time
     static constexpr bool F32MM = CT == CT_F32;  // the fp32 matrix cores
     static constexpr int QF = F32MM ? D / 16 : D / 32, QT = F32MM || !QF32 ? 1 : 3;  // q's fragments and their terms
     float o[SLOTS][16 * NB][D + 4];
@@ -181,12 +182,14 @@ struct Whole {
 // at part_o, [column][2] maximum and sum at part_ml. `of` may narrow the tokens
 // that are taken (takes, clip) and say where its columns are (position, whole),
 // which then are no one sequence's.
-template <int D, int CT, bool QF32, int NB, class OF = Whole, class SEEN = SeenTiles<TILE>>
-__device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF32, NB>& sh, const SeqRows& sq, int seq,
+template <int D, int CT, bool QF32, int NB, int W = ATTN_FEW_WAVES, class OF = Whole,
+          class SEEN = SeenTiles<TILE>>
+__device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF32, NB, W>& sh, const SeqRows& sq, int seq,
                                        int kvh, int cb, const SEEN& seen, int v0, int v1, float* part_o,
                                        float* part_ml, const OF& of = OF())
 {
-    using Sh = Shared<D, CT, QF32, NB>;
+    using Sh = Shared<D, CT, QF32, NB, W>;
+    constexpr int WAVES = Sh::WAVES, THREADS = Sh::THREADS, SLOTS = Sh::SLOTS;
     constexpr bool F32MM = Sh::F32MM;
     constexpr int NT = QF32 ? 3 : 1;  // bf16 terms of q and of the softmax's terms
     constexpr int DV = D / 16;

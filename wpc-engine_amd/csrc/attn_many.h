@@ -427,6 +427,30 @@ __device__ __forceinline__ void put_out(const PagedAttnArgs& p, const SeqRows& s
     }
 }
 
+// Its part, as column `col` of a workgroup's.
+template <int D, int CW>
+__device__ __forceinline__ void put_part(float* part_o, float* part_ml, int col, float m, float l,
+                                         const pf32x16 (&acc)[D / 32])
+{
+    constexpr int NCH = D / CW;
+    const int h = ((int)threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int a0 = 0; a0 < NCH / 8; a0++)
+#pragma unroll
+        for (int b0 = 0; b0 < 4; b0++)
+#pragma unroll
+            for (int j = 0; j < CW; j += 4) {
+                float o[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = acc[(j + i) * NCH / 32][4 * ((j + i) * NCH % 32 / 8 + a0) + b0];
+                *(pf32x4*)(part_o + col * D + CW * (8 * a0 + 4 * h + b0) + j) = (pf32x4){o[0], o[1], o[2], o[3]};
+            }
+    if (h == 0) {
+        part_ml[col * 2] = m;
+        part_ml[col * 2 + 1] = l;
+    }
+}
+
 // acc += a b over their bf16 terms, small products first; of two three-term
 // numbers the products below 2^-24 of the first are left out.
 template <int NA, int NB>
@@ -549,7 +573,7 @@ struct Shared {
 };
 
 // Four waves' 128 columns over the tiles of w: outputs, or parts. COLUMNS says
-// whose a wave's are and what they see; with LIMIT always parts.
+// whose a wave's are and what they see; with LIMIT parts, where w says.
 template <int D, int CT, bool QF32, class COLUMNS, class WORK>
 __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF32>& sh, const WORK& w)
 {
@@ -654,8 +678,11 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
     if (!live) return;
     l = sum_x32(l);
     if (sh.fault) l = __builtin_nanf("");
-    put_out<D, S::CW, QF32>(p, sq, w.seq, COLUMNS::LIMIT || (p.splits > 1 && seen.total() > p.chunk), w.split, row, head, m, l, acc,
-                            p.v_scale ? p.v_scale[kvh] : 1.0f);
+    if constexpr (COLUMNS::LIMIT)
+        put_part<D, S::CW>(w.part_o, w.part_ml, 32 * wave + c, m, l, acc);
+    else
+        put_out<D, S::CW, QF32>(p, sq, w.seq, p.splits > 1 && seen.total() > p.chunk, w.split, row, head, m, l, acc,
+                                p.v_scale ? p.v_scale[kvh] : 1.0f);
 }
 
 }  // namespace many

@@ -257,13 +257,12 @@ int plan_attention(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_atte
     return WPCG_OK;
 }
 
-// A batch whose groups share prefixes: how those are read, and the plans of the
-// batch without sharing, where that is what it takes.
+// A batch whose groups share prefixes: how the tiles are dealt out, and the plans
+// of the batch without sharing, where that is what it takes.
 struct PrefixPlan {
     bool shared;
     Plans plain;
-    PrefixArgs args;  // chunks, splits, blocks and columns
-    uint64_t pre_parts, own_parts;
+    PrefixArgs args;  // its weights, chunks, blocks, columns and places for parts
     uint64_t bytes;
 };
 int plan_prefix(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_kv_prefix* x, const wpcg_attention* a,
@@ -271,36 +270,35 @@ int plan_prefix(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_kv_pref
 {
     PrefixPlan& o = *out;
     o = {};
-    const int64_t group = a->n_heads / kv->n_kv_heads, cols = (int64_t)b.max_q * group;
-    const int64_t max_prefix = std::min<int64_t>(x->max_prefix, b.max_kv);
-    o.shared = b.n_rows > 0 && cols <= 2 * ATTN_FEW_COLS && x->n_groups > 0 && (int)x->n_groups < b.n_seq && max_prefix > 0;
+    const int64_t group = a->n_heads / kv->n_kv_heads, cols = (int64_t)b.max_q * group, n_kv = kv->n_kv_heads;
+    const int64_t max_prefix = std::min<int64_t>(x->max_prefix, b.max_kv), groups = x->n_groups;
+    const int64_t rows = std::min<int64_t>(b.n_rows, (int64_t)b.n_seq * b.max_q);
+    const int64_t cw = ATTN_MANY_COLS, tiles = (max_prefix + ATTN_MANY_TILE - 1) / ATTN_MANY_TILE;
+    const int64_t blocks = std::min(groups * ((rows * group + cw - 1) / cw), rows * group / cw + groups);
+    const int64_t own_cols = cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
+    const int64_t own_blocks = (cols + own_cols - 1) / own_cols, own_tiles = (b.max_kv + ATTN_FEW_TILE - 1) / ATTN_FEW_TILE;
+    PrefixArgs& p = o.args;
+    p.chunk = 64;
+    const int64_t chunks = (tiles + p.chunk - 1) / p.chunk;
+    const double cost = (double)n_kv * (blocks * (tiles + chunks * PREFIX_ITEM) +
+                                        b.n_seq * own_blocks * (own_tiles + OWN_ITEM));
+    o.shared = rows > 0 && cols <= 2 * ATTN_FEW_COLS && groups > 0 && groups < b.n_seq && groups <= PREFIX_GROUPS &&
+               b.n_seq <= PREFIX_SEQS && max_prefix > 0 && cost < (double)(1 << 30);
     if (!o.shared) {
         if (int rc = plan_attention(kv, b, a, &o.plain)) return rc;
         o.bytes = o.plain.bytes;
         return WPCG_OK;
     }
-    PrefixArgs& p = o.args;
-    p.n_groups = (int)x->n_groups;
+    p.n_groups = (int)groups;
     p.max_prefix = (int)max_prefix;
-    const int64_t cw = ATTN_MANY_COLS, tiles = (max_prefix + ATTN_MANY_TILE - 1) / ATTN_MANY_TILE;
-    const int64_t blocks = std::min(x->n_groups * ((b.n_rows * group + cw - 1) / cw), b.n_rows * group / cw + x->n_groups);
-    const int64_t room = a->dtype == WPCG_DTYPE_BF16 ? 2 * CUS : CUS;
-    const int64_t splits = std::max<int64_t>(1, std::min(room / std::max<int64_t>(1, blocks * kv->n_kv_heads), tiles / 2));
-    p.chunk = (int)((tiles + splits - 1) / splits);
-    p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
-    p.blocks = (int)blocks;
-    const int64_t own = (b.max_kv + ATTN_FEW_TILE - 1) / ATTN_FEW_TILE;
-    p.a.cols = cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
-    p.a.col_blocks = (int)((cols + p.a.cols - 1) / p.a.cols);
-    p.a.chunk = (int)std::max<int64_t>(32, (own + 15) / 16);
-    p.a.splits = (int)((own + p.a.chunk - 1) / p.a.chunk);
-    p.a.part_rows = b.n_rows;
-    const int64_t items = (int64_t)b.n_seq * kv->n_kv_heads * p.a.col_blocks * p.a.splits;
-    if (items >= GROUPS_512 || blocks * kv->n_kv_heads * p.splits >= GROUPS_512)
-        return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
-    o.pre_parts = (uint64_t)p.splits * b.n_rows * a->n_heads;
-    o.own_parts = (uint64_t)items * p.a.cols;
-    o.bytes = (o.pre_parts + o.own_parts) * (kv->head_dim + 2) * sizeof(float);
+    p.pre_weight = 2;
+    p.own_weight = 1;
+    p.a.blocks = a->dtype == WPCG_DTYPE_BF16 ? 2 * CUS : CUS;
+    p.a.cols = (int)own_cols;
+    p.pre_slots = (uint64_t)(n_kv * blocks * chunks + p.a.blocks);
+    p.own_slots = (uint64_t)(n_kv * own_blocks * b.n_seq + p.a.blocks);
+    o.bytes = (p.pre_slots * cw + p.own_slots * own_cols) * (kv->head_dim + 2) * sizeof(float) +
+              (groups + b.n_seq + 1) * sizeof(int2) + groups * sizeof(int) + sizeof(PrefixDeal);
     return WPCG_OK;
 }
 
@@ -624,15 +622,16 @@ int wpcg_prefix_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_
     const hipStream_t s = pick(ctx, stream);
     if (!plan.shared) return run_plans(a, plan.plain, kv, att, ws_dev, s);
     PrefixArgs& p = plan.args;
+    const uint64_t d = kv->head_dim, own = p.own_slots * p.a.cols, pre = p.pre_slots * ATTN_MANY_COLS;
     a.cols = p.a.cols;
-    a.col_blocks = p.a.col_blocks;
-    a.chunk = p.a.chunk;
-    a.splits = p.a.splits;
-    a.part_rows = p.a.part_rows;
+    a.blocks = p.a.blocks;
     a.part_o = (float*)ws_dev;
-    p.pre_o = a.part_o + plan.own_parts * kv->head_dim;
-    a.part_ml = p.pre_o + plan.pre_parts * kv->head_dim;
-    p.pre_ml = a.part_ml + plan.own_parts * 2;
+    p.pre_o = a.part_o + own * d;
+    a.part_ml = p.pre_o + pre * d;
+    p.pre_ml = a.part_ml + own * 2;
+    p.at = (int2*)(p.pre_ml + pre * 2);
+    p.tiles = (int*)(p.at + p.n_groups + a.b.n_seq + 1);
+    p.deal = (PrefixDeal*)(p.tiles + p.n_groups);
     p.a = a;
     p.group_start = prefix->group_start_dev;
     p.prefix_len = prefix->prefix_len_dev;

@@ -540,17 +540,29 @@ struct PagedAttnArgs {
 hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 
-// Attention whose sequences share prefixes in groups (attn_prefix.hip): `a` has the
-// batch and the part of the sequences' own tokens, in parts as few rows leave them.
-// Prefixes are read in chunks of `chunk` many-row tiles, `splits` at most, by
-// `blocks` workgroups a key-value head and chunk, whose parts lie by row:
-// (i * n_rows + row) * n_heads + head.
+// Attention whose sequences share prefixes in groups (attn_prefix.hip): a.blocks
+// workgroups, a multiple of 8, share the tiles: prefixes in tiles and columns of the
+// many rows, own tokens in those of few (a.cols). What an item costs to begin and
+// end, in its tiles: PREFIX_ITEM, OWN_ITEM; what a tile takes against the other kind's:
+// pre_weight, own_weight. A prefix's column blocks are taken by chunks of `chunk`
+// tiles. A part that a workgroup leaves is that of an item, numbered through, at place
+// item + workgroup: of prefixes at pre_o and pre_ml, of own tokens at a.part_o and
+// a.part_ml, as few rows leave them. at, tiles and deal: for the join.
+constexpr int PREFIX_SEQS = 512, PREFIX_GROUPS = 256;
+constexpr int PREFIX_ITEM = 3, OWN_ITEM = 6;
+struct PrefixDeal {
+    int pre, pre_share, own_share;  // workgroups of a die that take prefixes; tiles of one
+};
 struct PrefixArgs {
     PagedAttnArgs a;
     int n_groups, max_prefix;
     const int32_t *group_start, *prefix_len;
-    int chunk, splits, blocks;
+    int chunk, pre_weight, own_weight;
+    uint64_t pre_slots, own_slots;
     float *pre_o, *pre_ml;
+    int2* at;    // [n_groups + n_seq + 1] cost and items before the groups and sequences
+    int* tiles;  // [n_groups] of a prefix
+    PrefixDeal* deal;
 };
 hipError_t launch_attn_prefix(const PrefixArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 
