@@ -218,12 +218,19 @@ def test_prefix_refusals(kv, b, x, a, code, text):
 
 
 def test_prefix_workspace():
-    n = attend_ws(pages(), batch(), prefix(), attention())
+    # sharing pays where many bytes would be read again
+    b, x = batch(n_seq=64, n_rows=64, max_q=1, max_kv=10000, table_stride=1000), prefix(n_groups=1, max_prefix=9000)
+    n = attend_ws(pages(), b, x, attention())
     assert n > 0 and n % 4 == 0
-    refused(attend(pages(), batch(), prefix(), attention(), n=n - 1), E_ARG, "bytes of workspace")
-    refused(attend(pages(), batch(), prefix(), attention(), ws=None, n=0), E_ARG, "bytes of workspace")
-    refused(attend(pages(), batch(), prefix(), attention(), ws=AT + 4), E_ARG, "aligned")
+    refused(attend(pages(), b, x, attention(), n=n - 1), E_ARG, "bytes of workspace")
+    refused(attend(pages(), b, x, attention(), ws=None, n=0), E_ARG, "bytes of workspace")
+    refused(attend(pages(), b, x, attention(), ws=AT + 4), E_ARG, "aligned")
+    refused(attend(pages(), b, x, attention(), n=n), E_ARG, "null context")
     # without sharing that of the plain call
-    for x in (prefix(n_groups=0), prefix(max_prefix=0), prefix(n_groups=3)):
-        assert attend_ws(pages(), batch(), x, attention()) == 0
+    plain = C.c_uint64()
+    assert wpcg.lib.wpcg_paged_attention_workspace(ref(pages()), ref(b), ref(attention()), C.byref(plain)) == OK
+    for y in (prefix(n_groups=0), prefix(max_prefix=0), prefix(n_groups=64, max_prefix=9000), prefix(n_groups=1, max_prefix=500)):
+        assert attend_ws(pages(), b, y, attention()) == plain.value
     assert ATTEND_WS(ref(pages()), ref(batch()), ref(prefix()), ref(attention()), None) == E_ARG
+    # the parts' places hold whatever the bounds allow, loose rows too
+    assert attend_ws(pages(), batch(n_seq=64, n_rows=1 << 20, max_q=1, max_kv=10000, table_stride=1000), x, attention()) == n

@@ -22,10 +22,16 @@ def ctx():
 
 
 class Groups:
-    """A batch whose groups share: groups = [(prefix, [own tokens of each sequence])]."""
+    """A batch whose groups share: groups = [(prefix, [own tokens of each sequence])].
+    loose: a length by whose bounds the prefixes would be long enough (900 MB read
+    again) for sharing to be chosen."""
 
     def __init__(self, ctx, rng, groups, dtype, hkv, d, page, order="head", width=0):
         self.ctx, self.groups = ctx, groups
+        again = max(1, sum(len(own) - 1 for _, own in groups)) * 2 * hkv * d * R.SIZE[dtype]
+        self.loose = max(width * page, -(-int(900e6) // again // page) * page,
+                         max(p + max(own) for p, own in groups) // page * page + page)
+        width = self.loose // page
         self.size = [len(own) for _, own in groups]
         self.prefix = [p for p, _ in groups]
         lens = [p + m for p, own in groups for m in own]
@@ -43,12 +49,15 @@ class Groups:
                         pg.bits[n][pg.index(s, rest)] = pg.bits[n][pg.index(lead, rest)]
         pg.upload()
 
+    def batch(self, rows, **kw):
+        return self.pg.batch(rows, **{"max_kv": self.loose, **kw})
+
     def desc(self, max_prefix=None, start=None, prefix=None):
         self.d_start = self.ctx.upload(np.asarray(self.start if start is None else start, np.int32))
         prefix = self.prefix if prefix is None else prefix
         self.d_prefix = self.ctx.upload(np.asarray(prefix, np.int32))
         return wpcg.KvPrefix(len(prefix), self.d_start, self.d_prefix,
-                             max(max(self.prefix), 1) if max_prefix is None else max_prefix)
+                             self.loose if max_prefix is None else max_prefix)
 
 
 def expected(pg, q, rows, q_dtype, scale, window, sinks):
@@ -76,6 +85,7 @@ def run(ctx, pg, batch, prefix, q, heads, q_dtype, scale, window=0, sinks=0, str
     out = ctx.upload(np.full(rows * heads * pg.d * R.SIZE[q_dtype], 0x5A, np.uint8))
     qd = ctx.upload(q)
     op = wpcg.PrefixAttention(ctx, pg.kv, batch, prefix, heads, q_dtype, scale=scale, window=window, sinks=sinks)
+    run.workspace = op.workspace_bytes
     if op.workspace is not None:
         op.workspace.write(np.full(op.workspace_bytes, 0xFF, np.uint8))
     op.run(qd, out, stream)
@@ -89,10 +99,16 @@ def one(ctx, rng, groups, q_dtype, dtype, hkv, heads, d, page, rows=1, window=0,
     per = [rows] * n if np.isscalar(rows) else rows
     q = R.encode(rng.standard_normal((sum(per), heads, d)) * 1.5, q_dtype)
     scale = d ** -0.5
-    batch = g.pg.batch(None if null_start else per)
-    got = run(ctx, g.pg, batch, g.desc(), q, heads, q_dtype, scale, window, sinks)
     want, bound = expected(g.pg, q, per, q_dtype, scale, window, sinks)
+    # as the tight bounds have it, then shared
+    check(run(ctx, g.pg, g.pg.batch(None if null_start else per), g.desc(max_prefix=max([1] + g.prefix)),
+              q, heads, q_dtype, scale, window, sinks), want, bound)
+    batch = g.batch(None if null_start else per)
+    got = run(ctx, g.pg, batch, g.desc(), q, heads, q_dtype, scale, window, sinks)
     check(got, want, bound)
+    plain = wpcg.PagedAttention(ctx, g.pg.kv, batch, heads, q_dtype, scale=scale, window=window, sinks=sinks)
+    few = max(per) * heads // hkv <= 32 and n <= 512 and len(groups) <= 256 and n > len(groups)
+    assert (run.workspace != plain.workspace_bytes) == few
     return g, batch, q, got, want, bound
 
 
@@ -152,10 +168,10 @@ def test_bounds_that_are_loose(ctx, q_dtype, dtype):
     """More rows, tokens and prefix by the bounds than there are; rows of no
     sequence as they were."""
     rng = np.random.default_rng(4 + dtype)
-    g = Groups(ctx, rng, [(150, [4, 30, 9]), (20, [8, 8])], dtype, 2, 64, 16, width=7000)
+    g = Groups(ctx, rng, [(150, [4, 30, 9]), (20, [8, 8])], dtype, 2, 64, 16)
     q = R.encode(rng.standard_normal((5 + 20, 6, 64)), q_dtype)
-    batch = g.pg.batch([1] * 5, n_rows=25, max_kv=110000, max_q=3)
-    got = run(ctx, g.pg, batch, g.desc(max_prefix=100000), q, 6, q_dtype, 0.2)
+    batch = g.batch([1] * 5, n_rows=25, max_q=3)
+    got = run(ctx, g.pg, batch, g.desc(), q, 6, q_dtype, 0.2)
     check(got[:5], *expected(g.pg, q[:5], [1] * 5, q_dtype, 0.2, 0, 0))
     assert (got[5:] == R.decode(np.full(1, 0x5A5A if q_dtype == BF16 else 0x5A5A5A5A, R.BITS[q_dtype]), q_dtype)[0]).all()
 
@@ -167,13 +183,13 @@ def test_groups_that_are_none(ctx, q_dtype, dtype):
     rng = np.random.default_rng(5)
     g = Groups(ctx, rng, [(150, [4, 30, 9]), (70, [8, 8]), (33, [1, 2])], dtype, 2, 64, 16)
     q = R.encode(rng.standard_normal((7, 8, 64)), q_dtype)
-    batch = g.pg.batch([1] * 7)
+    batch = g.batch([1] * 7)
     want = expected(g.pg, q, [1] * 7, q_dtype, 0.125, 0, 0)
-    for start, prefix, most in (([0, 3, 5, 7], [-5, 70, -2 ** 31], 150), ([0, 3, 5, 7], [150, 70, 33], 60),
-                                ([0, 3, 5, 7], [150, 70, 33], 0), ([-1, 3, 5, 7], [150, 70, 33], 150),
-                                ([0, 3, 5, 8], [150, 70, 33], 150), ([0, 3, 5, 2 ** 31 - 1], [150, 70, 33], 150),
-                                ([0, 3, 3, 5, 7], [150, 9, 70, 33], 150), ([1, 3, 4, 6], [150, 70, 0], 150),
-                                ([3, 5], [70], 150)):
+    for start, prefix, most in (([0, 3, 5, 7], [-5, 70, -2 ** 31], g.loose), ([0, 3, 5, 7], [150, 70, 33], 60),
+                                ([0, 3, 5, 7], [150, 70, 33], 0), ([-1, 3, 5, 7], [150, 70, 33], g.loose),
+                                ([0, 3, 5, 8], [150, 70, 33], g.loose), ([0, 3, 5, 2 ** 31 - 1], [150, 70, 33], g.loose),
+                                ([0, 3, 3, 5, 7], [150, 9, 70, 33], g.loose), ([1, 3, 4, 6], [150, 70, 0], g.loose),
+                                ([3, 5], [70], g.loose)):
         check(run(ctx, g.pg, batch, g.desc(max_prefix=most, start=start, prefix=prefix), q, 8, q_dtype, 0.125), *want)
     none = wpcg.KvPrefix(0, None, None, 100)
     check(run(ctx, g.pg, batch, none, q, 8, q_dtype, 0.125), *want)
@@ -192,7 +208,7 @@ def test_lengths_and_pages_that_are_none(ctx, q_dtype, dtype):
         pg.d_len.write(np.asarray(lens, np.int32))
         pg.d_table.write(table)
         return run(ctx, pg, batch, prefix, q, 8, q_dtype, 0.125)
-    for bad in (-1, 10 ** 6, 2 ** 31 - 1, -2 ** 31):
+    for bad in (-1, g.loose + 1, 2 ** 31 - 1, -2 ** 31):
         for s in (0, 4):
             got = again([bad if i == s else m for i, m in enumerate(pg.kv_len)], pg.table)
             assert np.isnan(got[s]).all()
@@ -218,7 +234,7 @@ def test_values_that_are_not_finite(ctx, q_dtype, dtype):
     g = Groups(ctx, rng, [(100, [3, 60, 90]), (64, [5, 80])], dtype, 1, 64, 16)
     pg = g.pg
     q = R.encode(rng.standard_normal((5, 4, 64)), q_dtype)
-    batch = pg.batch([1] * 5)
+    batch = g.batch([1] * 5)
     want, bound = expected(pg, q, [1] * 5, q_dtype, 0.125, 70, 2)
     words = {F32: (0x7F800000, 0xFF800000, 0x7FC00000), BF16: (0x7F80, 0xFF80, 0x7FC0)}[dtype]
     # the row of sequence 0 (103 tokens) sees the prefix from 33 on, those of 1 and 2 from 90 and not at all
@@ -254,9 +270,12 @@ def test_many_sequences(ctx):
     groups than a wave looks through at once."""
     rng = np.random.default_rng(9)
     groups = [(int(rng.integers(0, 90)), [int(x) for x in rng.integers(1, 40, rng.integers(1, 9))]) for _ in range(150)]
-    one(ctx, rng, groups, BF16, BF16, 1, 4, 64, 16)
-    one(ctx, rng, [(40, [2] * 600)], BF16, E4M3, 1, 4, 64, 16)
-    one(ctx, rng, [(70, [1 + i % 30 for i in range(1100)])], F32, BF16, 1, 2, 64, 16)
+    one(ctx, rng, groups[:100], BF16, BF16, 1, 4, 64, 16)
+    one(ctx, rng, [(int(rng.integers(0, 90)), [1, 20]) for _ in range(256)], BF16, E4M3, 1, 4, 64, 16)
+    one(ctx, rng, [(40, [2] * 512)], BF16, E4M3, 1, 4, 64, 16)
+    one(ctx, rng, [(200, [1 + i % 30 for i in range(511)])], F32, BF16, 1, 2, 64, 16)
+    one(ctx, rng, groups, F32, F32, 1, 4, 64, 16)  # more than are shared
+    one(ctx, rng, [(40, [2] * 513)], BF16, BF16, 1, 4, 64, 16)
 
 
 @pytest.mark.parametrize("heads,hkv", [(4, 1), (3, 3), (10, 5), (8, 1)])
@@ -277,7 +296,7 @@ def test_graphs_and_streams(ctx):
     for groups, dtype in (([(400, [60] * 7), (90, [60] * 3)], BF16), ([(64, [40] * 4)], F32)):
         g = Groups(ctx, rng, groups, dtype, 2, 128, 16)
         n = len(g.pg.kv_len)
-        batch, prefix = g.pg.batch([1] * n), g.desc()
+        batch, prefix = g.batch([1] * n), g.desc()
         q, out = ctx.alloc(n * 8 * 128 * R.SIZE[dtype]), ctx.alloc(n * 8 * 128 * R.SIZE[dtype])
         op = wpcg.PrefixAttention(ctx, g.pg.kv, batch, prefix, 8, dtype, scale=0.1)
         made.append((g, dtype, n, q, out, ctx.capture(lambda op=op, q=q, out=out: op.run(q, out)), op, batch))

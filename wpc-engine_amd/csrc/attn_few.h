@@ -154,14 +154,14 @@ __device__ __forceinline__ void add_values(const Values<D, CT>& v, const pbf16x8
     }
 }
 
-// What a workgroup of W waves shares.
+// What a workgroup of W waves shares; with W = 1 a wave's own.
 template <int D, int CT, bool QF32, int NB, int W = ATTN_FEW_WAVES>
 struct Shared {
     static constexpr int WAVES = W, THREADS = 64 * W;
-    static constexpr int SLOTS = W / 2;  // waves whose outputs lie in LDS at a time
+    static constexpr int SLOTS = W > 1 ? W / 2 : 1;  // waves whose outputs lie in LDS at a time
     static constexpr bool F32MM = CT == CT_F32;  // the fp32 matrix cores
     static constexpr int QF = F32MM ? D / 16 : D / 32, QT = F32MM || !QF32 ? 1 : 3;  // q's fragments and their terms
-    float o[SLOTS][16 * NB][D + 4];
+    float o[SLOTS][W > 1 ? 16 * NB : 1][D + 4];
     float ml[WAVES][16 * NB][2];
     pu32x4 q[NB][QF][QT][64];
     uint64_t place[WAVES][64];
@@ -181,7 +181,8 @@ struct Whole {
 // that is all of them the outputs, else their part: [column][D] unnormalised
 // at part_o, [column][2] maximum and sum at part_ml. `of` may narrow the tokens
 // that are taken (takes, clip) and say where its columns are (position, whole),
-// which then are no one sequence's.
+// which then are no one sequence's. W = 1: by one wave of several that go their own
+// ways.
 template <int D, int CT, bool QF32, int NB, int W = ATTN_FEW_WAVES, class OF = Whole,
           class SEEN = SeenTiles<TILE>>
 __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF32, NB, W>& sh, const SeqRows& sq, int seq,
@@ -200,7 +201,7 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
     auto& s_ml = sh.ml;
     auto& s_q = sh.q;
     const int cols = sq.n * p.group;  // of this sequence and head
-    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lane = (int)threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int len = sq.bad ? 0 : sq.len;
     const int pos0 = len - sq.n;  // position of the sequence's row 0
@@ -307,7 +308,8 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
     }
 
     const float sc = p.scale * (p.k_scale ? p.k_scale[kvh] : 1.0f);
-    __syncthreads();
+    if constexpr (W > 1) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (LDS does a wave's operations in their order)
 
     pf32x4 acc[NB][DV] = {};
     float m[NB], l[NB];
@@ -443,7 +445,8 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
                 if constexpr (QF32) {
                     uint32_t t[4][3];
 #pragma unroll
-                    for (int x = 0; x < 4; x++) split3(e[2 * x], e[2 * x + 1], t[x]);
+                    for (int x = 0; x < 4; x++)
+                        OF::PART ? split3_finite(e[2 * x], e[2 * x + 1], t[x]) : split3(e[2 * x], e[2 * x + 1], t[x]);
 #pragma unroll
                     for (int k = 0; k < 3; k++)
                         b[k] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][k], t[1][k], t[2][k], t[3][k]});
@@ -477,11 +480,27 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
     for (int n = 0; n < NB; n++) {
         l[n] = sum_x16_32(l[n]);
         if (__any(fault)) l[n] = __builtin_nanf("");
+        if constexpr (W == 1) {
+            static_assert(W > 1 || OF::PART, "a wave leaves parts");
+            float* const to = part_o + (16 * n + c) * D;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < DV; j += 4)
+                    *(pf32x4*)(to + (4 * g + i) * DV + j) =
+                        (pf32x4){acc[n][j][i], acc[n][j + 1][i], acc[n][j + 2][i], acc[n][j + 3][i]};
+            if (g == 0) {
+                part_ml[(16 * n + c) * 2] = m[n];
+                part_ml[(16 * n + c) * 2 + 1] = l[n];
+            }
+            continue;
+        }
         if (g == 0) {
             s_ml[wave][16 * n + c][0] = m[n];
             s_ml[wave][16 * n + c][1] = l[n];
         }
     }
+    if constexpr (W == 1) return;
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NB; n++) {

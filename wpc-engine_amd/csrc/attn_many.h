@@ -375,8 +375,9 @@ __device__ __forceinline__ void load_q(const PagedAttnArgs& p, uint64_t at, bool
         }
     }
 }
-// Eight terms of a column (scores from s[i0] on) as a B fragment, added to l.
-template <int NQ>
+// Eight terms of a column (scores from s[i0] on) as a B fragment, added to l. FINITE:
+// an infinite term (of an infinite score) may be NaN.
+template <int NQ, bool FINITE = false>
 __device__ __forceinline__ void terms(const pf32x16& s, int i0, float sc, float base, float& l, pbf16x8 (&b)[NQ])
 {
     float e[8];
@@ -388,7 +389,7 @@ __device__ __forceinline__ void terms(const pf32x16& s, int i0, float sc, float 
     if constexpr (NQ == 3) {
         uint32_t t[4][3];
 #pragma unroll
-        for (int i = 0; i < 4; i++) split3(e[2 * i], e[2 * i + 1], t[i]);
+        for (int i = 0; i < 4; i++) FINITE ? split3_finite(e[2 * i], e[2 * i + 1], t[i]) : split3(e[2 * i], e[2 * i + 1], t[i]);
 #pragma unroll
         for (int n = 0; n < 3; n++) b[n] = __builtin_bit_cast(pbf16x8, (pu32x4){t[0][n], t[1][n], t[2][n], t[3][n]});
     } else {
@@ -597,8 +598,9 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
     __syncthreads();
     // q is there: else its first use in the loop would wait, every time
     // around, for all loads in flight
+    if (COLUMNS::LIMIT && v0 < v1) stage.fetch(v0);  // (few tiles: together with the first of them)
     __builtin_amdgcn_s_waitcnt(0);
-    if (v0 < v1) stage.fetch(v0);
+    if (!COLUMNS::LIMIT && v0 < v1) stage.fetch(v0);
     for (int vt = v0; vt < v1; vt++) {
         const int buf = (vt - v0) % S::NBUF;
         const bool all = stage.whole(vt);
@@ -657,12 +659,12 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
         if (t0 + TILE > my.hi || t0 < my.lo) mask<COLUMNS::LIMIT>(p, t0, pos, s, my.limit());
         const float base = follow(top_of(s) * sc, m, l, acc);
         pbf16x8 b[2][S::NQ];
-        terms<S::NQ>(s[0], 0, sc, base, l, b[0]);
+        terms<S::NQ, COLUMNS::LIMIT>(s[0], 0, sc, base, l, b[0]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (j < 3) load_values(j + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (j < 3) terms<S::NQ>(s[(j + 1) / 2], 8 * ((j + 1) % 2), sc, base, l, b[(j + 1) & 1]);
+            if (j < 3) terms<S::NQ, COLUMNS::LIMIT>(s[(j + 1) / 2], 8 * ((j + 1) % 2), sc, base, l, b[(j + 1) & 1]);
 #pragma unroll
             for (int d = 0; d < VF; d++) {
                 acc[d] = mul_terms(frag[j & 1][d], b[j & 1], acc[d]);

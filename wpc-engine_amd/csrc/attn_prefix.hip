@@ -7,16 +7,19 @@
 // The prefix of a group is read once for the rows of all its sequences, whose
 // (row, query head) pairs are the columns of the many-row kernel's workgroups
 // (attn_many.h), 128 at a time: what the memory bounds one sequence at a time, the
-// matrix cores do for many. Own tokens go through the few-row kernel's
-// (attn_few.h). Both are dealt out evenly, each over its workgroups of one launch,
-// which all fit on the chip at once: with BF16 queries two a CU, of which one as a
-// rule waits for the memory with own tokens while the other computes on a prefix.
-// Every piece of an item leaves its part, and a second launch joins them.
+// matrix cores do for many. Own tokens are single waves' work, a few tiles of a
+// sequence's key-value head each, by the few-row kernel's steps (attn_few.h) without
+// its barriers. All of it is one launch whose workgroups are on the chip together,
+// with BF16 queries two a CU: the first of them takes prefixes alone, the second
+// own tokens, which wait for the memory, and then what is left of its equal share
+// of the prefixes. Every piece leaves its part, and a second launch joins them.
 //
 // A CU gets some 20 GB/s from the memory, whatever it has in flight, and a few
 // times that from the L2. With prefixes in the few-row kernel's 32 columns, each
 // tile loaded for one wave, 8192 tokens shared by 64 rows of 32 / 4 heads took 45
-// us for that reason alone.
+// us for that reason alone. With own tokens in whole workgroups' items, dealt out
+// evenly beside the prefixes, each of them began and ended in 9 us, whatever its
+// tiles.
 #include "attn_few.h"
 #include "attn_many.h"
 
@@ -26,10 +29,10 @@ namespace {
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int PCOLS = ATTN_MANY_COLS;
 
-// The batch's row starts and lengths, in LDS, and the lowest and highest position
-// of a group's rows.
+// The batch in LDS: row starts and lengths, the groups' first sequences and prefix
+// lengths, the lowest and highest position of a group's rows.
 struct Batch {
-    const int *start, *len, *least, *most;
+    const int *start, *len, *group, *prefix, *least, *most;
 };
 __device__ __forceinline__ SeqRows rows_of(const PagedBatch& b, const Batch& x, int s)
 {
@@ -48,16 +51,16 @@ __device__ __forceinline__ Group group_of(const PrefixArgs& p, const Batch& x, i
 {
     const PagedBatch& b = p.a.b;
     Group r;
-    r.s0 = p.group_start[g];
-    const int s1 = p.group_start[g + 1];
+    r.s0 = x.group[g];
+    const int s1 = x.group[g + 1];
     const bool some = r.s0 >= 0 && r.s0 <= s1 - 2 && s1 <= b.n_seq;
     r.n = some ? s1 - r.s0 : 0;
-    r.a = b.q_start ? x.start[some ? r.s0 : 0] : r.s0;
-    const int end = b.q_start ? x.start[some ? s1 : 0] : s1;
+    r.a = x.start[some ? r.s0 : 0];
+    const int end = x.start[some ? s1 : 0];
     const bool rows = some && r.a >= 0 && r.a <= end && end <= b.n_rows && end - r.a <= (int64_t)r.n * b.max_q;
     // the pages are those of the first sequence, which has no more than its own
     const int len = x.len[some ? r.s0 : 0];
-    r.len = rows && len <= b.max_kv ? max(0, min(min(p.prefix_len[g], p.max_prefix), len)) : 0;
+    r.len = rows && len <= b.max_kv ? max(0, min(min(x.prefix[g], p.max_prefix), len)) : 0;
     r.rows = r.len > 0 ? end - r.a : 0;
     return r;
 }
@@ -67,7 +70,7 @@ __device__ __forceinline__ int group_with(const PrefixArgs& p, const Batch& x, i
     int lo = 0, hi = p.n_groups - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
-        if (p.group_start[mid] <= s) lo = mid;
+        if (x.group[mid] <= s) lo = mid;
         else hi = mid - 1;
     }
     g = group_of(p, x, lo);
@@ -175,79 +178,104 @@ __device__ __forceinline__ OwnTiles own_tiles(const PagedAttnArgs& p, const SeqR
 }
 
 // ---- the deal ------------------------------------------------------------------
-// Entries are the groups, then the sequences. A group's items are (key-value head,
-// chunk, column block), a sequence's (key-value head, column block): an order in
+// Prefixes: a group's items are (key-value head, chunk, column block), an order in
 // which neighbours read the same keys and values. An item costs its tiles and what
 // it takes to begin and end; a workgroup whose share of an item is no more than that
-// does nothing for it.
-//
-// What lies before entry e: at[e].x cost (sequences': behind all groups), at[e].y
-// items; tiles[g] of the groups.
-template <int OCOLS>
-__device__ __forceinline__ void deal(const PrefixArgs& p, const Batch& x, int2* at, int* tiles_of, int2* sums)
+// does nothing for it. Own tokens: a sequence's items are (key-value head, column
+// block, chunk of deal.own_chunk tiles), a wave's work each.
+struct Tables {
+    int2 at[PREFIX_GROUPS + 1];  // cost and items before a group
+    int tiles[PREFIX_GROUPS];    // of its prefix
+    int items[PREFIX_SEQS + 1];  // own items before a sequence
+};
+__device__ __forceinline__ int own_columns(const PagedAttnArgs& a, const SeqRows& sq, int cols)
 {
-    const PagedAttnArgs& a = p.a;
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const int entries = p.n_groups + a.b.n_seq;
-    int2 before = {0, 0};
-    for (int e0 = 0; e0 < entries; e0 += THREADS) {
-        const int e = e0 + (int)threadIdx.x;
-        int2 v = {0, 0};
-        if (e < p.n_groups) {
-            const Group g = group_of(p, x, e);
-            const int tiles = g.len > 0 ? prefix_tiles(a, g, x.least[e], x.most[e]).total() : 0;
-            const int cbs = (g.rows * a.group + PCOLS - 1) / PCOLS;
-            tiles_of[e] = tiles;
-            v.y = a.n_kv * cbs * ((tiles + p.chunk - 1) / p.chunk);
-            v.x = v.y * PREFIX_ITEM + a.n_kv * cbs * tiles;
-        } else if (e < entries) {
-            const int s = e - p.n_groups;
-            Group g;
-            group_with(p, x, s, g);
-            const SeqRows sq = rows_of(a.b, x, s);
-            const int tiles = own_tiles(a, sq, g.len).total();
-            v.y = tiles > 0 ? a.n_kv * ((sq.n * a.group + OCOLS - 1) / OCOLS) : 0;
-            v.x = v.y * (tiles + OWN_ITEM);
-        }
-        int2 t = v;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int ux = __shfl_up(t.x, d), uy = __shfl_up(t.y, d);
-            if (lane >= d) {
-                t.x += ux;
-                t.y += uy;
-            }
-        }
-        if (lane == 63) sums[wave] = t;
-        __syncthreads();
-        int2 all = {0, 0}, start = before;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            if (w < wave) {
-                start.x += sums[w].x;
-                start.y += sums[w].y;
-            }
-            all.x += sums[w].x;
-            all.y += sums[w].y;
-        }
-        if (e < entries) at[e] = {start.x + t.x - v.x, start.y + t.y - v.y};
-        before.x += all.x;
-        before.y += all.y;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) at[entries] = before;
-    __syncthreads();
+    return (sq.n * a.group + cols - 1) / cols;
 }
-// How many workgroups of each die's `blocks` take prefixes, and the shares.
-__device__ __forceinline__ PrefixDeal shares(const PrefixArgs& p, int pre, int own)
+// The sums over the threads before this one, and over all in total; s: WAVES int3s.
+__device__ __forceinline__ int wave_scan_i(int v)
 {
-    const int blocks = p.a.blocks / 8;
-    const double all = (double)pre * p.pre_weight + (double)own * p.own_weight;
+    v += wave_dpp_i<0x111>(0, v);  // lanes 1, 2, 4 and 8 before, in rows of 16
+    v += wave_dpp_i<0x112>(0, v);
+    v += wave_dpp_i<0x114>(0, v);
+    v += wave_dpp_i<0x118>(0, v);
+    v += wave_dpp_i<WDPP_BCAST15, 0xA>(0, v);
+    return v + wave_dpp_i<WDPP_BCAST31, 0xC>(0, v);
+}
+__device__ __forceinline__ int3 block_before(int3 v, int3* s, int3& total)
+{
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int3 t = {wave_scan_i(v.x), wave_scan_i(v.y), wave_scan_i(v.z)};
+    if (lane == 63) s[wave] = t;
+    __syncthreads();
+    int3 start = {0, 0, 0};
+    total = start;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        if (w == wave) start = total;
+        total = {total.x + s[w].x, total.y + s[w].y, total.z + s[w].z};
+    }
+    __syncthreads();
+    return {start.x + t.x - v.x, start.y + t.y - v.y, start.z + t.z - v.z};
+}
+template <int OCOLS>
+__device__ __forceinline__ PrefixDeal deal(const PrefixArgs& p, const Batch& x, Tables& t, int3* sums)
+{
+    static_assert(PREFIX_GROUPS <= THREADS && PREFIX_SEQS <= 2 * THREADS, "a group a thread, two sequences");
+    const PagedAttnArgs& a = p.a;
+    const int tid = (int)threadIdx.x;
+    int3 v = {0, 0, 0};  // cost and items of a group, own tiles of two sequences
+    if (tid < p.n_groups) {
+        const Group g = group_of(p, x, tid);
+        const int tiles = g.len > 0 ? prefix_tiles(a, g, x.least[tid], x.most[tid]).total() : 0;
+        const int cbs = (g.rows * a.group + PCOLS - 1) / PCOLS;
+        t.tiles[tid] = tiles;
+        v.y = a.n_kv * cbs * ((tiles + p.chunk - 1) / p.chunk);
+        v.x = v.y * PREFIX_ITEM + a.n_kv * cbs * tiles;
+    }
+    int tiles[2] = {0, 0}, cbs[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int s = 2 * tid + i;
+        if (s >= a.b.n_seq) continue;
+        Group g;
+        group_with(p, x, s, g);
+        const SeqRows sq = rows_of(a.b, x, s);
+        tiles[i] = own_tiles(a, sq, g.len).total();
+        cbs[i] = a.n_kv * own_columns(a, sq, OCOLS);
+        v.z += tiles[i] * cbs[i];
+    }
+    int3 total, none;
+    const int3 before = block_before(v, sums, total);
+    if (tid < p.n_groups) t.at[tid] = {before.x, before.y};
+    if (tid == 0) t.at[p.n_groups] = {total.x, total.y};
+    const int pre = uniform(total.x), own = uniform(total.z);
     PrefixDeal r;
-    r.pre = pre == 0 ? 0 : max(1, min(own == 0 ? blocks : blocks - 1, (int)(blocks * ((double)pre * p.pre_weight / all) + 0.5)));
-    const int n = 8 * r.pre, m = 8 * (blocks - r.pre);
-    r.pre_share = n == 0 ? 1 : max((pre + n - 1) / n, PREFIX_ITEM + 2);
-    r.own_share = m == 0 ? 1 : max((own + m - 1) / m, OWN_ITEM + WAVES);
+    // an item a wave, if that makes more than OWN_CHUNK tiles (each sequence's head has
+    // half an item more than its tiles make)
+    const int n = a.blocks / 8, second = n - p.first;  // workgroups of a die
+    const int waves = WAVES * 8 * second, full = waves - min(a.b.n_seq * a.n_kv, waves) / 2;
+    r.own_chunk = max(OWN_CHUNK, (own + full - 1) / full);
+    int items[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) items[i] = cbs[i] * ((tiles[i] + r.own_chunk - 1) / r.own_chunk);
+    const int first = block_before({items[0] + items[1], 0, 0}, sums, none).x;
+    if (2 * tid <= a.b.n_seq) t.items[2 * tid] = first;
+    if (2 * tid + 1 <= a.b.n_seq) t.items[2 * tid + 1] = first + items[0];
+    if (tid == THREADS - 1 && a.b.n_seq == 2 * THREADS) t.items[a.b.n_seq] = first + items[0] + items[1];
+    // the workgroups' shares of the prefixes: equal with what own tokens cost counted in
+    r.first = p.first;
+    const int cost = own > 0 ? OWN_ITEM + r.own_chunk : 0;
+    const int share = (int)(((int64_t)pre + (int64_t)8 * second * cost + 8 * n - 1) / (8 * n));
+    r.share[0] = share;
+    r.share[1] = share - cost;
+    if (r.first > 0 && r.share[1] < PREFIX_ITEM + 2) {
+        r.share[0] = (pre + 8 * r.first - 1) / (8 * r.first);
+        r.share[1] = 0;
+    }
+    r.share[0] = max(r.share[0], PREFIX_ITEM + 2);
+    if (r.first == 0 || r.share[1] > 0) r.share[1] = max(r.share[1], PREFIX_ITEM + 2);
+    __syncthreads();
     return r;
 }
 
@@ -256,25 +284,29 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
 {
     __shared__ union {
         many::Shared<D, CT, QF32> pre;
-        few::Shared<D, CT, QF32, NB, WAVES> own;
+        few::Shared<D, CT, QF32, NB, 1> own[WAVES];
     } sh;
-    __shared__ int2 s_at[PREFIX_SEQS + PREFIX_GROUPS + 1], s_sums[WAVES];
+    __shared__ Tables t;
+    __shared__ int3 s_sums[WAVES];
     __shared__ int s_start[PREFIX_SEQS + 1], s_len[PREFIX_SEQS];
-    __shared__ int s_least[PREFIX_GROUPS], s_most[PREFIX_GROUPS], s_tiles[PREFIX_GROUPS];
+    __shared__ int s_group[PREFIX_GROUPS + 1], s_prefix[PREFIX_GROUPS], s_least[PREFIX_GROUPS], s_most[PREFIX_GROUPS];
     constexpr int OCOLS = 16 * NB;
     const PagedAttnArgs& a = p.a;
-    const int n_seq = a.b.n_seq, entries = p.n_groups + n_seq;
-    const Batch x = {s_start, s_len, s_least, s_most};
-    for (int s = (int)threadIdx.x; s <= n_seq; s += THREADS) {
+    const int n_seq = a.b.n_seq, tid = (int)threadIdx.x;
+    const Batch x = {s_start, s_len, s_group, s_prefix, s_least, s_most};
+    for (int s = tid; s <= n_seq; s += THREADS) {
         s_start[s] = a.b.q_start ? a.b.q_start[s] : s;
         if (s < n_seq) s_len[s] = a.b.kv_len[s];
     }
-    for (int g = (int)threadIdx.x; g < p.n_groups; g += THREADS) {
+    for (int g = tid; g <= p.n_groups; g += THREADS) {
+        s_group[g] = p.group_start[g];
+        if (g == p.n_groups) break;
+        s_prefix[g] = p.prefix_len[g];
         s_least[g] = 0x7fffffff;
         s_most[g] = -1;
     }
     __syncthreads();
-    for (int s = (int)threadIdx.x; s < n_seq; s += THREADS) {
+    for (int s = tid; s < n_seq; s += THREADS) {
         Group g;
         const int which = group_with(p, x, s, g);
         const SeqRows r = rows_of(a.b, x, s);
@@ -284,87 +316,96 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         }
     }
     __syncthreads();
-    deal<OCOLS>(p, x, s_at, s_tiles, s_sums);
-    const int pre = uniform(s_at[p.n_groups].x), pre_items = uniform(s_at[p.n_groups].y);
-    const PrefixDeal sizes = shares(p, pre, uniform(s_at[entries].x) - pre);
+    const PrefixDeal dealt = deal<OCOLS>(p, x, t, s_sums);
     if (blockIdx.x == 0) {  // for the join
-        for (int e = (int)threadIdx.x; e <= entries; e += THREADS) p.at[e] = s_at[e];
-        for (int g = (int)threadIdx.x; g < p.n_groups; g += THREADS) p.tiles[g] = s_tiles[g];
-        if (threadIdx.x == 0) *p.deal = sizes;
-    }
-    // each die's workgroups take one stretch of the prefixes and one of own tokens;
-    // its first ones, one a CU, as a rule the former
-    const int die = (int)(blockIdx.x % 8u), j = (int)(blockIdx.x / 8u);
-    if (j < sizes.pre) {
-        const int b = die * sizes.pre + j;
-        const int64_t from = (int64_t)b * sizes.pre_share;
-        const int end = (int)min(from + sizes.pre_share, (int64_t)pre);
-        for (int64_t at = from; at < end;) {
-            int lo = 0, hi = p.n_groups - 1;  // the last group that begins at or before `at`
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (uniform(s_at[mid].x) <= at) lo = mid;
-                else hi = mid - 1;
-            }
-            const int2 base = {uniform(s_at[lo].x), uniform(s_at[lo].y)};
-            const int in = (int)at - base.x;
-            const Group g = uniform(group_of(p, x, lo));
-            const int least = uniform(s_least[lo]), most = uniform(s_most[lo]);
-            const int tiles = uniform(s_tiles[lo]), cbs = (g.rows * a.group + PCOLS - 1) / PCOLS;
-            const int chunks = (tiles + p.chunk - 1) / p.chunk;
-            const int of_kvh = cbs * (tiles + chunks * PREFIX_ITEM), kvh = in / of_kvh;
-            const int of_chunk = cbs * (p.chunk + PREFIX_ITEM), ch = in % of_kvh / of_chunk;
-            const int n = min(p.chunk, tiles - ch * p.chunk), c = in % of_kvh - ch * of_chunk;
-            const int cb = c / (n + PREFIX_ITEM), v = c % (n + PREFIX_ITEM);
-            const int take = min(n + PREFIX_ITEM - v, end - (int)at);
-            const int v0 = ch * p.chunk + max(0, v - PREFIX_ITEM), v1 = ch * p.chunk + max(0, v + take - PREFIX_ITEM);
-            const uint64_t slot = (uint64_t)(base.y + (kvh * chunks + ch) * cbs + cb + b);
-            if (v0 < v1 && slot < p.pre_slots) {
-                const PrefixWork w = {p, x, g, {g.a, g.rows, g.len, false}, g.s0, kvh, cb, 0, v0, v1, least, most,
-                                      prefix_tiles(a, g, least, most), p.pre_o + slot * PCOLS * D, p.pre_ml + slot * PCOLS * 2};
-                many::attend<D, CT, QF32, PrefixColumns>(a, sh.pre, w);
-            }
-            at += take;
-            __syncthreads();  // the tiles and states in LDS are read
-        }
-    } else {
-        const int b = die * (a.blocks / 8 - sizes.pre) + j - sizes.pre;
-        const int64_t from = pre + (int64_t)b * sizes.own_share;
-        const int end = (int)min(from + sizes.own_share, (int64_t)uniform(s_at[entries].x));
-        for (int64_t at = from; at < end;) {
-            int lo = p.n_groups, hi = entries - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (uniform(s_at[mid].x) <= at) lo = mid;
-                else hi = mid - 1;
-            }
-            const int2 base = {uniform(s_at[lo].x), uniform(s_at[lo].y)};
-            const int in = (int)at - base.x, s = lo - p.n_groups;
+        for (int s = tid; s < n_seq; s += THREADS) {
             Group g;
-            group_with(p, x, s, g);
-            g.len = uniform(g.len);
-            const SeqRows sq = uniform(rows_of(a.b, x, s));
-            const OwnTiles seen = own_tiles(a, sq, g.len);
-            const int of_item = seen.total() + OWN_ITEM, cbs = (sq.n * a.group + OCOLS - 1) / OCOLS;
-            const int item = in / of_item, v = in % of_item, take = min(of_item - v, end - (int)at);
-            const int v0 = max(0, v - OWN_ITEM), v1 = max(0, v + take - OWN_ITEM);
-            const uint64_t slot = (uint64_t)(base.y - pre_items + item + b);
-            if (v0 < v1 && slot < p.own_slots)
-                few::attend<D, CT, QF32, NB>(a, sh.own, sq, s, item / cbs, item % cbs, seen, v0, v1,
-                                             a.part_o + slot * OCOLS * D, a.part_ml + slot * OCOLS * 2, OwnTokens{g.len});
-            at += take;
-            __syncthreads();
+            const int which = group_with(p, x, s, g);
+            const int chunks = (own_tiles(a, rows_of(a.b, x, s), g.len).total() + dealt.own_chunk - 1) / dealt.own_chunk;
+            p.seqs[s] = {t.at[which].x, t.at[which].y, g.len > 0 ? t.tiles[which] : 0,
+                         g.len > 0 ? (t.tiles[which] + p.chunk - 1) / p.chunk : 0, g.a,
+                         (g.rows * a.group + PCOLS - 1) / PCOLS, t.items[s], chunks};
         }
+        if (tid == 0) *p.deal = dealt;
+    }
+
+    // own tokens: neighbouring items on different CUs
+    const int die = (int)(blockIdx.x % 8u), j = (int)(blockIdx.x / 8u);
+    if (j >= dealt.first) {
+        const int wave = uniform(tid >> 6), groups = a.blocks - 8 * dealt.first;
+        const int all = uniform(t.items[n_seq]);
+        for (int i = wave * groups + (int)blockIdx.x - 8 * dealt.first; i < all; i += WAVES * groups) {
+            int lo = 0, hi = n_seq - 1;  // the last sequence whose items begin at or before i
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (uniform(t.items[mid]) <= i) lo = mid;
+                else hi = mid - 1;
+            }
+            Group g;
+            group_with(p, x, lo, g);
+            g.len = uniform(g.len);
+            const SeqRows sq = uniform(rows_of(a.b, x, lo));
+            const OwnTiles seen = own_tiles(a, sq, g.len);
+            const int chunks = (seen.total() + dealt.own_chunk - 1) / dealt.own_chunk, cbs = own_columns(a, sq, OCOLS);
+            const int in = i - uniform(t.items[lo]), v0 = in % chunks * dealt.own_chunk;
+            if ((uint64_t)i < p.own_slots)
+                few::attend<D, CT, QF32, NB, 1>(a, sh.own[wave], sq, lo, in / chunks / cbs, in / chunks % cbs, seen, v0,
+                                                min(v0 + dealt.own_chunk, seen.total()), a.part_o + (uint64_t)i * OCOLS * D,
+                                                a.part_ml + (uint64_t)i * OCOLS * 2, OwnTokens{g.len});
+        }
+        __syncthreads();  // tiles of prefixes go where their queries lay
+    }
+
+    // prefixes: each die's workgroups take one stretch
+    const int share = dealt.share[j >= dealt.first];
+    const int of_die = dealt.first * dealt.share[0] + (a.blocks / 8 - dealt.first) * dealt.share[1];
+    const int64_t from = (int64_t)die * of_die + min(j, dealt.first) * dealt.share[0] + max(j - dealt.first, 0) * dealt.share[1];
+    const int end = (int)min(from + share, (int64_t)uniform(t.at[p.n_groups].x));
+    const int b = die * (dealt.share[1] > 0 ? a.blocks / 8 : dealt.first) + j;  // of those that take some
+    for (int64_t at = from; at < end;) {
+        int lo = 0, hi = p.n_groups - 1;  // the last group that begins at or before `at`
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (uniform(t.at[mid].x) <= at) lo = mid;
+            else hi = mid - 1;
+        }
+        const int2 base = {uniform(t.at[lo].x), uniform(t.at[lo].y)};
+        const int in = (int)at - base.x;
+        const Group g = uniform(group_of(p, x, lo));
+        const int least = uniform(s_least[lo]), most = uniform(s_most[lo]);
+        const int tiles = uniform(t.tiles[lo]), cbs = (g.rows * a.group + PCOLS - 1) / PCOLS;
+        const int chunks = (tiles + p.chunk - 1) / p.chunk;
+        const int of_kvh = cbs * (tiles + chunks * PREFIX_ITEM), kvh = in / of_kvh;
+        const int of_chunk = cbs * (p.chunk + PREFIX_ITEM), ch = in % of_kvh / of_chunk;
+        const int n = min(p.chunk, tiles - ch * p.chunk), c = in % of_kvh - ch * of_chunk;
+        const int cb = c / (n + PREFIX_ITEM), v = c % (n + PREFIX_ITEM);
+        const int take = min(n + PREFIX_ITEM - v, end - (int)at);
+        const int v0 = ch * p.chunk + max(0, v - PREFIX_ITEM), v1 = ch * p.chunk + max(0, v + take - PREFIX_ITEM);
+        const uint64_t slot = (uint64_t)(base.y + (kvh * chunks + ch) * cbs + cb + b);
+        if (v0 < v1 && slot < p.pre_slots) {
+            const PrefixWork w = {p, x, g, {g.a, g.rows, g.len, false}, g.s0, kvh, cb, 0, v0, v1, least, most,
+                                  prefix_tiles(a, g, least, most), p.pre_o + slot * PCOLS * D, p.pre_ml + slot * PCOLS * 2};
+            many::attend<D, CT, QF32, PrefixColumns>(a, sh.pre, w);
+        }
+        at += take;
+        __syncthreads();  // the tiles and states in LDS are read
     }
 }
 
 // ---- the join ------------------------------------------------------------------
-// Four groups of D/4 threads a (row, query head). The item that a row's column
-// is in has a part from each workgroup that takes some of its tiles.
+// x / d for quotients below 2^20, by = 1 / d.
+__device__ __forceinline__ int divided(int x, int d, float by)
+{
+    const int q = (int)((float)x * by), r = x - q * d;
+    return q + (r >= d) - (r < 0);
+}
+// Four groups of D/4 threads a (row, query head), which take its parts in turn. The
+// items that its column is in, of a prefix's chunks, have a part from each workgroup
+// that takes some of their tiles; those of its own tokens one each.
 template <int D, bool QF32, int OCOLS>
 __global__ __launch_bounds__(256) void k_attn_shared_join(PrefixArgs p)
 {
-    constexpr int TH = D / 4, PAR = 4, PER = 256 / (TH * PAR);
+    constexpr int TH = D / 4, PAR = 4, PER = 256 / (TH * PAR), AHEAD = 4;
     const PagedAttnArgs& a = p.a;
     __shared__ float s_o[PAR][PER][D];
     __shared__ float s_ml[PAR][PER][2];
@@ -376,77 +417,78 @@ __global__ __launch_bounds__(256) void k_attn_shared_join(PrefixArgs p)
     const int row = (int)(rest / (unsigned)a.b.n_seq), seq = (int)(rest % (unsigned)a.b.n_seq);
     SeqRows sq = {};
     if (row < a.b.max_q) sq = seq_rows(a.b, seq);
+    const PrefixSeq q = p.seqs[seq];
+    const PrefixDeal dealt = *p.deal;
     const bool live = row < sq.n;
     float m = -INFINITY, l = 0.0f;
     pf32x4 o = {};
     if (live) {
-        const PrefixDeal sizes = *p.deal;
-        const int kvh = head / a.group;
-        const Batch batch = {a.b.q_start, a.b.kv_len, nullptr, nullptr};
-        Group g;
-        const int which = group_with(p, batch, seq, g);
-        const int2 groups = p.at[p.n_groups];
-        // the prefix
-        int tiles = 0, cbs = 0, cb = 0, col = 0, chunks = 0;
-        int2 base = {0, 0};
-        if (g.len > 0) {
-            base = p.at[which];
-            tiles = p.tiles[which];
-            col = (sq.a + row - g.a) * a.group + head % a.group;
-            cb = col / PCOLS;
-            cbs = (g.rows * a.group + PCOLS - 1) / PCOLS;
-            chunks = (tiles + p.chunk - 1) / p.chunk;
-        }
-        // its own tokens
-        const int2 own = p.at[p.n_groups + seq], next = p.at[p.n_groups + seq + 1];
-        const int own_col = row * a.group + head % a.group;
-        const int of_item = next.y > own.y ? (next.x - own.x) / (next.y - own.y) : 0;
-        const int own_item = kvh * ((sq.n * a.group + OCOLS - 1) / OCOLS) + own_col / OCOLS;
-        for (int i = part; i <= chunks; i += PAR) {  // the last one: its own
-            int from, cost, share;  // where its tiles begin in the deal, and how many they are
-            const float *po, *pm;
-            uint64_t slot0, slots, at, step;
-            if (i < chunks) {
-                cost = min(p.chunk, tiles - i * p.chunk);
-                from = base.x + kvh * cbs * (tiles + chunks * PREFIX_ITEM) + i * cbs * (p.chunk + PREFIX_ITEM) +
-                       cb * (cost + PREFIX_ITEM) + PREFIX_ITEM;
-                share = sizes.pre_share;
-                slot0 = (uint64_t)(base.y + (kvh * chunks + i) * cbs + cb);
-                slots = p.pre_slots;
-                po = p.pre_o;
-                pm = p.pre_ml;
-                at = col % PCOLS;
-                step = PCOLS;
-            } else {
-                cost = of_item - OWN_ITEM;
-                from = own.x - groups.x + own_item * of_item + OWN_ITEM;
-                share = sizes.own_share;
-                slot0 = (uint64_t)(own.y - groups.y + own_item);
-                slots = p.own_slots;
-                po = a.part_o;
-                pm = a.part_ml;
-                at = own_col % OCOLS;
-                step = OCOLS;
+        const int kvh = head / a.group, of_row = head % a.group;
+        const int col = (sq.a + row - q.row) * a.group + of_row, cb = col / PCOLS;
+        int before = 0;  // parts of the chunks before
+        const auto load = [&](bool it, const float* po, const float* pm, uint64_t slot, uint64_t slots, int step, int at,
+                              float& mi, float& li, pf32x4& oi) {
+            pf32x2 ml = {-INFINITY, 0.0f};
+            oi = (pf32x4){};
+            if (it && slot < slots) {
+                const uint64_t to = slot * step + at;
+                ml = *(const pf32x2*)(pm + to * 2);
+                oi = *(const pf32x4*)(po + to * D + d);
             }
-            if (cost <= 0) continue;
-            const int b0 = from / share, n = (from + cost - 1) / share - b0 + 1;
-            for (int j0 = 0; j0 < n; j0 += 4) {  // four in flight
-                float mi[4], li[4];
-                pf32x4 oi[4];
+            mi = ml[0];
+            li = ml[1];
+        };
+        // own parts are on their way while the prefix's are looked for
+        const int own_col = row * a.group + of_row;
+        const uint64_t own = (uint64_t)(q.own + (kvh * own_columns(a, sq, OCOLS) + own_col / OCOLS) * q.own_chunks);
+        float mo[2], lo[2];
+        pf32x4 oo[2];
+        const auto load_own = [&](int i) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint64_t slot = slot0 + b0 + min(j0 + j, n - 1);
-                    const uint64_t to = (slot < slots ? slot : 0) * step + at;
-                    mi[j] = pm[to * 2];
-                    li[j] = pm[to * 2 + 1];
-                    oi[j] = *(const pf32x4*)(po + to * D + d);
-                    if (j0 + j >= n) {
-                        mi[j] = -INFINITY;
-                        li[j] = 0.0f;
-                    }
+            for (int j = 0; j < 2; j++)
+                load(i + j * PAR < q.own_chunks, a.part_o, a.part_ml, own + i + j * PAR, p.own_slots, OCOLS, own_col % OCOLS,
+                     mo[j], lo[j], oo[j]);
+        };
+        load_own(PAR - 1 - part);
+        // the workgroup in whose share a place of the prefixes' costs lies
+        const int first = dealt.first * dealt.share[0], of_die = first + (a.blocks / 8 - dealt.first) * dealt.share[1];
+        const int n = dealt.share[1] > 0 ? a.blocks / 8 : dealt.first;  // of a die
+        const float by_die = 1.0f / (float)of_die, by_first = 1.0f / (float)max(1, dealt.share[0]);
+        const float by_second = 1.0f / (float)max(1, dealt.share[1]);
+        const auto block_at = [&](int at) {
+            const int die = divided(at, of_die, by_die), in = at - die * of_die;
+            return die * n + (in < first ? divided(in, dealt.share[0], by_first)
+                                         : dealt.first + divided(in - first, dealt.share[1], by_second));
+        };
+        const int from0 = q.cost + kvh * q.cbs * (q.tiles + q.chunks * PREFIX_ITEM) + PREFIX_ITEM;
+        for (int i0 = 0; i0 < q.chunks; i0 += AHEAD) {
+            float mi[AHEAD], li[AHEAD];
+            pf32x4 oi[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                mi[j] = -INFINITY;
+                li[j] = 0.0f;
+                oi[j] = (pf32x4){};
+                const int i = i0 + j, cost = min(p.chunk, q.tiles - i * p.chunk);
+                if (i >= q.chunks) continue;
+                const int from = from0 + i * q.cbs * (p.chunk + PREFIX_ITEM) + cb * (cost + PREFIX_ITEM);
+                const int b0 = block_at(from), parts = block_at(from + cost - 1) - b0 + 1, k = (part - before) & (PAR - 1);
+                const uint64_t slot0 = (uint64_t)(q.item + (kvh * q.chunks + i) * q.cbs + cb + b0);
+                load(k < parts, p.pre_o, p.pre_ml, slot0 + k, p.pre_slots, PCOLS, col % PCOLS, mi[j], li[j], oi[j]);
+                for (int more = k + PAR; more < parts; more += PAR) {
+                    float mk[1], lk[1];
+                    pf32x4 ok[1];
+                    load(true, p.pre_o, p.pre_ml, slot0 + more, p.pre_slots, PCOLS, col % PCOLS, mk[0], lk[0], ok[0]);
+                    add_parts<1>(m, l, o, mk, lk, ok);
                 }
-                add_parts<4>(m, l, o, mi, li, oi);
+                before += parts;
             }
+            add_parts<AHEAD>(m, l, o, mi, li, oi);
+        }
+        add_parts<2>(m, l, o, mo, lo, oo);
+        for (int i = PAR - 1 - part + 2 * PAR; i < q.own_chunks; i += 2 * PAR) {
+            load_own(i);
+            add_parts<2>(m, l, o, mo, lo, oo);
         }
     }
     *(pf32x4*)&s_o[part][mine][d] = o;

@@ -278,12 +278,25 @@ int plan_prefix(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_kv_pref
     const int64_t own_cols = cols > ATTN_FEW_COLS && kv->dtype != WPCG_DTYPE_F32 ? 2 * ATTN_FEW_COLS : ATTN_FEW_COLS;
     const int64_t own_blocks = (cols + own_cols - 1) / own_cols, own_tiles = (b.max_kv + ATTN_FEW_TILE - 1) / ATTN_FEW_TILE;
     PrefixArgs& p = o.args;
-    p.chunk = 64;
+    // Chunks keep the column blocks' workgroups at keys and values that one die's L2
+    // holds; each makes a part more to join: four of a long prefix. (32 / 8 heads, 65536
+    // tokens, one column block: 16 chunks 125 us, 4 chunks 120.)
+    p.chunk = (int)std::max<int64_t>(64, (tiles + 3) / 4);
     const int64_t chunks = (tiles + p.chunk - 1) / p.chunk;
     const double cost = (double)n_kv * (blocks * (tiles + chunks * PREFIX_ITEM) +
                                         b.n_seq * own_blocks * (own_tiles + OWN_ITEM));
+    // Without sharing a prefix comes out of the caches for all sequences but the first,
+    // at some 11 TB/s, and the fixed costs are lower: it pays from a number of bytes on
+    // that are read again. Shared and not, us, prefixes of one group's sequences, own
+    // tokens up to 200; read again, MB:
+    //   BF16 queries, BF16 cache, 32 / 4 heads    246  33 29   459  35 47   1057  46 100
+    //                 E4M3, 32 / 8                115  25 22   246  28 33    516  40 54
+    //   F32 queries, BF16 cache, 32 / 8           229  39 31   369  64 56    492  41 49
+    //                F32 cache, 14 / 2 of 64      123  44 24   229  52 33
+    const double again = (double)(b.n_seq - groups) * max_prefix * 2 * n_kv * kv->head_dim * type_size(kv->dtype) / 1e6;
+    const double pays = a->dtype == WPCG_DTYPE_BF16 ? 250 : kv->dtype == WPCG_DTYPE_F32 ? 700 : 450;
     o.shared = rows > 0 && cols <= 2 * ATTN_FEW_COLS && groups > 0 && groups < b.n_seq && groups <= PREFIX_GROUPS &&
-               b.n_seq <= PREFIX_SEQS && max_prefix > 0 && cost < (double)(1 << 30);
+               b.n_seq <= PREFIX_SEQS && again >= pays && cost < (double)(1 << 30);
     if (!o.shared) {
         if (int rc = plan_attention(kv, b, a, &o.plain)) return rc;
         o.bytes = o.plain.bytes;
@@ -291,14 +304,14 @@ int plan_prefix(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_kv_pref
     }
     p.n_groups = (int)groups;
     p.max_prefix = (int)max_prefix;
-    p.pre_weight = 2;
-    p.own_weight = 1;
-    p.a.blocks = a->dtype == WPCG_DTYPE_BF16 ? 2 * CUS : CUS;
+    const bool bf16 = a->dtype == WPCG_DTYPE_BF16;
+    p.a.blocks = bf16 ? 2 * CUS : CUS;
+    p.first = bf16 ? CUS / 8 : 0;
     p.a.cols = (int)own_cols;
     p.pre_slots = (uint64_t)(n_kv * blocks * chunks + p.a.blocks);
-    p.own_slots = (uint64_t)(n_kv * own_blocks * b.n_seq + p.a.blocks);
+    p.own_slots = (uint64_t)(n_kv * own_blocks * b.n_seq + 4 * (p.a.blocks - 8 * p.first));
     o.bytes = (p.pre_slots * cw + p.own_slots * own_cols) * (kv->head_dim + 2) * sizeof(float) +
-              (groups + b.n_seq + 1) * sizeof(int2) + groups * sizeof(int) + sizeof(PrefixDeal);
+              b.n_seq * sizeof(PrefixSeq) + sizeof(PrefixDeal);
     return WPCG_OK;
 }
 
@@ -629,9 +642,8 @@ int wpcg_prefix_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_
     p.pre_o = a.part_o + own * d;
     a.part_ml = p.pre_o + pre * d;
     p.pre_ml = a.part_ml + own * 2;
-    p.at = (int2*)(p.pre_ml + pre * 2);
-    p.tiles = (int*)(p.at + p.n_groups + a.b.n_seq + 1);
-    p.deal = (PrefixDeal*)(p.tiles + p.n_groups);
+    p.seqs = (PrefixSeq*)(p.pre_ml + pre * 2);
+    p.deal = (PrefixDeal*)(p.seqs + a.b.n_seq);
     p.a = a;
     p.group_start = prefix->group_start_dev;
     p.prefix_len = prefix->prefix_len_dev;

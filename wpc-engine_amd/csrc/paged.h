@@ -150,6 +150,16 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&t)[3])
     t[1] = pk_upper(a, b);
     t[2] = pk_upper(below_bf16(a), below_bf16(b));
 }
+// The same without what keeps infinities from becoming NaN.
+__device__ __forceinline__ void split3_finite(float a, float b, uint32_t (&t)[3])
+{
+    const auto upper = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); };
+    t[0] = pk_upper(a, b);
+    a -= upper(a);
+    b -= upper(b);
+    t[1] = pk_upper(a, b);
+    t[2] = pk_upper(a - upper(a), b - upper(b));
+}
 // Two E4M3 bytes (the low or the high half of w) as two bf16, exact.
 template <bool HIGH>
 __device__ __forceinline__ uint32_t e4m3_bf16(uint32_t w)

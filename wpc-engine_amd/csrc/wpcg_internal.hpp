@@ -541,28 +541,33 @@ hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, in
 hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 
 // Attention whose sequences share prefixes in groups (attn_prefix.hip): a.blocks
-// workgroups, a multiple of 8, share the tiles: prefixes in tiles and columns of the
-// many rows, own tokens in those of few (a.cols). What an item costs to begin and
-// end, in its tiles: PREFIX_ITEM, OWN_ITEM; what a tile takes against the other kind's:
-// pre_weight, own_weight. A prefix's column blocks are taken by chunks of `chunk`
-// tiles. A part that a workgroup leaves is that of an item, numbered through, at place
-// item + workgroup: of prefixes at pre_o and pre_ml, of own tokens at a.part_o and
-// a.part_ml, as few rows leave them. at, tiles and deal: for the join.
+// workgroups, a multiple of 8, the first `first` of each die for prefixes alone.
+// Prefixes are in tiles and columns of the many rows, their column blocks taken by
+// chunks of `chunk` tiles; an item costs PREFIX_ITEM tiles to begin and end, a
+// workgroup's own tokens OWN_ITEM and one for each tile of a wave's item. Those
+// are in tiles of few rows and a.cols columns, by items of at least OWN_CHUNK, as
+// many as waves take them beside one for every sequence's head and columns. A
+// prefix's part that a workgroup leaves is at place item + workgroup of
+// pre_o and pre_ml, an own item's at its number in a.part_o and a.part_ml.
 constexpr int PREFIX_SEQS = 512, PREFIX_GROUPS = 256;
-constexpr int PREFIX_ITEM = 3, OWN_ITEM = 6;
+constexpr int PREFIX_ITEM = 3, OWN_ITEM = 2, OWN_CHUNK = 2;
 struct PrefixDeal {
-    int pre, pre_share, own_share;  // workgroups of a die that take prefixes; tiles of one
+    int first, share[2];  // of a die's workgroups; the shares of these and of the others
+    int own_chunk;        // tiles of an own item
+};
+struct PrefixSeq {
+    int cost, item, tiles, chunks, row, cbs;  // its group's: place in the deal, tiles, first row, column blocks
+    int own, own_chunks;                      // its first own item, how many a head and column block has
 };
 struct PrefixArgs {
     PagedAttnArgs a;
     int n_groups, max_prefix;
     const int32_t *group_start, *prefix_len;
-    int chunk, pre_weight, own_weight;
+    int first, chunk;
     uint64_t pre_slots, own_slots;
     float *pre_o, *pre_ml;
-    int2* at;    // [n_groups + n_seq + 1] cost and items before the groups and sequences
-    int* tiles;  // [n_groups] of a prefix
-    PrefixDeal* deal;
+    PrefixSeq* seqs;   // [n_seq] and
+    PrefixDeal* deal;  // for the join
 };
 hipError_t launch_attn_prefix(const PrefixArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s);
 
