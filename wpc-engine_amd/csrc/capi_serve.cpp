@@ -493,7 +493,9 @@ int check_logprobs(const wpcg_logprob* d, int* chunks, uint64_t* part_bytes, uin
     if (d->top > WPCG_LOGPROB_TOP) return fail(WPCG_E_ARG, "top is at most " + std::to_string(WPCG_LOGPROB_TOP));
     if (d->logits_stride && d->logits_stride < d->vocab) return fail(WPCG_E_SHAPE, "row stride shorter than the row");
     if (d->logits_stride >> 40) return fail(WPCG_E_ARG, "row stride too large");
-    *chunks = (int)((d->vocab + LOGPROB_CHUNK - 1) / LOGPROB_CHUNK);
+    // (a row that does not start on 16 bytes has up to seven places before it)
+    const uint64_t per = 16 / type_size(d->dtype), stride = d->logits_stride ? d->logits_stride : d->vocab;
+    *chunks = (int)((d->vocab + (stride % per ? per - 1 : 0) + LOGPROB_CHUNK - 1) / LOGPROB_CHUNK);
     if ((uint64_t)d->n_rows * ((*chunks + 3) / 4) >= (uint64_t)GROUPS_256)
         return fail(WPCG_E_UNSUPPORTED, "the batch needs too many workgroups");
     const uint64_t all = (uint64_t)d->n_rows * *chunks;
@@ -830,7 +832,8 @@ int wpcg_logprobs(wpcg_ctx* ctx, const wpcg_logprob* d, void* ws_dev, uint64_t w
     a.bf16 = d->dtype == WPCG_DTYPE_BF16;
     a.logits = d->logits_dev;
     a.row = d->logits_stride ? d->logits_stride : d->vocab;
-    a.vec = aligned(a.logits) && a.row * type_size(d->dtype) % 16 == 0;
+    a.all = (a.n_rows - 1) * a.row + a.vocab;
+    a.vec = aligned(a.logits);
     a.temperature = d->temperature_dev;
     a.tokens = d->tokens_dev;
     a.logprob = d->logprob_dev;

@@ -78,38 +78,6 @@ __device__ __forceinline__ double draft_rate(const DraftArgs& p, int s)
     return t > 0.0f ? fmax(1.4426950408889634 / (double)t, 0x1p-1000) : 0.0;
 }
 
-// Lane exchanges of doubles: 0 from lanes that there are none.
-constexpr int DPP_ROW_SHR = 0x110, DPP_WAVE_SHR1 = 0x138;  // from n lanes before, in a row of 16; of the wave
-template <int CTRL, int ROW_MASK = 0xF>
-__device__ __forceinline__ double dpp_d(double v)
-{
-    const uint64_t w = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)wave_dpp_i<CTRL, ROW_MASK>(0, (int)(uint32_t)w);
-    const uint32_t hi = (uint32_t)wave_dpp_i<CTRL, ROW_MASK>(0, (int)(w >> 32));
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ double lane_d(double v, int lane)
-{
-    const uint64_t w = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)w, lane);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), lane);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-// Every lane: the sum over its row of 16 lanes.
-__device__ __forceinline__ double row_sum_d(double v)
-{
-    v += dpp_d<WDPP_XOR1>(v);
-    v += dpp_d<WDPP_XOR2>(v);
-    v += dpp_d<WDPP_HALF_MIRROR>(v);
-    return v + dpp_d<WDPP_MIRROR>(v);
-}
-__device__ __forceinline__ double wave_sum_d(double v)
-{
-    v = row_sum_d(v);
-    v += dpp_d<WDPP_BCAST15, 0xA>(v);
-    v += dpp_d<WDPP_BCAST31, 0xC>(v);
-    return lane_d(v, 63);
-}
 // The sums over the lanes up to this one.
 __device__ __forceinline__ double wave_scan_d(double v)
 {

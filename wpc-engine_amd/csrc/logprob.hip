@@ -38,32 +38,40 @@ __device__ __forceinline__ float row_rate(const LogprobArgs& p, int row)
     return (float)fmin(row_rate_d(p, row), 3.0e38);
 }
 
-// A chunk's logits in registers: lane l holds ids PER * (l + 64 i) + 0 .. PER-1,
-// loads of 16 bytes; -inf behind the row's end.
+// Rows need not start on 16 bytes: chunks and segments are of places from the last
+// 16-byte border before the row's start on, `skew` places before its first id, and
+// what lies outside the row counts as -inf.
+__device__ __forceinline__ int row_skew(const LogprobArgs& p, int row)
+{
+    return p.vec ? (int)((uint64_t)row * p.row % (p.bf16 ? 8u : 4u)) : 0;
+}
+// A chunk's logits in registers: lane l holds places PER * (l + 64 i) + 0 .. PER-1,
+// loads of 16 bytes.
 template <bool BF16>
 struct Chunk {
     static constexpr int PER = BF16 ? 8 : 4, LOADS = VALUES / PER;
     float v[VALUES];
-    __device__ __forceinline__ static int id(int i)  // of v[i]
+    __device__ __forceinline__ static int place(int i)  // of v[i]
     {
         return PER * ((int)(threadIdx.x & 63) + 64 * (i / PER)) + i % PER;
     }
-    __device__ __forceinline__ void load(const LogprobArgs& p, int row, int c0)
+    // id0: the id at the chunk's first place
+    __device__ __forceinline__ void load(const LogprobArgs& p, int row, int id0)
     {
-        const uint64_t at = (uint64_t)row * p.row + c0;
         // one way for the whole wave, and no load behind a condition
-        if (p.vec && c0 + CHUNK <= p.vocab) {
+        const uint64_t at = (uint64_t)row * p.row + (uint64_t)(int64_t)id0;
+        if (p.vec && at + CHUNK <= p.all) {
 #pragma unroll
             for (int i = 0; i < LOADS; i++) {
                 if constexpr (BF16) {
-                    const pu32x4 w = *(const pu32x4*)((const uint16_t*)p.logits + at + id(i * PER));
+                    const pu32x4 w = *(const pu32x4*)((const uint16_t*)p.logits + at + place(i * PER));
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
                         v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
                     }
                 } else {
-                    const pf32x4 w = *(const pf32x4*)((const float*)p.logits + at + id(i * PER));
+                    const pf32x4 w = *(const pf32x4*)((const float*)p.logits + at + place(i * PER));
 #pragma unroll
                     for (int j = 0; j < 4; j++) v[4 * i + j] = w[j];
                 }
@@ -71,12 +79,14 @@ struct Chunk {
         } else {
 #pragma unroll
             for (int i = 0; i < VALUES; i++) {
-                const uint64_t x = (uint64_t)row * p.row + min(c0 + id(i), p.vocab - 1);
+                const uint64_t x = (uint64_t)row * p.row + min(max(id0 + place(i), 0), p.vocab - 1);
                 v[i] = BF16 ? __uint_as_float((uint32_t)((const uint16_t*)p.logits)[x] << 16) : ((const float*)p.logits)[x];
             }
+        }
+        if (id0 < 0 || id0 + CHUNK > p.vocab) {
 #pragma unroll
             for (int i = 0; i < VALUES; i++)
-                if (c0 + id(i) >= p.vocab) v[i] = -INFINITY;
+                if ((uint32_t)(id0 + place(i)) >= (uint32_t)p.vocab) v[i] = -INFINITY;
         }
     }
 };
@@ -94,10 +104,10 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
     const int row = (int)(blockIdx.x / (unsigned)groups);
     const int chunk = (int)(blockIdx.x % (unsigned)groups) * 4 + ((int)threadIdx.x >> 6);
     if (chunk >= p.chunks) return;
-    const int lane = (int)threadIdx.x & 63, c0 = chunk * CHUNK;
+    const int lane = (int)threadIdx.x & 63, id0 = chunk * CHUNK - row_skew(p, row);
     using C = Chunk<BF16>;
     C c;
-    c.load(p, row, c0);
+    c.load(p, row, id0);
     const int token = p.tokens ? p.tokens[row] : -1;
     const bool inside = token >= 0 && token < p.vocab;
     const float xt = inside ? logit(p, row, token) : INFINITY;
@@ -145,7 +155,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
     }
     if (__any(same)) {  // equal logits of lower ids come before, too
 #pragma unroll
-        for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] == xt && c0 + C::id(i) < token));
+        for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] == xt && id0 + C::place(i) < token));
     }
     const float zs = wave_sum(z[0] + z[1]), ss = wave_sum(s[0] + s[1]);
     if (lane == 0)
@@ -153,36 +163,24 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
 }
 
 // ---- the row's state -------------------------------------------------------------
-__device__ __forceinline__ double wave_sum_f64(double v)
-{
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ double block_sum_f64(double v, double* s)
-{
-    v = wave_sum_f64(v);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = (s[0] + s[1]) + (s[2] + s[3]);
-    __syncthreads();
-    return v;
-}
-__device__ __forceinline__ int block_sum_i(int v, int* s)
-{
-    v = wave_sum_i(v);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = s[0] + s[1] + s[2] + s[3];
-    __syncthreads();
-    return v;
-}
-
 // (x - M) / T for a logit in base 2, the rate in 64 bits
 __device__ __forceinline__ double scaled(float x, float m, double rate)
 {
     const double d = (double)x - (double)m;
     return rate == 0.0 ? (d == -INFINITY ? d : d * 0.0) : d * rate;
+}
+// Sums over the workgroup's four waves.
+struct RowSums {
+    double z, s;
+    int tops, before;
+};
+__device__ __forceinline__ RowSums block_sums(RowSums v, RowSums* s)
+{
+    v = {wave_sum_d(v.z), wave_sum_d(v.s), wave_sum_i(v.tops), wave_sum_i(v.before)};
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return {(s[0].z + s[1].z) + (s[2].z + s[3].z), (s[0].s + s[1].s) + (s[2].s + s[3].s),
+            s[0].tops + s[1].tops + s[2].tops + s[3].tops, s[0].before + s[1].before + s[2].before + s[3].before};
 }
 
 // ---- the K best ------------------------------------------------------------------
@@ -195,51 +193,64 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t at)
     const uint32_t order = b & 0x80000000u ? ~b : b | 0x80000000u;
     return (uint64_t)order << 32 | (uint32_t)~at;
 }
-__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane)
+__device__ __forceinline__ float value_of(uint64_t key)
 {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    const uint32_t order = (uint32_t)(key >> 32);
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ uint32_t place_of(uint64_t key) { return (uint32_t)~key; }
+
+struct Lists {
+    uint64_t key[LIST];
+    int n[THREADS / 64];
+};
+// All threads' keys at or above `from` (not 0) to the list; how many there are, which
+// may be more than it holds. each(f) calls f for the thread's keys, all threads
+// alike.
+template <class EACH>
+__device__ __forceinline__ int collect(Lists& l, uint64_t from, EACH each)
+{
+    const int wave = (int)threadIdx.x >> 6;
+    int mine = 0;
+    each([&](uint64_t key) { mine += __popcll(__ballot(key != 0 && key >= from)); });
+    if ((threadIdx.x & 63) == 0) l.n[wave] = mine;
+    __syncthreads();
+    int at = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+        if (w == wave) at = all;
+        all += l.n[w];
+    }
+    if (all <= LIST)
+        each([&](uint64_t key) {
+            const bool it = key != 0 && key >= from;
+            const uint64_t them = __ballot(it);
+            if (it) l.key[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0))] = key;
+            at += __popcll(them);
+        });
+    __syncthreads();
+    return all;
 }
 // The k-th largest of all threads' keys (0 where there are fewer), bit by bit: of
-// use where equal values make too many candidates to sort. each(f) calls f for
-// the thread's keys.
+// use where equal values make too many candidates to sort.
 template <class EACH>
-__device__ uint64_t kth_key(int k, int* s, EACH each)
+__device__ uint64_t kth_key(int k, Lists& l, EACH each)
 {
     uint64_t at = 0;
     for (int bit = 63; bit >= 0; bit--) {
         const uint64_t next = at | (uint64_t)1 << bit;
         int n = 0;
         each([&](uint64_t key) { n += key >= next; });
-        if (block_sum_i(n, s) >= k) at = next;
+        n = wave_sum_i(n);
+        if ((threadIdx.x & 63) == 0) l.n[threadIdx.x >> 6] = n;
+        __syncthreads();
+        if (l.n[0] + l.n[1] + l.n[2] + l.n[3] >= k) at = next;
+        __syncthreads();
     }
     return at;
 }
-
-struct Lists {
-    uint64_t key[LIST];
-    int n;
-};
-// All threads' keys at or above `from` to the list; how many there are, which may
-// be more than it holds.
-template <class EACH>
-__device__ __forceinline__ int collect(Lists& l, uint64_t from, EACH each)
-{
-    if (threadIdx.x == 0) l.n = 0;
-    __syncthreads();
-    each([&](uint64_t key) {
-        if (key != 0 && key >= from) {
-            const int at = atomicAdd(&l.n, 1);
-            if (at < LIST) l.key[at] = key;
-        }
-    });
-    __syncthreads();
-    const int n = l.n;
-    __syncthreads();
-    return n;
-}
-// The thread's entry of a list of n <= LIST and how many come before it.
-__device__ __forceinline__ int rank_of(const Lists& l, int n, uint64_t& key)
+// The list's entry of this thread, and how many come before it.
+__device__ __forceinline__ int rank_in(const Lists& l, int n, uint64_t& key)
 {
     const int tid = (int)threadIdx.x;
     key = tid < n ? l.key[tid] : 0;
@@ -249,124 +260,83 @@ __device__ __forceinline__ int rank_of(const Lists& l, int n, uint64_t& key)
     return before;
 }
 
-// The K best ids of a row with their keys to best[0 .. K), as many as there are.
-__device__ int best_ids(const LogprobArgs& p, int row, Lists& list, uint64_t* best, int* s_i)
-{
-    __shared__ uint64_t s_key[THREADS], s_from;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n_seg = p.chunks * SEGS, k = p.top;
-    const float* seg = p.seg + (uint64_t)row * n_seg;
-    const auto each_seg = [&](auto f) {
-        for (int i0 = tid; i0 < n_seg; i0 += 8 * THREADS) {  // eight in flight
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = seg[min(i0 + j * THREADS, n_seg - 1)];
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (i0 + j * THREADS < n_seg) f(key_of(v[j], (uint32_t)(i0 + j * THREADS)));
-        }
-    };
-    // the k-th of 64 groups' best is at most the k-th of all
-    uint64_t mine = 0;
-    each_seg([&](uint64_t key) { mine = key > mine ? key : mine; });
-    s_key[tid] = mine;
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-        for (int w = 1; w < THREADS / 64; w++) mine = s_key[64 * w + lane] > mine ? s_key[64 * w + lane] : mine;
-        int before = 0;
-#pragma unroll 8
-        for (int i = 0; i < 64; i++) before += lane_key(mine, i) > mine;
-        if (lane == 0) s_from = 0;
-        if (mine != 0 && before == k - 1) s_from = mine;  // (0: fewer groups than k hold any)
-    }
-    __syncthreads();
-    uint64_t from = s_from;
-    int n = collect(list, from, each_seg);
-    if (n > LIST) {
-        from = kth_key(k, s_i, each_seg);
-        n = collect(list, from, each_seg);
-    }
-    uint64_t key;
-    const int at = rank_of(list, n, key);
-    if (tid < n && at < k) s_key[at] = key;
-    __syncthreads();
-    const int segs = min(n, k);
-    // their ids: lane l the l-th of a wave's segments
-    constexpr int MOST = LOGPROB_TOP / (THREADS / 64);
-    const uint32_t least = segs < k ? 0u : (uint32_t)(s_key[segs - 1] >> 32);
-    uint64_t own[MOST];
-#pragma unroll
-    for (int i = 0; i < MOST; i++) {
-        const int x = wave + i * (THREADS / 64);
-        own[i] = 0;
-        if (x < segs) {
-            const uint32_t id = (uint32_t)~s_key[x] * SEG + lane;
-            own[i] = key_of(logit(p, row, min(id, (uint32_t)p.vocab - 1)), id);
-            if (id >= (uint32_t)p.vocab || (uint32_t)(own[i] >> 32) < least) own[i] = 0;
-        }
-    }
-    const auto each_id = [&](auto f) {
-#pragma unroll
-        for (int i = 0; i < MOST; i++) f(own[i]);
-    };
-    n = collect(list, 0, each_id);
-    if (n > LIST) n = collect(list, kth_key(k, s_i, each_id), each_id);
-    const int place = rank_of(list, n, key);
-    if (tid < n && place < k) best[place] = key;
-    __syncthreads();
-    return min(n, k);
-}
+constexpr int HELD = 10;  // segments' maxima that a thread has in registers: vocabularies up to 163840
 
+// One row a workgroup.
 __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
 {
-    __shared__ double s_d[4];
-    __shared__ float s_f[4];
-    __shared__ int s_i[4];
+    __shared__ RowSums s_sums[4];
+    __shared__ float s_max[4];
     __shared__ Lists s_list;
-    __shared__ uint64_t s_best[LOGPROB_TOP];
-    const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
+    __shared__ uint64_t s_key[THREADS];
+    const int row = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const LogprobPart* part = p.part + (uint64_t)row * p.chunks;
+    // everything that is read first, on its way together
+    const int n_seg = p.top > 0 ? p.chunks * SEGS : 0;
+    const float* seg = p.seg + (uint64_t)row * n_seg;
+    float held[HELD];
+    if (n_seg > 0) {
+#pragma unroll
+        for (int i = 0; i < HELD; i++) held[i] = seg[min(tid + i * THREADS, n_seg - 1)];
+    }
+    const LogprobPart mine = part[min(tid, p.chunks - 1)];
     const double rate = row_rate_d(p, row);
+    const int token = p.tokens ? p.tokens[row] : -1;
+    const bool inside = token >= 0 && token < p.vocab;
+    const float x = inside ? logit(p, row, token) : -INFINITY;
 
-    float m = -INFINITY;
-    for (int c = tid; c < p.chunks; c += THREADS) m = fmaxf(m, part[c].max);
+    float m = tid < p.chunks ? mine.max : -INFINITY;
+    for (int c = tid + THREADS; c < p.chunks; c += THREADS) m = fmaxf(m, part[c].max);
     m = wave_max(m);
-    if ((tid & 63) == 0) s_f[tid >> 6] = m;
+    if (lane == 0) s_max[wave] = m;
+    // the best of the thread's segments, for below
+    const auto each_seg = [&](auto f) {
+        if (n_seg <= HELD * THREADS) {
+#pragma unroll
+            for (int i = 0; i < HELD; i++) {
+                const int at = tid + i * THREADS;
+                f(at < n_seg ? key_of(held[i], (uint32_t)at) : 0);
+            }
+        } else {
+            for (int i0 = 0; i0 < n_seg; i0 += THREADS) {
+                const int at = i0 + tid;
+                f(at < n_seg ? key_of(seg[at], (uint32_t)at) : 0);
+            }
+        }
+    };
+    if (n_seg > 0) {
+        uint64_t best = 0;
+        each_seg([&](uint64_t key) { best = key > best ? key : best; });
+        s_key[tid] = best;
+    }
     __syncthreads();
-    m = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
     // Z without the ids at the maximum, how many those are, and sum e^t t, in base 2
-    double z = 0.0, s = 0.0;
-    int before = 0, tops = 0;
-    for (int c = tid; c < p.chunks; c += THREADS) {
-        const LogprobPart q = part[c];
-        before += q.before;
+    RowSums v = {0.0, 0.0, 0, 0};
+    const auto add = [&](const LogprobPart& q) {
+        v.before += q.before;
         if (q.max == m) {
-            z += (double)q.z;
-            tops += q.tops;
-            s += (double)q.s;
+            v.z += (double)q.z;
+            v.tops += q.tops;
+            v.s += (double)q.s;
         } else {
             const double t = scaled(q.max == -INFINITY ? m : q.max, m, rate), f = exp2(t), all = (double)q.z + (double)q.tops;
-            z += all * f;
-            s += ((double)q.s + all * t) * f;
+            v.z += all * f;
+            v.s += ((double)q.s + all * t) * f;
         }
-    }
-    z = block_sum_f64(z, s_d);
-    tops = block_sum_i(tops, s_i);
-    z += (double)(tops - 1);  // Z - 1
-    s = block_sum_f64(s, s_d);
-    before = block_sum_i(before, s_i);
+    };
+    if (tid < p.chunks) add(mine);
+    for (int c = tid + THREADS; c < p.chunks; c += THREADS) add(part[c]);
+    v = block_sums(v, s_sums);
+    const double z = v.z + (double)(v.tops - 1);  // Z - 1
     const double ln2 = 0.6931471805599453, nan = __builtin_nan("");
     const bool greedy = rate < 0.0;
     const bool none = !(m > -INFINITY) || (!greedy && m == INFINITY);
     const double log_z = none ? nan : greedy ? 0.0 : log1p(z);
     if (tid == 0) {
-        if (p.entropy) p.entropy[row] = (float)(none ? nan : greedy ? 0.0 : log_z - ln2 * s / (z + 1.0));
+        if (p.entropy) p.entropy[row] = (float)(none ? nan : greedy ? 0.0 : log_z - ln2 * v.s / (z + 1.0));
         if (p.tokens) {
-            const int token = p.tokens[row];
-            const bool inside = token >= 0 && token < p.vocab;
-            const float x = inside ? logit(p, row, token) : -INFINITY;
-            const int rank = inside && x == x ? 1 + before : 0;
+            const int rank = inside && x == x ? 1 + v.before : 0;
             if (p.rank) p.rank[row] = rank;
             if (p.logprob)
                 p.logprob[row] = (float)(none     ? nan
@@ -374,21 +344,57 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
                                                   : ln2 * scaled(x, m, rate) - log_z);
         }
     }
-    if (p.top == 0) return;
-    const int n = best_ids(p, row, s_list, s_best, s_i);
-    if (tid < p.top) {
-        const uint64_t at = (uint64_t)row * p.top + tid;
-        const int id = tid < n ? (int)(uint32_t)~s_best[tid] : -1;
-        if (p.top_ids) p.top_ids[at] = id;
-        if (p.top_logprob) {
-            double lp = -INFINITY;
-            if (none) lp = nan;
-            else if (greedy) lp = tid == 0 ? 0.0 : -INFINITY;
-            else if (id >= 0) lp = ln2 * scaled(logit(p, row, id), m, rate) - log_z;
-            else if (!(log_z == log_z)) lp = nan;
-            p.top_logprob[at] = (float)lp;
+    if (n_seg == 0) return;
+
+    // The segments: the k-th best of 64 groups (of the threads of one lane number) is
+    // no better than the k-th of all; its value is the least of those that fewer
+    // than k groups are above (none: all that there are).
+    const int k = p.top;
+    uint32_t group = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) group = max(group, (uint32_t)(s_key[64 * w + lane] >> 32));
+    int above = 0;
+#pragma unroll 16
+    for (int i = 0; i < 64; i++) above += (uint32_t)__builtin_amdgcn_readlane((int)group, i) > group;
+    const uint32_t least = ~(uint32_t)(0x80000000u ^ (uint32_t)wave_max_i((int)(0x80000000u ^ (above < k ? ~group : 0u))));
+    uint64_t from = (uint64_t)least << 32;
+    int n = collect(s_list, from, each_seg);
+    if (n > LIST) n = collect(s_list, kth_key(k, s_list, each_seg), each_seg);
+    uint64_t key;
+    const int at = rank_in(s_list, n, key);
+    if (tid < n && at < k) s_key[at] = key;
+    __syncthreads();
+    const int segs = min(n, k);
+    // their ids: lane l the l-th of a wave's segments
+    constexpr int MOST = LOGPROB_TOP / (THREADS / 64);
+    const uint32_t worst = segs < k ? 0u : (uint32_t)(s_key[segs - 1] >> 32);
+    const int skew = row_skew(p, row);
+    uint64_t own[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+        const int y = wave + i * (THREADS / 64);
+        own[i] = 0;
+        if (y < segs) {
+            const int id = (int)(place_of(s_key[y]) * SEG) + lane - skew;
+            own[i] = key_of(logit(p, row, min(max(id, 0), p.vocab - 1)), (uint32_t)id);
+            if ((uint32_t)id >= (uint32_t)p.vocab || (uint32_t)(own[i] >> 32) < worst) own[i] = 0;
         }
     }
+    const auto each_id = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < MOST; i++) f(own[i]);
+    };
+    n = collect(s_list, 0, each_id);
+    if (n > LIST) n = collect(s_list, kth_key(k, s_list, each_id), each_id);
+    const int place = rank_in(s_list, n, key);
+    const auto put = [&](int i, int id, double lp) {
+        if (p.top_ids) p.top_ids[(uint64_t)row * k + i] = id;
+        if (p.top_logprob) p.top_logprob[(uint64_t)row * k + i] = (float)lp;
+    };
+    if (tid < n && place < k)
+        put(place, (int)place_of(key),
+            none ? nan : greedy ? (place == 0 ? 0.0 : -INFINITY) : ln2 * scaled(value_of(key), m, rate) - log_z);
+    if (tid >= n && tid < k) put(tid, -1, log_z == log_z ? -INFINITY : nan);
 }
 
 }  // namespace

@@ -663,9 +663,9 @@ struct LogprobPart {
 };
 struct LogprobArgs {
     int n_rows, vocab, top, chunks;
-    int bf16, vec;  // vec: rows start on 16 bytes
+    int bf16, vec;  // vec: row 0 starts on 16 bytes
     const void* logits;
-    uint64_t row;
+    uint64_t row, all;  // elements from row to row, and to the last row's end
     const float* temperature;
     const int32_t* tokens;
     float *logprob, *entropy, *top_logprob;
