@@ -22,8 +22,8 @@ namespace wpcg {
 namespace {
 
 constexpr int THREADS = 256, CHUNK = LOGPROB_CHUNK, VALUES = CHUNK / 64;
+constexpr int LIST = THREADS;  // candidates that are sorted by counting
 constexpr int SEG = 64, SEGS = LOGPROB_SEGS;  // ids of a segment, segments of a chunk
-constexpr int LIST = 256;                    // candidates that are sorted by counting
 
 // log2(e) / T; 0: T is infinite, all ids with a logit above -inf are alike; -1:
 // greedy (T is not above 0).
@@ -169,95 +169,120 @@ __device__ __forceinline__ double scaled(float x, float m, double rate)
     const double d = (double)x - (double)m;
     return rate == 0.0 ? (d == -INFINITY ? d : d * 0.0) : d * rate;
 }
-// Sums over the workgroup's four waves.
+// Sums over the workgroup's four waves: from each wave, and with a barrier between
+// to all.
 struct RowSums {
     double z, s;
     int tops, before;
 };
-__device__ __forceinline__ RowSums block_sums(RowSums v, RowSums* s)
+__device__ __forceinline__ void give_sums(const RowSums& v, RowSums* s)
 {
-    v = {wave_sum_d(v.z), wave_sum_d(v.s), wave_sum_i(v.tops), wave_sum_i(v.before)};
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
+    const RowSums w = {wave_sum_d(v.z), wave_sum_d(v.s), wave_sum_i(v.tops), wave_sum_i(v.before)};
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = w;
+}
+__device__ __forceinline__ RowSums all_sums(const RowSums* s)
+{
     return {(s[0].z + s[1].z) + (s[2].z + s[3].z), (s[0].s + s[1].s) + (s[2].s + s[3].s),
             s[0].tops + s[1].tops + s[2].tops + s[3].tops, s[0].before + s[1].before + s[2].before + s[3].before};
 }
 
 // ---- the K best ------------------------------------------------------------------
 // Keys rise with the value, and fall with the place where values are equal; no
-// two are the same, and that of a place without a value (NaN, -inf) is 0.
-__device__ __forceinline__ uint64_t key_of(float v, uint32_t at)
+// two are the same, and that of a place without a value (NaN, -inf) is 0. Their
+// upper halves are the values' order.
+__device__ __forceinline__ uint32_t order_of(float v)
 {
-    if (!(v > -INFINITY)) return 0;
     const uint32_t b = __float_as_uint(v + 0.0f);  // -0 is 0
-    const uint32_t order = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (uint64_t)order << 32 | (uint32_t)~at;
+    const uint32_t order = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+    return v > -INFINITY ? order : 0;
 }
 __device__ __forceinline__ float value_of(uint64_t key)
 {
     const uint32_t order = (uint32_t)(key >> 32);
     return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
 }
+__device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t at) { return order ? (uint64_t)order << 32 | (uint32_t)~at : 0; }
 __device__ __forceinline__ uint32_t place_of(uint64_t key) { return (uint32_t)~key; }
 
-struct Lists {
-    uint64_t key[LIST];
-    int n[THREADS / 64];
+// Candidates, in no order; zeros behind them.
+struct List {
+    alignas(16) uint64_t key[LIST];
+    int n;
 };
-// All threads' keys at or above `from` (not 0) to the list; how many there are, which
-// may be more than it holds. each(f) calls f for the thread's keys, all threads
-// alike.
-template <class EACH>
-__device__ __forceinline__ int collect(Lists& l, uint64_t from, EACH each)
+// The wave's keys (each(f) calls f with the order and the place of each) for which
+// take(order, place) holds (not for the order 0), to the list. l.n may come to be more than it holds.
+template <class EACH, class TAKE>
+__device__ __forceinline__ void collect(List& l, EACH each, TAKE take)
 {
-    const int wave = (int)threadIdx.x >> 6;
-    int mine = 0;
-    each([&](uint64_t key) { mine += __popcll(__ballot(key != 0 && key >= from)); });
-    if ((threadIdx.x & 63) == 0) l.n[wave] = mine;
-    __syncthreads();
-    int at = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; w++) {
-        if (w == wave) at = all;
-        all += l.n[w];
-    }
-    if (all <= LIST)
-        each([&](uint64_t key) {
-            const bool it = key != 0 && key >= from;
-            const uint64_t them = __ballot(it);
-            if (it) l.key[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0))] = key;
-            at += __popcll(them);
-        });
-    __syncthreads();
-    return all;
+    int n = 0;
+    each([&](uint32_t order, uint32_t at) { n += __popcll(__ballot(take(order, at))); });
+    if (n == 0) return;
+    int to = 0;
+    if ((threadIdx.x & 63) == 0) to = atomicAdd(&l.n, n);
+    to = __builtin_amdgcn_readfirstlane(to);
+    each([&](uint32_t order, uint32_t at) {
+        const bool it = take(order, at);
+        const uint64_t them = __ballot(it);
+        const int x = to + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(them >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0));
+        if (it && x < LIST) l.key[x] = key_of(order, at);
+        to += __popcll(them);
+    });
 }
-// The k-th largest of all threads' keys (0 where there are fewer), bit by bit: of
-// use where equal values make too many candidates to sort.
+// The k-th largest of all threads' keys (0 where there are fewer), bit by bit, and
+// the list emptied: where equal values make too many candidates.
 template <class EACH>
-__device__ uint64_t kth_key(int k, Lists& l, EACH each)
+__device__ uint64_t kth_key(int k, List& l, EACH each)
 {
     uint64_t at = 0;
     for (int bit = 63; bit >= 0; bit--) {
         const uint64_t next = at | (uint64_t)1 << bit;
         int n = 0;
-        each([&](uint64_t key) { n += key >= next; });
+        each([&](uint32_t order, uint32_t at) { n += key_of(order, at) >= next; });
         n = wave_sum_i(n);
-        if ((threadIdx.x & 63) == 0) l.n[threadIdx.x >> 6] = n;
         __syncthreads();
-        if (l.n[0] + l.n[1] + l.n[2] + l.n[3] >= k) at = next;
+        if ((threadIdx.x & 63) == 0) l.key[threadIdx.x >> 6] = (uint64_t)n;
         __syncthreads();
+        if ((int)(l.key[0] + l.key[1] + l.key[2] + l.key[3]) >= k) at = next;
     }
+    __syncthreads();
+    l.key[threadIdx.x] = 0;
+    l.n = 0;
+    __syncthreads();
     return at;
 }
-// The list's entry of this thread, and how many come before it.
-__device__ __forceinline__ int rank_in(const Lists& l, int n, uint64_t& key)
+// The thread's entry of the list (0: none), and how many come before it.
+__device__ __forceinline__ int rank_in(const List& l, int n, uint64_t& key)
 {
     const int tid = (int)threadIdx.x;
-    key = tid < n ? l.key[tid] : 0;
+    key = 0;
     int before = 0;
-    if ((tid & ~63) < n)
-        for (int i = 0; i < n; i++) before += l.key[i] > key;
+    if (__builtin_amdgcn_readfirstlane(tid) >= n) return before;
+    key = l.key[tid];
+    for (int i = 0; i < n; i += 8) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) before += l.key[i + j] > key;
+    }
     return before;
+}
+// The k-th largest order of N a lane (0: there are fewer), its lower half cut off:
+// two bits a step, from the numbers of lanes at or above.
+template <int N>
+__device__ __forceinline__ uint32_t kth_about(const uint32_t (&v)[N], int k)
+{
+    uint32_t at = 0;
+#pragma unroll
+    for (int bit = 30; bit >= 16; bit -= 2) {
+        uint32_t up = 0;
+#pragma unroll
+        for (uint32_t x = 1; x < 4; x++) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < N; j++) n += __popcll(__ballot(v[j] >= (at | x << bit)));
+            up += n >= k;
+        }
+        at |= up << bit;
+    }
+    return at;
 }
 
 constexpr int HELD = 10;  // segments' maxima that a thread has in registers: vocabularies up to 163840
@@ -267,17 +292,25 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
 {
     __shared__ RowSums s_sums[4];
     __shared__ float s_max[4];
-    __shared__ Lists s_list;
-    __shared__ uint64_t s_key[THREADS];
-    const int row = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ List s_list[2];
+    __shared__ uint32_t s_best[THREADS];
+    __shared__ uint64_t s_key[LOGPROB_TOP];
+    const int row = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const LogprobPart* part = p.part + (uint64_t)row * p.chunks;
+    s_list[0].key[tid] = 0;
+    s_list[1].key[tid] = 0;
+    if (tid < 2) s_list[tid].n = 0;
     // everything that is read first, on its way together
     const int n_seg = p.top > 0 ? p.chunks * SEGS : 0;
     const float* seg = p.seg + (uint64_t)row * n_seg;
-    float held[HELD];
+    float maxima[HELD];
     if (n_seg > 0) {
 #pragma unroll
-        for (int i = 0; i < HELD; i++) held[i] = seg[min(tid + i * THREADS, n_seg - 1)];
+        for (int i = 0; i < HELD; i++) {
+            maxima[i] = -INFINITY;
+            if (i * THREADS < n_seg) maxima[i] = seg[min(tid + i * THREADS, n_seg - 1)];
+        }
     }
     const LogprobPart mine = part[min(tid, p.chunks - 1)];
     const double rate = row_rate_d(p, row);
@@ -290,24 +323,24 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     m = wave_max(m);
     if (lane == 0) s_max[wave] = m;
     // the best of the thread's segments, for below
+    uint32_t held[HELD];
     const auto each_seg = [&](auto f) {
         if (n_seg <= HELD * THREADS) {
 #pragma unroll
-            for (int i = 0; i < HELD; i++) {
-                const int at = tid + i * THREADS;
-                f(at < n_seg ? key_of(held[i], (uint32_t)at) : 0);
-            }
+            for (int i = 0; i < HELD; i++) f(held[i], (uint32_t)(tid + i * THREADS));
         } else {
             for (int i0 = 0; i0 < n_seg; i0 += THREADS) {
                 const int at = i0 + tid;
-                f(at < n_seg ? key_of(seg[at], (uint32_t)at) : 0);
+                f(at < n_seg ? order_of(seg[at]) : 0, (uint32_t)at);
             }
         }
     };
     if (n_seg > 0) {
-        uint64_t best = 0;
-        each_seg([&](uint64_t key) { best = key > best ? key : best; });
-        s_key[tid] = best;
+#pragma unroll
+        for (int i = 0; i < HELD; i++) held[i] = tid + i * THREADS < n_seg ? order_of(maxima[i]) : 0;
+        uint32_t best = 0;
+        each_seg([&](uint32_t order, uint32_t) { best = max(best, order); });
+        s_best[tid] = best;
     }
     __syncthreads();
     m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
@@ -327,7 +360,50 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     };
     if (tid < p.chunks) add(mine);
     for (int c = tid + THREADS; c < p.chunks; c += THREADS) add(part[c]);
-    v = block_sums(v, s_sums);
+    give_sums(v, s_sums);
+
+    // The segments: the k-th best of groups of them is no better than the k-th of
+    // all. Groups of the threads with one lane number are 64 and the k-th says
+    // enough up to k of 24; beyond, those of each thread.
+    const int k = p.top;
+    if (n_seg > 0) {
+        const uint32_t best[4] = {s_best[lane], s_best[64 + lane], s_best[128 + lane], s_best[192 + lane]};
+        const uint32_t all[1] = {max(max(best[0], best[1]), max(best[2], best[3]))};
+        const uint32_t least = max(k <= 24 ? kth_about(all, k) : kth_about(best, k), 1u);
+        collect(s_list[0], each_seg, [&](uint32_t order, uint32_t) { return order >= least; });
+    }
+    __syncthreads();
+    // their ids: lane l the l-th of a wave's segments
+    constexpr int MOST = LOGPROB_TOP / (THREADS / 64);
+    int id[MOST], segs = 0;
+    uint32_t own[MOST];  // as they are read
+    if (n_seg > 0) {
+        if (s_list[0].n > LIST) {
+            const uint64_t from = kth_key(k, s_list[0], each_seg);
+            collect(s_list[0], each_seg, [&](uint32_t order, uint32_t at) { return order != 0 && key_of(order, at) >= from; });
+            __syncthreads();
+        }
+        const int n = __builtin_amdgcn_readfirstlane(s_list[0].n);
+        uint64_t key;
+        const int at = rank_in(s_list[0], n, key);
+        if (key != 0 && at < k) s_key[at] = key;
+        segs = min(n, k);
+        __syncthreads();
+        const int skew = row_skew(p, row);
+#pragma unroll
+        for (int i = 0; i < MOST; i++) id[i] = (int)(place_of(s_key[wave + i * (THREADS / 64)]) * SEG) + lane - skew;
+        const auto read = [&](auto* x) {
+#pragma unroll
+            for (int i = 0; i < MOST; i++)
+                if (wave + i * (THREADS / 64) < segs) own[i] = x[min(max(id[i], 0), p.vocab - 1)];
+        };
+        if (p.bf16) read((const uint16_t*)p.logits + (uint64_t)row * p.row);
+        else read((const uint32_t*)p.logits + (uint64_t)row * p.row);
+    }
+
+    // (while they are on their way)
+    if (n_seg == 0 && wave > 0) return;
+    v = all_sums(s_sums);
     const double z = v.z + (double)(v.tops - 1);  // Z - 1
     const double ln2 = 0.6931471805599453, nan = __builtin_nan("");
     const bool greedy = rate < 0.0;
@@ -346,52 +422,33 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     }
     if (n_seg == 0) return;
 
-    // The segments: the k-th best of 64 groups (of the threads of one lane number) is
-    // no better than the k-th of all; its value is the least of those that fewer
-    // than k groups are above (none: all that there are).
-    const int k = p.top;
-    uint32_t group = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; w++) group = max(group, (uint32_t)(s_key[64 * w + lane] >> 32));
-    int above = 0;
-#pragma unroll 16
-    for (int i = 0; i < 64; i++) above += (uint32_t)__builtin_amdgcn_readlane((int)group, i) > group;
-    const uint32_t least = ~(uint32_t)(0x80000000u ^ (uint32_t)wave_max_i((int)(0x80000000u ^ (above < k ? ~group : 0u))));
-    uint64_t from = (uint64_t)least << 32;
-    int n = collect(s_list, from, each_seg);
-    if (n > LIST) n = collect(s_list, kth_key(k, s_list, each_seg), each_seg);
-    uint64_t key;
-    const int at = rank_in(s_list, n, key);
-    if (tid < n && at < k) s_key[at] = key;
-    __syncthreads();
-    const int segs = min(n, k);
-    // their ids: lane l the l-th of a wave's segments
-    constexpr int MOST = LOGPROB_TOP / (THREADS / 64);
     const uint32_t worst = segs < k ? 0u : (uint32_t)(s_key[segs - 1] >> 32);
-    const int skew = row_skew(p, row);
-    uint64_t own[MOST];
 #pragma unroll
-    for (int i = 0; i < MOST; i++) {
-        const int y = wave + i * (THREADS / 64);
-        own[i] = 0;
-        if (y < segs) {
-            const int id = (int)(place_of(s_key[y]) * SEG) + lane - skew;
-            own[i] = key_of(logit(p, row, min(max(id, 0), p.vocab - 1)), (uint32_t)id);
-            if ((uint32_t)id >= (uint32_t)p.vocab || (uint32_t)(own[i] >> 32) < worst) own[i] = 0;
+    for (int i = 0; i < MOST; i++)
+        if (wave + i * (THREADS / 64) < segs) {
+            const uint32_t order = order_of(__uint_as_float(p.bf16 ? own[i] << 16 : own[i]));
+            own[i] = (uint32_t)id[i] < (uint32_t)p.vocab && order >= worst ? order : 0;
         }
-    }
     const auto each_id = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < MOST; i++) f(own[i]);
+        for (int i = 0; i < MOST; i++)
+            if (wave + i * (THREADS / 64) < segs) f(own[i], (uint32_t)id[i]);
     };
-    n = collect(s_list, 0, each_id);
-    if (n > LIST) n = collect(s_list, kth_key(k, s_list, each_id), each_id);
-    const int place = rank_in(s_list, n, key);
+    collect(s_list[1], each_id, [](uint32_t order, uint32_t) { return order != 0; });
+    __syncthreads();
+    if (s_list[1].n > LIST) {
+        const uint64_t from = kth_key(k, s_list[1], each_id);
+        collect(s_list[1], each_id, [&](uint32_t order, uint32_t at) { return order != 0 && key_of(order, at) >= from; });
+        __syncthreads();
+    }
+    const int n = __builtin_amdgcn_readfirstlane(s_list[1].n);
+    uint64_t key;
+    const int place = rank_in(s_list[1], n, key);
     const auto put = [&](int i, int id, double lp) {
         if (p.top_ids) p.top_ids[(uint64_t)row * k + i] = id;
         if (p.top_logprob) p.top_logprob[(uint64_t)row * k + i] = (float)lp;
     };
-    if (tid < n && place < k)
+    if (key != 0 && place < k)
         put(place, (int)place_of(key),
             none ? nan : greedy ? (place == 0 ? 0.0 : -INFINITY) : ln2 * scaled(value_of(key), m, rate) - log_z);
     if (tid >= n && tid < k) put(tid, -1, log_z == log_z ? -INFINITY : nan);
