@@ -32,10 +32,13 @@ __device__ __forceinline__ double row_rate_d(const LogprobArgs& p, int row)
     const float t = p.temperature ? p.temperature[row] : 1.0f;
     return t > 0.0f ? 1.4426950408889634 / (double)t : -1.0;
 }
-// The same in fp32: finite, so that 0 times it is 0.
+// The same in fp32: finite, so that 0 times it is 0, and not 0, so that -inf times
+// it is -inf (the least one scales any difference to less than 2^-20: off by less
+// than exp2_fast is).
 __device__ __forceinline__ float row_rate(const LogprobArgs& p, int row)
 {
-    return (float)fmin(row_rate_d(p, row), 3.0e38);
+    const float rate = (float)fmin(row_rate_d(p, row), 3.0e38);
+    return rate == 0.0f ? 0x1p-149f : rate;
 }
 
 // Rows need not start on 16 bytes: chunks and segments are of places from the last
@@ -138,24 +141,30 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
     const float base = best == -INFINITY ? 0.0f : best;
     float z[2] = {0.0f, 0.0f}, s[2] = {0.0f, 0.0f};
     int tops = 0, before = 0;
-    bool same = false;
 #pragma unroll
     for (int i = 0; i < VALUES; i++) {
         const float d = c.v[i] - base;
-        float t = d * rate;
-        if (rate == 0.0f) t = d == -INFINITY ? d : t;
+        const float t = d * rate;
         const bool top = c.v[i] == best;
         // (a NaN reaches z here, and only here)
         const float e = top ? 0.0f : exp2_fast(t);
         z[i & 1] += e;
         s[i & 1] = fmaf(e, fmaxf(t, -200.0f), s[i & 1]);
         tops += __popcll(__ballot(top));
-        before += __popcll(__ballot(c.v[i] > xt));
-        same |= c.v[i] == xt;
     }
-    if (__any(same)) {  // equal logits of lower ids come before, too
+    // greater logits come before the token's, and equal ones of lower ids
+    if (inside) {
+        if (id0 > token) {
 #pragma unroll
-        for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] == xt && id0 + C::place(i) < token));
+            for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] > xt));
+        } else if (id0 >= 0 && id0 + CHUNK <= token) {
+#pragma unroll
+            for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] >= xt));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VALUES; i++)
+                before += __popcll(__ballot(c.v[i] > xt || (c.v[i] == xt && (uint32_t)(id0 + C::place(i)) < (uint32_t)token)));
+        }
     }
     const float zs = wave_sum(z[0] + z[1]), ss = wave_sum(s[0] + s[1]);
     if (lane == 0)
