@@ -95,17 +95,18 @@ __device__ __forceinline__ int block_before(int v, int* s, int& total)
     __syncthreads();
     return start + t - v;
 }
-// The blocks' counts before block b, and all of them.
-__device__ __forceinline__ void blocks_before(const int* count, int n, int b, int* s, int& before, int& total)
+// The blocks' counts before block b, and all of them. Every wave adds them up for
+// itself: no barrier before what comes next is loaded.
+__device__ __forceinline__ void blocks_before(const int* count, int n, int b, int& before, int& total)
 {
     int x = 0, y = 0;
-    for (int i = (int)threadIdx.x; i < n; i += THREADS) {
+    for (int i = (int)threadIdx.x & 63; i < n; i += 64) {
         const int v = count[i];
         x += i < b ? v : 0;
         y += v;
     }
-    block_before(x, s, before);
-    block_before(y, s, total);
+    before = wave_sum_i(x);
+    total = wave_sum_i(y);
 }
 
 // ---- fork ----------------------------------------------------------------------
@@ -194,43 +195,51 @@ __global__ __launch_bounds__(THREADS) void k_fork_plan(ForkArgs a)
     }
 }
 
+constexpr int BASES = 1024;  // sequences whose first fresh page is held in LDS
+
 __global__ __launch_bounds__(THREADS) void k_fork_apply(ForkArgs a)
 {
-    __shared__ int s_sums[WAVES];
+    __shared__ int s_sums[WAVES], s_base[BASES];
     const PoolArgs& p = a.p;
     const int tid = (int)threadIdx.x, b = (int)blockIdx.x, need = a.totals[0];
     int before, free;
-    blocks_before(a.count, a.blocks, b, s_sums, before, free);
+    blocks_before(a.count, a.blocks, b, before, free);
     const bool enough = need <= free;
     if (b == 0 && tid == 0) {
         a.result[0] = free - need;
         a.result[1] = enough ? a.totals[1] : 0;
     }
     if (b < a.blocks) {
-        if (!enough || before >= need) return;
         // thread t: pages PER t .. of the block, so that ranks rise with threads
         const int page0 = b * BLOCK + PER * tid;
         bool is[PER];
         int n = 0, all;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            is[i] = page0 + i < p.n_pages && p.refs[page0 + i] == 0;
-            n += is[i];
-        }
+        for (int i = 0; i < PER; i++) is[i] = page0 + i < p.n_pages && p.refs[page0 + i] == 0;
+        // every step-th sequence's base, so that few steps of a search read memory
+        const int step = max(1, (p.n_seq + BASES - 1) / BASES), bases = (p.n_seq + step - 1) / step;
+        if (tid < bases) s_base[tid] = a.rows[tid * step].base;
+        if (!enough || before >= need) return;
+#pragma unroll
+        for (int i = 0; i < PER; i++) n += is[i];
         int rank = before + block_before(n, s_sums, all);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             if (!is[i] || rank >= need) continue;
             // the last sequence whose fresh pages begin at or before this one
-            int lo = 0, hi = p.n_seq - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (a.rows[mid].base <= rank) lo = mid;
-                else hi = mid - 1;
-            }
-            const ForkRow r = a.rows[lo];
+            const auto last = [&](int lo, int hi, auto base) {
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) / 2;
+                    if (base(mid) <= rank) lo = mid;
+                    else hi = mid - 1;
+                }
+                return lo;
+            };
+            int to = last(0, bases - 1, [&](int x) { return s_base[x]; }) * step;
+            to = last(to, min(to + step, p.n_seq) - 1, [&](int x) { return a.rows[x].base; });
+            const ForkRow r = a.rows[to];
             const int j = r.from + rank - r.base;
-            p.table[(uint64_t)lo * p.stride + j] = page0 + i;
+            p.table[(uint64_t)to * p.stride + j] = page0 + i;
             p.refs[page0 + i] = 1;
             if (r.copy >= 0 && j == r.from) {
                 int32_t* c = a.copies + (uint64_t)r.copy * 3;
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(THREADS) void k_compact_rank(CompactArgs a)
     __shared__ int s_sums[WAVES];
     const int b = (int)blockIdx.x, page0 = b * BLOCK + PER * (int)threadIdx.x;
     int before, used;
-    blocks_before(a.count, a.blocks, b, s_sums, before, used);
+    blocks_before(a.count, a.blocks, b, before, used);
     if (b == 0 && threadIdx.x == 0) *a.total = used;
     bool is[PER];
     int n = 0, all;
