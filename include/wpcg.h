@@ -471,6 +471,19 @@ int wpcg_model_verify(wpcg_model* m, const uint32_t* tokens, uint32_t n, uint32_
  * next token is fed. No reference counterpart. */
 int wpcg_model_verify_sampled(wpcg_model* m, const uint32_t* tokens, uint32_t n, const float* draft_probs,
                               const float* u, float u_next, float temperature, uint32_t* accepted, int32_t* out);
+/* How likely the model holds what it is fed, and what it would say instead: the n
+ * tokens at the next n positions as with wpcg_model_verify, and from row i's
+ * logits, those after tokens[0..i], wpcg_logprobs' outputs for targets[i]: its
+ * log probability and rank, the entropy, the top (<= WPCG_LOGPROB_TOP) best ids
+ * and theirs, at one temperature (1: the model's own). Targets are mostly the
+ * tokens that follow: tokens[i + 1], and any for the last row. An answer's score
+ * is the sum of its log probabilities. All arrays are the host's; any output may
+ * be null (targets with logprob and rank), and is as wpcg_logprobs says.
+ * 1 <= n <= WPCG_VERIFY_MAX; longer answers in turns of it. No reference
+ * counterpart. */
+int wpcg_model_score(wpcg_model* m, const uint32_t* tokens, uint32_t n, const int32_t* targets, float temperature,
+                     uint32_t top, float* logprob, float* entropy, int32_t* rank, int32_t* top_ids,
+                     float* top_logprob);
 /* Move the position back to pos (<= the current one): later cache entries
  * are ignored and overwritten by the next steps. No reference counterpart. */
 int wpcg_model_set_position(wpcg_model* m, uint32_t pos);

@@ -54,6 +54,11 @@ def test_right_scores_end_at_the_context():
     refused(score(None), E_ARG, "null")
 
 
+def test_model_scores():
+    call = wpcg.lib.wpcg_model_score
+    refused(call(None, AT, 4, AT, 1.0, 0, AT, None, None, None, None), E_ARG, "null")
+
+
 def test_score_workspace():
     n = C.c_uint64(7)
     assert SCORE_WS(ref(scores()), C.byref(n)) == OK and n.value == 5 * 20 + 12 + 5 * 32 * 4

@@ -48,6 +48,7 @@ struct Prefill {
     uint32_t* vids = nullptr;  // [WPCG_VERIFY_MAX]
     float* draft_probs = nullptr;  // sampled verification: [WPCG_VERIFY_MAX - 1][vocab], made on first use
     void* draft = nullptr;         // its other arrays and workspace
+    void* score = nullptr;         // the arrays and the workspace of scores, made on first use
 };
 
 }  // namespace
@@ -1307,6 +1308,80 @@ int wpcg_model_verify_sampled(wpcg_model* m, const uint32_t* tokens, uint32_t n,
     if (int rc = take_state(m, nullptr)) return rc;  // waits for the stream
     *accepted = words[2 * WPCG_VERIFY_MAX + 2];
     std::memcpy(out, words + 3 * WPCG_VERIFY_MAX, n * 4);
+    return WPCG_OK;
+}
+
+int wpcg_model_score(wpcg_model* m, const uint32_t* tokens, uint32_t n, const int32_t* targets, float temperature,
+                     uint32_t top, float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprob)
+{
+    if (!m || !tokens) return fail(WPCG_E_ARG, "null argument");
+    if (!targets && (logprob || rank)) return fail(WPCG_E_ARG, "log probabilities and ranks need tokens");
+    if (n == 0 || n > WPCG_VERIFY_MAX) return fail(WPCG_E_ARG, "score takes 1.." + std::to_string(WPCG_VERIFY_MAX) + " tokens");
+    if (top > WPCG_LOGPROB_TOP) return fail(WPCG_E_ARG, "top is at most " + std::to_string(WPCG_LOGPROB_TOP));
+    for (uint32_t i = 0; i < n; i++)
+        if (tokens[i] >= m->cfg.vocab) return fail(WPCG_E_ARG, "token id out of range");
+    if (int rc = ready(m)) return rc;
+    hipStream_t s = m->ctx->stream;
+    const size_t V = m->cfg.vocab;
+    if (int rc = host_state(m)) return rc;
+    DecodeState st = m->hst;
+    if ((uint64_t)st.pos + n > m->cfg.max_pos) return fail(WPCG_E_ARG, "KV cache full (max_pos reached)");
+    const uint32_t pos0 = st.pos;
+    if (int rc = make_verify(m)) return rc;
+    // beside the logits, for WPCG_VERIFY_MAX rows: targets, temperature; logprob,
+    // entropy, rank, the best ids and theirs; then the workspace
+    constexpr uint32_t ROWS = WPCG_VERIFY_MAX, IN = 2 * ROWS, WORDS = IN + 3 * ROWS + 2 * ROWS * WPCG_LOGPROB_TOP;
+    wpcg_logprob d{};
+    d.n_rows = ROWS;
+    d.vocab = (uint32_t)V;
+    d.top = WPCG_LOGPROB_TOP;
+    d.dtype = WPCG_DTYPE_F32;
+    uint64_t ws = 0;
+    if (int rc = wpcg_logprobs_workspace(&d, &ws)) return rc;
+    Prefill& P = m->pf;
+    if (!P.score) {
+        WPCG_HIP(hipMalloc(&P.score, WORDS * 4 + ws));
+        m->allocs.push_back(P.score);
+    }
+    uint32_t* w = (uint32_t*)P.score;
+    uint32_t words[WORDS] = {};
+    if (targets) std::memcpy(words, targets, n * 4);
+    for (uint32_t i = 0; i < n; i++) std::memcpy(&words[ROWS + i], &temperature, 4);
+    WPCG_HIP(hipMemcpyAsync(w, words, IN * 4, hipMemcpyHostToDevice, s));
+    WPCG_HIP(hipStreamSynchronize(s));  // `words` is read
+    st.n_prompt = 0xffffffffu;
+    if (int rc = put_state(m, st, tokens, n)) return rc;
+    m->hst_ok = false;
+    if (m->mode == WPCG_MODE_FAST && m->use_prefill && prefill_ok(m)) {
+        if (int rc = verify_run(m, pos0, n)) return rc;
+    } else {
+        for (uint32_t i = 0; i < n; i++) {
+            if (int rc = run_step(m, pos0 + i)) return rc;
+            WPCG_HIP(launch_copy_words(P.vlogits + i * V, m->logits, (uint32_t)V, s));
+        }
+    }
+    d.n_rows = n;
+    d.top = top;
+    d.logits_dev = P.vlogits;
+    d.tokens_dev = targets ? (const int32_t*)w : nullptr;
+    d.temperature_dev = (const float*)w + ROWS;
+    float* f = (float*)w + IN;
+    d.logprob_dev = logprob ? f : nullptr;
+    d.entropy_dev = entropy ? f + ROWS : nullptr;
+    d.rank_dev = rank ? (int32_t*)f + 2 * ROWS : nullptr;
+    d.top_ids_dev = top_ids ? (int32_t*)f + 3 * ROWS : nullptr;
+    d.top_logprob_dev = top_logprob ? f + 3 * ROWS + ROWS * WPCG_LOGPROB_TOP : nullptr;
+    if (int rc = wpcg_logprobs(m->ctx, &d, w + WORDS, ws, s)) return rc;
+    WPCG_HIP(hipMemcpyAsync(words + IN, f, (WORDS - IN) * 4, hipMemcpyDeviceToHost, s));
+    if (int rc = take_state(m, nullptr)) return rc;  // waits for the stream
+    const auto give = [&](void* to, uint32_t at, uint32_t count) {
+        if (to && count) std::memcpy(to, &words[IN + at], (size_t)count * 4);
+    };
+    give(logprob, 0, n);
+    give(entropy, ROWS, n);
+    give(rank, 2 * ROWS, n);
+    give(top_ids, 3 * ROWS, n * top);
+    give(top_logprob, 3 * ROWS + ROWS * WPCG_LOGPROB_TOP, n * top);
     return WPCG_OK;
 }
 

@@ -125,6 +125,7 @@ _SIGS = {
     "wpcg_model_prefill": (C.c_int, [_p, _p, C.c_uint32, _p, C.POINTER(C.c_uint32)]),
     "wpcg_model_set_prefill": (C.c_int, [_p, C.c_int]),
     "wpcg_model_verify": (C.c_int, [_p, _p, C.c_uint32, _p, _p]),
+    "wpcg_model_score": (C.c_int, [_p, _p, C.c_uint32, _p, C.c_float, C.c_uint32] + [_p] * 5),
     "wpcg_model_verify_sampled": (C.c_int, [_p, _p, C.c_uint32, _p, _p, C.c_float, C.c_float,
                                             C.POINTER(C.c_uint32), _p]),
     "wpcg_model_set_position": (C.c_int, [_p, C.c_uint32]),
@@ -1265,6 +1266,24 @@ class Model:
                                             None if draft_probs is None else _np_ptr(draft_probs),
                                             _np_ptr(u), u_next, temperature, C.byref(n), _np_ptr(out)))
         return n.value, out
+
+    def score(self, tokens, targets=None, temperature: float = 1.0, top: int = 0):
+        """dict of, for the rows after each token: logprob and rank of targets
+        (None: of none), entropy, and top_ids, top_logprob [n][top]"""
+        t = np.ascontiguousarray(tokens, np.uint32)
+        n = t.size
+        out = {"entropy": np.empty(n, np.float32), "top_ids": np.empty((n, top), np.int32),
+               "top_logprob": np.empty((n, top), np.float32)}
+        if targets is not None:
+            targets = np.ascontiguousarray(targets, np.int32)
+            if targets.size != n:
+                raise ValueError(f"{n} tokens need {n} targets, not {targets.size}")
+            out.update(logprob=np.empty(n, np.float32), rank=np.empty(n, np.int32))
+        p = {k: _np_ptr(v) for k, v in out.items()}
+        check(lib.wpcg_model_score(self.h, _np_ptr(t), n, None if targets is None else _np_ptr(targets), temperature,
+                                   top, p.get("logprob"), p["entropy"], p.get("rank"), p["top_ids"],
+                                   p["top_logprob"]))
+        return out
 
     def set_position(self, pos: int):
         check(lib.wpcg_model_set_position(self.h, pos))
