@@ -236,6 +236,11 @@ def test_prefix_workspace():
     assert wpcg.lib.wpcg_paged_attention_workspace(ref(pages()), ref(b), ref(attention()), C.byref(plain)) == OK
     for y in (prefix(n_groups=0), prefix(max_prefix=0), prefix(n_groups=64, max_prefix=9000), prefix(n_groups=1, max_prefix=500)):
         assert attend_ws(pages(), b, y, attention()) == plain.value
+    # a window reads no more again than it sees
+    assert attend_ws(pages(), b, x, attention(window=8000, sinks=10)) == n
+    narrow = attention(window=700, sinks=10)
+    assert wpcg.lib.wpcg_paged_attention_workspace(ref(pages()), ref(b), ref(narrow), C.byref(plain)) == OK
+    assert attend_ws(pages(), b, x, narrow) == plain.value
     assert ATTEND_WS(ref(pages()), ref(batch()), ref(prefix()), ref(attention()), None) == E_ARG
     # the parts' places hold whatever the bounds allow, loose rows too
     assert attend_ws(pages(), batch(n_seq=64, n_rows=1 << 20, max_q=1, max_kv=10000, table_stride=1000), x, attention()) == n

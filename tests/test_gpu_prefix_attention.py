@@ -24,9 +24,9 @@ def ctx():
 class Groups:
     """A batch whose groups share: groups = [(prefix, [own tokens of each sequence])].
     loose: a length by whose bounds the prefixes would be long enough (900 MB read
-    again) for sharing to be chosen."""
+    again) for sharing to be chosen. Behind the groups are `empty` sequences."""
 
-    def __init__(self, ctx, rng, groups, dtype, hkv, d, page, order="head", width=0):
+    def __init__(self, ctx, rng, groups, dtype, hkv, d, page, order="head", width=0, empty=0):
         self.ctx, self.groups = ctx, groups
         again = max(1, sum(len(own) - 1 for _, own in groups)) * 2 * hkv * d * R.SIZE[dtype]
         self.loose = max(width * page, -(-int(900e6) // again // page) * page,
@@ -34,7 +34,7 @@ class Groups:
         width = self.loose // page
         self.size = [len(own) for _, own in groups]
         self.prefix = [p for p, _ in groups]
-        lens = [p + m for p, own in groups for m in own]
+        lens = [p + m for p, own in groups for m in own] + [0] * empty
         self.pg = pg = R.Paged(ctx, rng, dtype, hkv, d, page, lens, order=order, scales=dtype == E4M3, width=width)
         self.start = np.cumsum([0] + self.size)
         for g, (p, own) in enumerate(groups):
@@ -74,7 +74,7 @@ def expected(pg, q, rows, q_dtype, scale, window, sinks):
 
 
 def check(got, want, bound):
-    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.isnan(got), np.isnan(want)), f"NaN in rows, heads {np.argwhere(np.isnan(got).any(-1))[:40].tolist()}"
     off = np.abs(got - want) - bound
     i = np.unravel_index(np.nanargmax(off), off.shape)
     assert not (off > 0).any(), f"{(off > 0).sum()} of {off.size} off, worst {i}: {got[i]} for {want[i]} +- {bound[i]}"
@@ -93,10 +93,17 @@ def run(ctx, pg, batch, prefix, q, heads, q_dtype, scale, window=0, sinks=0, str
     return R.decode(out.read(R.BITS[q_dtype], rows * heads * pg.d).reshape(rows, heads, pg.d), q_dtype)
 
 
-def one(ctx, rng, groups, q_dtype, dtype, hkv, heads, d, page, rows=1, window=0, sinks=0, order="head", null_start=False):
-    g = Groups(ctx, rng, groups, dtype, hkv, d, page, order)
+def least_window(q_dtype, dtype, hkv, d, n):
+    """The fewest tokens that n sequences can read again for sharing to be chosen."""
+    pays = 250e6 if q_dtype == BF16 else 700e6 if dtype == F32 else 450e6
+    return -(-int(pays) // (n * 2 * hkv * d * R.SIZE[dtype]))
+
+
+def one(ctx, rng, groups, q_dtype, dtype, hkv, heads, d, page, rows=1, window=0, sinks=0, order="head", null_start=False,
+        empty=0):
+    g = Groups(ctx, rng, groups, dtype, hkv, d, page, order, empty=empty)
     n = len(g.pg.kv_len)
-    per = [rows] * n if np.isscalar(rows) else rows
+    per = [rows] * (n - empty) + [0] * empty if np.isscalar(rows) else rows
     q = R.encode(rng.standard_normal((sum(per), heads, d)) * 1.5, q_dtype)
     scale = d ** -0.5
     want, bound = expected(g.pg, q, per, q_dtype, scale, window, sinks)
@@ -108,6 +115,8 @@ def one(ctx, rng, groups, q_dtype, dtype, hkv, heads, d, page, rows=1, window=0,
     check(got, want, bound)
     plain = wpcg.PagedAttention(ctx, g.pg.kv, batch, heads, q_dtype, scale=scale, window=window, sinks=sinks)
     few = max(per) * heads // hkv <= 32 and n <= 512 and len(groups) <= 256 and n > len(groups)
+    if window:  # what a window lets be read again
+        few &= window + sinks + max(per) >= least_window(q_dtype, dtype, hkv, d, n - len(groups))
     assert (run.workspace != plain.workspace_bytes) == few
     return g, batch, q, got, want, bound
 
@@ -149,6 +158,19 @@ def test_windows(ctx, q_dtype, dtype, window, sinks):
     rng = np.random.default_rng(window + sinks + 10 * q_dtype + dtype)
     groups = [(200, [3, 40, 130, 90]), (37, [120, 3, 8]), (300, [20] * 5), (10, [400, 5])]
     one(ctx, rng, groups, q_dtype, dtype, 2, 8, 64, 16, rows=3, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("more,sinks", [(0, 0), (1, 3), (17, 16), (30, 70), (100, 4), (0, 330), (3000, 5)])
+def test_windows_over_shared_prefixes(ctx, q_dtype, dtype, more, sinks):
+    """The same with windows wide enough, by a batch's bounds, for sharing to be
+    chosen: 512 sequences, most of them empty."""
+    print(f"[gpu] prefix shared window {q_dtype}/{dtype} {more} {sinks}", flush=True)
+    rng = np.random.default_rng(more + sinks + 10 * q_dtype + dtype)
+    w = least_window(q_dtype, dtype, 16, 128, 512 - 4)
+    groups = [(w + 50, [3, 40, 130, 90]), (37, [120, 3, 8]), (w + 150, [20] * 5), (10, [w + 200, 5])]
+    # (one() says that the call shares)
+    one(ctx, rng, groups, q_dtype, dtype, 16, 32, 128, 16, rows=3, window=w + more, sinks=sinks, empty=512 - 14)
 
 
 @pytest.mark.parametrize("q_dtype,dtype", TYPES)
@@ -231,19 +253,24 @@ def test_values_that_are_not_finite(ctx, q_dtype, dtype):
     """NaN and infinities at tokens that a window hides from some rows reach those
     that see them alone."""
     rng = np.random.default_rng(7 + dtype)
-    g = Groups(ctx, rng, [(100, [3, 60, 90]), (64, [5, 80])], dtype, 1, 64, 16)
+    # (the batch's other sequences are empty: enough of them for a window to share)
+    w = least_window(q_dtype, dtype, 8, 128, 510)
+    g = Groups(ctx, rng, [(w + 30, [3, 60, 90]), (64, [5, 80])], dtype, 8, 128, 16, empty=507)
     pg = g.pg
-    q = R.encode(rng.standard_normal((5, 4, 64)), q_dtype)
-    batch = g.batch([1] * 5)
-    want, bound = expected(pg, q, [1] * 5, q_dtype, 0.125, 70, 2)
+    q = R.encode(rng.standard_normal((5, 16, 128)), q_dtype)
+    batch = g.batch([1] * 5 + [0] * 507)
+    want, bound = expected(pg, q, [1] * 5, q_dtype, 0.125, w, 2)
+    plain = wpcg.PagedAttention(ctx, pg.kv, batch, 16, q_dtype, scale=0.125, window=w, sinks=2).workspace_bytes
     words = {F32: (0x7F800000, 0xFF800000, 0x7FC00000), BF16: (0x7F80, 0xFF80, 0x7FC0)}[dtype]
-    # the row of sequence 0 (103 tokens) sees the prefix from 33 on, those of 1 and 2 from 90 and not at all
-    for w in words:
+    # the row of sequence 0 sees the prefix from its 33rd token on, those of 1 and 2 from the 90th and the 120th
+    for word in words:
         for n in "kv":
             x = pg.bits[n].copy()
-            x[pg.index(0, [60])] = w
+            x[pg.index(0, [60])] = word
             (pg.dk if n == "k" else pg.dv).write(x)
-            got = run(ctx, pg, batch, g.desc(), q, 4, q_dtype, 0.125, 70, 2)
+            got = run(ctx, pg, batch, g.desc(), q, 16, q_dtype, 0.125, w, 2)
+            print(f"[gpu] prefix with {word:#x} in {n}", flush=True)
+            assert run.workspace != plain
             check(got[1:], want[1:], bound[1:])
             assert not (np.abs(got[0] - want[0]) <= bound[0]).all()
             (pg.dk if n == "k" else pg.dv).write(pg.bits[n])
