@@ -155,16 +155,17 @@ class Cache:
                 b.write(w)
 
 
+@pytest.mark.parametrize("stride", [7, 1100])
 @pytest.mark.parametrize("dtype,hkv,d,page,order,n_layers", [
     (BF16, 2, 128, 16, "head", 3), (F32, 1, 64, 32, "token", 2), (E4M3, 3, 64, 16, "token", 2), (E4M3, 2, 128, 64, "head", 1),
     (F32, 2, 128, 16, "head", 2), (BF16, 1, 64, 256, "token", 70)])
-def test_lives_of_sequences(ctx, dtype, hkv, d, page, order, n_layers):
+def test_lives_of_sequences(ctx, dtype, hkv, d, page, order, n_layers, stride):
     """Begun, grown, forked, cut back, ended and moved together at random, with
-    the tokens followed."""
+    the tokens followed; rows short enough for one workgroup, and long ones."""
     print(f"[gpu] pool lives {dtype} {hkv}x{d} page {page} layers {n_layers}", flush=True)
     rng = np.random.default_rng(page + d + dtype)
     n = 6
-    ref = Pool(40, page, n, 7)
+    ref = Pool(40, page, n, stride)
     cache = Cache(ctx, ref, n_layers, hkv, d, dtype, order)
     dev = Device(ctx, ref, cache.layers)
     shortages = 0
@@ -279,7 +280,8 @@ def test_running_out_and_just_enough(ctx):
 
 
 @pytest.mark.parametrize("n_pages,n,stride", [(1, 1, 1), (4095, 3, 1023), (4096, 2, 1024), (4097, 2, 1025), (9000, 2100, 3),
-                                              (20000, 5, 3000), (300000, 1025, 2)])
+                                              (20000, 5, 3000), (300000, 1025, 2), (8192, 64, 128), (8193, 64, 128),
+                                              (2000, 65, 32), (4096, 33, 129), (3000, 32, 256), (900, 10, 512), (100, 17, 7)])
 def test_sizes_of_pools(ctx, n_pages, n, stride):
     """Around the blocks of pages, of a row's entries and of sequences."""
     print(f"[gpu] pool of {n_pages} pages, {n} sequences of {stride}", flush=True)

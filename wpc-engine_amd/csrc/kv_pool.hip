@@ -60,6 +60,10 @@ __device__ __forceinline__ bool writes_tail(const PoolArgs& p, const ForkRow& r)
 {
     return (r.keep & (p.page - 1)) != 0 && r.size > r.keep;
 }
+__device__ __forceinline__ bool keeps(const ForkRow& r, int j)
+{
+    return j < r.kept_pages && !(j >= r.dead0 && j < r.dead1);
+}
 // The row's entry j before, and what it keeps there (-1: none).
 __device__ __forceinline__ int old_entry(const PoolArgs& p, const ForkRow& r, int s, int j)
 {
@@ -68,8 +72,7 @@ __device__ __forceinline__ int old_entry(const PoolArgs& p, const ForkRow& r, in
 }
 __device__ __forceinline__ int kept_entry(const PoolArgs& p, const ForkRow& r, int j)
 {
-    const bool some = j < r.kept_pages && !(j >= r.dead0 && j < r.dead1);
-    const int id = some ? p.table[(uint64_t)r.parent * p.stride + j] : -1;
+    const int id = keeps(r, j) ? p.table[(uint64_t)r.parent * p.stride + j] : -1;
     return is_page(p, id) ? id : -1;
 }
 
@@ -274,6 +277,159 @@ __global__ __launch_bounds__(THREADS) void k_fork_apply(ForkArgs a)
     }
 }
 
+// A whole fork by one workgroup, where every thread has ONE_ENTRIES table entries at
+// most and a wave's pages are ONE_PAGES rows of 64: the same three steps with barriers
+// between them instead of launches. Thread t: of sequence t / team, the entries
+// t % team, + team ..
+constexpr int ONE_SEQS = 64, ONE_ENTRIES = 8, ONE_PAGES = 8;
+__global__ __launch_bounds__(THREADS) void k_fork_one(ForkArgs a, int team_shift)
+{
+    __shared__ int s_sums[WAVES];
+    __shared__ __attribute__((aligned(16))) int s_tail[ONE_SEQS];
+    __shared__ ForkRow s_rows[ONE_SEQS];
+    const PoolArgs& p = a.p;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int team = 1 << team_shift, s = tid >> team_shift, t = tid & (team - 1);
+    const bool live = s < p.n_seq, leads = live && t == 0;
+    const auto count_of = [&](int page) { return __hip_atomic_load(&p.refs[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
+    const auto add = [&](int page, int n) {
+        (void)__hip_atomic_fetch_add(&p.refs[page], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    ForkRow r = {};
+    r.parent = -1;
+    if (live) r = fork_row(a, s);
+    const int entries = max(r.old_pages, r.kept_pages);
+    const bool writer = writes_tail(p, r);
+    if (leads && !writer) s_tail[s] = -1;
+    if (tid >= p.n_seq && tid < (p.n_seq + 3) / 4 * 4) s_tail[tid] = -1;
+    const int32_t* const old = p.table + (uint64_t)(live ? s : 0) * p.stride;
+    const int32_t* const from_row = p.table + (uint64_t)max(r.parent, 0) * p.stride;
+    int is[ONE_ENTRIES];
+    int was[ONE_ENTRIES];
+#pragma unroll
+    for (int i = 0; i < ONE_ENTRIES; i++) {
+        const int x = min(t + i * team, p.stride - 1);
+        was[i] = is[i] = -1;
+        if (__any(t + i * team < entries)) {  // (no load behind a condition of its lanes)
+            was[i] = old[x];
+            is[i] = from_row[x];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ONE_ENTRIES; i++) {
+        const int j = t + i * team;
+        if (!__any(j < entries)) continue;
+        const int w = j < r.old_pages && is_page(p, was[i]) ? was[i] : -1;
+        const int x = keeps(r, j) && is_page(p, is[i]) ? is[i] : -1;
+        is[i] = x;
+        if (w != x) {
+            if (w >= 0) add(w, -1);
+            if (x >= 0) add(x, 1);
+        }
+        if (writer && j == r.keep >> p.shift) s_tail[s] = x;
+    }
+    __syncthreads();
+
+    // the free pages, ranks rising with the wave's rows
+    const int rows = (p.n_pages + THREADS - 1) / THREADS, page0 = wave * rows * 64 + lane;
+    int refs[ONE_PAGES];
+#pragma unroll
+    for (int i = 0; i < ONE_PAGES; i++) {
+        refs[i] = 1;
+        if (i < rows) refs[i] = count_of(min(page0 + 64 * i, p.n_pages - 1));
+    }
+    const int tail = leads ? s_tail[s] : -1, held = tail >= 0 ? count_of(tail) : 0;
+    uint64_t free_row[ONE_PAGES];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < ONE_PAGES; i++) {
+        free_row[i] = 0;
+        if (i < rows) free_row[i] = __ballot(refs[i] == 0 && page0 + 64 * i < p.n_pages);
+        mine += __popcll(free_row[i]);
+    }
+    // the first writer of a tail keeps it if nobody else has it
+    bool copy = false;
+    if (tail >= 0) {
+        int n = 0, first = ONE_SEQS;
+        for (int i = (p.n_seq + 3) / 4 * 4 - 4; i >= 0; i -= 4) {
+            const int4 x = *(const int4*)&s_tail[i];
+            const int v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 3; j >= 0; j--) {
+                n += v[j] == tail;
+                if (v[j] == tail) first = i + j;
+            }
+        }
+        copy = first != s || held > n;
+    }
+    r.src = tail;
+    r.from = copy ? r.keep >> p.shift : r.kept_pages;
+    int need, copies, free;
+    r.base = block_before(leads ? r.pages - r.from : 0, s_sums, need);
+    const int at = block_before(copy, s_sums, copies);
+    const int before = block_before(lane == 0 ? mine : 0, s_sums, free);
+    r.copy = copy ? at : -1;
+    if (leads) s_rows[s] = r;
+    __syncthreads();
+    const bool enough = need <= free;
+    if (tid == 0) {
+        a.result[0] = free - need;
+        a.result[1] = enough ? copies : 0;
+    }
+    if (!enough) {
+        for (int j = t; j < entries; j += team) {
+            const int was = old_entry(p, r, s, j), x = kept_entry(p, r, j);
+            if (was != x) {
+                if (was >= 0) add(was, 1);
+                if (x >= 0) add(x, -1);
+            }
+        }
+        return;
+    }
+    int rank = __builtin_amdgcn_readfirstlane(before);
+#pragma unroll
+    for (int i = 0; i < ONE_PAGES; i++) {
+        if (i >= rows || rank >= need) continue;
+        const int at_page = rank + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(free_row[i] >> 32),
+                                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)free_row[i], 0));
+        if ((free_row[i] >> lane & 1) != 0 && at_page < need) {
+            int lo = 0, hi = p.n_seq - 1;  // the last sequence whose fresh pages begin at or before this one
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (s_rows[mid].base <= at_page) lo = mid;
+                else hi = mid - 1;
+            }
+            const ForkRow to = s_rows[lo];
+            const int j = to.from + at_page - to.base, page = page0 + 64 * i;
+            p.table[(uint64_t)lo * p.stride + j] = page;
+            p.refs[page] = 1;
+            if (to.copy >= 0 && j == to.from) {
+                int32_t* c = a.copies + (uint64_t)to.copy * 3;
+                c[0] = to.src;
+                c[1] = page;
+                c[2] = to.keep & (p.page - 1);
+                add(to.src, -1);
+            }
+        }
+        rank += __popcll(free_row[i]);
+    }
+    if (!live) return;
+    if (leads) p.kv_len[s] = r.size;
+    const int from = s_rows[s].from;
+#pragma unroll
+    for (int i = 0; i < ONE_ENTRIES; i++) {
+        const int j = t + i * team;
+        if (!__any(j < entries)) continue;
+        int32_t* to = p.table + (uint64_t)s * p.stride + j;
+        if (j < from) {
+            if (r.parent != s) *to = is[i];
+            else if (j >= r.dead0 && j < r.dead1) *to = -1;
+        } else if (j >= r.pages && j < r.old_pages) {
+            *to = -1;
+        }
+    }
+}
+
 // ---- compact -------------------------------------------------------------------
 __global__ __launch_bounds__(THREADS) void k_compact_count(CompactArgs a)
 {
@@ -400,6 +556,16 @@ __global__ __launch_bounds__(COPY_THREADS) void k_kv_copy(CopyArgs a)
 
 hipError_t launch_kv_fork(const ForkArgs& a, hipStream_t s)
 {
+    // One workgroup for small pools. It and the three launches, us, sequences x pages
+    // each: 8 x 30 6.9 and 11.9, 32 x 38 8.2 and 12.0, 64 x 126 12.6 and 15.5; with room
+    // for 256 sequences, 16 entries and 16 rows of pages the first two took 8.6 and 9.7,
+    // 100 x 20 13.5 and 14.0, 256 x 62 27 and 16.
+    int shift = 10;
+    while (shift > 0 && THREADS >> shift < a.p.n_seq) shift--;
+    if (a.p.n_seq > 0 && a.p.n_seq <= ONE_SEQS && a.p.stride <= ONE_ENTRIES << shift && a.p.n_pages <= ONE_PAGES * THREADS) {
+        k_fork_one<<<dim3(1), dim3(THREADS), 0, s>>>(a, shift);
+        return hipGetLastError();
+    }
     const unsigned rows = (unsigned)a.p.n_seq * (unsigned)((a.p.stride + THREADS - 1) / THREADS);
     if (rows) k_fork_count<<<dim3(rows), dim3(THREADS), 0, s>>>(a);
     k_fork_plan<<<dim3((unsigned)a.blocks + 1), dim3(THREADS), 0, s>>>(a);
