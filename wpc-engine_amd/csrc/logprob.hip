@@ -373,11 +373,11 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
 
     // The segments: the k-th best of groups of them is no better than the k-th of
     // all. Groups of the threads with one lane number are 64 and the k-th says
-    // enough up to k of 24; beyond, those of each thread.
+    // enough up to k of 24; beyond, half as large ones.
     const int k = p.top;
     if (n_seg > 0) {
-        const uint32_t best[4] = {s_best[lane], s_best[64 + lane], s_best[128 + lane], s_best[192 + lane]};
-        const uint32_t all[1] = {max(max(best[0], best[1]), max(best[2], best[3]))};
+        const uint32_t best[2] = {max(s_best[lane], s_best[64 + lane]), max(s_best[128 + lane], s_best[192 + lane])};
+        const uint32_t all[1] = {max(best[0], best[1])};
         const uint32_t least = max(k <= 24 ? kth_about(all, k) : kth_about(best, k), 1u);
         collect(s_list[0], each_seg, [&](uint32_t order, uint32_t) { return order >= least; });
     }
