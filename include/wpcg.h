@@ -643,9 +643,11 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  * and the first sequence's length; sequences of no group, groups of one and
  * groups whose numbers are not within the batch share nothing. Each sequence's
  * rows come after its group's prefix as a rule, but need not. Work is shared out
- * by the lengths, so that a sequence's last bits may depend on the others; the same call on the
- * same arrays gives the same bits. Sharing is for single tokens and drafts: with
- * more than 32 rows times query heads a key-value head, the call is
+ * by the lengths, so that a sequence's last bits may depend on the others; the same
+ * call on the same arrays gives the same bits. Sharing is for single tokens and
+ * drafts, at most 32 rows times query heads a key-value head, and up to 512
+ * sequences in 256 groups, where by the bounds (max_prefix and window) some 250 to
+ * 700 MB of keys and values would be read again; else the call is
  * wpcg_paged_attention itself. Where group_start falls, which group a sequence is
  * of is open. Workspace and streams as for wpcg_paged_attention. */
 typedef struct wpcg_kv_prefix_s {

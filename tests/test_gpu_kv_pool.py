@@ -195,11 +195,11 @@ def test_lives_of_sequences(ctx, dtype, hkv, d, page, order, n_layers, stride):
 
 
 @pytest.mark.parametrize("keep", [0, 1, 15, 16, 17, 31, 32, 33, 47])
-@pytest.mark.parametrize("grow", [0, 1, 2, 16, 17])
-def test_many_from_one(ctx, keep, grow):
+@pytest.mark.parametrize("grow,stride", [(0, 5), (1, 5), (2, 5), (16, 5), (17, 5), (1, 1100), (17, 1100)])
+def test_many_from_one(ctx, keep, grow, stride):
     """All rows from row 0, which is not or is itself among them; the tail is
     copied for all but one, and not at all where nothing is written or it is full."""
-    ref = Pool(60, 16, 9, 5)
+    ref = Pool(60, 16, 9, stride)
     dev = Device(ctx, ref)
     first = np.zeros(9, np.int32)
     first[0] = 47
@@ -241,10 +241,11 @@ def test_a_page_held_by_the_host(ctx):
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (16, 0), (17, 0), (33, 5), (40, 16), (40, 17), (100, 3), (5, 200)])
-def test_windows(ctx, window, sinks):
+@pytest.mark.parametrize("stride", [12, 1100])
+def test_windows(ctx, window, sinks, stride):
     """Pages go free as the window moves on, token by token and in jumps; forked
     rows with holes; the tokens that rows see are all there."""
-    ref = Pool(64, 16, 4, 12)
+    ref = Pool(64, 16, 4, stride)
     cache = Cache(ctx, ref, 1, 1, 64, BF16, "head")
     dev = Device(ctx, ref, cache.layers)
     lo = [0] * 4
@@ -265,10 +266,11 @@ def test_windows(ctx, window, sinks):
         assert (ref.table[:, 1:3] == -1).any()
 
 
-def test_running_out_and_just_enough(ctx):
+@pytest.mark.parametrize("stride", [8, 1100])
+def test_running_out_and_just_enough(ctx, stride):
     """One page missing: nothing changes and none is copied; the pages that the
     call itself frees are enough for it."""
-    ref = Pool(8, 16, 3, 8)
+    ref = Pool(8, 16, 3, stride)
     dev = Device(ctx, ref)
     dev.fork(grow=[40, 50, 10])
     assert (ref.refs > 0).sum() == 8
@@ -300,12 +302,13 @@ def test_sizes_of_pools(ctx, n_pages, n, stride):
     dev.fork(np.full(n, -1))
 
 
-def test_arrays_that_hold_anything(ctx):
+@pytest.mark.parametrize("stride", [5, 1100])
+def test_arrays_that_hold_anything(ctx, stride):
     """Ids of no page, lengths that are none, parents and keeps out of range:
     nothing is touched outside the arrays, and the sequences beside them are right."""
     rng = np.random.default_rng(3)
     for turn in range(20):
-        ref = Pool(50, 16, 8, 5)
+        ref = Pool(50, 16, 8, stride)
         ref.table[:] = rng.integers(-4, 54, ref.table.shape)
         ref.table[rng.random(ref.table.shape) < 0.1] = 2 ** 31 - 1
         ref.kv_len[:] = rng.choice([-5, 0, 3, 16, 33, 79, 80, 81, 2 ** 31 - 1, -2 ** 31], 8)
@@ -356,8 +359,8 @@ def test_graphs_and_streams(ctx):
     print("[gpu] pool graphs", flush=True)
     rng = np.random.default_rng(12)
     twins = []
-    for n, pages in ((6, 60), (3, 30)):
-        ref = Pool(pages, 16, n, 6)
+    for n, pages, stride in ((6, 60, 6), (3, 30, 1100)):
+        ref = Pool(pages, 16, n, stride)
         cache = Cache(ctx, ref, 2, 2, 64, BF16, "head")
         dev = Device(ctx, ref, cache.layers)
         dev.fork(grow=rng.integers(1, 40, n))

@@ -20,6 +20,13 @@
 // us for that reason alone. With own tokens in whole workgroups' items, dealt out
 // evenly beside the prefixes, each of them began and ended in 9 us, whatever its
 // tiles.
+//
+// 64 rows of 32 / 4 heads, 8192 shared tokens and up to 1000 own, BF16: 40 us and
+// the join's 8, of which the deal 4.5, a workgroup's prefix 5 and 2.2 a tile (64
+// tokens, 128 columns: 490 TFLOP/s with the CU's other workgroup waiting for own
+// tokens, and twice that with both at prefixes). Six groups of 16 over E4M3, 32 / 8
+// heads: 30 and 8. 32 rows over 65536 shared tokens, F32 queries over E4M3, three
+// products each: 116 and 9, 0.84 PFLOP/s in all, one wave a SIMD.
 #include "attn_few.h"
 #include "attn_many.h"
 
@@ -91,17 +98,15 @@ __device__ __forceinline__ SeqRows uniform(const SeqRows& r)
 // ---- prefixes ------------------------------------------------------------------
 // A workgroup's 128 columns of a group's rows over some tiles of its prefix.
 struct PrefixWork {
-    const PrefixArgs& args;
     const Batch& x;
     const Group& g;
     SeqRows sq;  // the group's rows
-    int seq, kvh, cb, split, v0, v1;
+    int seq, kvh, cb, v0, v1;
     int least, most;  // its rows' positions
     SeenTiles<many::TILE> seen;
     float *part_o, *part_ml;
     __device__ __forceinline__ int all_hi() const { return min(least, g.len - 1) + 1; }
     __device__ __forceinline__ int all_lo(const PagedAttnArgs& p) const { return p.window > 0 ? most - p.window + 1 : 0; }
-    __device__ __forceinline__ bool part() const { return true; }
 };
 __device__ __forceinline__ SeenTiles<many::TILE> prefix_tiles(const PagedAttnArgs& p, const Group& g, int least, int most)
 {
@@ -383,7 +388,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         const int v0 = ch * p.chunk + max(0, v - PREFIX_ITEM), v1 = ch * p.chunk + max(0, v + take - PREFIX_ITEM);
         const uint64_t slot = (uint64_t)(base.y + (kvh * chunks + ch) * cbs + cb + b);
         if (v0 < v1 && slot < p.pre_slots) {
-            const PrefixWork w = {p, x, g, {g.a, g.rows, g.len, false}, g.s0, kvh, cb, 0, v0, v1, least, most,
+            const PrefixWork w = {x, g, {g.a, g.rows, g.len, false}, g.s0, kvh, cb, v0, v1, least, most,
                                   prefix_tiles(a, g, least, most), p.pre_o + slot * PCOLS * D, p.pre_ml + slot * PCOLS * 2};
             many::attend<D, CT, QF32, PrefixColumns>(a, sh.pre, w);
         }

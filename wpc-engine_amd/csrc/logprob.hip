@@ -11,10 +11,14 @@
 // Two launches. The first cuts rows into chunks of 2048 ids, a wave each, held in
 // registers: the chunk's maximum, how many reach it, the sums over the others
 // relative to it, how many ids come before the given token, and the maximum of
-// every 64 ids. Every logit is read once, so memory bounds it. The second, a
+// every 64 ids. Every logit is read once, so memory bounds it: 1500 rows of 151936
+// F32 logits (912 MB) 151 us, 6.0 TB/s; 777 rows of 32003 BF16 logits 20 us for 50
+// MB, where the vector work of an id (some 14 operations) is as long. The second, a
 // workgroup a row, joins the chunks' states in fp64 and finds the K best: they
 // lie in the K segments of 64 ids whose maxima come first (each of these comes
 // before anything in another segment), so 64 K logits are read again, not a row.
+// It is a chain of two reads and four barriers: 7.2 us for up to 64 rows, 13 for
+// 777 rows and K of 50, which are instructions (1500 a wave) rather than waits.
 #include "paged.h"
 #include "wave.h"
 
