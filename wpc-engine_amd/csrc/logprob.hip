@@ -109,7 +109,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
 {
     const int groups = (p.chunks + 3) / 4;
     const int row = (int)(blockIdx.x / (unsigned)groups);
-    const int chunk = (int)(blockIdx.x % (unsigned)groups) * 4 + ((int)threadIdx.x >> 6);
+    const int chunk = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % (unsigned)groups) * 4 + ((int)threadIdx.x >> 6));
     if (chunk >= p.chunks) return;
     const int lane = (int)threadIdx.x & 63, id0 = chunk * CHUNK - row_skew(p, row);
     using C = Chunk<BF16>;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
         tops += __popcll(__ballot(top));
     }
     // greater logits come before the token's, and equal ones of lower ids
-    if (inside) {
+    if (inside && best >= xt) {
         if (id0 > token) {
 #pragma unroll
             for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] > xt));
