@@ -104,6 +104,16 @@ __device__ __forceinline__ float logit(const LogprobArgs& p, int row, int id)
     return p.bf16 ? __uint_as_float((uint32_t)((const uint16_t*)p.logits)[x] << 16) : ((const float*)p.logits)[x];
 }
 
+// The lane's share of two maxima: b's with `upper`, a's without, over itself and its
+// partner, which is the other kind.
+constexpr int DPP_QUAD_MIRROR = 0x1B;
+template <int CTRL>
+__device__ __forceinline__ float max_over(bool upper, float a, float b)
+{
+    const float give = upper ? a : b;
+    return fmaxf(upper ? b : a, wave_dpp<CTRL>(give, give));
+}
+
 template <bool BF16>
 __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
 {
@@ -123,38 +133,62 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
     // maxima of the 64-id segments, which are SEG / PER lanes of one load, and
     // of the chunk
     constexpr int LANES = SEG / C::PER;
-    float best = -INFINITY, seg = -INFINITY;
+    float m[C::LOADS], best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < C::LOADS; i++) {
-        float m = -INFINITY;
+        m[i] = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < C::PER; j++) m = fmaxf(m, c.v[C::PER * i + j]);
-        if (p.top > 0) {
-            m = fmaxf(m, wave_dpp<WDPP_XOR1>(m, m));
-            m = fmaxf(m, wave_dpp<WDPP_XOR2>(m, m));
-            m = fmaxf(m, wave_dpp<WDPP_HALF_MIRROR>(m, m));
-            if (LANES == 16) m = fmaxf(m, wave_dpp<WDPP_MIRROR>(m, m));
-            if (lane % LANES == i) seg = m;  // lane i of a segment's keeps load i's
-        }
-        best = fmaxf(best, m);
+        for (int j = 0; j < C::PER; j++) m[i] = fmaxf(m[i], c.v[C::PER * i + j]);
+        best = fmaxf(best, m[i]);
     }
-    if (p.top > 0 && lane % LANES < C::LOADS)
-        p.seg[((uint64_t)row * p.chunks + chunk) * SEGS + lane % LANES * (64 / LANES) + lane / LANES] = seg;
+    if (p.top > 0) {
+        // a lane keeps half of its loads and hands its partner the others, so that
+        // one is left in the end, the same in lanes 2 n and 2 n + 1
+        int load = 0;
+        if constexpr (LANES == 16) {
+            load = lane >> 3 & 1;
+#pragma unroll
+            for (int i = 0; i < 4; i++) m[i] = max_over<WDPP_MIRROR>(lane & 8, m[2 * i], m[2 * i + 1]);
+        }
+        load += (lane >> 2 & 1) * (LANES / 8);
+#pragma unroll
+        for (int i = 0; i < 2; i++) m[i] = max_over<WDPP_HALF_MIRROR>(lane & 4, m[2 * i], m[2 * i + 1]);
+        load += (lane >> 1 & 1) * (LANES / 4);
+        m[0] = max_over<DPP_QUAD_MIRROR>(lane & 2, m[0], m[1]);
+        m[0] = fmaxf(m[0], wave_dpp<WDPP_XOR1>(m[0], m[0]));
+        if (lane % 2 == 0)
+            p.seg[((uint64_t)row * p.chunks + chunk) * SEGS + load * (64 / LANES) + lane / LANES] = m[0];
+    }
     best = wave_max(best);
 
+    // Of the maximum itself e^0 = 1 is added like any other term where the sum is
+    // 3 and more: 16 additions' roundings of it are 24 of what is left without it.
+    // Else ids at the maximum are counted and the others summed again.
     const float base = best == -INFINITY ? 0.0f : best;
-    float z[2] = {0.0f, 0.0f}, s[2] = {0.0f, 0.0f};
-    int tops = 0, before = 0;
+    float z[4] = {}, s[2] = {};
+    int tops = 1, before = 0;
 #pragma unroll
     for (int i = 0; i < VALUES; i++) {
-        const float d = c.v[i] - base;
-        const float t = d * rate;
-        const bool top = c.v[i] == best;
-        // (a NaN reaches z here, and only here)
-        const float e = top ? 0.0f : exp2_fast(t);
-        z[i & 1] += e;
+        const float t = (c.v[i] - base) * rate, e = exp2_fast(t);  // (a NaN reaches z)
+        z[i & 3] += e;
         s[i & 1] = fmaf(e, fmaxf(t, -200.0f), s[i & 1]);
-        tops += __popcll(__ballot(top));
+    }
+    // (s is summed here: behind the branch below all terms would have to be kept)
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]));
+    float zs = wave_sum((z[0] + z[1]) + (z[2] + z[3])) - 1.0f;
+    if (!(zs >= 2.0f)) {
+        z[0] = z[1] = z[2] = z[3] = 0.0f;
+        tops = 0;
+        float from = base;  // (differences anew: kept, they would be 32 registers more)
+        asm volatile("" : "+v"(from));
+#pragma unroll
+        for (int i = 0; i < VALUES; i++) {
+            const bool top = c.v[i] == best;
+            z[i & 3] += top ? 0.0f : exp2_fast((c.v[i] - from) * rate);
+            tops += __popcll(__ballot(top));
+        }
+        zs = wave_sum((z[0] + z[1]) + (z[2] + z[3]));
+        if (best == -INFINITY) tops = 0;
     }
     // greater logits come before the token's, and equal ones of lower ids
     if (inside && best >= xt) {
@@ -170,9 +204,8 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
                 before += __popcll(__ballot(c.v[i] > xt || (c.v[i] == xt && (uint32_t)(id0 + C::place(i)) < (uint32_t)token)));
         }
     }
-    const float zs = wave_sum(z[0] + z[1]), ss = wave_sum(s[0] + s[1]);
-    if (lane == 0)
-        p.part[(uint64_t)row * p.chunks + chunk] = LogprobPart{best, zs, ss, best == -INFINITY ? 0 : tops, before};
+    const float ss = wave_sum(s[0] + s[1]);
+    if (lane == 0) p.part[(uint64_t)row * p.chunks + chunk] = LogprobPart{best, zs, ss, tops, before};
 }
 
 // ---- the row's state -------------------------------------------------------------
