@@ -41,7 +41,9 @@ def row(x, token, k, temperature=1.0):
     h = log_z - (p[some] * t[some]).sum()
     # Terms: the hardware's exponential 2 eps; its argument (base 2) has three
     # roundings, 3 eps |t|, and so has the term, relatively. Sums: 16 additions in a
-    # lane, 7 over lanes. log Z of 1 + (Z - 1) errs by the error of Z - 1 over Z.
+    # lane, 7 over lanes; or 10 and 6 with the maximum's own term among them, where the
+    # sum is at least 3, 3/2 times as much of what is left without it. log Z of
+    # 1 + (Z - 1) errs by the error of Z - 1 over Z.
     # The entropy's other part sums e t alike, with one product's rounding more.
     # Results are rounded to fp32; the given logit's own t has the rate's rounding
     # (fp64 else).

@@ -85,6 +85,37 @@ def test_sizes(ctx, dtype, v, top):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("top", [1, 24, 25, 64])
+def test_segments_that_do_not_fit_in_registers(ctx, dtype, top):
+    rng = np.random.default_rng(170001 + top)
+    bits, x = logits(rng, 2, 170001, dtype)
+    tokens = rng.integers(0, 170001, 2)
+    check(run(ctx, bits, dtype, tokens, top), x, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_rows(ctx, dtype):
+    """Many rounds of workgroups."""
+    rng = np.random.default_rng(8300)
+    bits, x = logits(rng, 8300, 501, dtype)
+    tokens = rng.integers(0, 501, 8300)
+    got = run(ctx, bits, dtype, tokens, 3)
+    some = np.append(np.arange(0, 8300, 13), 8299)
+    check({k: a[some] for k, a in got.items()}, x[some], tokens[some], 3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [1e-3, 0.1, 0.5, 1.0, 3.0, 5.0, 8.0, 20.0])
+def test_flat_and_peaked(ctx, dtype, width):
+    """Sums of nearly all ids, of some, and of hardly more than the maximum; the
+    likeliest ids' log probabilities among them."""
+    rng = np.random.default_rng(int(width * 1000))
+    bits, x = logits(rng, 12, 4500, dtype, width)
+    tokens = np.argsort(-x, -1)[np.arange(12), [0, 0, 0, 0, 1, 1, 2, 3, 10, 100, 1000, 4000]]
+    check(run(ctx, bits, dtype, tokens, 5), x, tokens, 5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("stride,offset", [(5008, 0), (5001, 0), (5008, 1), (5003, 3)])
 def test_strides_and_alignment(ctx, dtype, stride, offset):
     """Rows on 16 bytes and off them; what lies between them is not looked at."""

@@ -4,16 +4,16 @@
 // With M the row's largest logit, t_i = (x_i - M) / T and Z = sum e^(t_i):
 //   log p_i = t_i - ln Z,   H = ln Z - sum e^(t_i) t_i / Z
 // Every term of H's sum has one sign, so nothing cancels. For a confident row
-// ln Z is that of a number just above 1: the ids at the maximum are counted, not
-// summed, so that the small terms beside them keep their 24 bits, and ln Z is
-// log1p of what is left.
+// ln Z is that of a number just above 1: where there is little beside the ids at the
+// maximum they are counted, not summed, so that the small terms keep their 24 bits,
+// and ln Z is log1p of what is left.
 //
 // Two launches. The first cuts rows into chunks of 2048 ids, a wave each, held in
 // registers: the chunk's maximum, how many reach it, the sums over the others
 // relative to it, how many ids come before the given token, and the maximum of
 // every 64 ids. Every logit is read once, so memory bounds it: 1500 rows of 151936
-// F32 logits (912 MB) 151 us, 6.0 TB/s; 777 rows of 32003 BF16 logits 20 us for 50
-// MB, where the vector work of an id (some 14 operations) is as long. The second, a
+// F32 logits (912 MB) 147 us, 6.2 TB/s; 777 rows of 32003 BF16 logits 17.6 us for 50
+// MB, where the vector work of an id (some 11 operations) is longer. The second, a
 // workgroup a row, joins the chunks' states in fp64 and finds the K best: they
 // lie in the K segments of 64 ids whose maxima come first (each of these comes
 // before anything in another segment), so 64 K logits are read again, not a row.
@@ -506,8 +506,12 @@ hipError_t launch_logprobs(const LogprobArgs& p, hipStream_t s)
 {
     if (p.n_rows == 0) return hipSuccess;
     const dim3 grid((unsigned)p.n_rows * ((unsigned)(p.chunks + 3) / 4));
+    // F32 rows in many rounds of workgroups come from the memory faster to four of them a
+    // CU than to eight, which unused LDS sees to: 1500 rows of 151936 151 us and 158; 64
+    // rows, less than a round, 17.3 and 17.0.
+    const unsigned room = !p.bf16 && grid.x >= 4 * 8 * 256 ? 40000 : 0;
     if (p.bf16) k_logprob_stats<true><<<grid, dim3(THREADS), 0, s>>>(p);
-    else k_logprob_stats<false><<<grid, dim3(THREADS), 0, s>>>(p);
+    else k_logprob_stats<false><<<grid, dim3(THREADS), room, s>>>(p);
     k_logprob_finish<<<dim3((unsigned)p.n_rows), dim3(THREADS), 0, s>>>(p);
     return hipGetLastError();
 }
