@@ -338,6 +338,8 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
 {
     __shared__ RowSums s_sums[4];
     __shared__ float s_max[4];
+    __shared__ uint32_t s_least;
+    __shared__ double s_log_z;
     __shared__ List s_list[2];
     __shared__ uint32_t s_best[THREADS];
     __shared__ uint64_t s_key[LOGPROB_TOP];
@@ -413,9 +415,13 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     // enough up to k of 24; beyond, half as large ones.
     const int k = p.top;
     if (n_seg > 0) {
-        const uint32_t best[2] = {max(s_best[lane], s_best[64 + lane]), max(s_best[128 + lane], s_best[192 + lane])};
-        const uint32_t all[1] = {max(best[0], best[1])};
-        const uint32_t least = max(k <= 24 ? kth_about(all, k) : kth_about(best, k), 1u);
+        if (wave == THREADS / 64 - 1) {  // (the last wave: it has fewest chunks)
+            const uint32_t best[2] = {max(s_best[lane], s_best[64 + lane]), max(s_best[128 + lane], s_best[192 + lane])};
+            const uint32_t all[1] = {max(best[0], best[1])};
+            s_least = max(k <= 24 ? kth_about(all, k) : kth_about(best, k), 1u);
+        }
+        __syncthreads();
+        const uint32_t least = __builtin_amdgcn_readfirstlane(s_least);
         collect(s_list[0], each_seg, [&](uint32_t order, uint32_t) { return order >= least; });
     }
     __syncthreads();
@@ -448,22 +454,24 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     }
 
     // (while they are on their way)
-    if (n_seg == 0 && wave > 0) return;
-    v = all_sums(s_sums);
-    const double z = v.z + (double)(v.tops - 1);  // Z - 1
     const double ln2 = 0.6931471805599453, nan = __builtin_nan("");
     const bool greedy = rate < 0.0;
     const bool none = !(m > -INFINITY) || (!greedy && m == INFINITY);
-    const double log_z = none ? nan : greedy ? 0.0 : log1p(z);
-    if (tid == 0) {
-        if (p.entropy) p.entropy[row] = (float)(none ? nan : greedy ? 0.0 : log_z - ln2 * v.s / (z + 1.0));
-        if (p.tokens) {
-            const int rank = inside && x == x ? 1 + v.before : 0;
-            if (p.rank) p.rank[row] = rank;
-            if (p.logprob)
-                p.logprob[row] = (float)(none     ? nan
-                                         : greedy ? (rank == 1 && x > -INFINITY ? 0.0 : -INFINITY)
-                                                  : ln2 * scaled(x, m, rate) - log_z);
+    if (wave == 0) {
+        v = all_sums(s_sums);
+        const double z = v.z + (double)(v.tops - 1);  // Z - 1
+        const double log_z = none ? nan : greedy ? 0.0 : log1p(z);
+        if (tid == 0) {
+            s_log_z = log_z;
+            if (p.entropy) p.entropy[row] = (float)(none ? nan : greedy ? 0.0 : log_z - ln2 * v.s / (z + 1.0));
+            if (p.tokens) {
+                const int rank = inside && x == x ? 1 + v.before : 0;
+                if (p.rank) p.rank[row] = rank;
+                if (p.logprob)
+                    p.logprob[row] = (float)(none     ? nan
+                                             : greedy ? (rank == 1 && x > -INFINITY ? 0.0 : -INFINITY)
+                                                      : ln2 * scaled(x, m, rate) - log_z);
+            }
         }
     }
     if (n_seg == 0) return;
@@ -490,6 +498,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     const int n = __builtin_amdgcn_readfirstlane(s_list[1].n);
     uint64_t key;
     const int place = rank_in(s_list[1], n, key);
+    const double log_z = s_log_z;
     const auto put = [&](int i, int id, double lp) {
         if (p.top_ids) p.top_ids[(uint64_t)row * k + i] = id;
         if (p.top_logprob) p.top_logprob[(uint64_t)row * k + i] = (float)lp;
