@@ -17,8 +17,8 @@
 // workgroup a row, joins the chunks' states in fp64 and finds the K best: they
 // lie in the K segments of 64 ids whose maxima come first (each of these comes
 // before anything in another segment), so 64 K logits are read again, not a row.
-// It is a chain of two reads and four barriers: 7.2 us for up to 64 rows, 13 for
-// 777 rows and K of 50, which are instructions (1500 a wave) rather than waits.
+// It is a chain of two reads and five barriers: 7.4 us for up to 64 rows, 12 for
+// 777 rows and K of 50, which are instructions (1400 a wave) rather than waits.
 #include "paged.h"
 #include "wave.h"
 
