@@ -178,6 +178,29 @@ def test_ties(ctx, dtype, top):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v,top", [(20001, 1), (40000, 20), (40000, 64), (170001, 20)])
+def test_many_alike(ctx, dtype, v, top):
+    """More equal candidates than can be sorted: rows masked by the type's lowest
+    value but for a few ids (none, fewer and more than are asked for), neighbouring
+    values in every number, and a value above, between and below many equal ones."""
+    rng = np.random.default_rng(v + top)
+    low = -3.4028234663852886e38 if dtype == F32 else -3.3895313892515355e38
+    x = np.full((11, v), low)
+    for i, n in enumerate((0, 1, top - 1, top, top + 1, 300)):
+        x[i, rng.permutation(v)[:n]] = rng.standard_normal(n) * 3
+    step = 2.0 ** (-23 if dtype == F32 else -7)
+    x[6] = 1 + step * rng.integers(0, 6, v)
+    x[7] = 1 + step * rng.integers(0, 2, v) * (np.arange(v) > v // 2)
+    x[8] = np.where(rng.random(v) < 0.01, 2.0, 1.0)
+    x[9] = np.where(np.arange(v) % 3 == 0, -1.0, np.where(np.arange(v) % 3 == 1, -1.0 - step, -1.0 - 2 * step))
+    x[10] = np.where(rng.random(v) < 0.5, -np.inf, -5.0)
+    bits = R.encode(x, dtype)
+    x = R.decode(bits, dtype)
+    tokens = np.array([0, v - 1] + [int(i) for i in rng.integers(0, v, 9)])
+    check(run(ctx, bits, dtype, tokens, top), x, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_what_is_not_finite(ctx, dtype):
     """Masked rows and rows that are no distribution; the rows beside them stay
     right; lowest values of the type as masks."""

@@ -274,27 +274,65 @@ __device__ __forceinline__ void collect(List& l, EACH each, TAKE take)
         to += __popcll(them);
     });
 }
-// The k-th largest of all threads' keys (0 where there are fewer), bit by bit, and
-// the list emptied: where equal values make too many candidates.
+// A key that at least k, and no more of all threads' keys than the list holds, are at or
+// above, and the list emptied: where equal values make too many candidates to sort, a
+// row of which most is masked by the type's lowest value, say. The k-th key's order is
+// `lower` at least, places are below `places`.
 template <class EACH>
-__device__ uint64_t kth_key(int k, List& l, EACH each)
+__device__ uint64_t enough_from(int k, uint32_t lower, int places, List& l, EACH each)
 {
-    uint64_t at = 0;
-    for (int bit = 63; bit >= 0; bit--) {
-        const uint64_t next = at | (uint64_t)1 << bit;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const auto all_waves = [&](int x, uint64_t (&got)[4]) {
+        __syncthreads();
+        if (lane == 0) l.key[wave] = (uint32_t)x;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; w++) got[w] = l.key[w];
+    };
+    const auto sum = [&](int x) {
+        uint64_t g[4];
+        all_waves(x, g);
+        return __builtin_amdgcn_readfirstlane((int)(g[0] + g[1] + g[2] + g[3]));
+    };
+    const auto from_order = [&](uint32_t order0) {  // how many are of an order from order0 on
         int n = 0;
-        each([&](uint32_t order, uint32_t at) { n += key_of(order, at) >= next; });
-        n = wave_sum_i(n);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) l.key[threadIdx.x >> 6] = (uint64_t)n;
-        __syncthreads();
-        if ((int)(l.key[0] + l.key[1] + l.key[2] + l.key[3]) >= k) at = next;
+        each([&](uint32_t order, uint32_t) { n += __popcll(__ballot(order >= order0)); });
+        return sum(n);
+    };
+    // the k-th key's order: mostly the least of those from `lower` on, else by bisection
+    int low = 0x7fffffff;  // (as a signed number)
+    each([&](uint32_t order, uint32_t) { low = order >= max(lower, 1u) ? min(low, (int)(order ^ 0x80000000u)) : low; });
+    uint64_t g[4];
+    all_waves(~wave_max_i(~low), g);
+    uint32_t of = (uint32_t)min(min((int)g[0], (int)g[1]), min((int)g[2], (int)g[3])) ^ 0x80000000u;
+    int above = from_order(of + 1);
+    bool found = above < k;
+    if (!found) {
+        of = 0;
+        for (int bit = 31; bit >= 0 && !found; bit--) {
+            const int n = from_order(of | 1u << bit);
+            if (n < k) above = n;
+            else of |= 1u << bit;
+            found = n >= k && n <= LIST;
+        }
+        if (!found) above = from_order(of + 1);
+    }
+    // of this order the lowest places
+    int first = 0, last = places - 1;
+    while (first < last) {
+        const int mid = (int)((uint32_t)(first + last) / 2);
+        int n = 0;
+        each([&](uint32_t order, uint32_t at) { n += __popcll(__ballot(order == of && at <= (uint32_t)mid)); });
+        n = sum(n);
+        if (above + n < k) first = mid + 1;
+        else last = mid;
+        if (above + n >= k && above + n <= LIST) break;
     }
     __syncthreads();
     l.key[threadIdx.x] = 0;
     l.n = 0;
     __syncthreads();
-    return at;
+    return key_of(of, (uint32_t)last);
 }
 // The thread's entry of the list (0: none), and how many come before it.
 __device__ __forceinline__ int rank_in(const List& l, int n, uint64_t& key)
@@ -431,7 +469,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     uint32_t own[MOST];  // as they are read
     if (n_seg > 0) {
         if (s_list[0].n > LIST) {
-            const uint64_t from = kth_key(k, s_list[0], each_seg);
+            const uint64_t from = enough_from(k, s_least, n_seg, s_list[0], each_seg);
             collect(s_list[0], each_seg, [&](uint32_t order, uint32_t at) { return order != 0 && key_of(order, at) >= from; });
             __syncthreads();
         }
@@ -491,7 +529,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
     collect(s_list[1], each_id, [](uint32_t order, uint32_t) { return order != 0; });
     __syncthreads();
     if (s_list[1].n > LIST) {
-        const uint64_t from = kth_key(k, s_list[1], each_id);
+        const uint64_t from = enough_from(k, worst, p.vocab, s_list[1], each_id);
         collect(s_list[1], each_id, [&](uint32_t order, uint32_t at) { return order != 0 && key_of(order, at) >= from; });
         __syncthreads();
     }
