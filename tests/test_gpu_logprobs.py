@@ -296,3 +296,64 @@ def test_many_rows_streams_and_graphs(ctx):
             assert np.array_equal(d["lp"].read(np.float32, rows), first["logprob"][at:at + rows])
             assert np.array_equal(d["ids"].read(np.int32, 10 * rows).reshape(rows, 10), first["top_ids"][at:at + rows])
     other.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [257, 300, 1000, 4096, 32003])
+@pytest.mark.parametrize("top", [20, 64])
+def test_ties_at_the_border(ctx, dtype, v, top):
+    """The last of the best ids is one of many equal ones, zeros and powers of two among
+    them, with none, a few and nearly enough above, and any number below: more
+    candidates than can be sorted, in fewer segments than ids are asked for."""
+    print(f"[gpu] ties at the border {dtype} {v} top {top}", flush=True)
+    rng = np.random.default_rng(v + top + dtype)
+    low = -3.4028234663852886e38 if dtype == F32 else -3.3895313892515355e38
+    rows, tokens = [], []
+    for tie in (0.0, 2.0, 1.0, -0.5):
+        for below in ("spread", low, -1e4, -np.inf):
+            for above, more in ((0, 10), (3, 90), (top - 1, 40)):
+                x = tie - 1 - np.abs(rng.standard_normal(v)) if below == "spread" else np.full(v, below)
+                n = top + more
+                at = int(rng.integers(0, v - n + 1))
+                x[at:at + n] = tie
+                x[at + rng.permutation(n)[:above]] = tie + 1 + rng.integers(0, 4, above) / 4
+                rows.append(x)
+                tokens.append(at + n - 1)
+    # rounded values in every number, and masks that leave 300 neighbours
+    rows += [np.round(rng.standard_normal(v) * w) / 4 for w in (1, 4, 16)]
+    x = np.full(v, -np.inf)
+    at = int(rng.integers(0, max(1, v - 300)))
+    x[at:at + 300] = np.round(rng.standard_normal(len(x[at:at + 300])) * 4) / 4
+    rows.append(x)
+    bits = R.encode(np.array(rows), dtype)
+    if dtype == BF16:
+        bits = np.where(np.isneginf(rows), 0xFF80, bits).astype(np.uint16)
+    tokens += [int(i) for i in rng.integers(0, v, 4)]
+    x = R.decode(bits, dtype)
+    check(run(ctx, bits, dtype, np.array(tokens), top), x, tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v,top", [(32000, 20), (151936, 20), (151936, 64), (170016, 24)])
+def test_ties_at_the_border_of_segments(ctx, dtype, v, top):
+    """The same among the segments of 64 ids: more segments than can be sorted, the
+    K-th best maximum at zero or two, in few of the groups that they are looked at in."""
+    print(f"[gpu] ties of segments {dtype} {v} top {top}", flush=True)
+    rng = np.random.default_rng(v + top + dtype)
+    rows = []
+    for tie in (0.0, 2.0, 1.0):
+        for groups in ((5,), (5, 6, 40)):
+            x = np.full(v, -1e4)
+            segs = [s for s in range(v // 64) if s % 64 in groups]
+            for s in segs:
+                x[64 * s + rng.integers(0, 64, 2)] = tie
+            for s in rng.permutation(segs)[:3]:
+                x[64 * s + 7] = tie + 1
+            rows.append(x)
+    x = np.full(v, -1e4)  # ten above neighbouring zeros
+    x[v // 2:v // 2 + 30 + top] = 0.0
+    x[v // 2 + rng.permutation(30)[:10]] = rng.standard_normal(10) ** 2 + 0.25
+    rows.append(x)
+    bits = R.encode(np.array(rows), dtype)
+    tokens = [int(i) for i in rng.integers(0, v, len(rows))]
+    check(run(ctx, bits, dtype, np.array(tokens), top), R.decode(bits, dtype), tokens, top)

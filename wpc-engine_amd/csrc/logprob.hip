@@ -21,6 +21,8 @@
 // 777 rows and K of 50, which are instructions (1400 a wave) rather than waits.
 #include "paged.h"
 #include "wave.h"
+#define KTH_KEY_FN __device__ __forceinline__
+#include "kth_key.h"
 
 namespace wpcg {
 namespace {
@@ -294,45 +296,28 @@ __device__ uint64_t enough_from(int k, uint32_t lower, int places, List& l, EACH
         all_waves(x, g);
         return __builtin_amdgcn_readfirstlane((int)(g[0] + g[1] + g[2] + g[3]));
     };
-    const auto from_order = [&](uint32_t order0) {  // how many are of an order from order0 on
-        int n = 0;
-        each([&](uint32_t order, uint32_t) { n += __popcll(__ballot(order >= order0)); });
-        return sum(n);
-    };
-    // the k-th key's order: mostly the least of those from `lower` on, else by bisection
     int low = 0x7fffffff;  // (as a signed number)
     each([&](uint32_t order, uint32_t) { low = order >= max(lower, 1u) ? min(low, (int)(order ^ 0x80000000u)) : low; });
     uint64_t g[4];
     all_waves(~wave_max_i(~low), g);
-    uint32_t of = (uint32_t)min(min((int)g[0], (int)g[1]), min((int)g[2], (int)g[3])) ^ 0x80000000u;
-    int above = from_order(of + 1);
-    bool found = above < k;
-    if (!found) {
-        of = 0;
-        for (int bit = 31; bit >= 0 && !found; bit--) {
-            const int n = from_order(of | 1u << bit);
-            if (n < k) above = n;
-            else of |= 1u << bit;
-            found = n >= k && n <= LIST;
-        }
-        if (!found) above = from_order(of + 1);
-    }
-    // of this order the lowest places
-    int first = 0, last = places - 1;
-    while (first < last) {
-        const int mid = (int)((uint32_t)(first + last) / 2);
-        int n = 0;
-        each([&](uint32_t order, uint32_t at) { n += __popcll(__ballot(order == of && at <= (uint32_t)mid)); });
-        n = sum(n);
-        if (above + n < k) first = mid + 1;
-        else last = mid;
-        if (above + n >= k && above + n <= LIST) break;
-    }
+    const uint32_t least = (uint32_t)min(min((int)g[0], (int)g[1]), min((int)g[2], (int)g[3])) ^ 0x80000000u;
+    const KthKey found = kth_key(
+        k, LIST, least, places,
+        [&](uint32_t order0) {
+            int n = 0;
+            each([&](uint32_t order, uint32_t) { n += __popcll(__ballot(order >= order0)); });
+            return sum(n);
+        },
+        [&](uint32_t of, int place) {
+            int n = 0;
+            each([&](uint32_t order, uint32_t at) { n += __popcll(__ballot(order == of && at <= (uint32_t)place)); });
+            return sum(n);
+        });
     __syncthreads();
     l.key[threadIdx.x] = 0;
     l.n = 0;
     __syncthreads();
-    return key_of(of, (uint32_t)last);
+    return key_of(found.order, (uint32_t)found.place);
 }
 // The thread's entry of the list (0: none), and how many come before it.
 __device__ __forceinline__ int rank_in(const List& l, int n, uint64_t& key)
