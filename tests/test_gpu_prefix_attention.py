@@ -354,3 +354,100 @@ def test_graphs_and_streams(ctx):
     other.sync()
     assert np.array_equal(out.read(R.BITS[dtype], n * 8 * 128), first)
     other.close()
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("sinks", [0, 20])
+def test_windows_that_left_the_first_sequence_ahead(ctx, q_dtype, dtype, sinks):
+    """A group's first sequence is further on than others, or has ended: pages behind
+    its window, which others still see, are no longer in its row of the table, nor
+    are any behind theirs in the others'. Ids of no page there, and ids of pages that hold
+    something else."""
+    print(f"[gpu] prefix window, first ahead {q_dtype}/{dtype} sinks {sinks}", flush=True)
+    rng = np.random.default_rng(100 + sinks + 10 * q_dtype + dtype)
+    w = least_window(q_dtype, dtype, 16, 128, 512 - 5) + 5
+    # longest first; ended first; ended and longest; shortest first; rows that begin before the prefix ends
+    groups = [(w + 90, [w + 300, 3, 40, w + 130]), (w + 40, [0, 70, 3]), (2 * w + 100, [200, 20, 20, 130]),
+              (300, [9, w + 20]), (150, [w + 60, 0, 2 * w])]
+    live = sum(len(own) for _, own in groups)
+    g = Groups(ctx, rng, groups, dtype, 16, 128, 16, empty=512 - live)
+    pg = g.pg
+    per = [3] * live + [0] * (512 - live)
+    per[4], pg.kv_len[4] = 0, 0
+    for n in "kv":
+        pg.real[n][4] = pg.real[n][4][:0]
+    # sequence 14's only rows lie before its group's prefix ends
+    pg.kv_len[14] = 60
+    for n in "kv":
+        pg.real[n][14] = pg.real[n][14][:60]
+    q = R.encode(rng.standard_normal((sum(per), 32, 128)) * 1.5, q_dtype)
+    batch = g.batch(per)
+    want, bound = expected(pg, q, per, q_dtype, 128 ** -0.5, w, sinks)
+    plain = wpcg.PagedAttention(ctx, pg.kv, batch, 32, q_dtype, scale=128 ** -0.5, window=w, sinks=sinks).workspace_bytes
+    whole = pg.table.copy()
+    for gone in (-1, 2 ** 31 - 1, pg.n_pages, "others"):
+        table = whole.copy()
+        for s in range(live):
+            pages = -(-pg.kv_len[s] // 16)
+            lo = pg.kv_len[s] - per[s] - w + 1  # the first token that its rows see
+            for j in range(table.shape[1]):
+                seen = j < pages and per[s] and (16 * (j + 1) > lo or 16 * j < sinks)
+                if not seen:
+                    table[s, j] = int(rng.integers(0, pg.n_pages)) if gone == "others" else gone
+        pg.d_table.write(table)
+        got = run(ctx, pg, batch, g.desc(), q, 32, q_dtype, 128 ** -0.5, w, sinks)
+        assert run.workspace != plain  # it shares
+        check(got, want, bound)
+
+
+@pytest.mark.parametrize("q_dtype,dtype", [(BF16, BF16), (F32, E4M3)])
+def test_windows_whose_pages_a_fork_gave_back(ctx, q_dtype, dtype):
+    """The same with the tables that wpcg_kv_fork leaves, in steps of uneven numbers of
+    tokens a sequence."""
+    print(f"[gpu] prefix window after forks {q_dtype}/{dtype}", flush=True)
+    rng = np.random.default_rng(200 + dtype)
+    w = least_window(q_dtype, dtype, 16, 128, 512 - 2) + 3
+    groups = [(w + 90, [5, 3, 40, 1]), (2 * w, [1, 1, 1])]
+    live = 7
+    g = Groups(ctx, rng, groups, dtype, 16, 128, 16, empty=512 - live)
+    pg = g.pg
+    stride = pg.table.shape[1]
+    pg.table[:, :] = np.where(np.arange(stride) < -(-np.array(pg.kv_len)[:, None] // 16), pg.table, -1)
+    refs = np.bincount(pg.table[pg.table >= 0], minlength=pg.n_pages).astype(np.int32)
+    pool = wpcg.KvPool(ctx, pg.n_pages, 16, 512, stride, refs=ctx.upload(refs), table=ctx.upload(pg.table),
+                       kv_len=ctx.upload(np.array(pg.kv_len, np.int32)))
+    copies, result, grow = ctx.alloc(12 * 512), ctx.alloc(8), ctx.alloc(4 * 512)
+    fork = wpcg.KvFork(ctx, pool, copies, result, grow_each=grow, window=w)
+    copy = wpcg.KvCopy(ctx, [pg.kv], copies, result, 512)
+    gone = 0
+    for turn in range(5):
+        # the first sequence is ahead of the others
+        more = np.zeros(512, np.int32)
+        more[:live] = [3, 1, 2, 1, 3, 1, 2] if turn else [w + 60, 1, 1, 2, w // 2, 1, 1]
+        per = [min(3, int(m)) for m in more]
+        grow.write(more)
+        fork.run()
+        copy.run()
+        ctx.sync()
+        assert result.read(np.int32, 2)[0] >= 0
+        pg.table = pool.table.read(np.int32, 512 * stride).reshape(512, stride)
+        for n, buf in (("k", pg.dk), ("v", pg.dv)):
+            pg.bits[n] = buf.read(R.BITS[dtype], pg.bits[n].size).reshape(pg.bits[n].shape)
+        for s in range(live):
+            m = int(more[s])
+            new = np.arange(pg.kv_len[s], pg.kv_len[s] + m)
+            for n in "kv":
+                x = R.encode(rng.standard_normal((m, 16, 128)), dtype)
+                pg.bits[n][pg.index(s, new)] = x
+                pg.real[n][s] = np.concatenate([pg.real[n][s], R.decode(x, dtype) * pg.scale[n][:, None].astype(np.float64)])
+            pg.kv_len[s] += m
+        pg.dk.write(pg.bits["k"])
+        pg.dv.write(pg.bits["v"])
+        gone += int((pg.table[0] == -1)[:5].sum())
+        q = R.encode(rng.standard_normal((sum(per), 32, 128)) * 1.5, q_dtype)
+        batch = g.batch(per)
+        want, bound = expected(pg, q, per, q_dtype, 0.1, w, 0)
+        check(run(ctx, pg, batch, g.desc(), q, 32, q_dtype, 0.1, w, 0), want, bound)
+        plain = wpcg.PagedAttention(ctx, pg.kv, batch, 32, q_dtype, scale=0.1, window=w)
+        assert run.workspace != plain.workspace_bytes
+    assert gone > 0

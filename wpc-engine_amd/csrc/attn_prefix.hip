@@ -36,10 +36,12 @@ namespace {
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int PCOLS = ATTN_MANY_COLS;
 
-// The batch in LDS: row starts and lengths, the groups' first sequences and prefix
-// lengths, the lowest and highest position of a group's rows.
+// The batch in LDS: row starts and lengths, the groups' first sequences, how many tokens
+// they share and from whose pages these are read, the lowest and highest position of a
+// group's rows.
 struct Batch {
     const int *start, *len, *group, *prefix, *least, *most;
+    const uint16_t* from;
 };
 __device__ __forceinline__ SeqRows rows_of(const PagedBatch& b, const Batch& x, int s)
 {
@@ -49,30 +51,42 @@ __device__ __forceinline__ SeqRows rows_of(const PagedBatch& b, const Batch& x, 
 }
 
 // Group g: sequences s0 .. s0 + n - 1, rows a .. a + rows - 1, and how many tokens
-// they share; len = 0: it shares nothing (it has one sequence or none, or its
-// numbers are out of bounds).
+// they share; n = 0: its numbers are out of bounds, or it has one sequence or none.
 struct Group {
     int s0, n, a, rows, len;
 };
-__device__ __forceinline__ Group group_of(const PrefixArgs& p, const Batch& x, int g)
+__device__ __forceinline__ Group group_rows(const PrefixArgs& p, const Batch& x, int g)
 {
     const PagedBatch& b = p.a.b;
-    Group r;
+    Group r = {};
     r.s0 = x.group[g];
     const int s1 = x.group[g + 1];
     const bool some = r.s0 >= 0 && r.s0 <= s1 - 2 && s1 <= b.n_seq;
-    r.n = some ? s1 - r.s0 : 0;
     r.a = x.start[some ? r.s0 : 0];
-    const int end = x.start[some ? s1 : 0];
-    const bool rows = some && r.a >= 0 && r.a <= end && end <= b.n_rows && end - r.a <= (int64_t)r.n * b.max_q;
-    // the pages are those of the first sequence, which has no more than its own
-    const int len = x.len[some ? r.s0 : 0];
-    r.len = rows && len <= b.max_kv ? max(0, min(min(x.prefix[g], p.max_prefix), len)) : 0;
-    r.rows = r.len > 0 ? end - r.a : 0;
+    const int end = x.start[some ? s1 : 0], n = some ? s1 - r.s0 : 0;
+    if (some && r.a >= 0 && r.a <= end && end <= b.n_rows && end - r.a <= (int64_t)n * b.max_q) {
+        r.n = n;
+        r.rows = end - r.a;
+    }
     return r;
 }
-// The group that sequence s is of, if any is: its number, and what is shared.
-__device__ __forceinline__ int group_with(const PrefixArgs& p, const Batch& x, int s, Group& g)
+// How many tokens it shares, `prefix` of them by its own number, from the pages of
+// sequence `from`, which has no more than its own.
+__device__ __forceinline__ int group_length(const PrefixArgs& p, const Batch& x, int g, int from, int prefix)
+{
+    const Group r = group_rows(p, x, g);
+    const int len = x.len[r.n > 0 ? from : 0];
+    return r.n > 0 && len <= p.a.b.max_kv ? max(0, min(min(prefix, p.max_prefix), len)) : 0;
+}
+__device__ __forceinline__ Group group_of(const PrefixArgs& p, const Batch& x, int g)
+{
+    Group r = group_rows(p, x, g);
+    r.len = x.prefix[g];
+    if (r.len == 0) r.rows = 0;
+    return r;
+}
+// The last group that begins at or before sequence s.
+__device__ __forceinline__ int group_at(const PrefixArgs& p, const Batch& x, int s)
 {
     int lo = 0, hi = p.n_groups - 1;
     while (lo < hi) {
@@ -80,9 +94,15 @@ __device__ __forceinline__ int group_with(const PrefixArgs& p, const Batch& x, i
         if (x.group[mid] <= s) lo = mid;
         else hi = mid - 1;
     }
-    g = group_of(p, x, lo);
-    if (s < g.s0 || s >= g.s0 + g.n) g.len = g.rows = 0;
     return lo;
+}
+// The group that sequence s is of, if any is: its number, and what is shared.
+__device__ __forceinline__ int group_with(const PrefixArgs& p, const Batch& x, int s, Group& g)
+{
+    const int which = group_at(p, x, s);
+    g = group_of(p, x, which);
+    if (s < g.s0 || s >= g.s0 + g.n) g.len = g.rows = 0;
+    return which;
 }
 // What came from LDS and is the same in a whole wave, in scalar registers.
 using few::uniform;
@@ -295,10 +315,11 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
     __shared__ int3 s_sums[WAVES];
     __shared__ int s_start[PREFIX_SEQS + 1], s_len[PREFIX_SEQS];
     __shared__ int s_group[PREFIX_GROUPS + 1], s_prefix[PREFIX_GROUPS], s_least[PREFIX_GROUPS], s_most[PREFIX_GROUPS];
+    __shared__ uint16_t s_from[PREFIX_GROUPS];  // (two workgroups fill a CU's LDS but for some 300 bytes each)
     constexpr int OCOLS = 16 * NB;
     const PagedAttnArgs& a = p.a;
     const int n_seq = a.b.n_seq, tid = (int)threadIdx.x;
-    const Batch x = {s_start, s_len, s_group, s_prefix, s_least, s_most};
+    const Batch x = {s_start, s_len, s_group, s_prefix, s_least, s_most, s_from};
     for (int s = tid; s <= n_seq; s += THREADS) {
         s_start[s] = a.b.q_start ? a.b.q_start[s] : s;
         if (s < n_seq) s_len[s] = a.b.kv_len[s];
@@ -309,18 +330,47 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         s_prefix[g] = p.prefix_len[g];
         s_least[g] = 0x7fffffff;
         s_most[g] = -1;
+        t.tiles[g] = 0x7fffffff;  // (below the sequence whose pages are read)
     }
     __syncthreads();
-    for (int s = tid; s < n_seq; s += THREADS) {
-        Group g;
-        const int which = group_with(p, x, s, g);
+    int which[2], least[2];  // of the thread's sequences that see something: group and first position
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int s = tid + i * THREADS;
+        which[i] = -1;
+        if (s >= n_seq) continue;
+        const int g = group_at(p, x, s);
+        const Group of = group_rows(p, x, g);
         const SeqRows r = rows_of(a.b, x, s);
-        if (g.len > 0 && r.n > 0 && !r.bad) {
-            atomicMin(&s_least[which], r.len - r.n);
-            atomicMax(&s_most[which], r.len - 1);
-        }
+        if (s < of.s0 || s >= of.s0 + of.n || r.n == 0 || r.bad || r.len == 0) continue;
+        which[i] = g;
+        least[i] = r.len - r.n;
+        atomicMin(&s_least[g], least[i]);
+        atomicMax(&s_most[g], r.len - 1);
+    }
+    const int own_group = THREADS - 1 - tid;  // (of the waves with fewest sequences)
+    if (a.window <= 0 && own_group < p.n_groups) {
+        const int from = max(0, min(s_group[own_group], n_seq - 1));  // the first sequence
+        s_from[own_group] = (uint16_t)from;
+        s_prefix[own_group] = group_length(p, x, own_group, from, s_prefix[own_group]);
     }
     __syncthreads();
+    // With a window only the sequence whose rows begin lowest is sure to have all
+    // pages that the others' rows see, as far as its own rows go: those that are further on
+    // may have given theirs away.
+    if (a.window > 0) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (which[i] >= 0 && least[i] == s_least[which[i]]) atomicMin(&t.tiles[which[i]], tid + i * THREADS);
+        __syncthreads();
+        if (own_group < p.n_groups) {
+            const bool some = t.tiles[own_group] < n_seq;
+            const int from = some ? t.tiles[own_group] : 0;
+            s_from[own_group] = (uint16_t)from;
+            s_prefix[own_group] = some ? group_length(p, x, own_group, from, s_prefix[own_group]) : 0;
+        }
+        __syncthreads();
+    }
     const PrefixDeal dealt = deal<OCOLS>(p, x, t, s_sums);
     if (blockIdx.x == 0) {  // for the join
         for (int s = tid; s < n_seq; s += THREADS) {
@@ -388,7 +438,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         const int v0 = ch * p.chunk + max(0, v - PREFIX_ITEM), v1 = ch * p.chunk + max(0, v + take - PREFIX_ITEM);
         const uint64_t slot = (uint64_t)(base.y + (kvh * chunks + ch) * cbs + cb + b);
         if (v0 < v1 && slot < p.pre_slots) {
-            const PrefixWork w = {x, g, {g.a, g.rows, g.len, false}, g.s0, kvh, cb, v0, v1, least, most,
+            const PrefixWork w = {x, g, {g.a, g.rows, g.len, false}, uniform((int)s_from[lo]), kvh, cb, v0, v1, least, most,
                                   prefix_tiles(a, g, least, most), p.pre_o + slot * PCOLS * D, p.pre_ml + slot * PCOLS * 2};
             many::attend<D, CT, QF32, PrefixColumns>(a, sh.pre, w);
         }
