@@ -451,3 +451,17 @@ def test_windows_whose_pages_a_fork_gave_back(ctx, q_dtype, dtype):
         plain = wpcg.PagedAttention(ctx, pg.kv, batch, 32, q_dtype, scale=0.1, window=w)
         assert run.workspace != plain.workspace_bytes
     assert gone > 0
+
+
+@pytest.mark.parametrize("start", [[0, 12, -2 ** 31], [0, 2 ** 31 - 1, -2 ** 31, 12], [3, -2 ** 31, 0, 12], [-2 ** 31, 0, 2 - 2 ** 31, 12]])
+@pytest.mark.parametrize("q_dtype,dtype", [(BF16, BF16), (F32, F32)])
+def test_group_starts_that_are_the_least_number(ctx, q_dtype, dtype, start):
+    """Groups that end two and fewer above the least number, where a difference of the two overflows."""
+    print(f"[gpu] prefix least starts {q_dtype}/{dtype} {start}", flush=True)
+    rng = np.random.default_rng(320 + dtype)
+    g = Groups(ctx, rng, [(90, list(range(1, 13)))], dtype, 2, 64, 16)
+    q = R.encode(rng.standard_normal((12, 8, 64)) * 1.5, q_dtype)
+    want = expected(g.pg, q, [1] * 12, q_dtype, 0.125, 0, 0)
+    prefix = g.desc(start=start, prefix=[90] * (len(start) - 1))
+    check(run(ctx, g.pg, g.batch([1] * 12), prefix, q, 8, q_dtype, 0.125), *want)
+    assert run.workspace != wpcg.PagedAttention(ctx, g.pg.kv, g.batch([1] * 12), 8, q_dtype, scale=0.125).workspace_bytes

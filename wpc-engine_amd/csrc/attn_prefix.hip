@@ -61,7 +61,7 @@ __device__ __forceinline__ Group group_rows(const PrefixArgs& p, const Batch& x,
     Group r = {};
     r.s0 = x.group[g];
     const int s1 = x.group[g + 1];
-    const bool some = r.s0 >= 0 && r.s0 <= s1 - 2 && s1 <= b.n_seq;
+    const bool some = r.s0 >= 0 && r.s0 < s1 && s1 <= b.n_seq && s1 - r.s0 > 1;  // (in this order nothing overflows)
     r.a = x.start[some ? r.s0 : 0];
     const int end = x.start[some ? s1 : 0], n = some ? s1 - r.s0 : 0;
     if (some && r.a >= 0 && r.a <= end && end <= b.n_rows && end - r.a <= (int64_t)n * b.max_q) {
