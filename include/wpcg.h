@@ -650,8 +650,8 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  * drafts, at most 32 rows times query heads a key-value head, and up to 512
  * sequences in 256 groups, where by the bounds (max_prefix and window) some 250 to
  * 700 MB of keys and values would be read again; else the call is
- * wpcg_paged_attention itself. Where group_start falls, which group a sequence is
- * of is open. Workspace and streams as for wpcg_paged_attention. */
+ * wpcg_paged_attention itself. Where group_start or q_start falls nothing is
+ * shared. Workspace and streams as for wpcg_paged_attention. */
 typedef struct wpcg_kv_prefix_s {
     uint32_t n_groups, max_prefix;
     const int32_t* group_start_dev; /* n_groups + 1 */

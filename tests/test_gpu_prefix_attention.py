@@ -465,3 +465,21 @@ def test_group_starts_that_are_the_least_number(ctx, q_dtype, dtype, start):
     prefix = g.desc(start=start, prefix=[90] * (len(start) - 1))
     check(run(ctx, g.pg, g.batch([1] * 12), prefix, q, 8, q_dtype, 0.125), *want)
     assert run.workspace != wpcg.PagedAttention(ctx, g.pg.kv, g.batch([1] * 12), 8, q_dtype, scale=0.125).workspace_bytes
+
+
+@pytest.mark.parametrize("start", [[512 if i % 2 else 4 * i for i in range(129)], [0, 512, 256, 512, 512], [0, 512] * 9 + [0],
+                                   [0, 100, 50, 512], [100, 0, 512],
+                                   [5, 512, 5, 2 ** 30, 7]])
+@pytest.mark.parametrize("q_dtype,dtype", [(BF16, BF16), (F32, BF16)])
+def test_group_starts_that_fall(ctx, q_dtype, dtype, start):
+    """Groups that lie over each other or end before they begin: the outputs are those of
+    the sequences all the same."""
+    print(f"[gpu] prefix falling starts {q_dtype}/{dtype} {start[:5]}", flush=True)
+    rng = np.random.default_rng(300 + dtype)
+    g = Groups(ctx, rng, [(100, [1 + i % 20 for i in range(512)])], dtype, 2, 64, 16)
+    q = R.encode(rng.standard_normal((512, 8, 64)) * 1.5, q_dtype)
+    want = expected(g.pg, q, [1] * 512, q_dtype, 0.125, 0, 0)
+    batch = g.batch([1] * 512)
+    prefix = g.desc(start=start, prefix=[100] * (len(start) - 1))
+    check(run(ctx, g.pg, batch, prefix, q, 8, q_dtype, 0.125), *want)
+    assert run.workspace != wpcg.PagedAttention(ctx, g.pg.kv, batch, 8, q_dtype, scale=0.125).workspace_bytes

@@ -70,13 +70,13 @@ __device__ __forceinline__ Group group_rows(const PrefixArgs& p, const Batch& x,
     }
     return r;
 }
-// How many tokens it shares, `prefix` of them by its own number, from the pages of
-// sequence `from`, which has no more than its own.
+// How many tokens it shares, at most `prefix` and from the pages of sequence `from`,
+// which has no more than its own.
 __device__ __forceinline__ int group_length(const PrefixArgs& p, const Batch& x, int g, int from, int prefix)
 {
     const Group r = group_rows(p, x, g);
     const int len = x.len[r.n > 0 ? from : 0];
-    return r.n > 0 && len <= p.a.b.max_kv ? max(0, min(min(prefix, p.max_prefix), len)) : 0;
+    return r.n > 0 && len <= p.a.b.max_kv ? max(0, min(prefix, len)) : 0;
 }
 __device__ __forceinline__ Group group_of(const PrefixArgs& p, const Batch& x, int g)
 {
@@ -333,12 +333,14 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         t.tiles[g] = 0x7fffffff;  // (below the sequence whose pages are read)
     }
     __syncthreads();
+    bool falls = false;
     int which[2], least[2];  // of the thread's sequences that see something: group and first position
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const int s = tid + i * THREADS;
         which[i] = -1;
         if (s >= n_seq) continue;
+        falls |= s_start[s + 1] < s_start[s];
         const int g = group_at(p, x, s);
         const Group of = group_rows(p, x, g);
         const SeqRows r = rows_of(a.b, x, s);
@@ -349,10 +351,13 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         atomicMax(&s_most[g], r.len - 1);
     }
     const int own_group = THREADS - 1 - tid;  // (of the waves with fewest sequences)
+    if (own_group < p.n_groups) falls |= s_group[own_group + 1] < s_group[own_group];
+    falls = __any(falls);
+    if ((tid & 63) == 0) t.items[tid >> 6] = falls;  // (the deal writes there behind a barrier of its own)
     if (a.window <= 0 && own_group < p.n_groups) {
         const int from = max(0, min(s_group[own_group], n_seq - 1));  // the first sequence
         s_from[own_group] = (uint16_t)from;
-        s_prefix[own_group] = group_length(p, x, own_group, from, s_prefix[own_group]);
+        s_prefix[own_group] = group_length(p, x, own_group, from, min(s_prefix[own_group], p.max_prefix));
     }
     __syncthreads();
     // With a window only the sequence whose rows begin lowest is sure to have all
@@ -367,8 +372,14 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
             const bool some = t.tiles[own_group] < n_seq;
             const int from = some ? t.tiles[own_group] : 0;
             s_from[own_group] = (uint16_t)from;
-            s_prefix[own_group] = some ? group_length(p, x, own_group, from, s_prefix[own_group]) : 0;
+            s_prefix[own_group] = some ? group_length(p, x, own_group, from, min(s_prefix[own_group], p.max_prefix)) : 0;
         }
+        __syncthreads();
+    }
+    // Where starts fall, groups or their rows may lie over each other and be more than
+    // the parts' places are for: nothing is shared.
+    if (t.items[0] | t.items[1] | t.items[2] | t.items[3]) {
+        if (own_group < p.n_groups) s_prefix[own_group] = 0;
         __syncthreads();
     }
     const PrefixDeal dealt = deal<OCOLS>(p, x, t, s_sums);
