@@ -244,3 +244,21 @@ def test_prefix_workspace():
     assert ATTEND_WS(ref(pages()), ref(batch()), ref(prefix()), ref(attention()), None) == E_ARG
     # the parts' places hold whatever the bounds allow, loose rows too
     assert attend_ws(pages(), batch(n_seq=64, n_rows=1 << 20, max_q=1, max_kv=10000, table_stride=1000), x, attention()) == n
+
+
+def test_prefixes_of_too_many_rows_and_heads_are_plain():
+    """Outputs for 2^32 threads of one launch: the plain call, which takes them."""
+    plain = C.c_uint64()
+    for n_kv, heads, rows in ((2048, 65536, 512), (65536, 65536, 512 * 32)):
+        kv = pages(n_kv_heads=n_kv)
+        b = batch(n_seq=512, n_rows=rows, max_q=rows // 512, max_kv=64, table_stride=4)
+        rc = wpcg.lib.wpcg_paged_attention_workspace(ref(kv), ref(b), ref(attention(n_heads=heads)), C.byref(plain))
+        n = attend_ws(kv, b, prefix(n_groups=1, max_prefix=64), attention(n_heads=heads))
+        if rc != OK:
+            assert n == rc == E_UNSUPPORTED
+            continue
+        assert n == plain.value
+    # a row less of each is shared
+    kv, b = pages(n_kv_heads=2048), batch(n_seq=511, n_rows=511, max_q=1, max_kv=64, table_stride=4)
+    assert wpcg.lib.wpcg_paged_attention_workspace(ref(kv), ref(b), ref(attention(n_heads=65536)), C.byref(plain)) == OK
+    assert attend_ws(kv, b, prefix(n_groups=1, max_prefix=64), attention(n_heads=65536)) != plain.value

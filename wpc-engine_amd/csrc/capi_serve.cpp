@@ -298,7 +298,8 @@ int plan_prefix(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_kv_pref
     const double again = (double)(b.n_seq - groups) * seen * 2 * n_kv * kv->head_dim * type_size(kv->dtype) / 1e6;
     const double pays = a->dtype == WPCG_DTYPE_BF16 ? 250 : kv->dtype == WPCG_DTYPE_F32 ? 700 : 450;
     o.shared = rows > 0 && cols <= 2 * ATTN_FEW_COLS && groups > 0 && groups < b.n_seq && groups <= PREFIX_GROUPS &&
-               b.n_seq <= PREFIX_SEQS && again >= pays && cost < (double)(1 << 30);
+               b.n_seq <= PREFIX_SEQS && again >= pays && cost < (double)(1 << 30) &&
+               (double)b.n_seq * b.max_q * a->n_heads * kv->head_dim < 256.0 * GROUPS_256;  // the join's workgroups
     if (!o.shared) {
         if (int rc = plan_attention(kv, b, a, &o.plain)) return rc;
         o.bytes = o.plain.bytes;
