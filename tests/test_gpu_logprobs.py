@@ -357,3 +357,30 @@ def test_ties_at_the_border_of_segments(ctx, dtype, v, top):
     bits = R.encode(np.array(rows), dtype)
     tokens = [int(i) for i in rng.integers(0, v, len(rows))]
     check(run(ctx, bits, dtype, np.array(tokens), top), R.decode(bits, dtype), tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logits_as_wide_as_the_type(ctx, dtype):
+    """Differences beyond the type's range: at +inf all finite logits are alike, at
+    temperatures of their size they are told apart; differences of the least numbers at
+    the least temperatures."""
+    rng = np.random.default_rng(12)
+    v = 5000
+    most = 3.4028234663852886e38 if dtype == F32 else 3.3895313892515355e38
+    temp = np.array([np.inf, np.inf, np.inf, 1e38, 3.4e38, 2e37, 1e35, 1.0, 1e6, 1e-38, 1e-45, 3e-45, 1e-40], np.float32)
+    x = rng.uniform(-1, 1, (len(temp), v)) * most
+    x[1, ::2] = -np.inf
+    x[2] = rng.standard_normal(v)
+    x[2, ::3] = -most
+    x[2, 17] = most
+    x[7, 100:] = -most  # a mask beneath ordinary logits
+    x[7, :100] = rng.standard_normal(100)
+    x[8] = rng.standard_normal(v) * 1e6
+    least = 2.0 ** (-149 if dtype == F32 else -133)
+    x[9:] = rng.integers(-5, 6, (4, v)) * least
+    x[9] = rng.integers(-5, 6, v) * 2.0 ** -127
+    bits = R.encode(x, dtype)
+    x = R.decode(bits, dtype)
+    tokens = rng.integers(0, v, len(temp))
+    tokens[3:7] = [int(np.argmax(r)) for r in x[3:7]]
+    check(run(ctx, bits, dtype, tokens, 9, temp), x, tokens, 9, temp)

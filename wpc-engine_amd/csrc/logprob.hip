@@ -38,14 +38,23 @@ __device__ __forceinline__ double row_rate_d(const LogprobArgs& p, int row)
     const float t = p.temperature ? p.temperature[row] : 1.0f;
     return t > 0.0f ? 1.4426950408889634 / (double)t : -1.0;
 }
-// The same in fp32: finite, so that 0 times it is 0, and not 0, so that -inf times
-// it is -inf (the least one scales any difference to less than 2^-20: off by less
-// than exp2_fast is).
-__device__ __forceinline__ float row_rate(const LogprobArgs& p, int row)
-{
-    const float rate = (float)fmin(row_rate_d(p, row), 3.0e38);
-    return rate == 0.0f ? 0x1p-149f : rate;
-}
+// (x - from) times any rate in fp32. With low rates a difference may be too large for
+// fp32 and its product not: the logits are scaled down before. With high ones it may be a
+// denormal, and the rate too large: it is scaled up. The rate stays finite, so that 0
+// times it is 0, and not 0, so that -inf times it is -inf (2^-149 makes less than 2^-50 of
+// any difference that is left).
+__device__ __forceinline__ bool ordinary(double rate) { return rate < 0.0 || (rate >= 0x1p-100 && rate <= 0x1p100); }
+struct WideRate {
+    float fit, grow, by;
+    __device__ __forceinline__ explicit WideRate(double rate)
+    {
+        const bool low = rate < 1.0;
+        fit = low ? 0x1p-32f : 1.0f;
+        grow = low ? 1.0f : 0x1p32f;
+        by = fmaxf((float)(rate * (low ? 0x1p32 : 0x1p-32)), 0x1p-149f);
+    }
+    __device__ __forceinline__ float operator()(float x, float from) const { return (x * fit - from * fit) * grow * by; }
+};
 
 // Rows need not start on 16 bytes: chunks and segments are of places from the last
 // 16-byte border before the row's start on, `skew` places before its first id, and
@@ -130,7 +139,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
     const int token = p.tokens ? p.tokens[row] : -1;
     const bool inside = token >= 0 && token < p.vocab;
     const float xt = inside ? logit(p, row, token) : INFINITY;
-    const float rate = row_rate(p, row);
+    const double rate_d = row_rate_d(p, row);
 
     // maxima of the 64-id segments, which are SEG / PER lanes of one load, and
     // of the chunk
@@ -163,12 +172,35 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
     }
     best = wave_max(best);
 
+    int before = 0;
+    // greater logits come before the token's, and equal ones of lower ids
+    if (inside && best >= xt) {
+        if (id0 > token) {
+#pragma unroll
+            for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] > xt));
+        } else if (id0 >= 0 && id0 + CHUNK <= token) {
+#pragma unroll
+            for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] >= xt));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VALUES; i++)
+                before += __popcll(__ballot(c.v[i] > xt || (c.v[i] == xt && (uint32_t)(id0 + C::place(i)) < (uint32_t)token)));
+        }
+    }
+
     // Of the maximum itself e^0 = 1 is added like any other term where the sum is
     // 3 and more: 16 additions' roundings of it are 24 of what is left without it.
     // Else ids at the maximum are counted and the others summed again.
-    const float base = best == -INFINITY ? 0.0f : best;
+    float base = best == -INFINITY ? 0.0f : best, most = best, rate = (float)rate_d;
+    if (!ordinary(rate_d)) {  // t itself in the logits' place
+        const WideRate scaled(rate_d);
+#pragma unroll
+        for (int i = 0; i < VALUES; i++) c.v[i] = scaled(c.v[i], base);
+        base = most = 0.0f;
+        rate = 1.0f;
+    }
     float z[4] = {}, s[2] = {};
-    int tops = 1, before = 0;
+    int tops = 1;
 #pragma unroll
     for (int i = 0; i < VALUES; i++) {
         const float t = (c.v[i] - base) * rate, e = exp2_fast(t);  // (a NaN reaches z)
@@ -185,26 +217,12 @@ __global__ __launch_bounds__(THREADS) void k_logprob_stats(LogprobArgs p)
         asm volatile("" : "+v"(from));
 #pragma unroll
         for (int i = 0; i < VALUES; i++) {
-            const bool top = c.v[i] == best;
+            const bool top = c.v[i] == most;
             z[i & 3] += top ? 0.0f : exp2_fast((c.v[i] - from) * rate);
             tops += __popcll(__ballot(top));
         }
         zs = wave_sum((z[0] + z[1]) + (z[2] + z[3]));
         if (best == -INFINITY) tops = 0;
-    }
-    // greater logits come before the token's, and equal ones of lower ids
-    if (inside && best >= xt) {
-        if (id0 > token) {
-#pragma unroll
-            for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] > xt));
-        } else if (id0 >= 0 && id0 + CHUNK <= token) {
-#pragma unroll
-            for (int i = 0; i < VALUES; i++) before += __popcll(__ballot(c.v[i] >= xt));
-        } else {
-#pragma unroll
-            for (int i = 0; i < VALUES; i++)
-                before += __popcll(__ballot(c.v[i] > xt || (c.v[i] == xt && (uint32_t)(id0 + C::place(i)) < (uint32_t)token)));
-        }
     }
     const float ss = wave_sum(s[0] + s[1]);
     if (lane == 0) p.part[(uint64_t)row * p.chunks + chunk] = LogprobPart{best, zs, ss, tops, before};
