@@ -167,11 +167,9 @@ struct Shared {
     uint64_t place[WAVES][64];
 };
 
-// Which tokens the columns of attend() see, and who they are: a sequence's rows
-// over all that their positions see.
+// Which tokens the columns of attend() take of those that their positions see: all.
 struct Whole {
     static constexpr bool PART = false;  // outputs, where no part is asked for
-    static constexpr bool POSITIONS = false;
     __device__ __forceinline__ bool takes(int) const { return true; }
     __device__ __forceinline__ void clip(int&, int&) const {}
 };
@@ -180,15 +178,15 @@ struct Whole {
 // those that `seen` lists (all that the columns see, and then some). Where
 // that is all of them the outputs, else their part: [column][D] unnormalised
 // at part_o, [column][2] maximum and sum at part_ml. `of` may narrow the tokens
-// that are taken (takes, clip) and say where its columns are (position, whole),
-// which then are no one sequence's. W = 1: by one wave of several that go their own
-// ways.
+// that are taken (takes, clip). W = 1: a part, by one wave of several that go their
+// own ways.
 template <int D, int CT, bool QF32, int NB, int W = ATTN_FEW_WAVES, class OF = Whole,
           class SEEN = SeenTiles<TILE>>
 __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF32, NB, W>& sh, const SeqRows& sq, int seq,
                                        int kvh, int cb, const SEEN& seen, int v0, int v1, float* part_o,
                                        float* part_ml, const OF& of = OF())
 {
+    static_assert(OF::PART == (W == 1), "a wave leaves parts");
     using Sh = Shared<D, CT, QF32, NB, W>;
     constexpr int WAVES = Sh::WAVES, THREADS = Sh::THREADS, SLOTS = Sh::SLOTS;
     constexpr bool F32MM = Sh::F32MM;
@@ -212,18 +210,6 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
     int pos[NB];  // of this lane's columns
 #pragma unroll
     for (int n = 0; n < NB; n++) pos[n] = pos0 + min(cb * COLS + 16 * n + c, cols - 1) / p.group;
-    if constexpr (OF::POSITIONS) {
-#pragma unroll
-        for (int n = 0; n < NB; n++) pos[n] = of.position(sq.a + min(cb * COLS + 16 * n + c, cols - 1) / p.group);
-        int least = pos[0], most = pos[0];
-#pragma unroll
-        for (int n = 1; n < NB; n++) {
-            least = min(least, pos[n]);
-            most = max(most, pos[n]);
-        }
-        all_hi = ~wave_max_i(~least) + 1;
-        all_lo = p.window > 0 ? wave_max_i(most) - p.window + 1 : 0;
-    }
     of.clip(all_hi, all_lo);
 
     const uint8_t* const kp = (const uint8_t*)p.k + (uint64_t)kvh * p.head_stride * ES;
@@ -481,7 +467,6 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
         l[n] = sum_x16_32(l[n]);
         if (__any(fault)) l[n] = __builtin_nanf("");
         if constexpr (W == 1) {
-            static_assert(W > 1 || OF::PART, "a wave leaves parts");
             float* const to = part_o + (16 * n + c) * D;
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -548,7 +533,7 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& p, Shared<D, CT, QF3
 #pragma unroll
         for (int w = 1; w < SLOTS; w++) o += *(const pf32x4*)&s_o[w][oc][od];
         const int orow = ocol / p.group, ohead = kvh * p.group + ocol % p.group;
-        if (OF::PART || part_o) {
+        if (part_o) {
             *(pf32x4*)(part_o + oc * D + od) = o;
             if (od == 0) {
                 part_ml[oc * 2] = om;

@@ -191,7 +191,7 @@ struct OwnTiles {
     __device__ __forceinline__ bool some(int t) const { return (t < hi && t >= lo) || (t < sinks && t >= from); }
 };
 struct OwnTokens {
-    static constexpr bool PART = true, POSITIONS = false;
+    static constexpr bool PART = true;
     int from;
     __device__ __forceinline__ bool takes(int t) const { return t >= from; }
     __device__ __forceinline__ void clip(int&, int& lo) const { lo = max(lo, from); }
