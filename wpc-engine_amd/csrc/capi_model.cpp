@@ -73,6 +73,7 @@ struct wpcg_model {
     // and the tokens as a call takes them (max_pos of them)
     float* pin_out = nullptr;
     uint32_t* pin_tok = nullptr;
+    uint32_t* pin_score = nullptr;  // what a score takes and gives, made on first use
     uint32_t* tokens = nullptr;                // [max_pos + 1]
     float *residual = nullptr, *normed = nullptr, *q = nullptr, *k = nullptr, *v = nullptr;
     float *attn = nullptr, *g = nullptr, *u = nullptr,
@@ -166,6 +167,7 @@ void free_model(wpcg_model* m)
     for (void* p : m->pf.allocs) (void)hipFree(p);
     if (m->pin_out) (void)hipHostFree(m->pin_out);
     if (m->pin_tok) (void)hipHostFree(m->pin_tok);
+    if (m->pin_score) (void)hipHostFree(m->pin_score);
 }
 
 // Every call on a model waits for the stream or queues work that later calls
@@ -1339,16 +1341,17 @@ int wpcg_model_score(wpcg_model* m, const uint32_t* tokens, uint32_t n, const in
     uint64_t ws = 0;
     if (int rc = wpcg_logprobs_workspace(&d, &ws)) return rc;
     Prefill& P = m->pf;
+    if (!m->pin_score) WPCG_HIP(hipHostMalloc((void**)&m->pin_score, WORDS * 4));
     if (!P.score) {
         WPCG_HIP(hipMalloc(&P.score, WORDS * 4 + ws));
         m->allocs.push_back(P.score);
     }
-    uint32_t* w = (uint32_t*)P.score;
-    uint32_t words[WORDS] = {};
-    if (targets) std::memcpy(words, targets, n * 4);
-    for (uint32_t i = 0; i < n; i++) std::memcpy(&words[ROWS + i], &temperature, 4);
-    WPCG_HIP(hipMemcpyAsync(w, words, IN * 4, hipMemcpyHostToDevice, s));
-    WPCG_HIP(hipStreamSynchronize(s));  // `words` is read
+    uint32_t *const w = (uint32_t*)P.score, *const words = m->pin_score;
+    for (uint32_t i = 0; i < n; i++) {
+        words[i] = targets ? (uint32_t)targets[i] : 0;
+        std::memcpy(&words[ROWS + i], &temperature, 4);
+    }
+    WPCG_HIP(launch_copy_words(w, words, ROWS + n, s));
     st.n_prompt = 0xffffffffu;
     if (int rc = put_state(m, st, tokens, n)) return rc;
     m->hst_ok = false;
@@ -1370,9 +1373,9 @@ int wpcg_model_score(wpcg_model* m, const uint32_t* tokens, uint32_t n, const in
     d.entropy_dev = entropy ? f + ROWS : nullptr;
     d.rank_dev = rank ? (int32_t*)f + 2 * ROWS : nullptr;
     d.top_ids_dev = top_ids ? (int32_t*)f + 3 * ROWS : nullptr;
-    d.top_logprob_dev = top_logprob ? f + 3 * ROWS + ROWS * WPCG_LOGPROB_TOP : nullptr;
+    d.top_logprob_dev = top_logprob ? f + 3 * ROWS + n * top : nullptr;
     if (int rc = wpcg_logprobs(m->ctx, &d, w + WORDS, ws, s)) return rc;
-    WPCG_HIP(hipMemcpyAsync(words + IN, f, (WORDS - IN) * 4, hipMemcpyDeviceToHost, s));
+    WPCG_HIP(launch_copy_words(words + IN, f, 3 * ROWS + 2 * n * top, s));
     if (int rc = take_state(m, nullptr)) return rc;  // waits for the stream
     const auto give = [&](void* to, uint32_t at, uint32_t count) {
         if (to && count) std::memcpy(to, &words[IN + at], (size_t)count * 4);
@@ -1381,7 +1384,7 @@ int wpcg_model_score(wpcg_model* m, const uint32_t* tokens, uint32_t n, const in
     give(entropy, ROWS, n);
     give(rank, 2 * ROWS, n);
     give(top_ids, 3 * ROWS, n * top);
-    give(top_logprob, 3 * ROWS + ROWS * WPCG_LOGPROB_TOP, n * top);
+    give(top_logprob, 3 * ROWS + n * top, n * top);
     return WPCG_OK;
 }
 
