@@ -635,9 +635,9 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  * their first tokens (answers to one prompt, beams, questions about one document):
  * group g is sequences group_start[g] .. group_start[g+1]-1, and the first
  * prefix_len[g] tokens of all of them are the same, so that their keys and values
- * are read once for the group, from the pages of its first sequence, or, with a
- * window, of the one whose rows begin lowest, which sees all that the others do (a
- * sequence that is further on may have given those pages away). Tables,
+ * are read once for the group, from the pages of its first sequence that has rows,
+ * or, with a window, of the one whose rows begin lowest, which sees all that the
+ * others do (a sequence that is further on may have given those pages away). Tables,
  * lengths and everything else are as for wpcg_paged_attention, which gives the
  * same outputs within rounding: every sequence's row of the table lists all the
  * pages that its rows see, the shared ones among them (where a prefix ends inside a

@@ -483,3 +483,33 @@ def test_group_starts_that_fall(ctx, q_dtype, dtype, start):
     prefix = g.desc(start=start, prefix=[100] * (len(start) - 1))
     check(run(ctx, g.pg, batch, prefix, q, 8, q_dtype, 0.125), *want)
     assert run.workspace != wpcg.PagedAttention(ctx, g.pg.kv, batch, 8, q_dtype, scale=0.125).workspace_bytes
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+def test_first_sequences_without_rows(ctx, q_dtype, dtype):
+    """Sequences of a step that have no rows, at their groups' begin: ended ones, and
+    ones whose rows of the table hold anything, as no row sees their pages."""
+    print(f"[gpu] prefix first without rows {q_dtype}/{dtype}", flush=True)
+    rng = np.random.default_rng(400 + dtype)
+    groups = [(150, [4, 30, 9]), (200, [8, 40, 20, 1]), (70, [8, 8, 5]), (33, [1, 2])]
+    g = Groups(ctx, rng, groups, dtype, 2, 64, 16)
+    pg = g.pg
+    per = [0, 2, 2, 0, 0, 1, 2, 0, 2, 2, 0, 0]
+    pg.kv_len[3] = 0
+    for n in "kv":
+        pg.real[n][3] = pg.real[n][3][:0]
+    whole = pg.table.copy()
+    for s in (0, 4, 7, 10, 11):
+        pg.table[s] = rng.integers(0, pg.n_pages, pg.table.shape[1]) if s != 4 else -1
+    pg.table[7] = 2 ** 31 - 1
+    q = R.encode(rng.standard_normal((sum(per), 8, 64)) * 1.5, q_dtype)
+    batch = g.batch(per)
+    want = expected(pg, q, per, q_dtype, 0.125, 0, 0)
+    check(run(ctx, pg, batch, g.desc(), q, 8, q_dtype, 0.125), *want)
+    assert run.workspace != wpcg.PagedAttention(ctx, pg.kv, batch, 8, q_dtype, scale=0.125).workspace_bytes
+    # a length that is none in their place, and with their own pages
+    pg.table = whole
+    for bad in (-1, 2 ** 31 - 1):
+        batch = g.batch(per)
+        pg.d_len.write(np.array([bad if i in (0, 7) else m for i, m in enumerate(pg.kv_len)], np.int32))
+        check(run(ctx, pg, batch, g.desc(), q, 8, q_dtype, 0.125), *want)

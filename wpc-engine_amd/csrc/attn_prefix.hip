@@ -333,6 +333,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         t.tiles[g] = 0x7fffffff;  // (below the sequence whose pages are read)
     }
     __syncthreads();
+    const auto sees = [](const SeqRows& r) { return r.n > 0 && !r.bad && r.len > 0; };
     bool falls = false;
     int which[2], least[2];  // of the thread's sequences that see something: group and first position
 #pragma unroll
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         const int g = group_at(p, x, s);
         const Group of = group_rows(p, x, g);
         const SeqRows r = rows_of(a.b, x, s);
-        if (s < of.s0 || s >= of.s0 + of.n || r.n == 0 || r.bad || r.len == 0) continue;
+        if (s < of.s0 || s >= of.s0 + of.n || !sees(r)) continue;
         which[i] = g;
         least[i] = r.len - r.n;
         atomicMin(&s_least[g], least[i]);
@@ -355,7 +356,10 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
     falls = __any(falls);
     if ((tid & 63) == 0) t.items[tid >> 6] = falls;  // (the deal writes there behind a barrier of its own)
     if (a.window <= 0 && own_group < p.n_groups) {
-        const int from = max(0, min(s_group[own_group], n_seq - 1));  // the first sequence
+        // the first sequence that has rows: others' pages are not looked at
+        const Group of = group_rows(p, x, own_group);
+        int from = of.n > 0 ? of.s0 : 0;
+        while (from < of.s0 + of.n - 1 && !sees(rows_of(a.b, x, from))) from++;
         s_from[own_group] = (uint16_t)from;
         s_prefix[own_group] = group_length(p, x, own_group, from, min(s_prefix[own_group], p.max_prefix));
     }
