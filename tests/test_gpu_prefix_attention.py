@@ -513,3 +513,43 @@ def test_first_sequences_without_rows(ctx, q_dtype, dtype):
         batch = g.batch(per)
         pg.d_len.write(np.array([bad if i in (0, 7) else m for i, m in enumerate(pg.kv_len)], np.int32))
         check(run(ctx, pg, batch, g.desc(), q, 8, q_dtype, 0.125), *want)
+
+
+def test_errors_of_other_calls(ctx):
+    """A refused allocation before them is not reported by calls that work."""
+    rng = np.random.default_rng(500)
+    g = Groups(ctx, rng, [(150, [4, 30, 9])], BF16, 2, 64, 16)
+    q = ctx.upload(R.encode(rng.standard_normal((3, 8, 64)), BF16))
+    out, ints, flt = ctx.alloc(3 * 8 * 64 * 2), ctx.upload(np.zeros(64, np.int32)), ctx.alloc(4096)
+    batch = g.batch([1] * 3)
+    shared = wpcg.PrefixAttention(ctx, g.pg.kv, batch, g.desc(), 8, BF16)
+    plain = wpcg.PagedAttention(ctx, g.pg.kv, batch, 8, BF16)
+    assert shared.workspace_bytes != plain.workspace_bytes
+    prompt = wpcg.PagedAttention(ctx, g.pg.kv, g.batch([40] * 3, n_rows=120), 8, BF16)  # (many rows; not run)
+    assert prompt.workspace_bytes >= 0
+    many_q = ctx.upload(R.encode(rng.standard_normal((120, 8, 64)), BF16))
+    many_out = ctx.alloc(120 * 8 * 64 * 2)
+    pool = wpcg.KvPool(ctx, 20, 16, 3, 4)
+    copies, result = ctx.alloc(400), ctx.alloc(8)
+    k = ctx.upload(R.encode(rng.standard_normal((3, 2, 64)), BF16))
+    scratch = wpcg.PagedKv(ctx, 20, 16, 2, 64, BF16)
+    room = wpcg.KvBatch(3, 3, pool.kv_len, pool.table, 4, 64)
+    score = wpcg.LogProbs(ctx, 2, 100, top=3)
+    logits = ctx.upload(rng.standard_normal((2, 100)).astype(np.float32))
+    u = ctx.upload(np.full(8, 0.5, np.float32))
+    draft = wpcg.DraftVerify(ctx, 1, 2, 2, 100)
+    ids = ctx.alloc(400)
+    calls = {"fork": lambda: wpcg.KvFork(ctx, pool, copies, result, grow=5).run(),
+             "large fork": lambda: wpcg.KvFork(ctx, wpcg.KvPool(ctx, 20, 16, 70, 4), ctx.alloc(1024), result).run(),
+             "compact": lambda: wpcg.KvCompact(ctx, pool, copies, result, 5).run(),
+             "copy": lambda: wpcg.KvCopy(ctx, [scratch], copies, result, 3).run(),
+             "append": lambda: wpcg.KvAppend(ctx, scratch, room, 8, BF16).run(None, k, k, None),
+             "shared": lambda: shared.run(q, out), "plain": lambda: plain.run(q, out),
+             "prompt": lambda: prompt.run(many_q, many_out), "score": lambda: score.run(logits, ints, flt, top_ids=ids),
+             "draft": lambda: draft.run(logits, ints, u, u, flt, out)}
+    for name, call in calls.items():
+        with pytest.raises(wpcg.WpcgError):
+            ctx.alloc(1 << 50)
+        print(f"[gpu] after a refused allocation: {name}", flush=True)
+        call()
+        ctx.sync()

@@ -349,6 +349,7 @@ void go_types(const PagedAttnArgs& p, int q_dtype, int cache_dtype, hipStream_t 
 
 hipError_t launch_attn_few(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     if (p.b.n_seq == 0) return hipSuccess;
     if (head_dim == 128) go_types<128>(p, q_dtype, cache_dtype, s);
     else go_types<64>(p, q_dtype, cache_dtype, s);

@@ -255,6 +255,7 @@ void join(const PagedAttnArgs& p, hipStream_t s)
 
 hipError_t launch_attn_many(const PagedAttnArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     const uint64_t blocks =
         (p.blocks ? (uint64_t)p.blocks : (uint64_t)p.b.n_seq * p.col_blocks) * p.n_kv * p.splits;
     if (blocks == 0) return hipSuccess;

@@ -619,6 +619,7 @@ void go_types(const PrefixArgs& p, int q_dtype, int cache_dtype, hipStream_t s)
 
 hipError_t launch_attn_prefix(const PrefixArgs& p, int head_dim, int q_dtype, int cache_dtype, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     if (head_dim == 128) go_types<128>(p, q_dtype, cache_dtype, s);
     else go_types<64>(p, q_dtype, cache_dtype, s);
     return hipGetLastError();

@@ -478,6 +478,7 @@ __global__ __launch_bounds__(THREADS) void k_draft_choose(DraftArgs p)
 
 hipError_t launch_draft_verify(const DraftArgs& p, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     if (p.n_seq == 0) return hipSuccess;
     const unsigned groups = (unsigned)(p.chunks + 3) / 4;
     if (p.n_rows > 0) k_draft_stats<<<dim3((unsigned)p.n_rows * groups), dim3(THREADS), 0, s>>>(p);

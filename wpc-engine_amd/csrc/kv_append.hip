@@ -169,6 +169,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(KvAppendArgs p)
 
 hipError_t launch_kv_append(const KvAppendArgs& p, int head_dim, bool bf16, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     const int heads = THREADS * 8 / head_dim;
     const uint64_t blocks = (uint64_t)p.b.n_rows * (uint64_t)((p.n_units + heads - 1) / heads);
     if (blocks == 0) return hipSuccess;

@@ -561,6 +561,7 @@ __global__ __launch_bounds__(COPY_THREADS) void k_kv_copy(CopyArgs a)
 
 hipError_t launch_kv_fork(const ForkArgs& a, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     // One workgroup for small pools. It and the three launches, us, sequences x pages
     // each: 8 x 30 6.9 and 11.9, 32 x 38 8.2 and 12.0, 64 x 126 12.6 and 15.5; with room
     // for 256 sequences, 16 entries and 16 rows of pages the first two took 8.6 and 9.7,
@@ -580,6 +581,7 @@ hipError_t launch_kv_fork(const ForkArgs& a, hipStream_t s)
 
 hipError_t launch_kv_compact(CompactArgs a, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     const unsigned rows = (unsigned)a.p.n_seq * (unsigned)((a.p.stride + THREADS - 1) / THREADS);
     a.move_blocks = std::max(1, (std::min(a.p.n_pages / 2, a.max_copies) + THREADS - 1) / THREADS);
     k_compact_count<<<dim3((unsigned)a.blocks), dim3(THREADS), 0, s>>>(a);
@@ -590,6 +592,7 @@ hipError_t launch_kv_compact(CompactArgs a, hipStream_t s)
 
 hipError_t launch_kv_copy(CopyArgs a, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     // 16 waves a CU at most: enough loads in flight
     const uint64_t all = (uint64_t)a.max_copies * a.units;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((all + COPY_WAVES - 1) / COPY_WAVES, 256 * 4);

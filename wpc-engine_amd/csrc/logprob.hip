@@ -554,6 +554,7 @@ __global__ __launch_bounds__(THREADS) void k_logprob_finish(LogprobArgs p)
 
 hipError_t launch_logprobs(const LogprobArgs& p, hipStream_t s)
 {
+    (void)hipGetLastError();  // report only these launches
     if (p.n_rows == 0) return hipSuccess;
     const dim3 grid((unsigned)p.n_rows * ((unsigned)(p.chunks + 3) / 4));
     // F32 rows in many rounds of workgroups come from the memory faster to four of them a
