@@ -639,19 +639,22 @@ int wpcg_paged_attention(wpcg_ctx* ctx, const wpcg_kv_pages* kv, const wpcg_kv_b
  * or, with a window, of the one whose rows begin lowest, which sees all that the
  * others do (a sequence that is further on may have given those pages away). Tables,
  * lengths and everything else are as for wpcg_paged_attention, which gives the
- * same outputs within rounding: every sequence's row of the table lists all the
- * pages that its rows see, the shared ones among them (where a prefix ends inside a
- * page, each sequence may have a copy of that page). A prefix is taken as far as
- * max_prefix and that sequence's length; sequences of no group, groups of one and
- * groups whose numbers are not within the batch share nothing. Each sequence's
- * rows come after its group's prefix as a rule, but need not. Work is shared out
- * by the lengths, so that a sequence's last bits may depend on the others; the same
- * call on the same arrays gives the same bits. Sharing is for single tokens and
- * drafts, at most 32 rows times query heads a key-value head, and up to 512
- * sequences in 256 groups, where by the bounds (max_prefix and window) some 250 to
- * 700 MB of keys and values would be read again; else the call is
- * wpcg_paged_attention itself. Where group_start or q_start falls nothing is
- * shared. Workspace and streams as for wpcg_paged_attention. */
+ * same outputs within its rounding (BF16 queries: a term of the softmax is rounded
+ * to bf16 relative to the largest of the part that it is in, and the two calls' parts
+ * are others): every sequence's row of the table lists all the pages that its rows
+ * see, the shared ones among them (where a prefix ends inside a page, each sequence
+ * may have a copy of that page). A prefix is taken as far as max_prefix and that
+ * sequence's length; sequences of no group, groups of one and groups whose numbers
+ * are not within the batch share nothing, and where group_start or q_start falls
+ * none does. Each sequence's rows come after its group's prefix as a rule, but need
+ * not. Work is shared out by the lengths, so that a sequence's last bits may depend
+ * on the others; the same call on the same arrays gives the same bits. Sharing is
+ * for single tokens and drafts, at most 32 rows times query heads a key-value head,
+ * and up to 512 sequences in 256 groups, where by the bounds (n_seq, n_groups,
+ * max_prefix and window) some 250 to 700 MB of keys and values would be read again;
+ * else the call is wpcg_paged_attention itself. Bounds far above the lengths make it
+ * share short prefixes, where what it costs in any case (25 to 70 us) is more than
+ * it saves. Workspace and streams as for wpcg_paged_attention. */
 typedef struct wpcg_kv_prefix_s {
     uint32_t n_groups, max_prefix;
     const int32_t* group_start_dev; /* n_groups + 1 */

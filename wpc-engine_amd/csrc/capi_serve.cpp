@@ -287,13 +287,24 @@ int plan_prefix(const wpcg_kv_pages* kv, const PagedBatch& b, const wpcg_kv_pref
                                         b.n_seq * own_blocks * (own_tiles + OWN_ITEM));
     // Without sharing a prefix comes out of the caches for all sequences but the first,
     // at some 11 TB/s, and the fixed costs are lower: it pays from a number of bytes on
-    // that are read again. Shared and not, us, prefixes of one group's sequences, own
-    // tokens up to 200; read again, MB:
-    //   BF16 queries, BF16 cache, 32 / 4 heads    246  33 29   459  35 47   1057  46 100
-    //                 E4M3, 32 / 8                115  25 22   246  28 33    516  40 54
-    //   F32 queries, BF16 cache, 32 / 8           229  39 31   369  64 56    492  41 49
-    //                F32 cache, 14 / 2 of 64      123  44 24   229  52 33
-    // (36316 tokens, 22 rows of which see the last 106: 44 us and 9.)
+    // that are read again. Shared and not, us, one group's prefix and up to 200 own tokens;
+    // read again, MB (sequences x rows; heads of 128 but for 14 / 2):
+    //                                     120     250     450     700     1000
+    //   BF16 queries
+    //     BF16 cache, 32 / 4, 64 x 1    33 16   35 25   35 38   38 68   41  89
+    //                 14 / 2, 64 x 1    24 21   26 31   30 48   34 76   43  99
+    //                 32 / 8, 16 x 5    36 25   39 34   45 49   56 86   65 104
+    //     E4M3        32 / 8, 32 x 1    30 19   31 30   34 45   35 79   39 104
+    //   F32 queries
+    //     BF16 cache, 32 / 8, 32 x 1    44 18   44 28   46 43   47 74   48  95
+    //                 14 / 2, 64 x 1    34 22   36 32   42 47   48 76   56 100
+    //                 32 / 8, 16 x 5    51 30   56 42   69 64   84 102 104 131
+    //     E4M3        32 / 8, 32 x 1    45 23   46 38   48 58   50 101  58 134
+    //     F32         32 / 8, 32 x 1    68 27   70 38   70 54   71 93   72 119
+    //                 14 / 2, 64 x 1    43 24   45 34   47 48   52 80   58 104
+    // One bound for a pair of types, so that some batches near it take up to 10 us longer
+    // than the other way would (BF16, 32 / 4 heads, 250 to 400; F32 cache, 14 / 2, 450 to
+    // 700). (36316 tokens, 22 rows of which see the last 106: 44 us and 9.)
     const int64_t seen = a->window > 0 ? std::min<int64_t>(max_prefix, (int64_t)a->window + a->sinks + b.max_q) : max_prefix;
     const double again = (double)(b.n_seq - groups) * seen * 2 * n_kv * kv->head_dim * type_size(kv->dtype) / 1e6;
     const double pays = a->dtype == WPCG_DTYPE_BF16 ? 250 : kv->dtype == WPCG_DTYPE_F32 ? 700 : 450;
