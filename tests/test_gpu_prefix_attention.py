@@ -553,3 +553,30 @@ def test_errors_of_other_calls(ctx):
         print(f"[gpu] after a refused allocation: {name}", flush=True)
         call()
         ctx.sync()
+
+
+@pytest.mark.parametrize("q_dtype,dtype", TYPES)
+@pytest.mark.parametrize("sinks", [0, 40, 500])
+def test_windows_that_have_left_the_prefix(ctx, q_dtype, dtype, sinks):
+    """Groups none of whose rows, or of whose later ones, see a token of the prefix but
+    for the sinks; the prefixes' pages are others' by now. Prefixes that end inside tiles
+    and pages, and at their borders."""
+    print(f"[gpu] prefix window beyond {q_dtype}/{dtype} sinks {sinks}", flush=True)
+    rng = np.random.default_rng(600 + sinks + 10 * q_dtype + dtype)
+    w = least_window(q_dtype, dtype, 16, 128, 512 - 6) + 5
+    groups = [(361, [w + 90, w + 50, w + 70]), (64, [w + 1, w + 200]), (100, [w + 70, 5, w]), (17, [w + 39, w + 80]), (128, [w, w - 1]),
+              (360, [w + 300, w + 31])]
+    live = sum(len(own) for _, own in groups)
+    g = Groups(ctx, rng, groups, dtype, 16, 128, 32, empty=512 - live)
+    pg = g.pg
+    per = [1] * live + [0] * (512 - live)
+    q = R.encode(rng.standard_normal((live, 32, 128)) * 1.5, q_dtype)
+    lo = np.array(pg.kv_len) - w  # the first token in the row's window
+    first = np.arange(pg.table.shape[1])[None] * 32
+    seen = (first < np.array(pg.kv_len)[:, None]) & ((first + 32 > lo[:, None]) | (first < sinks))
+    pg.table = np.where(seen, pg.table, -1).astype(np.int32)
+    batch = g.batch(per)
+    want, bound = expected(pg, q, per, q_dtype, 0.1, w, sinks)
+    plain = wpcg.PagedAttention(ctx, pg.kv, batch, 32, q_dtype, scale=0.1, window=w, sinks=sinks).workspace_bytes
+    check(run(ctx, pg, batch, g.desc(), q, 32, q_dtype, 0.1, w, sinks), want, bound)
+    assert run.workspace != plain

@@ -116,6 +116,16 @@ __device__ __forceinline__ SeqRows uniform(const SeqRows& r)
 }
 
 // ---- prefixes ------------------------------------------------------------------
+// The tiles of a prefix of len tokens that rows at positions least .. most see.
+__device__ __forceinline__ SeenTiles<many::TILE> prefix_tiles(const PagedAttnArgs& p, int len, int least, int most)
+{
+    SeenTiles<many::TILE> r = seen_tiles<many::TILE>(least, min(most, len - 1), p.window, p.sinks);
+    if (r.lo == r.hi) {  // the windows have left it: none but the sinks'
+        r.lo = r.hi = 0;
+        r.end = r.first;
+    }
+    return r;
+}
 // A workgroup's 128 columns of a group's rows over some tiles of its prefix.
 struct PrefixWork {
     const Batch& x;
@@ -128,10 +138,6 @@ struct PrefixWork {
     __device__ __forceinline__ int all_hi() const { return min(least, g.len - 1) + 1; }
     __device__ __forceinline__ int all_lo(const PagedAttnArgs& p) const { return p.window > 0 ? most - p.window + 1 : 0; }
 };
-__device__ __forceinline__ SeenTiles<many::TILE> prefix_tiles(const PagedAttnArgs& p, const Group& g, int least, int most)
-{
-    return seen_tiles<many::TILE>(least, min(most, g.len - 1), p.window, p.sinks);
-}
 // A wave's 32 columns from w0 on.
 struct PrefixColumns {
     static constexpr bool LIMIT = true;
@@ -160,7 +166,7 @@ struct PrefixColumns {
         const int least = ~wave_max_i(~pos), most = wave_max_i(pos);
         hi = min(least + 1, len);
         lo = p.window > 0 ? most - p.window + 1 : 0;
-        seen = seen_tiles<many::TILE>(least, min(most, len - 1), p.window, p.sinks);
+        seen = prefix_tiles(p, len, least, most);
     }
 };
 
@@ -252,7 +258,7 @@ __device__ __forceinline__ PrefixDeal deal(const PrefixArgs& p, const Batch& x, 
     int3 v = {0, 0, 0};  // cost and items of a group, own tiles of two sequences
     if (tid < p.n_groups) {
         const Group g = group_of(p, x, tid);
-        const int tiles = g.len > 0 ? prefix_tiles(a, g, x.least[tid], x.most[tid]).total() : 0;
+        const int tiles = g.len > 0 ? prefix_tiles(a, g.len, x.least[tid], x.most[tid]).total() : 0;
         const int cbs = (g.rows * a.group + PCOLS - 1) / PCOLS;
         t.tiles[tid] = tiles;
         v.y = a.n_kv * cbs * ((tiles + p.chunk - 1) / p.chunk);
@@ -454,7 +460,7 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         const uint64_t slot = (uint64_t)(base.y + (kvh * chunks + ch) * cbs + cb + b);
         if (v0 < v1 && slot < p.pre_slots) {
             const PrefixWork w = {x, g, {g.a, g.rows, g.len, false}, uniform((int)s_from[lo]), kvh, cb, v0, v1, least, most,
-                                  prefix_tiles(a, g, least, most), p.pre_o + slot * PCOLS * D, p.pre_ml + slot * PCOLS * 2};
+                                  prefix_tiles(a, g.len, least, most), p.pre_o + slot * PCOLS * D, p.pre_ml + slot * PCOLS * 2};
             many::attend<D, CT, QF32, PrefixColumns>(a, sh.pre, w);
         }
         at += take;
