@@ -362,42 +362,33 @@ __global__ __launch_bounds__(THREADS, QF32 ? 1 : 2) void k_attn_shared(PrefixArg
         least[i] = r.len - r.n;
         atomicMin(&s_least[g], least[i]);
         atomicMax(&s_most[g], r.len - 1);
+        if (a.window <= 0) atomicMin(&t.tiles[g], s);
     }
     const int own_group = THREADS - 1 - tid;  // (of the waves with fewest sequences)
     if (own_group < p.n_groups) falls |= s_group[own_group + 1] < s_group[own_group];
     falls = __any(falls);
     if ((tid & 63) == 0) t.items[tid >> 6] = falls;  // (the deal writes there behind a barrier of its own)
-    if (a.window <= 0 && own_group < p.n_groups) {
-        // the first sequence that has rows: others' pages are not looked at
-        const Group of = group_rows(p, x, own_group);
-        int from = of.n > 0 ? of.s0 : 0;
-        while (from < of.s0 + of.n - 1 && !sees(rows_of(a.b, x, from))) from++;
-        s_from[own_group] = (uint16_t)from;
-        s_prefix[own_group] = group_length(p, x, own_group, from, min(s_prefix[own_group], p.max_prefix));
-    }
     __syncthreads();
-    // With a window only the sequence whose rows begin lowest is sure to have all
-    // pages that the others' rows see, as far as its own rows go: those that are further on
-    // may have given theirs away.
+    // Pages are those of the first sequence that has rows: nobody looks at the others'. With a
+    // window only the sequence whose rows begin lowest is sure to have all pages that
+    // the others' rows see, as far as its own rows go: those that are further on may have
+    // given theirs away.
     if (a.window > 0) {
 #pragma unroll
         for (int i = 0; i < 2; i++)
             if (which[i] >= 0 && least[i] == s_least[which[i]]) atomicMin(&t.tiles[which[i]], tid + i * THREADS);
         __syncthreads();
-        if (own_group < p.n_groups) {
-            const bool some = t.tiles[own_group] < n_seq;
-            const int from = some ? t.tiles[own_group] : 0;
-            s_from[own_group] = (uint16_t)from;
-            s_prefix[own_group] = some ? group_length(p, x, own_group, from, min(s_prefix[own_group], p.max_prefix)) : 0;
-        }
-        __syncthreads();
     }
     // Where starts fall, groups or their rows may lie over each other and be more than
     // the parts' places are for: nothing is shared.
-    if (t.items[0] | t.items[1] | t.items[2] | t.items[3]) {
-        if (own_group < p.n_groups) s_prefix[own_group] = 0;
-        __syncthreads();
+    falls = (t.items[0] | t.items[1] | t.items[2] | t.items[3]) != 0;
+    if (own_group < p.n_groups) {
+        const bool some = t.tiles[own_group] < n_seq && !falls;
+        const int from = some ? t.tiles[own_group] : 0;
+        s_from[own_group] = (uint16_t)from;
+        s_prefix[own_group] = some ? group_length(p, x, own_group, from, min(s_prefix[own_group], p.max_prefix)) : 0;
     }
+    __syncthreads();
     const PrefixDeal dealt = deal<OCOLS>(p, x, t, s_sums);
     if (blockIdx.x == 0) {  // for the join
         for (int s = tid; s < n_seq; s += THREADS) {
