@@ -580,3 +580,38 @@ def test_windows_that_have_left_the_prefix(ctx, q_dtype, dtype, sinks):
     plain = wpcg.PagedAttention(ctx, pg.kv, batch, 32, q_dtype, scale=0.1, window=w, sinks=sinks).workspace_bytes
     check(run(ctx, pg, batch, g.desc(), q, 32, q_dtype, 0.1, w, sinks), want, bound)
     assert run.workspace != plain
+
+
+@pytest.mark.parametrize("window", [False, True])
+def test_captured_calls_whose_first_sequences_change(ctx, window):
+    """One captured call: which sequence of a group has rows, or is furthest on, and what
+    the tables hold for the others, changes between the replays."""
+    print(f"[gpu] prefix captured, window {window}", flush=True)
+    rng = np.random.default_rng(700)
+    w = least_window(BF16, BF16, 16, 128, 512 - 2) + 5 if window else 0
+    g = Groups(ctx, rng, [(w + 90, [w + 300] * 4), (200, [w + 200] * 3)], BF16, 16, 128, 16, empty=505)
+    pg = g.pg
+    whole = {"table": pg.table.copy(), "real": pg.real}
+    batch, prefix = g.batch([1] * 7 + [0] * 505), g.desc()
+    lens, table, start = pg.d_len, pg.d_table, pg.d_start
+    q, out = ctx.alloc(7 * 32 * 128 * 2), ctx.alloc(7 * 32 * 128 * 2)
+    op = wpcg.PrefixAttention(ctx, pg.kv, batch, prefix, 32, BF16, scale=0.1, window=w)
+    assert op.workspace_bytes != wpcg.PagedAttention(ctx, pg.kv, batch, 32, BF16, scale=0.1, window=w).workspace_bytes
+    graph = ctx.capture(lambda: op.run(q, out))
+    for turn in range(6):
+        per = [1] * 7 + [0] * 505
+        per[turn % 4] = per[4 + turn % 3] = 0  # the first one of both groups in turn 0
+        n = [int(m - rng.integers(0, 150)) for m in (w + 90 + w + 300,) * 4 + (200 + w + 200,) * 3] + [0] * 505
+        pg.kv_len, pg.real = n, {k: [x[:m] for x, m in zip(whole["real"][k], n)] for k in "kv"}
+        lo = np.where(np.array(per) > 0, np.array(n) - w if window else 0, 2 ** 30)
+        first = np.arange(pg.table.shape[1])[None] * 16
+        seen = (first < np.array(n)[:, None]) & (first + 16 > lo[:, None])
+        table.write(np.where(seen, whole["table"], turn % 2 * (2 ** 31 - 1) - 1).astype(np.int32))
+        lens.write(np.array(n, np.int32))
+        start.write(np.cumsum([0] + per).astype(np.int32))
+        x = R.encode(rng.standard_normal((5, 32, 128)) * 1.5, BF16)
+        q.write(np.concatenate([x, x[:2]]))
+        graph.launch()
+        ctx.sync()
+        got = R.decode(out.read(np.uint16, 5 * 32 * 128).reshape(5, 32, 128), BF16)
+        check(got, *expected(pg, x, per, BF16, 0.1, w, 0))

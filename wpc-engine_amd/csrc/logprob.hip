@@ -314,8 +314,9 @@ __device__ uint64_t enough_from(int k, uint32_t lower, int places, List& l, EACH
         all_waves(x, g);
         return __builtin_amdgcn_readfirstlane((int)(g[0] + g[1] + g[2] + g[3]));
     };
+    if (lower == 0) lower = 1;
     int low = 0x7fffffff;  // (as a signed number)
-    each([&](uint32_t order, uint32_t) { low = order >= max(lower, 1u) ? min(low, (int)(order ^ 0x80000000u)) : low; });
+    each([&](uint32_t order, uint32_t) { low = order >= lower ? min(low, (int)(order ^ 0x80000000u)) : low; });
     uint64_t g[4];
     all_waves(~wave_max_i(~low), g);
     const uint32_t least = (uint32_t)min(min((int)g[0], (int)g[1]), min((int)g[2], (int)g[3])) ^ 0x80000000u;
